@@ -15,8 +15,8 @@ OK, VERSION_MISMATCH, INVALID_ARGUMENT, UNSUPPORTED, INTERNAL_ERROR = range(5)
 STATUS_NAMES = {OK: "OK", VERSION_MISMATCH: "VERSION_MISMATCH",
                 INVALID_ARGUMENT: "INVALID_ARGUMENT", UNSUPPORTED: "UNSUPPORTED",
                 INTERNAL_ERROR: "INTERNAL_ERROR"}
-# DType (abi/buffers.py:22-28) + F16
-F32, F64, BF16, I32, I64, U8, F16 = range(7)
+# DType (abi/buffers.py:22-28) + F16, I8
+F32, F64, BF16, I32, I64, U8, F16, I8 = range(8)
 MASK_BIDIRECTIONAL, MASK_D2F_HYBRID, MASK_FULL = range(3)
 LOGITS_RAW, LOGITS_DREAM_AR_SHIFT = range(2)
 
@@ -128,6 +128,19 @@ SIGNATURES = {
     "drt_op_lm_head_workspace_bytes": (_SZ, [_I32, _I32, _I32]),
     "drt_op_lm_head_score": (_I32, [_VP, _VP, _VP, _I32, _I32, _I32, _VP, C.c_float, _U64, _I32,
                                     _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "drt_op_kv8_store": (_I32, [_VP, _VP, _I32, _I32, _I32, _I32, _VP, _I64, _VP, _VP, _VP]),
+    "drt_op_kv_sums": (_I32, [_VP, _I64, _I32, _I32, _I32, _I32, _VP, _VP]),
+    "drt_op_kv_load": (_I32, [_VP, _I64, _I32, _VP, _I32, _I32, _I32, _VP, _VP, _I32, _VP]),
+    "drt_op_attention_kv8_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32]),
+    "drt_op_attention_kv8": (_I32, [_VP, _I32, _VP, _I64, _VP, _I32, _I32, _I32, _I32, _I32,
+                                    _I32, _I32, _I32, _VP, _I32, _VP, _SZ, _VP]),
+    "drt_op_select_blocks_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32]),
+    "drt_op_select_blocks": (_I32, [_VP, _I32, _VP, _I64, _I32, _I32, _I32, _I32, _I32, _I32,
+                                    _I32, _I32, _I32, _I32, _I32, _I32, _VP, _VP, _SZ, _VP]),
+    "drt_op_sparse_attention_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32, _I32]),
+    "drt_op_sparse_attention": (_I32, [_VP, _I32, _VP, _I64, _I32, _VP, _I32, _I32, _I32, _I32,
+                                       _I32, _I32, _I32, _I32, _VP, _I32, _I32, _VP, _I32, _VP,
+                                       _SZ, _VP]),
 }
 
 _lib = None

@@ -1,0 +1,234 @@
+// Rows into and out of the prefix cache where the cache is more than a copy of them: the
+// 8-bit store, the reading back of rows, and the sums of a tile's keys.
+#include "kv8.h"
+#include "launch.h"
+
+namespace {
+
+// One 256-thread work-group per (tile, K/V head); thread t holds 16 head dims of key t / 8, of K
+// and of V: the new rows from their source, the tile's other rows as they read. The largest
+// magnitudes choose the powers of two (a comparison of bits, in which NaN and infinities are
+// the largest), every value is rounded once (x / scale is exact), and the codes meet in LDS, from where the
+// tile leaves in 16-byte pieces.
+//   e = the least integer >= -40 with max <= 127 * 2^e;  code = rint(x * 2^-e)
+// A power of two, not max / 127: a tile that is stored to again is quantized anew from
+// what it reads as, which with these scales is one more rounding only when e rises, each time to half
+// the resolution or less, so any number of stores stays within one step of what they wrote
+// (1/2 + 1/4 + ...); and x / scale never falls on the wrong side of a rounding.
+template <bool SRC_BF16>
+__global__ __launch_bounds__(256) void kv8_store_kernel(
+    const void* __restrict__ k_src, const void* __restrict__ v_src, int n, int Hkv, int pos0,
+    uint8_t* __restrict__ kv, int64_t kv_head_stride, float* __restrict__ scales,
+    float* __restrict__ sums) {
+  const int t = (pos0 >> 5) + blockIdx.x, h = blockIdx.y;
+  const int64_t tiles = kv_head_stride / KV8_TILE;
+  const int64_t row_t = (int64_t)32 * t - pos0;  // source row of the tile's key 0 (may be negative)
+  uint8_t* tile = kv + h * kv_head_stride + (int64_t)t * KV8_TILE;
+  float* sc = scales + (h * tiles + t) * 2;
+  __shared__ __align__(16) uint8_t codes[KV8_TILE];
+  __shared__ uint32_t most[2][4];
+  __shared__ int part[4][128];
+  const int tid = threadIdx.x, kk = tid >> 3, d0 = (tid & 7) * 16;
+  const int64_t src_row = row_t + kk;
+  const bool fresh = src_row >= 0 && src_row < n;
+  float x[2][16];
+  if (fresh) {
+    const int64_t at = (src_row * Hkv + h) * 128 + d0;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const void* s = w ? v_src : k_src;
+      if (SRC_BF16) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const u32x4 r = *(const u32x4_e*)((const uint16_t*)s + at + 8 * c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[w][8 * c + 2 * e] = bf16_bits_to_float(r[e] & 0xffffu);
+            x[w][8 * c + 2 * e + 1] = bf16_bits_to_float(r[e] >> 16);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const f32x4 r = *(const f32x4_e*)((const float*)s + at + 4 * c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[w][4 * c + e] = r[e];
+        }
+      }
+    }
+  } else {  // a row that stays
+    const float sk = sc[0], sv = sc[1];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      x[0][e] = sk * (float)((int)tile[kv8_k_at(kk, d0 + e)] - 128);
+      x[1][e] = sv * (float)((int)tile[kv8_v_at(kk, d0 + e)] - 128);
+    }
+  }
+  uint32_t m[2] = {0u, 0u};
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) m[w] = max(m[w], __float_as_uint(x[w][e]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m[w] = max(m[w], (uint32_t)__shfl_xor((int)m[w], o, 64));
+    if ((tid & 63) == 0) most[w][tid >> 6] = m[w];
+  }
+  __syncthreads();  // (also: every row that stays has been read)
+  float scale[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const uint32_t b = max(max(most[w][0], most[w][1]), max(most[w][2], most[w][3]));
+    // 127 = 1.984375 * 2^6
+    const int e = max(KV8_MIN_EXP, (int)(b >> 23) - 133 + ((b & 0x7fffffu) > 0x7e0000u ? 1 : 0));
+    const bool fits = e <= KV8_MAX_EXP;
+    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    scale[w] = fits ? __uint_as_float((uint32_t)(127 + e) << 23) : __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int c = fits ? (int)rintf(x[w][i] * inv) : 0;
+      codes[w ? kv8_v_at(kk, d0 + i) : kv8_k_at(kk, d0 + i)] = (uint8_t)(c + 128);
+      x[w][i] = (float)c;
+    }
+  }
+  if (sums) {  // whole numbers below 2^12: exact in any order
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      int s = (int)x[0][i];  // the eight keys of this wave (lanes 8 apart)
+      s += __shfl_xor(s, 8, 64);
+      s += __shfl_xor(s, 16, 64);
+      s += __shfl_xor(s, 32, 64);
+      if ((tid & 63) < 8) part[tid >> 6][d0 + i] = s;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    *(u32x4*)(tile + (tid + 256 * i) * 16) = *(const u32x4*)(codes + (tid + 256 * i) * 16);
+  if (tid < 2) sc[tid] = tid ? scale[1] : scale[0];
+  if (sums && tid < 128)
+    sums[(h * tiles + t) * 128 + tid] =
+        scale[0] * (float)(part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid]);
+}
+
+// Rows [pos0, pos0 + n) of a cache back as [n][Hkv][128] values. One 256-thread work-group
+// per (tile, head), which reads the tile whole.
+// DT: 0 = 8-bit, 1 = fp16, 2 = bf16.
+DRT_DEV int kv16_k_at(int kk, int hd) { return ((hd >> 3) * 32 + kk) * 8 + (hd & 7); }
+DRT_DEV int kv16_v_at(int kk, int hd) {
+  return 4096 + ((((hd >> 5) * 2 + (kk >> 4)) * 2 + ((kk >> 2) & 1)) * 32 + (hd & 31)) * 8 +
+         (kk & 3) + 4 * ((kk >> 3) & 1);
+}
+template <int DT> DRT_DEV float kv_value(const void* tile, int at, float scale) {
+  if (DT == 0) return scale * (float)((int)((const uint8_t*)tile)[at] - 128);
+  if (DT == 1) return (float)((const _Float16*)tile)[at];
+  return bf16_bits_to_float(((const uint16_t*)tile)[at]);
+}
+
+template <int DT, bool OUT_BF16>
+__global__ __launch_bounds__(256) void kv_load_kernel(const uint8_t* __restrict__ kv,
+                                                      int64_t head_stride_bytes,
+                                                      const float* __restrict__ scales, int n,
+                                                      int Hkv, int pos0, void* __restrict__ k_out,
+                                                      void* __restrict__ v_out) {
+  constexpr int TILE = DT == 0 ? KV8_TILE : 2 * KV8_TILE;
+  const int t = (pos0 >> 5) + blockIdx.x, h = blockIdx.y;
+  const int64_t tiles = head_stride_bytes / TILE;
+  __shared__ __align__(16) uint8_t tile[TILE];
+  const int tid = threadIdx.x;
+  const uint8_t* src = kv + h * head_stride_bytes + (int64_t)t * TILE;
+#pragma unroll
+  for (int i = 0; i < TILE / 4096; ++i)
+    *(u32x4*)(tile + (tid + 256 * i) * 16) = *(const u32x4*)(src + (tid + 256 * i) * 16);
+  const float sk = DT == 0 ? scales[(h * tiles + t) * 2] : 1.f;
+  const float sv = DT == 0 ? scales[(h * tiles + t) * 2 + 1] : 1.f;
+  __syncthreads();
+  for (int it = tid; it < 32 * 32; it += 256) {  // four head dims of a key
+    const int kk = it >> 5, d = (it & 31) * 4;
+    const int64_t row = (int64_t)32 * t - pos0 + kk;
+    if (row < 0 || row >= n) continue;
+    const int64_t at = (row * Hkv + h) * 128 + d;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[e] = kv_value<DT>(tile,
+                            DT == 0 ? (w ? kv8_v_at(kk, d + e) : kv8_k_at(kk, d + e))
+                                    : (w ? kv16_v_at(kk, d + e) : kv16_k_at(kk, d + e)),
+                            w ? sv : sk);
+      void* out = w ? v_out : k_out;
+      if (OUT_BF16) {
+        uint32_t p[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          p[e] = (uint32_t)float_to_bf16_bits(x[2 * e]) |
+                 ((uint32_t)float_to_bf16_bits(x[2 * e + 1]) << 16);
+        *(uint2*)((uint16_t*)out + at) = make_uint2(p[0], p[1]);
+      } else {
+        *(f32x4*)((float*)out + at) = f32x4{x[0], x[1], x[2], x[3]};
+      }
+    }
+  }
+}
+
+// The keys of a 16-bit tile added up, in 64 bits and rounded once (an 8-bit tile's sums are
+// the store's own). One 128-thread work-group per (tile, head), thread = head dim.
+template <int DT>
+__global__ __launch_bounds__(128) void kv_sums_kernel(const uint8_t* __restrict__ kv,
+                                                      int64_t head_stride_bytes, int t0,
+                                                      float* __restrict__ sums) {
+  const int t = t0 + blockIdx.x, h = blockIdx.y, hd = threadIdx.x;
+  const uint8_t* tile = kv + h * head_stride_bytes + (int64_t)t * 2 * KV8_TILE;
+  double s = 0.0;
+#pragma unroll
+  for (int kk = 0; kk < 32; ++kk) s += (double)kv_value<DT>(tile, kv16_k_at(kk, hd), 1.f);
+  sums[(h * (head_stride_bytes / (2 * KV8_TILE)) + t) * 128 + hd] = (float)s;
+}
+
+unsigned tiles_of(int pos0, int n) { return (unsigned)(((int64_t)pos0 + n - 1) / 32 - pos0 / 32 + 1); }
+
+}  // namespace
+
+namespace drt {
+
+void kv8_store(const void* k, const void* v, bool src_bf16, int n, int Hkv, int pos0, void* kv,
+               int64_t head_stride, float* scales, float* sums, hipStream_t s) {
+  const dim3 grid(tiles_of(pos0, n), (unsigned)Hkv);
+  if (src_bf16)
+    hipLaunchKernelGGL(kv8_store_kernel<true>, grid, dim3(256), 0, s, k, v, n, Hkv, pos0,
+                       (uint8_t*)kv, head_stride, scales, sums);
+  else
+    hipLaunchKernelGGL(kv8_store_kernel<false>, grid, dim3(256), 0, s, k, v, n, Hkv, pos0,
+                       (uint8_t*)kv, head_stride, scales, sums);
+  DRT_HIP(hipGetLastError());
+}
+
+void kv_load(KvType type, const void* kv, int64_t head_stride, const float* scales, int n, int Hkv,
+             int pos0, void* k, void* v, bool out_bf16, hipStream_t s) {
+  const dim3 grid(tiles_of(pos0, n), (unsigned)Hkv);
+  const int64_t bytes = type == KvType::I8 ? head_stride : 2 * head_stride;
+#define DRT_KVL(DT, B)                                                                       \
+  hipLaunchKernelGGL((kv_load_kernel<DT, B>), grid, dim3(256), 0, s, (const uint8_t*)kv,     \
+                     bytes, scales, n, Hkv, pos0, k, v)
+#define DRT_KVL2(DT) do { if (out_bf16) DRT_KVL(DT, true); else DRT_KVL(DT, false); } while (0)
+  if (type == KvType::I8) DRT_KVL2(0);
+  else if (type == KvType::F16) DRT_KVL2(1);
+  else DRT_KVL2(2);
+#undef DRT_KVL2
+#undef DRT_KVL
+  DRT_HIP(hipGetLastError());
+}
+
+void kv_sums(bool bf16, const void* kv, int64_t head_stride, int Hkv, int pos0, int n, float* sums,
+             hipStream_t s) {
+  const dim3 grid(tiles_of(pos0, n), (unsigned)Hkv);
+  if (bf16)
+    hipLaunchKernelGGL(kv_sums_kernel<2>, grid, dim3(128), 0, s, (const uint8_t*)kv,
+                       2 * head_stride, pos0 / 32, sums);
+  else
+    hipLaunchKernelGGL(kv_sums_kernel<1>, grid, dim3(128), 0, s, (const uint8_t*)kv,
+                       2 * head_stride, pos0 / 32, sums);
+  DRT_HIP(hipGetLastError());
+}
+
+}  // namespace drt

@@ -201,6 +201,49 @@ void attention_decode(bool bf16, const void* q, const void* kv_layer, int64_t kv
 void kv_pack(bool kv_bf16, const void* k, const void* v, bool src_bf16, int n, int Hkv, int pos0,
              void* kv_layer, int64_t kv_head_stride, hipStream_t s);
 
+// The partials of n_splits key ranges, [n_splits][Hkv][n_rows * G][128] and [..][2], to rows.
+// out_fmt: 2 = fp32, 3 = bf16.
+void attn_combine(const float* o_part, const float* ml_part, int n_splits, int n_rows, int Hq,
+                  int Hkv, void* out, int out_fmt, hipStream_t s);
+
+// The 8-bit cache (kv8.h; head strides in elements, a multiple of 8192) and what reads it.
+enum class KvType { I8, F16, BF16 };
+// Which keys a row sees: the first n_keys, or under the d2f_hybrid mask (masked) those up to
+// the end of its own block.
+struct AttnWhere {
+  int n_keys, row_pos0, masked, prompt_len, block;
+};
+void kv8_store(const void* k, const void* v, bool src_bf16, int n, int Hkv, int pos0, void* kv,
+               int64_t head_stride, float* scales, float* sums, hipStream_t s);
+void kv_load(KvType type, const void* kv, int64_t head_stride, const float* scales, int n, int Hkv,
+             int pos0, void* k, void* v, bool out_bf16, hipStream_t s);
+void kv_sums(bool bf16, const void* kv, int64_t head_stride, int Hkv, int pos0, int n, float* sums,
+             hipStream_t s);
+struct Attn8Plan {
+  int qw = 1, qgroups = 1, splits = 1, tiles_per_split = 1;
+  bool wide = false;  // two query tiles a wave
+};
+Attn8Plan plan_attention8(int n_rows, int Hq, int Hkv, int n_keys);
+size_t attention8_part_bytes(const Attn8Plan& p, int n_rows, int Hq);
+void attention8(const void* q, bool q_bf16, const void* kv_layer, int64_t kv_head_stride,
+                const float* scales, int n_rows, int Hq, int Hkv, const AttnWhere& where,
+                const Attn8Plan& p, float* part, void* out, bool out_bf16, hipStream_t s);
+
+// Block-sparse attention over either cache. Blocks are `block` keys (a multiple of 32).
+struct SparseSel {
+  int block, count, sinks, local;
+};
+size_t select_blocks_bytes(int n_rows, int Hkv, int n_keys, int block);
+void select_blocks(const void* q, bool q_bf16, const float* sums, int64_t sums_head_stride,
+                   int n_rows, int Hq, int Hkv, const AttnWhere& where, const SparseSel& sel,
+                   void* workspace, int32_t* blocks, hipStream_t s);
+int sparse_splits(int n_rows, int Hq, int Hkv, int count, int block);
+size_t sparse_part_bytes(int n_rows, int Hq, int splits);
+void sparse_attention(KvType type, const void* q, bool q_bf16, const void* kv_layer,
+                      int64_t kv_head_stride, const float* scales, int n_rows, int Hq, int Hkv,
+                      const AttnWhere& where, const int32_t* blocks, int count, int block,
+                      int splits, float* part, void* out, bool out_bf16, hipStream_t s);
+
 // Epilogues.
 // rot (optional): receives the XCD rotation of the launch (see probe_round_robin).
 // ss_out (optional, M <= 32): per-32-column partial sums of squares of the rows,

@@ -2766,4 +2766,188 @@ int32_t drt_op_lm_head_score(const void* qw, const void* sb, const void* wb, int
   });
 }
 
+// ------------------------------------------------------------------ the 8-bit cache, sparse attention
+
+namespace {
+
+AttnWhere where_of(int32_t rows, int32_t n_keys, int32_t row_pos0, int32_t mask_kind,
+                   int32_t mask_prompt_len, int32_t mask_block_size, const char* what) {
+  const std::string op(what);
+  require(n_keys > 0 && n_keys <= INT32_MAX - 64, op + " n_keys out of range");
+  require(row_pos0 >= 0 && rows <= INT32_MAX - row_pos0, op + " row positions out of range");
+  require(mask_kind == DRT_MASK_BIDIRECTIONAL || mask_kind == DRT_MASK_D2F_HYBRID,
+          op + " mask kind must be bidirectional or d2f_hybrid");
+  const bool masked = mask_kind == DRT_MASK_D2F_HYBRID;
+  if (masked)
+    require(mask_block_size >= 1 && mask_prompt_len >= 0, "d2f_hybrid needs a mask geometry");
+  return AttnWhere{n_keys, row_pos0, masked, mask_prompt_len, std::max(1, mask_block_size)};
+}
+
+KvType kv_type(int32_t dtype, const char* what) {
+  require(dtype == DRT_I8 || dtype == DRT_F16 || dtype == DRT_BF16,
+          std::string(what) + " cache must be I8, F16 or BF16");
+  return dtype == DRT_I8 ? KvType::I8 : dtype == DRT_F16 ? KvType::F16 : KvType::BF16;
+}
+
+void require_kv(const void* cache, int64_t head_stride, const void* scales, int32_t kv_dtype,
+                int64_t keys, const char* what) {
+  const std::string op(what);
+  require(head_stride > 0 && head_stride % 8192 == 0, op + " head stride must be whole tiles of 8192");
+  require((keys + 31) / 32 <= head_stride / 8192, op + " positions exceed the cache head stride");
+  require(((uintptr_t)cache & 15) == 0, op + " cache must be 16-byte aligned");
+  if (kv_dtype == DRT_I8)
+    require(scales && ((uintptr_t)scales & 7) == 0, op + " 8-bit cache needs its scales, 8-byte aligned");
+}
+
+// The queries' type: either 16-bit one over an 8-bit cache, the cache's own otherwise.
+bool q_is_bf16(int32_t q_dtype, int32_t kv_dtype, const void* q, const char* what) {
+  const std::string op(what);
+  require(q_dtype == DRT_F16 || q_dtype == DRT_BF16, op + " q must be F16 or BF16");
+  require(kv_dtype == DRT_I8 || q_dtype == kv_dtype, op + " q must be of the cache's type");
+  require(((uintptr_t)q & 15) == 0, op + " q must be 16-byte aligned");
+  return q_dtype == DRT_BF16;
+}
+
+void require_out(const void* out, int32_t out_dtype, const char* what) {
+  const std::string op(what);
+  require(out_dtype == DRT_F32 || out_dtype == DRT_BF16, op + " out must be F32 or BF16");
+  require(((uintptr_t)out & 15) == 0, op + " out must be 16-byte aligned");
+}
+
+}  // namespace
+
+int32_t drt_op_kv8_store(const void* k, const void* v, int32_t src_dtype, int32_t n, int32_t hkv,
+                         int32_t pos0, void* cache, int64_t head_stride, float* scales,
+                         float* sums, void* stream) {
+  return guarded([&] {
+    require(k && v && cache && n > 0 && hkv > 0 && hkv <= 65535 && pos0 >= 0,
+            "bad kv8_store arguments");
+    require(src_dtype == DRT_F32 || src_dtype == DRT_BF16, "kv8_store source must be F32 or BF16");
+    require_kv(cache, head_stride, scales, DRT_I8, (int64_t)pos0 + n, "kv8_store");
+    kv8_store(k, v, src_dtype == DRT_BF16, n, hkv, pos0, cache, head_stride, scales, sums,
+              as_stream(stream));
+  });
+}
+
+int32_t drt_op_kv_sums(const void* cache, int64_t head_stride, int32_t kv_dtype, int32_t n,
+                       int32_t hkv, int32_t pos0, float* sums, void* stream) {
+  return guarded([&] {
+    require(cache && sums && n > 0 && hkv > 0 && hkv <= 65535 && pos0 >= 0, "bad kv_sums arguments");
+    require(kv_dtype == DRT_F16 || kv_dtype == DRT_BF16, "kv_sums cache must be F16 or BF16");
+    require_kv(cache, head_stride, nullptr, kv_dtype, (int64_t)pos0 + n, "kv_sums");
+    kv_sums(kv_dtype == DRT_BF16, cache, head_stride, hkv, pos0, n, sums, as_stream(stream));
+  });
+}
+
+int32_t drt_op_kv_load(const void* cache, int64_t head_stride, int32_t kv_dtype,
+                       const float* scales, int32_t n, int32_t hkv, int32_t pos0, void* k, void* v,
+                       int32_t out_dtype, void* stream) {
+  return guarded([&] {
+    require(cache && k && v && n > 0 && hkv > 0 && hkv <= 65535 && pos0 >= 0, "bad kv_load arguments");
+    const KvType type = kv_type(kv_dtype, "kv_load");
+    require_kv(cache, head_stride, scales, kv_dtype, (int64_t)pos0 + n, "kv_load");
+    require_out(k, out_dtype, "kv_load");
+    require_out(v, out_dtype, "kv_load");
+    kv_load(type, cache, head_stride, scales, n, hkv, pos0, k, v, out_dtype == DRT_BF16,
+            as_stream(stream));
+  });
+}
+
+size_t drt_op_attention_kv8_workspace_bytes(int32_t rows, int32_t hq, int32_t hkv, int32_t n_keys) {
+  if (rows <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || n_keys <= 0) return 0;
+  return attention8_part_bytes(plan_attention8(rows, hq, hkv, n_keys), rows, hq);
+}
+
+int32_t drt_op_attention_kv8(const void* q, int32_t q_dtype, const void* cache, int64_t head_stride,
+                             const float* scales, int32_t rows, int32_t hq, int32_t hkv,
+                             int32_t n_keys, int32_t row_pos0, int32_t mask_kind,
+                             int32_t mask_prompt_len, int32_t mask_block_size, void* out,
+                             int32_t out_dtype, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  return guarded([&] {
+    require(q && cache && out && rows > 0 && hq > 0 && hkv > 0 && hq % hkv == 0,
+            "bad attention_kv8 arguments");
+    const AttnWhere where = where_of(rows, n_keys, row_pos0, mask_kind, mask_prompt_len,
+                                     mask_block_size, "attention_kv8");
+    require_kv(cache, head_stride, scales, DRT_I8, n_keys, "attention_kv8");
+    const bool qb = q_is_bf16(q_dtype, DRT_I8, q, "attention_kv8");
+    require_out(out, out_dtype, "attention_kv8");
+    const Attn8Plan p = plan_attention8(rows, hq, hkv, n_keys);
+    require(p.qgroups <= 65535 && (int64_t)p.splits * hkv < (1ll << 31) &&
+                (int64_t)rows * (hq / hkv) < INT32_MAX - 512,
+            "attention_kv8: too many rows for one call");
+    const size_t need = attention8_part_bytes(p, rows, hq);
+    require(workspace_bytes >= need && (workspace || !need) && ((uintptr_t)workspace & 15) == 0,
+            "attention_kv8 workspace too small or not 16-byte aligned");
+    attention8(q, qb, cache, head_stride, scales, rows, hq, hkv, where, p,
+               need ? (float*)workspace : nullptr, out, out_dtype == DRT_BF16, as_stream(stream));
+  });
+}
+
+static bool sparse_shape_ok(int32_t rows, int32_t hq, int32_t hkv, int32_t block_size, int32_t count) {
+  return rows > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 && block_size > 0 && block_size % 32 == 0 &&
+         count > 0 && count <= 1024;
+}
+
+size_t drt_op_select_blocks_workspace_bytes(int32_t rows, int32_t hkv, int32_t n_keys,
+                                            int32_t block_size) {
+  if (rows <= 0 || hkv <= 0 || n_keys <= 0 || block_size <= 0 || block_size % 32) return 0;
+  return select_blocks_bytes(rows, hkv, n_keys, block_size);
+}
+
+int32_t drt_op_select_blocks(const void* q, int32_t q_dtype, const float* sums, int64_t sums_tiles,
+                             int32_t rows, int32_t hq, int32_t hkv, int32_t n_keys,
+                             int32_t row_pos0, int32_t mask_kind, int32_t mask_prompt_len,
+                             int32_t mask_block_size, int32_t block_size, int32_t count,
+                             int32_t sinks, int32_t local, int32_t* blocks, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    require(q && sums && blocks && sparse_shape_ok(rows, hq, hkv, block_size, count),
+            "bad select_blocks arguments (block_size is a multiple of 32, count 1..1024)");
+    require(sinks >= 0 && local >= 1 && (int64_t)sinks + local <= count,
+            "select_blocks needs sinks >= 0, local >= 1 and sinks + local <= count");
+    const AttnWhere where = where_of(rows, n_keys, row_pos0, mask_kind, mask_prompt_len,
+                                     mask_block_size, "select_blocks");
+    require(q_dtype == DRT_F16 || q_dtype == DRT_BF16, "select_blocks q must be F16 or BF16");
+    require((n_keys + 31) / 32 <= sums_tiles, "select_blocks n_keys exceed the sums");
+    require(workspace && ((uintptr_t)workspace & 7) == 0 &&
+                workspace_bytes >= select_blocks_bytes(rows, hkv, n_keys, block_size),
+            "select_blocks workspace too small or not 8-byte aligned");
+    select_blocks(q, q_dtype == DRT_BF16, sums, sums_tiles * 128, rows, hq, hkv, where,
+                  SparseSel{block_size, count, sinks, local}, workspace, blocks, as_stream(stream));
+  });
+}
+
+size_t drt_op_sparse_attention_workspace_bytes(int32_t rows, int32_t hq, int32_t hkv,
+                                               int32_t block_size, int32_t count) {
+  if (!sparse_shape_ok(rows, hq, hkv, block_size, count)) return 0;
+  return sparse_part_bytes(rows, hq, sparse_splits(rows, hq, hkv, count, block_size));
+}
+
+int32_t drt_op_sparse_attention(const void* q, int32_t q_dtype, const void* cache,
+                                int64_t head_stride, int32_t kv_dtype, const float* scales,
+                                int32_t rows, int32_t hq, int32_t hkv, int32_t n_keys,
+                                int32_t row_pos0, int32_t mask_kind, int32_t mask_prompt_len,
+                                int32_t mask_block_size, const int32_t* blocks, int32_t block_size,
+                                int32_t count, void* out, int32_t out_dtype, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    require(q && cache && blocks && out && sparse_shape_ok(rows, hq, hkv, block_size, count),
+            "bad sparse_attention arguments (block_size is a multiple of 32, count 1..1024)");
+    const KvType type = kv_type(kv_dtype, "sparse_attention");
+    const AttnWhere where = where_of(rows, n_keys, row_pos0, mask_kind, mask_prompt_len,
+                                     mask_block_size, "sparse_attention");
+    require_kv(cache, head_stride, scales, kv_dtype, n_keys, "sparse_attention");
+    const bool qb = q_is_bf16(q_dtype, kv_dtype, q, "sparse_attention");
+    require_out(out, out_dtype, "sparse_attention");
+    const int splits = sparse_splits(rows, hq, hkv, count, block_size);
+    const size_t need = sparse_part_bytes(rows, hq, splits);
+    require(workspace_bytes >= need && (workspace || !need) && ((uintptr_t)workspace & 15) == 0,
+            "sparse_attention workspace too small or not 16-byte aligned");
+    sparse_attention(type, q, qb, cache, head_stride, scales, rows, hq, hkv, where, blocks, count,
+                     block_size, splits, need ? (float*)workspace : nullptr, out,
+                     out_dtype == DRT_BF16, as_stream(stream));
+  });
+}
+
 }  // extern "C"

@@ -21,6 +21,7 @@ import math
 
 from . import _lib
 
+_I32_MAX = 2**31 - 1
 KV_TILE_ELEMS = 8192  # one 32-key tile: K block + V block, 2-byte elements
 
 
@@ -161,29 +162,105 @@ def swiglu(gate, up):
     return y
 
 
+class _on:
+    """The current device set to ``t``'s for the launches inside (nothing where it is already)."""
+
+    def __init__(self, t):
+        self.index = t.device.index
+
+    def __enter__(self):
+        torch = _torch()
+        self.back = torch.cuda.current_device()
+        if self.index != self.back:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.index != self.back:
+            _torch().cuda.set_device(self.back)
+
+
+def _workspace(nbytes, t):
+    """(pointer or None, bytes, the tensor that holds them)."""
+    if not nbytes:
+        return None, 0, None
+    ws = _torch().empty(nbytes, dtype=_torch().uint8, device=t.device)
+    return _ptr(ws), nbytes, ws
+
+
 class PrefixKVCache:
     """Tiled K/V cache for ``layers`` layers on one device.
 
     The build's prefix-cache object: rows are written once (``store``) at
     absolute positions and read by :meth:`attention`. Layout per (layer, kv
     head): 32-key tiles of 8192 elements (K block then V block) in the MFMA
-    operand order of the attention kernel. Unwritten slots stay zero."""
+    operand order of the attention kernel. Unwritten slots stay zero.
 
-    def __init__(self, layers: int, kv_heads: int, capacity: int, *, dtype="f16", device=None):
+    ``dtype`` is ``"f16"``, ``"bf16"`` or ``"i8"``: whole numbers of [-127, 127] times
+    one power of two for each tile's K and V (``scales [layers, kv_heads, tiles, 2]``), half the
+    bytes of a 16-bit cache. A store into an ``"i8"`` cache quantizes each tile it touches as a whole, from
+    the rows it keeps (as they read) and the new ones, to the least power of two >= 2^-40 that
+    holds them: a value is off by at most half of it (max / 127 to 2 max / 127), a row that later stores
+    of its tile went past by less than one of the last scale. A tile with a value that is not finite, or beyond
+    127 * 2^40, reads as NaN until every row of it is stored anew.
+
+    ``block_sums=True`` keeps the sum of each tile's keys (``sums [layers, kv_heads, tiles,
+    128]``) up to date, which :meth:`select_blocks` scores blocks by."""
+
+    def __init__(self, layers: int, kv_heads: int, capacity: int, *, dtype="f16", device=None,
+                 block_sums: bool = False):
         torch = _torch()
         self.layers, self.kv_heads = int(layers), int(kv_heads)
         self.tiles = (int(capacity) + 31) // 32
         self.capacity = self.tiles * 32
         self.head_stride = self.tiles * KV_TILE_ELEMS
-        self.kv_dtype = _lib.BF16 if dtype == "bf16" else _lib.F16
-        tdt = torch.bfloat16 if dtype == "bf16" else torch.float16
-        self.data = torch.zeros((self.layers, self.kv_heads, self.head_stride), dtype=tdt,
-                                device=device or "cuda")
+        self.kv_dtype = {"bf16": _lib.BF16, "i8": _lib.I8}.get(dtype, _lib.F16)
+        shape = (self.layers, self.kv_heads, self.head_stride)
+        device = device or "cuda"
+        self.scales = self.sums = None
+        if dtype == "i8":  # a byte is a code + 128
+            self.data = torch.full(shape, 128, dtype=torch.uint8, device=device)
+            self.scales = torch.ones((*shape[:2], self.tiles, 2), dtype=torch.float32,
+                                     device=device)
+        else:
+            self.data = torch.zeros(shape, dtype=torch.bfloat16 if dtype == "bf16"
+                                    else torch.float16, device=device)
+        if block_sums:
+            self.sums = torch.zeros((*shape[:2], self.tiles, 128), dtype=torch.float32,
+                                    device=device)
         self.length = 0
 
     @property
     def nbytes(self) -> int:
-        return self.data.numel() * self.data.element_size()
+        return sum(t.numel() * t.element_size() for t in (self.data, self.scales, self.sums)
+                   if t is not None)
+
+    def _layer(self, layer, *tensors):
+        """(data, scales or None, sums or None) of a layer, as pointers; the new operators' checks
+        of where things are."""
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer must be in [0, {self.layers})")
+        _require_cuda(*tensors)
+        if any(t.device != self.data.device for t in tensors):
+            raise ValueError("tensors must be on the cache's device")
+        return tuple(None if t is None else _ptr(t[layer])
+                     for t in (self.data, self.scales, self.sums))
+
+    def _queries(self, q):
+        """(rows, query heads, dtype code) of ``q``, checked against the cache."""
+        torch = _torch()
+        if q.dim() != 3 or q.shape[2] != 128 or q.shape[1] < 1 or q.shape[1] % self.kv_heads:
+            raise ValueError("attention needs q [rows, Hq, 128] and Hq % Hkv == 0")
+        code = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}.get(q.dtype)
+        if code is None or (self.kv_dtype != _lib.I8 and code != self.kv_dtype):
+            raise ValueError("q must be float16 or bfloat16 over an 8-bit cache, and of the "
+                             "cache's own type over a 16-bit one")
+        return q.shape[0], q.shape[1], code
+
+    def _keys(self, n_keys, rows, row_pos0):
+        if n_keys < 1 or n_keys > self.capacity:
+            raise ValueError("n_keys outside the cache")
+        if rows < 1 or row_pos0 < 0 or row_pos0 + rows > _I32_MAX:
+            raise ValueError("attention needs a query row, and row positions of 32 bits")
 
     def store(self, layer: int, k, v, pos0: int) -> None:
         """Write ``k/v [n, Hkv, 128]`` (fp32 or bf16) at positions ``pos0..pos0+n-1``."""
@@ -197,16 +274,53 @@ class PrefixKVCache:
         if k.dtype not in (torch.float32, torch.bfloat16) or v.dtype != k.dtype:
             raise ValueError("store takes fp32 or bf16 k/v")
         src = _lib.BF16 if k.dtype == torch.bfloat16 else _lib.F32
+        if self.kv_dtype == _lib.I8 or self.sums is not None:
+            data, scales, sums = self._layer(layer, k, v)
+            with _on(k):
+                if self.kv_dtype == _lib.I8:
+                    _lib.check(_lib.load().drt_op_kv8_store(
+                        _ptr(k), _ptr(v), src, n, self.kv_heads, pos0, data, self.head_stride,
+                        scales, sums, _stream(k)))
+                else:
+                    _lib.check(_lib.load().drt_op_kv_pack(
+                        _ptr(k), _ptr(v), src, n, self.kv_heads, pos0, data, self.head_stride,
+                        self.kv_dtype, _stream(k)))
+                    _lib.check(_lib.load().drt_op_kv_sums(
+                        data, self.head_stride, self.kv_dtype, n, self.kv_heads, pos0, sums,
+                        _stream(k)))
+            self.length = max(self.length, pos0 + n)
+            return
         layer_view = self.data[layer]
         _lib.check(_lib.load().drt_op_kv_pack(_ptr(k), _ptr(v), src, n, self.kv_heads, pos0,
                                               _ptr(layer_view), self.head_stride, self.kv_dtype,
                                               _stream(k)))
         self.length = max(self.length, pos0 + n)
 
+    def load(self, layer: int, pos0: int, n: int, out_dtype=None):
+        """``(k, v) [n, Hkv, 128]`` of positions ``pos0..pos0+n-1`` as the cache holds them, in
+        fp32 (or bf16): what attention reads."""
+        torch = _torch()
+        out_dtype = out_dtype or torch.float32
+        if out_dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("load gives float32 or bfloat16")
+        if n < 1 or pos0 < 0 or pos0 + n > self.capacity:
+            raise ValueError("load positions outside the cache")
+        data, scales, _ = self._layer(layer, self.data)
+        k = torch.empty((n, self.kv_heads, 128), dtype=out_dtype, device=self.data.device)
+        v = torch.empty_like(k)
+        with _on(k):
+            _lib.check(_lib.load().drt_op_kv_load(
+                data, self.head_stride, self.kv_dtype, scales, n, self.kv_heads, pos0, _ptr(k),
+                _ptr(v), _lib.F32 if out_dtype == torch.float32 else _lib.BF16, _stream(k)))
+        return k, v
+
     def attention(self, layer: int, q, *, n_keys: int, row_pos0: int, kind: str,
                   mask_geometry=None, out_dtype=None):
-        """Attention of ``q [rows, Hq, 128]`` (cache dtype) over keys ``[0, n_keys)``."""
+        """Attention of ``q [rows, Hq, 128]`` (cache dtype; fp16 or bf16 over an ``"i8"`` cache)
+        over keys ``[0, n_keys)``."""
         torch = _torch()
+        if self.kv_dtype == _lib.I8:
+            return self._attention8(layer, q, n_keys, row_pos0, kind, mask_geometry, out_dtype)
         _require_cuda(q)
         rows, hq, hd = q.shape
         if hd != 128 or hq % self.kv_heads:
@@ -227,6 +341,95 @@ class PrefixKVCache:
                                         self.kv_dtype, rows, hq, self.kv_heads, n_keys, row_pos0,
                                         mk, p, b, _ptr(out), odt, _ptr(ws), ws_bytes, _stream(q)))
         return out
+
+    def _attention8(self, layer, q, n_keys, row_pos0, kind, mask_geometry, out_dtype):
+        data, scales, _ = self._layer(layer, q)
+        rows, hq, qdt = self._queries(q)
+        self._keys(n_keys, rows, row_pos0)
+        mk, p, b = _mask_args(kind, mask_geometry)
+        out, odt = _attention_out(q, out_dtype)
+        lib = _lib.load()
+        with _on(q):
+            ws, ws_bytes, _held = _workspace(
+                lib.drt_op_attention_kv8_workspace_bytes(rows, hq, self.kv_heads, n_keys), q)
+            _lib.check(lib.drt_op_attention_kv8(
+                _ptr(q), qdt, data, self.head_stride, scales, rows, hq, self.kv_heads, n_keys,
+                row_pos0, mk, p, b, _ptr(out), odt, ws, ws_bytes, _stream(q)))
+        return out
+
+    def select_blocks(self, layer: int, q, *, block_size: int, count: int, n_keys: int,
+                      row_pos0: int, kind: str, mask_geometry=None, sinks: int = 0,
+                      local: int = 1):
+        """The blocks of ``block_size`` keys (a multiple of 32) that each row of ``q`` reads of
+        keys ``[0, n_keys)``: int32 ``[rows, kv_heads, count]``, ascending.
+
+        They are the first ``sinks`` and the last ``local`` blocks that the row sees and, of
+        those between, the ones whose keys' sum has the largest product with the sum of
+        the row's queries of the head's group (compared in 64 bits; equal ones: the lower block). A row that sees no
+        more than ``count`` blocks lists them all, then ``-1``. Needs ``block_sums=True``."""
+        torch = _torch()
+        if self.sums is None:
+            raise ValueError("select_blocks needs a cache with block_sums=True")
+        _, _, sums = self._layer(layer, q)
+        rows, hq, qdt = self._queries(q)
+        self._keys(n_keys, rows, row_pos0)
+        _sparse_args(block_size, count)
+        if sinks < 0 or local < 1 or sinks + local > count:
+            raise ValueError("select_blocks needs sinks >= 0, local >= 1, sinks + local <= count")
+        mk, p, b = _mask_args(kind, mask_geometry)
+        blocks = torch.empty((rows, self.kv_heads, count), dtype=torch.int32, device=q.device)
+        lib = _lib.load()
+        with _on(q):
+            ws, ws_bytes, _held = _workspace(lib.drt_op_select_blocks_workspace_bytes(
+                rows, self.kv_heads, n_keys, block_size), q)
+            _lib.check(lib.drt_op_select_blocks(
+                _ptr(q), qdt, sums, self.tiles, rows, hq, self.kv_heads, n_keys, row_pos0, mk, p,
+                b, block_size, count, sinks, local, _ptr(blocks), ws, ws_bytes, _stream(q)))
+        return blocks
+
+    def sparse_attention(self, layer: int, q, blocks, *, block_size: int, n_keys: int,
+                         row_pos0: int, kind: str, mask_geometry=None, out_dtype=None):
+        """:meth:`attention` over the keys of ``blocks`` (int32 ``[rows, kv_heads, count]``, as
+        :meth:`select_blocks` gives them or a caller's own) that the row sees.
+
+        An entry that is no larger than one before it in its list, or lies beyond the row's
+        keys, is passed over (so ``-1`` is none); a row without any gives zeros."""
+        torch = _torch()
+        data, scales, _ = self._layer(layer, q, blocks)
+        rows, hq, qdt = self._queries(q)
+        self._keys(n_keys, rows, row_pos0)
+        if (blocks.dtype != torch.int32 or blocks.dim() != 3
+                or blocks.shape[:2] != (rows, self.kv_heads)):
+            raise ValueError("blocks must be int32 [rows, kv_heads, count]")
+        count = blocks.shape[2]
+        _sparse_args(block_size, count)
+        mk, p, b = _mask_args(kind, mask_geometry)
+        out, odt = _attention_out(q, out_dtype)
+        lib = _lib.load()
+        with _on(q):
+            ws, ws_bytes, _held = _workspace(lib.drt_op_sparse_attention_workspace_bytes(
+                rows, hq, self.kv_heads, block_size, count), q)
+            _lib.check(lib.drt_op_sparse_attention(
+                _ptr(q), qdt, data, self.head_stride, self.kv_dtype, scales, rows, hq,
+                self.kv_heads, n_keys, row_pos0, mk, p, b, _ptr(blocks), block_size, count,
+                _ptr(out), odt, ws, ws_bytes, _stream(q)))
+        return out
+
+
+def _attention_out(q, out_dtype):
+    torch = _torch()
+    out_dtype = out_dtype or torch.float32
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("attention out must be float32 or bfloat16")
+    out = torch.empty((q.shape[0], q.shape[1] * 128), dtype=out_dtype, device=q.device)
+    return out, _lib.F32 if out_dtype == torch.float32 else _lib.BF16
+
+
+def _sparse_args(block_size, count):
+    if block_size < 32 or block_size % 32 or block_size > _I32_MAX:
+        raise ValueError("block_size must be a multiple of 32")
+    if not 1 <= count <= 1024:
+        raise ValueError("a row lists 1 to 1024 blocks")
 
 
 def _mask_args(kind, mask_geometry):
@@ -278,7 +481,10 @@ def attention(q, k, v, *, head_dim: int, kind: str, mask_geometry=None, q_positi
     kd = k if k.dtype in (torch.float32, torch.bfloat16) else k.float()
     vd = v if v.dtype == kd.dtype else v.to(kd.dtype)
     cache.store(0, kd.contiguous(), vd.contiguous(), 0)
-    qc = q.to(torch.bfloat16 if kv_dtype == "bf16" else torch.float16).contiguous()
+    if kv_dtype == "i8":  # queries keep a 16-bit type of their own
+        qc = (q if q.dtype in (torch.float16, torch.bfloat16) else q.half()).contiguous()
+    else:
+        qc = q.to(torch.bfloat16 if kv_dtype == "bf16" else torch.float16).contiguous()
     out = cache.attention(0, qc, n_keys=rk, row_pos0=pos0, kind=kind, mask_geometry=mask_geometry,
                           out_dtype=torch.float32)
     return out.to(q.dtype)

@@ -39,8 +39,10 @@ enum {
   DRT_INTERNAL_ERROR = 4
 };
 
-/* DType (abi/buffers.py:22-28); DRT_F16 is appended after the reference's values. */
-enum { DRT_F32 = 0, DRT_F64 = 1, DRT_BF16 = 2, DRT_I32 = 3, DRT_I64 = 4, DRT_U8 = 5, DRT_F16 = 6 };
+/* DType (abi/buffers.py:22-28); DRT_F16 and DRT_I8 (an 8-bit cache) are appended after the
+ * reference's values. */
+enum { DRT_F32 = 0, DRT_F64 = 1, DRT_BF16 = 2, DRT_I32 = 3, DRT_I64 = 4, DRT_U8 = 5, DRT_F16 = 6,
+       DRT_I8 = 7 };
 
 /* DecodeStrategy / CommitPolicy / AttentionMaskKind values (abi/enums.py:14-43). */
 enum { DRT_DECODE_BLOCK_THRESHOLD = 0, DRT_DECODE_FIXED_QUOTA = 6, DRT_DECODE_BD3_FIXED_QUOTA = 7 };
@@ -291,6 +293,66 @@ int32_t drt_op_lm_head_score(const void* qw, const void* sb, const void* wb, int
                              uint64_t seed, int32_t step, const int32_t* positions,
                              double* scores, int32_t* tokens, float* logits, void* workspace,
                              size_t workspace_bytes, void* stream);
+
+/* ---- the 8-bit cache (no counterpart in the reference) ----
+ * A cache of hkv heads, head_stride bytes each, in tiles of 32 keys and 8192 bytes (K, then V): a
+ * byte is a code + 128, a value code * scale, with scales [hkv][head_stride / 8192][2] fp32 (a
+ * tile's K and V), powers of two. For a tile's K, and for its V: scale = the least power of two >=
+ * 2^-40 with max|x| <= 127 * scale, code = x / scale rounded to nearest, ties to even. A tile with
+ * a value that is not finite, or beyond 127 * 2^40, reads as NaN as a whole. Codes start as 128,
+ * scales as 1. Caches are 16-byte aligned and head strides whole tiles. */
+
+/* Rows k, v ([n, hkv, 128] fp32 or bf16) to positions pos0..pos0+n-1. A tile is quantized as a
+ * whole from the rows it keeps, as they read, and the new ones. sums: NULL or [hkv][head_stride / 8192][128]
+ * fp32, which receive each touched tile's keys added up. */
+int32_t drt_op_kv8_store(const void* k, const void* v, int32_t src_dtype, int32_t n, int32_t hkv,
+                         int32_t pos0, void* cache, int64_t head_stride, float* scales, float* sums,
+                         void* stream);
+/* The same sums for the tiles of positions pos0..pos0+n-1 of a 16-bit cache (drt_op_kv_pack). */
+int32_t drt_op_kv_sums(const void* cache, int64_t head_stride, int32_t kv_dtype, int32_t n,
+                       int32_t hkv, int32_t pos0, float* sums, void* stream);
+/* Rows of a cache of any type (DRT_I8, DRT_F16, DRT_BF16; scales for DRT_I8) as values:
+ * k, v [n, hkv, 128] of out_dtype (DRT_F32 or DRT_BF16). */
+int32_t drt_op_kv_load(const void* cache, int64_t head_stride, int32_t kv_dtype, const float* scales,
+                       int32_t n, int32_t hkv, int32_t pos0, void* k, void* v, int32_t out_dtype,
+                       void* stream);
+/* drt_op_attention over an 8-bit cache; q fp16 or bf16 (q_dtype), row_pos0 >= 0. Calls that overlap must
+ * not share a workspace (it may be NULL where 0 bytes are asked for). */
+size_t drt_op_attention_kv8_workspace_bytes(int32_t rows, int32_t hq, int32_t hkv, int32_t n_keys);
+int32_t drt_op_attention_kv8(const void* q, int32_t q_dtype, const void* cache, int64_t head_stride,
+                             const float* scales, int32_t rows, int32_t hq, int32_t hkv,
+                             int32_t n_keys, int32_t row_pos0, int32_t mask_kind,
+                             int32_t mask_prompt_len, int32_t mask_block_size, void* out,
+                             int32_t out_dtype, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* ---- block-sparse attention (no counterpart in the reference) ----
+ * Blocks are block_size keys (a multiple of 32). For each row and K/V head drt_op_select_blocks
+ * lists `count` (1..1024) of the blocks the row sees: the first `sinks`, the last `local` (>= 1) and,
+ * of those between, the ones whose keys' sum has the largest product with the sum of the head
+ * group's queries (in 64 bits; equal ones: the lower block; a NaN is the largest). Blocks ascend in
+ * blocks [rows, hkv, count]; a row that sees fewer lists them all, then -1. sums: [hkv][sums_tiles][128] of
+ * drt_op_kv8_store or drt_op_kv_sums. Neither call's overlapping ones may share a workspace. */
+size_t drt_op_select_blocks_workspace_bytes(int32_t rows, int32_t hkv, int32_t n_keys,
+                                            int32_t block_size);
+int32_t drt_op_select_blocks(const void* q, int32_t q_dtype, const float* sums, int64_t sums_tiles,
+                             int32_t rows, int32_t hq, int32_t hkv, int32_t n_keys,
+                             int32_t row_pos0, int32_t mask_kind, int32_t mask_prompt_len,
+                             int32_t mask_block_size, int32_t block_size, int32_t count,
+                             int32_t sinks, int32_t local, int32_t* blocks, void* workspace,
+                             size_t workspace_bytes, void* stream);
+/* drt_op_attention (or _kv8) over the listed blocks' keys only, blocks [rows, hkv, count] of any origin:
+ * an entry that is no larger than one before it, or beyond the row's keys, is passed over; a row
+ * without any is zeros. q: fp16 or bf16 over DRT_I8, else of the cache's type. */
+size_t drt_op_sparse_attention_workspace_bytes(int32_t rows, int32_t hq, int32_t hkv,
+                                               int32_t block_size, int32_t count);
+int32_t drt_op_sparse_attention(const void* q, int32_t q_dtype, const void* cache,
+                                int64_t head_stride, int32_t kv_dtype, const float* scales,
+                                int32_t rows, int32_t hq, int32_t hkv, int32_t n_keys,
+                                int32_t row_pos0, int32_t mask_kind, int32_t mask_prompt_len,
+                                int32_t mask_block_size, const int32_t* blocks, int32_t block_size,
+                                int32_t count, void* out, int32_t out_dtype, void* workspace,
+                                size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,147 @@
+"""The 8-bit K/V cache and the block-sparse attention in float64 (oracle; test-only).
+
+The reference has neither (its K/V stays in the compute dtype,
+``backends/mlx_ops.py:347-443``): these are the definitions of
+``diffusorrt_amd.kernels.PrefixKVCache``'s, parity unpinned.
+"""
+from __future__ import annotations
+
+import numpy as np
+
+TILE = 32
+MIN_EXP, MAX_EXP = -40, 40
+
+
+def exponent(most: float):
+    """The least e >= -40 with most <= 127 * 2^e; None where the tile is NaN."""
+    if not np.isfinite(most) or most > 127 * 2.0 ** MAX_EXP:
+        return None
+    e = MIN_EXP
+    while 127 * 2.0 ** e < most:
+        e += 1
+    return e
+
+
+def quantize_tile(x):
+    """One head's 32 keys ``[32, 128]`` -> (whole numbers or None, exponent or None)."""
+    x = np.asarray(x, np.float64)
+    with np.errstate(invalid="ignore"):
+        e = exponent(np.abs(x).max())
+    return (None, None) if e is None else (np.rint(x * 2.0 ** -e), e)  # rint: ties to even
+
+
+class Cache8:
+    """Values an 8-bit cache reads as, ``[tiles * 32, hkv, 128]``, with its tile exponents."""
+
+    def __init__(self, hkv: int, capacity: int):
+        tiles = -(-capacity // TILE)
+        self.hkv = hkv
+        self.values = np.zeros((2, tiles * TILE, hkv, 128))
+        self.scales = np.ones((hkv, tiles, 2))
+
+    def store(self, k, v, pos0: int) -> None:
+        n = len(k)
+        for w, x in enumerate((k, v)):
+            self.values[w, pos0:pos0 + n] = np.asarray(x, np.float64)
+        for t in range(pos0 // TILE, (pos0 + n - 1) // TILE + 1):
+            for h in range(self.hkv):
+                for w in range(2):
+                    tile = self.values[w, t * TILE:(t + 1) * TILE, h]
+                    q, e = quantize_tile(tile)
+                    tile[:] = np.nan if e is None else q * 2.0 ** e
+                    self.scales[h, t, w] = np.nan if e is None else 2.0 ** e
+
+    def sums(self):
+        """``[hkv, tiles, 128]``: each tile's keys added up."""
+        return tile_sums(self.values[0])
+
+
+def tile_sums(k):
+    return np.asarray(k, np.float64).reshape(-1, TILE, *k.shape[1:]).sum(1).transpose(1, 0, 2)
+
+
+def key_ends(rows: int, n_keys: int, row_pos0: int, mask=None):
+    """Keys that each row sees, always the first ones; mask: None or (prompt_len, block)."""
+    p = row_pos0 + np.arange(rows)
+    if mask is None:
+        return np.full(rows, n_keys)
+    prompt, block = mask
+    return np.minimum(n_keys, np.where(p < prompt, prompt,
+                                       prompt + ((p - prompt) // block + 1) * block))
+
+
+def select_blocks(q, sums, ends, *, block: int, count: int, sinks: int = 0, local: int = 1):
+    """int32 ``[rows, hkv, count]``: forced blocks and the best scores, ascending, -1 behind."""
+    q = np.asarray(q, np.float64)
+    rows, hq, _ = q.shape
+    hkv, tiles, _ = sums.shape
+    m = block // TILE
+    out = np.full((rows, hkv, count), -1, np.int32)
+    for r in range(rows):
+        n = -(-int(ends[r]) // block)
+        for h in range(hkv):
+            if n <= count:
+                out[r, h, :n] = np.arange(n)
+                continue
+            mid = np.arange(sinks, n - local)
+            whole = sums[h, :(n - 1) * m].reshape(n - 1, m, 128).sum(1)
+            g = hq // hkv
+            score = whole[mid] @ q[r, h * g:(h + 1) * g].sum(0)
+            score = np.where(np.isnan(score), np.inf, score)
+            best = mid[np.lexsort((mid, -score))][:count - sinks - local]
+            out[r, h] = np.sort(np.concatenate([np.arange(sinks), best,
+                                                np.arange(n - local, n)]))
+    return out
+
+
+def attention(q, k, v, ends, blocks=None, block: int = 0):
+    """(out, weight) ``[rows, hq, 128]``: softmax(q k^T / sqrt(128)) v over each row's first
+    ``ends`` keys (those of its listed blocks), and the same sum of |v|. No key: zeros."""
+    q = np.asarray(q, np.float64)
+    rows, hq, _ = q.shape
+    hkv = k.shape[1]
+    out, weight = np.zeros((2, rows, hq, 128))
+    for r in range(rows):
+        for h in range(hq):
+            kv = h // (hq // hkv)
+            keys = np.arange(ends[r])
+            if blocks is not None:
+                listed, top = [], -1
+                for b in blocks[r, kv]:
+                    if b > top:
+                        listed.append(b)
+                        top = b
+                keys = keys[np.isin(keys // block, listed)]
+            if not len(keys):
+                continue
+            s = k[keys, kv] @ q[r, h] * 128 ** -0.5
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            out[r, h] = p @ v[keys, kv]
+            weight[r, h] = p @ np.abs(v[keys, kv])
+    return out, weight
+
+
+def attention_bound(q, k, v, ends, weight, p_half: float, n_keys: int, *, q_bf16_scaled=False):
+    """How far a kernel's fp32 result may be from :func:`attention`'s, from its roundings.
+
+    - a weighted value p is rounded once to the product's type: ``p_half`` of it (2^-11 for
+      fp16, 2^-8 for bf16), or below fp16's normal numbers 2^-25 absolute against a largest of
+      at least 1, times a code of at most 127 where the tile's largest is over 63: 2^-24 of the
+      largest |v| per key;
+    - a score is a sum of 128 exact products in fp32, and two more roundings: 130 * 2^-24 of
+      the sum of their magnitudes, in the exponent, so that times p; once in p, once in the
+      normaliser; exp2 and the sums over keys in fp32 add (n_keys / 32 + 64) * 2^-24;
+    - bf16 queries that are scaled to fp16 lose at most 2^-25 of the vector's largest each.
+    """
+    q = np.abs(np.asarray(q, np.float64))
+    k, v = np.abs(np.nan_to_num(k)), np.abs(np.nan_to_num(v))
+    kmax = k.max(0)                                                      # [hkv, 128]
+    g = q.shape[1] // k.shape[1]
+    s = (q * kmax.repeat(g, 0)[None]).sum(-1) * 128 ** -0.5              # [rows, hq]
+    e = 130 * 2.0 ** -24 * s
+    if q_bf16_scaled:
+        e = e + 128 ** -0.5 * 2.0 ** -25 * q.max(-1) * kmax.sum(-1).repeat(g)[None]
+    rel = p_half + 2 * e + (n_keys / 32 + 64) * 2.0 ** -24
+    floor = n_keys * 2.0 ** -24 * v.max()
+    return rel[..., None] * weight + floor
