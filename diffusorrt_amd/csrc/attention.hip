@@ -1206,15 +1206,6 @@ void attention(bool bf16, const void* q, const void* kv_layer, int64_t kv_head_s
   DRT_HIP(hipGetLastError());
 }
 
-void attn_combine(const float* o_part, const float* ml_part, int n_splits, int n_rows, int Hq,
-                  int Hkv, void* out, int out_fmt, hipStream_t s) {
-  const int64_t threads = (int64_t)n_rows * Hq * 16;
-  hipLaunchKernelGGL(attn_combine_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s,
-                     o_part, ml_part, n_splits, n_rows, Hq, Hkv, out, (float*)nullptr, out_fmt,
-                     (int*)nullptr);
-  DRT_HIP(hipGetLastError());
-}
-
 size_t attention_decode_part_bytes(int ranges, int Hkv, int n_qv) {
   const int qt = n_qv <= 64 ? (n_qv + 31) / 32 : 4;
   return (size_t)ranges * Hkv * ((size_t)qt * 4096 + (size_t)qt * 32 * 2) * 4;

@@ -26,17 +26,27 @@ DRT_DEV int kv8_v_at(int kk, int hd) {
          (kk & 3) + 4 * ((kk >> 3) & 1);
 }
 
-// Eight codes as exact fp16 values: a byte b under the exponent of 1024 is the fp16 1024 + b,
-// and one packed subtraction of 1152 leaves b - 128.
-DRT_DEV uint32_t kv8_pair_to_f16(uint32_t codes, uint32_t which) {
-  const f16x2 bias = {(_Float16)-1152.f, (_Float16)-1152.f};
-  const uint32_t w = __builtin_amdgcn_perm(codes, 0x64646464u, which);
-  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, w) + bias);
-}
+// Eight bytes as fp16 operands in one instruction a pair: a byte b alone is the subnormal fp16
+// b * 2^-24, which the matrix instructions (and v_dot2_f32_f16) multiply exactly. With a code
+// c = b - 128, a product with x is 2^-24 (sum x c + 128 sum x): the 2^24 goes where a scale is applied
+// anyway, and 128 times the sum of x is taken off in fp32 (x the query: once per query vector; x the
+// weights: one running sum). The exact fp16 c (1024 + b, less 1152) takes twice the instructions.
 DRT_DEV f16x8 kv8_to_f16(uint32_t lo, uint32_t hi) {
-  const u32x4 r = {kv8_pair_to_f16(lo, 0x00050004u), kv8_pair_to_f16(lo, 0x00070006u),
-                   kv8_pair_to_f16(hi, 0x00050004u), kv8_pair_to_f16(hi, 0x00070006u)};
+  const u32x4 r = {__builtin_amdgcn_perm(lo, lo, 0x0c050c04u), __builtin_amdgcn_perm(lo, lo, 0x0c070c06u),
+                   __builtin_amdgcn_perm(hi, hi, 0x0c050c04u), __builtin_amdgcn_perm(hi, hi, 0x0c070c06u)};
   return __builtin_bit_cast(f16x8, r);
+}
+constexpr float KV8_POW = 16777216.f;  // 2^24
+constexpr float KV8_BIAS = 128.f;
+// c + the sum of eight fp16 values, in fp32.
+DRT_DEV float kv8_add8(const f16x8 p, float c) {
+  const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
+  const u32x4 w = __builtin_bit_cast(u32x4, p);
+  const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3];
+  c = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w0), one, c, false);
+  c = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w1), one, c, false);
+  c = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w2), one, c, false);
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w3), one, c, false);
 }
 
 // The number of keys a row sees, always the first ones (no more than n_keys).

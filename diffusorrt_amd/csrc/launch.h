@@ -201,10 +201,10 @@ void attention_decode(bool bf16, const void* q, const void* kv_layer, int64_t kv
 void kv_pack(bool kv_bf16, const void* k, const void* v, bool src_bf16, int n, int Hkv, int pos0,
              void* kv_layer, int64_t kv_head_stride, hipStream_t s);
 
-// The partials of n_splits key ranges, [n_splits][Hkv][n_rows * G][128] and [..][2], to rows.
-// out_fmt: 2 = fp32, 3 = bf16.
-void attn_combine(const float* o_part, const float* ml_part, int n_splits, int n_rows, int Hq,
-                  int Hkv, void* out, int out_fmt, hipStream_t s);
+// The parts of `splits` key ranges, [splits][n][128] and their base and sum [splits][n][2], to n
+// (row, head) results; one that no range has a key of gives zeros.
+void part_combine(const float* o_part, const float* ml_part, int splits, int64_t n, void* out,
+                  bool bf16, hipStream_t s);
 
 // The 8-bit cache (kv8.h; head strides in elements, a multiple of 8192) and what reads it.
 enum class KvType { I8, F16, BF16 };

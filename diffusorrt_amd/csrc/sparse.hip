@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256) void sparse_attn_kernel(
   // queries: column = head kvh * G + cg * 16 + col
   const int gi = cg * 16 + col, head = kvh * G + min(gi, G - 1);
   vec qf[4];
-  float cq = c;
+  float cq = c, nq = 0.f;  // (8-bit: kv8.h's 2^24 in c, -128 * 2^-24 the queries' sum)
   {
     const uint16_t* p = q + ((int64_t)row * Hq + head) * 128;
     u32x4 raw[4];
@@ -270,8 +270,16 @@ __global__ __launch_bounds__(256) void sparse_attn_kernel(
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) qf[i] = __builtin_bit_cast(vec, raw[i]);
+    if constexpr (DT == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) nq = kv8_add8(qf[i], nq);
+      nq += __shfl_xor(nq, 16, 64);
+      nq += __shfl_xor(nq, 32, 64);
+      nq *= -KV8_BIAS / KV8_POW;
+    }
   }
-  float m_run = -INFINITY, l_run = 0.f;
+  float m_run = -INFINITY, l_run = 0.f, p_run = 0.f;
+  int fold = 16;
   f32x4 o[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) o[i] = f32x4{};
@@ -353,7 +361,7 @@ __global__ __launch_bounds__(256) void sparse_attn_kernel(
           }
       }
     }
-    float a = DT == 0 ? fmaxf(sk * cq, 1e-37f) : cq;
+    float a = DT == 0 ? __builtin_amdgcn_fmed3f(sk * cq, 1e-37f, 3e38f) : cq;
     const float lb = DT == 0 ? (float)((int)(__float_as_uint(sv) >> 23) - 127) : 0.f;
     const float inv_sv = DT == 0 ? __uint_as_float((254u << 23) - __float_as_uint(sv)) : 1.f;
     float tmax = s[0][0];
@@ -361,22 +369,36 @@ __global__ __launch_bounds__(256) void sparse_attn_kernel(
     for (int n = 0; n < 4; ++n)
 #pragma unroll
       for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, s[n][r]);
-    float u = fmaf(tmax, a, lb);
+    const float off0 = DT == 0 ? fmaf(nq, a, lb) : 0.f;
+    float u = fmaf(tmax, a, off0);
     u = fmaxf(u, __shfl_xor(u, 16, 64));
     u = fmaxf(u, __shfl_xor(u, 32, 64));
     const bool up = u > m_run + 8.f;
-    if (__ballot(up)) {
+    if (__ballot(up) || (DT == 0 && --fold == 0)) {
       const float alpha = up ? __builtin_amdgcn_exp2f(m_run - u) : 1.f;
+      float less = 0.f;
+      if (DT == 0) {  // (kv8.h: the bytes' 128)
+        less = p_run + __shfl_xor(p_run, 16, 64);
+        less = alpha * (-KV8_BIAS / KV8_POW) * (less + __shfl_xor(less, 32, 64));
+        p_run = 0.f;
+        fold = 16;
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] *= alpha;
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = fmaf(o[i][e], alpha, less);
       l_run *= alpha;
       m_run = up ? u : m_run;
     }
-    const float off = lb - (m_run == -INFINITY ? 0.f : m_run);
-    if (__ballot(fabsf(m_run) > 1048576.f)) {  // (attention8.hip: A8_LARGE)
+    const float mb = m_run == -INFINITY ? 0.f : m_run;
+    float off = off0 - mb;
+    if (__ballot(fabsf(mb) > 1048576.f)) {  // (attention8.hip: A8_LARGE)
 #pragma unroll
-      for (int n = 0; n < 4; ++n) s[n] *= a;
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[n][r] = fmaf(s[n][r], a, off0);
       a = 1.f;
+      off = -mb;
     }
     float psum = 0.f;
     vec pf[2];
@@ -389,6 +411,7 @@ __global__ __launch_bounds__(256) void sparse_attn_kernel(
         if constexpr (DT == 2) pf[kh][e] = (__bf16)p;
         else pf[kh][e] = (_Float16)p;
       }
+    if constexpr (DT == 0) p_run = kv8_add8(pf[1], kv8_add8(pf[0], p_run));
     l_run = fmaf(psum, inv_sv, l_run);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -402,6 +425,14 @@ __global__ __launch_bounds__(256) void sparse_attn_kernel(
   }
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);
+  if (DT == 0) {
+    p_run += __shfl_xor(p_run, 16, 64);
+    p_run += __shfl_xor(p_run, 32, 64);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = fmaf(o[i][e], KV8_POW, -KV8_BIAS * p_run);
+  }
   if (gi >= G) return;
   if (splits > 1) {
     const int64_t at = ((int64_t)split * n_rows + row) * Hq + head;
@@ -423,35 +454,6 @@ __global__ __launch_bounds__(256) void sparse_attn_kernel(
     else
       *(f32x4*)((float*)ao.out + at + 16 * i) = y;
   }
-}
-
-// The key ranges of a (row, head) joined: 32 threads of four head dims each.
-__global__ __launch_bounds__(256) void sparse_combine_kernel(const float* __restrict__ o_part,
-                                                             const float* __restrict__ ml_part,
-                                                             int splits, int64_t n, void* out,
-                                                             int bf16) {
-  const int64_t id = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
-  if (id >= n) return;
-  const int ch = threadIdx.x & 31;
-  float mm = -INFINITY;
-  for (int s = 0; s < splits; ++s) mm = fmaxf(mm, ml_part[(s * n + id) * 2]);
-  float l = 0.f;
-  f32x4 y = f32x4{};
-  for (int s = 0; s < splits; ++s) {
-    const float2 ml = *(const float2*)(ml_part + (s * n + id) * 2);
-    // (a NaN sum counts whatever its base)
-    const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mm);
-    l = fmaf(w, ml.y, l);
-    y += w * *(const f32x4*)(o_part + (s * n + id) * 128 + 4 * ch);
-  }
-  y *= l == 0.f ? 0.f : 1.f / l;
-  const int64_t at = id * 128 + 4 * ch;
-  if (bf16)
-    *(uint2*)((uint16_t*)out + at) =
-        make_uint2((uint32_t)float_to_bf16_bits(y[0]) | ((uint32_t)float_to_bf16_bits(y[1]) << 16),
-                   (uint32_t)float_to_bf16_bits(y[2]) | ((uint32_t)float_to_bf16_bits(y[3]) << 16));
-  else
-    *(f32x4*)((float*)out + at) = y;
 }
 
 // Rows whose scores one pass holds: 256 MiB of them at most.
@@ -510,7 +512,7 @@ void sparse_attention(KvType type, const void* q, bool q_bf16, const void* kv_la
                       int64_t kv_head_stride, const float* scales, int n_rows, int Hq, int Hkv,
                       const AttnWhere& where, const int32_t* blocks, int count, int block,
                       int splits, float* part, void* out, bool out_bf16, hipStream_t s) {
-  const float c = 1.44269504088896340736f / sqrtf(128.0f);
+  const float c = 1.44269504088896340736f / sqrtf(128.0f) * (type == KvType::I8 ? KV8_POW : 1.f);
   const int cgroups = (Hq / Hkv + 15) / 16;
   const int64_t grid = ((int64_t)n_rows + 3) / 4 * splits * cgroups * Hkv;
   require(grid < ((int64_t)1 << 31), "sparse_attention: too many rows for one call");
@@ -527,11 +529,7 @@ void sparse_attention(KvType type, const void* q, bool q_bf16, const void* kv_la
   else DRT_SPARSE(2);
 #undef DRT_SPARSE
   DRT_HIP(hipGetLastError());
-  if (splits > 1) {
-    hipLaunchKernelGGL(sparse_combine_kernel, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, s, part,
-                       ml, splits, n, out, (int)out_bf16);
-    DRT_HIP(hipGetLastError());
-  }
+  if (splits > 1) part_combine(part, ml, splits, n, out, out_bf16, s);
 }
 
 }  // namespace drt

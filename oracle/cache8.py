@@ -122,7 +122,8 @@ def attention(q, k, v, ends, blocks=None, block: int = 0):
     return out, weight
 
 
-def attention_bound(q, k, v, ends, weight, p_half: float, n_keys: int, *, q_bf16_scaled=False):
+def attention_bound(q, k, v, ends, weight, p_half: float, n_keys: int, *, q_bf16_scaled=False,
+                    scales8=(0.0, 0.0)):
     """How far a kernel's fp32 result may be from :func:`attention`'s, from its roundings.
 
     - a weighted value p is rounded once to the product's type: ``p_half`` of it (2^-11 for
@@ -132,16 +133,21 @@ def attention_bound(q, k, v, ends, weight, p_half: float, n_keys: int, *, q_bf16
     - a score is a sum of 128 exact products in fp32, and two more roundings: 130 * 2^-24 of
       the sum of their magnitudes, in the exponent, so that times p; once in p, once in the
       normaliser; exp2 and the sums over keys in fp32 add (n_keys / 32 + 64) * 2^-24;
+    - over 8 bits (scales8: the largest scales of a tile's K and V) both go into the products as
+      bytes code + 128 <= 255, and 128 times the sum of the query, or of the weights, is taken off:
+      |k| is up to 128 scales larger, and O an fp32 sum of up to 255 scales instead of |v|,
+      which a product rounds at most once a key and a fold once more (a tile's sum of weights: 32
+      times), 2 n_keys times in all;
     - bf16 queries that are scaled to fp16 lose at most 2^-25 of the vector's largest each.
     """
     q = np.abs(np.asarray(q, np.float64))
     k, v = np.abs(np.nan_to_num(k)), np.abs(np.nan_to_num(v))
-    kmax = k.max(0)                                                      # [hkv, 128]
+    kmax = k.max(0) + 128 * scales8[0]                                   # [hkv, 128]
     g = q.shape[1] // k.shape[1]
     s = (q * kmax.repeat(g, 0)[None]).sum(-1) * 128 ** -0.5              # [rows, hq]
     e = 130 * 2.0 ** -24 * s
     if q_bf16_scaled:
         e = e + 128 ** -0.5 * 2.0 ** -25 * q.max(-1) * kmax.sum(-1).repeat(g)[None]
     rel = p_half + 2 * e + (n_keys / 32 + 64) * 2.0 ** -24
-    floor = n_keys * 2.0 ** -24 * v.max()
+    floor = n_keys * 2.0 ** -24 * v.max() + (2 * n_keys + 4) * 2.0 ** -24 * 255 * scales8[1]
     return rel[..., None] * weight + floor

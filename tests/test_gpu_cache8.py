@@ -43,6 +43,14 @@ def _filled(gen, n, hkv, dtype, capacity=None, block_sums=True):
     return (cache, *(_np(torch.cat([x, pad]).to(TDT[dtype])) for x in (k, v)))
 
 
+def _scales(cache, layer):
+    """The largest scales of a tile's K and V of an 8-bit cache, for attention_bound."""
+    if cache.scales is None:
+        return (0.0, 0.0)
+    x = torch.nan_to_num(cache.scales[layer]).amax((0, 1))
+    return float(x[0]), float(x[1])
+
+
 def _check(got, out, bound, out_dtype):
     g = _np(got).reshape(out.shape)
     last = 2.0 ** -8 if out_dtype == torch.bfloat16 else 2.0 ** -24
@@ -179,7 +187,7 @@ def test_attention_over_8_bits(rows, hq, hkv, n_keys, pos0, mask, qdt, odt):
     ends = X.key_ends(rows, n_keys, pos0, mask)
     out, weight = X.attention(_np(q), k, v, ends)
     bound = X.attention_bound(_np(q), k, v, ends, weight, HALF["i8"], n_keys,
-                              q_bf16_scaled=qdt == "bf16")
+                              q_bf16_scaled=qdt == "bf16", scales8=_scales(cache, 1))
     _check(got, out, bound, TDT[odt])
 
 
@@ -196,7 +204,8 @@ def test_attention_of_the_kernel_table_over_8_bits():
     ref.store(k.numpy(), v.numpy(), 0)
     ends = X.key_ends(32, 96, 64)
     out, weight = X.attention(_np(q), *ref.values, ends)
-    bound = X.attention_bound(_np(q), *ref.values, ends, weight, HALF["i8"], 96)
+    bound = X.attention_bound(_np(q), *ref.values, ends, weight, HALF["i8"], 96,
+                              scales8=ref.scales.max((0, 1)))
     assert got.dtype == torch.float16 and got.shape == (32, 512)
     assert (np.abs(_np(got).reshape(out.shape) - out)
             <= bound + 2.0 ** -11 * (np.abs(out) + bound)).all()
@@ -232,7 +241,8 @@ def test_tiles_of_very_different_scales(rows, sparse):
             got = cache.attention(0, q.cuda(), n_keys=n_keys, row_pos0=0, kind="full")
         k8, v8 = ref.values[0][:n_keys], ref.values[1][:n_keys]
         out, weight = X.attention(_np(q), k8, v8, ends)
-        _check(got, out, X.attention_bound(_np(q), k8, v8, ends, weight, HALF["i8"], n_keys),
+        _check(got, out, X.attention_bound(_np(q), k8, v8, ends, weight, HALF["i8"], n_keys,
+                                            scales8=ref.scales[:, :n_keys // 32].max((0, 1))),
                torch.float32)
 
 
@@ -259,7 +269,8 @@ def test_bf16_queries_of_any_size(qsize):
             assert (off[sure] <= 2.0 ** -20 * np.abs(out).max()).all()
         else:
             _check(got, out, X.attention_bound(_np(q), k, v, ends, weight, HALF["i8"], 90,
-                                               q_bf16_scaled=True), torch.float32)
+                                               q_bf16_scaled=True, scales8=_scales(cache, 1)),
+                   torch.float32)
 
 
 @pytest.mark.parametrize("dtype", ["i8", "f16", "bf16"])
@@ -425,7 +436,8 @@ def test_sparse_attention(dtype, rows, hq, hkv, n_keys, pos0, mask, qdt, odt, bl
     ends = X.key_ends(rows, n_keys, pos0, mask)
     out, weight = X.attention(_np(q), k, v, ends, blocks.cpu().numpy(), block)
     bound = X.attention_bound(_np(q), k, v, ends, weight, HALF[dtype], n_keys,
-                              q_bf16_scaled=dtype == "i8" and qdt == "bf16")
+                              q_bf16_scaled=dtype == "i8" and qdt == "bf16",
+                              scales8=_scales(cache, 1))
     _check(got, out, bound, TDT[odt])
 
 
@@ -455,7 +467,7 @@ def test_sparse_attention_of_lists_of_any_origin(dtype, rows):
     ends = X.key_ends(rows, n_keys, pos0, (2950, 24))
     out, weight = X.attention(_np(q[some]), k, v, ends[some], blocks[some], 32)
     _check(got[some], out, X.attention_bound(_np(q[some]), k, v, ends[some], weight, HALF[dtype],
-                                             n_keys), torch.float32)
+                                             n_keys, scales8=_scales(cache, 1)), torch.float32)
     assert not got[0].any()
     # row 1 lists block 2^31 - 1 first: it lies beyond the row, and nothing after is larger
     assert not got[1].any()
@@ -516,7 +528,8 @@ def test_a_blocks_step_against_the_oracle(dtype):
     np.testing.assert_array_equal(blocks.cpu().numpy(), want)
     for got, y, lists in ((a, ya, want), (b, yb, None)):
         out, weight = X.attention(_np(q), k8, v8, ends, lists, 64)
-        bound = X.attention_bound(_np(q), k8, v8, ends, weight, HALF[dtype], 1024)
+        bound = X.attention_bound(_np(q), k8, v8, ends, weight, HALF[dtype], 1024,
+                                  scales8=_scales(cache, 0))
         if dtype == "i8" or lists is not None:
             _check(got, out, bound, torch.bfloat16)
         # the projection of what came out: half a bf16 step and the fp32 sums
