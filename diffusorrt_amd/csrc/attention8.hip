@@ -54,15 +54,15 @@ struct A8Out {
 // QW waves over query tiles, KW waves over keys (wave kw of a query tile takes key
 // tiles kw, kw + KW, ...; their parts meet in LDS at the end). OUT: one key range, the
 // result itself; otherwise a part for the combine.
-template <int QW, int KW, bool OUT>
-__global__ __launch_bounds__(64 * QW * KW, KW == 1 ? 3 : 2) void attn8_kernel(
+template <int QT, int QW, int KW, bool OUT>
+__global__ __launch_bounds__(64 * QW * KW, 2) void attn8_kernel(
     const uint16_t* __restrict__ q, const uint8_t* __restrict__ kv, int64_t kv_head_stride,
     const float* __restrict__ scales, int q_bf16, int n_rows, int Hq, int Hkv,
     int tiles_per_split, float c, const AttnWhere where, const A8Out ao) {
-  constexpr int NW = QW * KW, THREADS = 64 * NW, NQ = 32 * QW;
-  constexpr int O_BYTES = 16384;  // a query tile's O
-  constexpr int Q_BYTES = NQ * A8_QROW * 2, OUT_BYTES = QW * O_BYTES / 2;
-  constexpr int MRG = KW > 1 ? (NW / 2) * (O_BYTES + 512) : 0;
+  constexpr int NW = QW * KW, THREADS = 64 * NW, NQ = 32 * QT * QW;
+  constexpr int O_BYTES = QT * 16384;  // a wave's O
+  constexpr int Q_BYTES = NQ * A8_QROW * 2, OUT_BYTES = QW * 8192;
+  constexpr int ML_BYTES = QT * 512, MRG = KW > 1 ? (NW / 2) * (O_BYTES + ML_BYTES) : 0;
   constexpr int LDS = Q_BYTES > MRG ? (Q_BYTES > OUT_BYTES ? Q_BYTES : OUT_BYTES)
                                     : (MRG > OUT_BYTES ? MRG : OUT_BYTES);
   __shared__ __align__(16) char smem[LDS];
@@ -72,7 +72,8 @@ __global__ __launch_bounds__(64 * QW * KW, KW == 1 ? 3 : 2) void attn8_kernel(
   const int qw = wave % QW, kw = wave / QW;
   const int G = Hq / Hkv, n_qv = n_rows * G;
   const int kvh = blockIdx.x % Hkv, split = blockIdx.x / Hkv;
-  const int qt0 = blockIdx.y * QW;  // the work-group's first query tile
+  // the work-group's first query tile: the last rows, which see the most keys, start first
+  const int qt0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * (QW * QT);
   const int n_tiles = (where.n_keys + 31) >> 5;
 
   // queries into LDS, 16 threads (eight elements each) a query vector
@@ -109,24 +110,32 @@ __global__ __launch_bounds__(64 * QW * KW, KW == 1 ? 3 : 2) void attn8_kernel(
   }
   __syncthreads();
 
-  const _Float16* ql = (const _Float16*)smem + (qw * 32 + (lane & 31)) * A8_QROW + 8 * (lane >> 5);
-  constexpr bool HOLD = KW > 1;  // the queries' operands in registers (two waves a SIMD)
+  const _Float16* ql = (const _Float16*)smem + (qw * QT * 32 + (lane & 31)) * A8_QROW + 8 * (lane >> 5);
+  constexpr bool HOLD = QT == 1;  // the queries' operands in registers
   f16x8 qr[HOLD ? 8 : 1];
   if (HOLD) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) qr[HOLD ? i : 0] = *(const f16x8*)(ql + 16 * i);
   }
-  const int my_qv = (qt0 + qw) * 32 + (lane & 31);
-  const int q_end = key_end_of(min(my_qv, n_qv - 1) / G, where);
-  const float cq = qinfo[qw * 32 + (lane & 31)].x, nq = qinfo[qw * 32 + (lane & 31)].y;
-  float m_run = -INFINITY, l_run = 0.f, p_run = 0.f;
-  f32x16 o[4];
+  const int wt0 = qt0 + qw * QT;  // the wave's first query tile
+  int q_end[QT];
+  float cq[QT], nq[QT], m_run[QT], l_run[QT], p_run[QT];
+  f32x16 o[QT][4];
 #pragma unroll
-  for (int hb = 0; hb < 4; ++hb) o[hb] = f32x16{};
+  for (int j = 0; j < QT; ++j) {
+    q_end[j] = key_end_of(min((wt0 + j) * 32 + (lane & 31), n_qv - 1) / G, where);
+    const float2 x = qinfo[(qw * QT + j) * 32 + (lane & 31)];
+    cq[j] = x.x;
+    nq[j] = x.y;
+    m_run[j] = -INFINITY;
+    l_run[j] = p_run[j] = 0.f;
+#pragma unroll
+    for (int hb = 0; hb < 4; ++hb) o[j][hb] = f32x16{};
+  }
   // (ends never fall from row to row) keys every row of the wave sees, and any of them
-  const int wave_full = key_end_of(min((qt0 + qw) * 32, n_qv - 1) / G, where);
-  const int wave_end = key_end_of(min((qt0 + qw) * 32 + 31, n_qv - 1) / G, where);
-  const bool idle = (qt0 + qw) * 32 >= n_qv;
+  const int wave_full = key_end_of(min(wt0 * 32, n_qv - 1) / G, where);
+  const int wave_end = key_end_of(min((wt0 + QT) * 32 - 1, n_qv - 1) / G, where);
+  const bool idle = wt0 * 32 >= n_qv;
   const int t_begin = split * tiles_per_split;
   const int t_end = idle ? 0 : min(min(n_tiles, t_begin + tiles_per_split), (wave_end + 31) >> 5);
 
@@ -148,114 +157,143 @@ __global__ __launch_bounds__(64 * QW * KW, KW == 1 ? 3 : 2) void attn8_kernel(
     const float sk = st.x, sv = st.y;
     const int tn = min(t + KW, t_end - 1);  // (the last tile's own again: loaded, not used)
     const uint8_t* p = base + (int64_t)tn * KV8_TILE;
-    f32x16 s = f32x16{};
+    f32x16 s[QT];
+#pragma unroll
+    for (int j = 0; j < QT; ++j) s[j] = f32x16{};
+    if (!HOLD) asm volatile("" ::: "memory");  // (read the queries here, tile by tile)
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const f16x8 kf = kv8_to_f16(kr[i >> 1][2 * (i & 1)], kr[i >> 1][2 * (i & 1) + 1]);
-      s = mfma_f16(kf, HOLD ? qr[HOLD ? i : 0] : *(const f16x8*)(ql + 16 * i), s);
+#pragma unroll
+      for (int j = 0; j < QT; ++j)
+        s[j] = mfma_f16(kf, HOLD ? qr[HOLD ? i : 0] : *(const f16x8*)(ql + j * 32 * A8_QROW + 16 * i),
+                        s[j]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) kr[i] = *(const u32x4*)(p + i * 1024);
+    __builtin_amdgcn_s_setprio(0);
+    asm volatile("" ::: "memory");  // (a scalar load among the reads of LDS would be waited for with them)
     st = sc[tn];
     const bool bad = !(sk + sv < INFINITY);  // a tile that is NaN: so is every row that sees it
-    if (bad && key0 < q_end) {
-      l_run = NAN;
-      m_run = m_run == -INFINITY ? 0.f : m_run;
-    }
     if (key0 + 32 > wave_full || bad) {
-      const int end = bad ? 0 : q_end;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = key0 + mfma_row(r, lane) < end ? s[r] : -INFINITY;
+      for (int j = 0; j < QT; ++j) {
+        if (bad && key0 < q_end[j]) {
+          l_run[j] = NAN;
+          m_run[j] = m_run[j] == -INFINITY ? 0.f : m_run[j];
+        }
+        const int end = bad ? 0 : q_end[j];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[j][r] = key0 + mfma_row(r, lane) < end ? s[j][r] : -INFINITY;
+      }
     }
     const float lb = bad ? 0.f : (float)((int)(__float_as_uint(sv) >> 23) - 127);  // sv = 2^lb
     const float inv_sv = bad ? 0.f : __uint_as_float((254u << 23) - __float_as_uint(sv));
-    // (within the finite numbers above zero whatever the powers of two: no 0 * inf)
-    float a = bad ? 1.f : __builtin_amdgcn_fmed3f(sk * cq, 1e-37f, 3e38f);
-    float tmax = s[0];
+    f16x8 pf[QT][2];
 #pragma unroll
-    for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, s[r]);
-    const float off0 = fmaf(nq, a, lb);
-    const float u = fmaf(a8_max_xor32(tmax), a, off0);  // -inf: no visible key in the tile
-    const bool up = u > m_run + A8_RESCALE_LOG2;
-    if (__ballot(up) || --fold == 0) {
-      const float alpha = up ? __builtin_amdgcn_exp2f(m_run - u) : 1.f;  // 0 from -inf
-      const float less = alpha * (-KV8_BIAS / KV8_POW) * (p_run + __shfl_xor(p_run, 32, 64));
+    for (int j = 0; j < QT; ++j) {
+      // (within the finite numbers above zero whatever the powers of two: no 0 * inf)
+      float a = bad ? 1.f : __builtin_amdgcn_fmed3f(sk * cq[j], 1e-37f, 3e38f);
+      float tmax = s[j][0];
 #pragma unroll
-      for (int hb = 0; hb < 4; ++hb)
+      for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, s[j][r]);
+      const float off0 = fmaf(nq[j], a, lb);
+      const float u = fmaf(a8_max_xor32(tmax), a, off0);  // -inf: no visible key in the tile
+      const bool up = u > m_run[j] + A8_RESCALE_LOG2;
+      if (__ballot(up) || fold == 1) {
+        const float alpha = up ? __builtin_amdgcn_exp2f(m_run[j] - u) : 1.f;  // 0 from -inf
+        const float less = alpha * (-KV8_BIAS / KV8_POW) * (p_run[j] + __shfl_xor(p_run[j], 32, 64));
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[hb][r] = fmaf(o[hb][r], alpha, less);
-      l_run *= alpha;
-      p_run = 0.f;
-      fold = A8_FOLD;
-      m_run = up ? u : m_run;
-    }
-    const float mb = m_run == -INFINITY ? 0.f : m_run;
-    float off = off0 - mb;
-    if (__ballot(fabsf(mb) > A8_LARGE)) {  // exponents rounded as the base was
+        for (int hb = 0; hb < 4; ++hb)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], a, off0);
-      a = 1.f;
-      off = -mb;
-    }
-    f16x8 pf[2];
-    float psum = 0.f;
-#pragma unroll
-    for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[kh * 8 + e], a, off));
-        psum += p;
-        pf[kh][e] = (_Float16)p;
+          for (int r = 0; r < 16; ++r) o[j][hb][r] = fmaf(o[j][hb][r], alpha, less);
+        l_run[j] *= alpha;
+        p_run[j] = 0.f;
+        m_run[j] = up ? u : m_run[j];
       }
-    p_run = kv8_add8(pf[1], kv8_add8(pf[0], p_run));
-    l_run = fmaf(psum, inv_sv, l_run);
+      const float mb = m_run[j] == -INFINITY ? 0.f : m_run[j];
+      float off = off0 - mb;
+      if (__ballot(fabsf(mb) > A8_LARGE)) {  // exponents rounded as the base was
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[j][r] = fmaf(s[j][r], a, off0);
+        a = 1.f;
+        off = -mb;
+      }
+      float psum = 0.f;
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[j][kh * 8 + e], a, off));
+          psum += x;
+          pf[j][kh][e] = (_Float16)x;
+        }
+      p_run[j] = kv8_add8(pf[j][1], kv8_add8(pf[j][0], p_run[j]));
+      l_run[j] = fmaf(psum, inv_sv, l_run[j]);
+    }
+    fold = fold == 1 ? A8_FOLD : fold - 1;
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int hb = 0; hb < 4; ++hb)
 #pragma unroll
-      for (int kh = 0; kh < 2; ++kh)
-        o[hb] = mfma_f16(kv8_to_f16(vr[hb][2 * kh], vr[hb][2 * kh + 1]), pf[kh], o[hb]);
+      for (int kh = 0; kh < 2; ++kh) {
+        const f16x8 vf = kv8_to_f16(vr[hb][2 * kh], vr[hb][2 * kh + 1]);
+#pragma unroll
+        for (int j = 0; j < QT; ++j) o[j][hb] = mfma_f16(vf, pf[j][kh], o[j][hb]);
+      }
 #pragma unroll
     for (int i = 0; i < 4; ++i) vr[i] = *(const u32x4*)(p + 4096 + i * 1024);
   }
-  l_run += __shfl_xor(l_run, 32, 64);
-  p_run += __shfl_xor(p_run, 32, 64);
 #pragma unroll
-  for (int hb = 0; hb < 4; ++hb)
+  for (int j = 0; j < QT; ++j) {
+    l_run[j] += __shfl_xor(l_run[j], 32, 64);
+    p_run[j] += __shfl_xor(p_run[j], 32, 64);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) o[hb][r] = fmaf(o[hb][r], KV8_POW, -KV8_BIAS * p_run);
+    for (int hb = 0; hb < 4; ++hb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[j][hb][r] = fmaf(o[j][hb][r], KV8_POW, -KV8_BIAS * p_run[j]);
+  }
 
-  // the key ways of a query tile in pairs
+  // the key ways of a wave's queries in pairs
   if (KW > 1) {
 #pragma unroll
     for (int half = KW / 2; half > 0; half >>= 1) {
       __syncthreads();  // the queries, or the round before, have been read
       if (kw >= half && kw < 2 * half) {
-        f32x4* d = (f32x4*)(smem + ((kw - half) * QW + qw) * (O_BYTES + 512));
+        char* d = smem + ((kw - half) * QW + qw) * (O_BYTES + ML_BYTES);
 #pragma unroll
-        for (int hb = 0; hb < 4; ++hb)
+        for (int j = 0; j < QT; ++j) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            d[(hb * 4 + r) * 64 + lane] =
-                f32x4{o[hb][4 * r], o[hb][4 * r + 1], o[hb][4 * r + 2], o[hb][4 * r + 3]};
-        ((float2*)((char*)d + O_BYTES))[lane] = make_float2(m_run, l_run);
+          for (int hb = 0; hb < 4; ++hb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              ((f32x4*)d)[(j * 16 + hb * 4 + r) * 64 + lane] =
+                  f32x4{o[j][hb][4 * r], o[j][hb][4 * r + 1], o[j][hb][4 * r + 2], o[j][hb][4 * r + 3]};
+          ((float2*)(d + O_BYTES))[j * 64 + lane] = make_float2(m_run[j], l_run[j]);
+        }
       }
       __syncthreads();
       if (kw < half) {
-        const f32x4* d = (const f32x4*)(smem + (kw * QW + qw) * (O_BYTES + 512));
-        const float2 ml = ((const float2*)((const char*)d + O_BYTES))[lane];
-        const float mm = fmaxf(m_run, ml.x);
-        const float w0 = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - mm);
-        const float w1 = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mm);
+        const char* d = smem + (kw * QW + qw) * (O_BYTES + ML_BYTES);
 #pragma unroll
-        for (int hb = 0; hb < 4; ++hb)
+        for (int j = 0; j < QT; ++j) {
+          const float2 ml = ((const float2*)(d + O_BYTES))[j * 64 + lane];
+          const float mm = fmaxf(m_run[j], ml.x);
+          const float w0 = m_run[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[j] - mm);
+          const float w1 = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mm);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const f32x4 y = d[(hb * 4 + r) * 64 + lane];
+          for (int hb = 0; hb < 4; ++hb)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[hb][4 * r + e] = fmaf(w1, y[e], w0 * o[hb][4 * r + e]);
-          }
-        l_run = fmaf(w1, ml.y, w0 * l_run);
-        m_run = mm;
+            for (int r = 0; r < 4; ++r) {
+              const f32x4 y = ((const f32x4*)d)[(j * 16 + hb * 4 + r) * 64 + lane];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                o[j][hb][4 * r + e] = fmaf(w1, y[e], w0 * o[j][hb][4 * r + e]);
+            }
+          l_run[j] = fmaf(w1, ml.y, w0 * l_run[j]);
+          m_run[j] = mm;
+        }
       }
     }
   }
@@ -263,20 +301,21 @@ __global__ __launch_bounds__(64 * QW * KW, KW == 1 ? 3 : 2) void attn8_kernel(
   if (kw > 0) return;  // (no barrier follows)
   // Rows out: half a query tile's O^T (64 head dims) at a time through 8 KiB of the wave's own, as 16-byte
   // pieces (query v, piece p at p ^ v: every bank in turn both ways), eight lanes a query vector.
-  f32x4* ot = (f32x4*)(smem + qw * (O_BYTES / 2));
+  f32x4* ot = (f32x4*)(smem + qw * 8192);
 #pragma unroll
-  for (int hf = 0; hf < 2; ++hf) {
+  for (int jh = 0; jh < 2 * QT; ++jh) {
+    const int j = jh >> 1, hf = jh & 1;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         ot[(lane & 31) * 16 + ((b * 8 + 2 * r + (lane >> 5)) ^ (lane & 15))] =
-            f32x4{o[2 * hf + b][4 * r], o[2 * hf + b][4 * r + 1], o[2 * hf + b][4 * r + 2],
-                  o[2 * hf + b][4 * r + 3]};
+            f32x4{o[j][2 * hf + b][4 * r], o[j][2 * hf + b][4 * r + 1], o[j][2 * hf + b][4 * r + 2],
+                  o[j][2 * hf + b][4 * r + 3]};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int v = (lane >> 3) + 8 * i, ch = lane & 7, qv = (qt0 + qw) * 32 + v;
-      const float m = __shfl(m_run, v, 64), l = __shfl(l_run, v, 64);
+      const int v = (lane >> 3) + 8 * i, ch = lane & 7, qv = (wt0 + j) * 32 + v;
+      const float m = __shfl(m_run[j], v, 64), l = __shfl(l_run[j], v, 64);
       f32x4 y0 = ot[v * 16 + ((2 * ch) ^ (v & 15))], y1 = ot[v * 16 + ((2 * ch + 1) ^ (v & 15))];
       if (qv >= n_qv) continue;
       const int row = qv / G;
@@ -400,14 +439,20 @@ void part_combine(const float* o_part, const float* ml_part, int splits, int64_t
 Attn8Plan plan_attention8(int n_rows, int Hq, int Hkv, int n_keys) {
   Attn8Plan p;
   const int qtiles = (int)(((int64_t)n_rows * (Hq / Hkv) + 31) / 32);
-  p.qw = qtiles == 1 ? 1 : qtiles == 2 ? 2 : 4;
+  // Many queries: two query tiles a wave (a tile's codes made operands once for both), four key
+  // ways in a work-group of their own, so that work-groups are as many as can be (2048 rows x 16
+  // heads over 4096 keys: 72 us; two and one key ways, which need key ranges to fill the chip:
+  // 101, 110). Few: eight waves over the one, two or four query tiles.
   p.wide = qtiles > 4;
-  p.qgroups = (qtiles + p.qw - 1) / p.qw;
-  const int n_tiles = (n_keys + 31) / 32, kw = p.wide ? 1 : 8 / p.qw;
+  p.qw = p.wide || qtiles == 1 ? 1 : qtiles == 2 ? 2 : 4;
+  p.kw = p.wide ? 4 : 8 / p.qw;
+  const int per = p.wide ? 2 : p.qw;  // query tiles of a work-group
+  p.qgroups = (qtiles + per - 1) / per;
+  const int n_tiles = (n_keys + 31) / 32;
   const int64_t wgs = (int64_t)Hkv * p.qgroups;
-  const int target = p.wide ? 768 : 256;
+  const int target = p.wide ? 512 : 256;
   int64_t splits = std::max<int64_t>(1, target / wgs);
-  splits = std::min<int64_t>({splits, (n_tiles + kw - 1) / kw, 64});
+  splits = std::min<int64_t>({splits, (n_tiles + p.kw - 1) / p.kw, 64});
   p.tiles_per_split = (int)((n_tiles + splits - 1) / splits);
   p.splits = (n_tiles + p.tiles_per_split - 1) / p.tiles_per_split;
   return p;
@@ -424,16 +469,16 @@ void attention8(const void* q, bool q_bf16, const void* kv_layer, int64_t kv_hea
   float* ml = part ? part + (size_t)p.splits * n_rows * Hq * 128 : nullptr;
   const A8Out ao{out, part, ml, out_bf16};
   const dim3 grid((unsigned)(p.splits * Hkv), (unsigned)p.qgroups);
-#define DRT_A8(QW, KW, OUT)                                                                   \
-  hipLaunchKernelGGL((attn8_kernel<QW, KW, OUT>), grid, dim3(64 * QW * KW), 0, s,             \
+#define DRT_A8(QT, QW, KW, OUT)                                                                   \
+  hipLaunchKernelGGL((attn8_kernel<QT, QW, KW, OUT>), grid, dim3(64 * QW * KW), 0, s,             \
                      (const uint16_t*)q, (const uint8_t*)kv_layer, kv_head_stride, scales,    \
                      (int)q_bf16, n_rows, Hq, Hkv, p.tiles_per_split, c, where, ao)
-#define DRT_A8O(QW, KW)                                                                       \
-  do { if (p.splits == 1) DRT_A8(QW, KW, true); else DRT_A8(QW, KW, false); } while (0)
-  if (p.wide) DRT_A8O(4, 1);
-  else if (p.qw == 1) DRT_A8O(1, 8);
-  else if (p.qw == 2) DRT_A8O(2, 4);
-  else DRT_A8O(4, 2);
+#define DRT_A8O(QT, QW, KW)                                                                       \
+  do { if (p.splits == 1) DRT_A8(QT, QW, KW, true); else DRT_A8(QT, QW, KW, false); } while (0)
+  if (p.wide) DRT_A8O(2, 1, 4);
+  else if (p.qw == 1) DRT_A8O(1, 1, 8);
+  else if (p.qw == 2) DRT_A8O(1, 2, 4);
+  else DRT_A8O(1, 4, 2);
 #undef DRT_A8O
 #undef DRT_A8
   DRT_HIP(hipGetLastError());

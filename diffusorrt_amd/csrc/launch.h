@@ -220,7 +220,7 @@ void kv_load(KvType type, const void* kv, int64_t head_stride, const float* scal
 void kv_sums(bool bf16, const void* kv, int64_t head_stride, int Hkv, int pos0, int n, float* sums,
              hipStream_t s);
 struct Attn8Plan {
-  int qw = 1, qgroups = 1, splits = 1, tiles_per_split = 1;
+  int qw = 1, kw = 8, qgroups = 1, splits = 1, tiles_per_split = 1;
   bool wide = false;  // two query tiles a wave
 };
 Attn8Plan plan_attention8(int n_rows, int Hq, int Hkv, int n_keys);

@@ -17,6 +17,7 @@ the reference's fail-closed checks.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 from . import _lib
@@ -162,29 +163,35 @@ def swiglu(gate, up):
     return y
 
 
-class _on:
-    """The current device set to ``t``'s for the launches inside (nothing where it is already)."""
+_Q_CODES = {}  # torch dtype -> code of what a query may be (filled on first use)
 
-    def __init__(self, t):
-        self.index = t.device.index
 
-    def __enter__(self):
+def _q_codes():
+    if not _Q_CODES:
         torch = _torch()
-        self.back = torch.cuda.current_device()
-        if self.index != self.back:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.index != self.back:
-            _torch().cuda.set_device(self.back)
+        _Q_CODES.update({torch.float16: _lib.F16, torch.bfloat16: _lib.BF16})
+    return _Q_CODES
 
 
-def _workspace(nbytes, t):
-    """(pointer or None, bytes, the tensor that holds them)."""
-    if not nbytes:
-        return None, 0, None
-    ws = _torch().empty(nbytes, dtype=_torch().uint8, device=t.device)
-    return _ptr(ws), nbytes, ws
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name, *shape) -> int:
+    return getattr(_lib.load(), name)(*shape)
+
+
+def _launch(torch, fn, index, *args):
+    """``fn(*args, stream)`` on device ``index`` and its current stream. (A short call is mostly
+    host time: addresses go as plain integers, and the device is only set where it differs.)"""
+    back = torch._C._cuda_getDevice()
+    if back == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        torch.cuda.set_device(index)
+        try:
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        finally:
+            torch.cuda.set_device(back)
+    if status:
+        _lib.check(status)
 
 
 class PrefixKVCache:
@@ -228,39 +235,51 @@ class PrefixKVCache:
             self.sums = torch.zeros((*shape[:2], self.tiles, 128), dtype=torch.float32,
                                     device=device)
         self.length = 0
+        self._index = self.data.get_device()  # (-1: on the host, where nothing runs)
 
     @property
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.data, self.scales, self.sums)
                    if t is not None)
 
-    def _layer(self, layer, *tensors):
-        """(data, scales or None, sums or None) of a layer, as pointers; the new operators' checks
-        of where things are."""
+    def _check(self, layer, *tensors):
+        """The layer, and where the tensors of a call are."""
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer must be in [0, {self.layers})")
-        _require_cuda(*tensors)
-        if any(t.device != self.data.device for t in tensors):
-            raise ValueError("tensors must be on the cache's device")
-        return tuple(None if t is None else _ptr(t[layer])
-                     for t in (self.data, self.scales, self.sums))
+        for t in tensors:
+            if t.get_device() != self._index or self._index < 0:
+                raise ValueError("tensors must be on the cache's device, a GPU")
+            if not t.is_contiguous():
+                raise ValueError("the cache's calls take contiguous tensors")
 
-    def _queries(self, q):
-        """(rows, query heads, dtype code) of ``q``, checked against the cache."""
-        torch = _torch()
-        if q.dim() != 3 or q.shape[2] != 128 or q.shape[1] < 1 or q.shape[1] % self.kv_heads:
+    def _data(self, layer):
+        return self.data.data_ptr() + layer * self.kv_heads * self.head_stride * \
+            (1 if self.scales is not None else 2)
+
+    def _scales(self, layer):
+        return None if self.scales is None else \
+            self.scales.data_ptr() + layer * self.kv_heads * self.tiles * 8
+
+    def _sums(self, layer):
+        return None if self.sums is None else \
+            self.sums.data_ptr() + layer * self.kv_heads * self.tiles * 512
+
+    def _queries(self, q, n_keys, row_pos0):
+        """(rows, query heads, dtype code) of a call's queries, checked against the cache."""
+        if q.dim() != 3:
+            raise ValueError("attention needs q [rows, Hq, 128]")
+        rows, hq, hd = q.shape
+        if hd != 128 or hq < 1 or hq % self.kv_heads:
             raise ValueError("attention needs q [rows, Hq, 128] and Hq % Hkv == 0")
-        code = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}.get(q.dtype)
-        if code is None or (self.kv_dtype != _lib.I8 and code != self.kv_dtype):
+        code = _q_codes().get(q.dtype)
+        if code is None or (self.scales is None and code != self.kv_dtype):
             raise ValueError("q must be float16 or bfloat16 over an 8-bit cache, and of the "
                              "cache's own type over a 16-bit one")
-        return q.shape[0], q.shape[1], code
-
-    def _keys(self, n_keys, rows, row_pos0):
         if n_keys < 1 or n_keys > self.capacity:
             raise ValueError("n_keys outside the cache")
         if rows < 1 or row_pos0 < 0 or row_pos0 + rows > _I32_MAX:
             raise ValueError("attention needs a query row, and row positions of 32 bits")
+        return rows, hq, code
 
     def store(self, layer: int, k, v, pos0: int) -> None:
         """Write ``k/v [n, Hkv, 128]`` (fp32 or bf16) at positions ``pos0..pos0+n-1``."""
@@ -274,20 +293,17 @@ class PrefixKVCache:
         if k.dtype not in (torch.float32, torch.bfloat16) or v.dtype != k.dtype:
             raise ValueError("store takes fp32 or bf16 k/v")
         src = _lib.BF16 if k.dtype == torch.bfloat16 else _lib.F32
-        if self.kv_dtype == _lib.I8 or self.sums is not None:
-            data, scales, sums = self._layer(layer, k, v)
-            with _on(k):
-                if self.kv_dtype == _lib.I8:
-                    _lib.check(_lib.load().drt_op_kv8_store(
-                        _ptr(k), _ptr(v), src, n, self.kv_heads, pos0, data, self.head_stride,
-                        scales, sums, _stream(k)))
-                else:
-                    _lib.check(_lib.load().drt_op_kv_pack(
-                        _ptr(k), _ptr(v), src, n, self.kv_heads, pos0, data, self.head_stride,
-                        self.kv_dtype, _stream(k)))
-                    _lib.check(_lib.load().drt_op_kv_sums(
-                        data, self.head_stride, self.kv_dtype, n, self.kv_heads, pos0, sums,
-                        _stream(k)))
+        if self.scales is not None or self.sums is not None:
+            self._check(layer, k, v)
+            lib, data, sums = _lib.load(), self._data(layer), self._sums(layer)
+            if self.scales is not None:
+                _launch(torch, lib.drt_op_kv8_store, self._index, k.data_ptr(), v.data_ptr(), src,
+                        n, self.kv_heads, pos0, data, self.head_stride, self._scales(layer), sums)
+            else:
+                _launch(torch, lib.drt_op_kv_pack, self._index, k.data_ptr(), v.data_ptr(), src,
+                        n, self.kv_heads, pos0, data, self.head_stride, self.kv_dtype)
+                _launch(torch, lib.drt_op_kv_sums, self._index, data, self.head_stride,
+                        self.kv_dtype, n, self.kv_heads, pos0, sums)
             self.length = max(self.length, pos0 + n)
             return
         layer_view = self.data[layer]
@@ -305,13 +321,13 @@ class PrefixKVCache:
             raise ValueError("load gives float32 or bfloat16")
         if n < 1 or pos0 < 0 or pos0 + n > self.capacity:
             raise ValueError("load positions outside the cache")
-        data, scales, _ = self._layer(layer, self.data)
+        self._check(layer, self.data)
         k = torch.empty((n, self.kv_heads, 128), dtype=out_dtype, device=self.data.device)
         v = torch.empty_like(k)
-        with _on(k):
-            _lib.check(_lib.load().drt_op_kv_load(
-                data, self.head_stride, self.kv_dtype, scales, n, self.kv_heads, pos0, _ptr(k),
-                _ptr(v), _lib.F32 if out_dtype == torch.float32 else _lib.BF16, _stream(k)))
+        _launch(torch, _lib.load().drt_op_kv_load, self._index, self._data(layer),
+                self.head_stride, self.kv_dtype, self._scales(layer), n, self.kv_heads, pos0,
+                k.data_ptr(), v.data_ptr(),
+                _lib.F32 if out_dtype is torch.float32 else _lib.BF16)
         return k, v
 
     def attention(self, layer: int, q, *, n_keys: int, row_pos0: int, kind: str,
@@ -343,18 +359,18 @@ class PrefixKVCache:
         return out
 
     def _attention8(self, layer, q, n_keys, row_pos0, kind, mask_geometry, out_dtype):
-        data, scales, _ = self._layer(layer, q)
-        rows, hq, qdt = self._queries(q)
-        self._keys(n_keys, rows, row_pos0)
+        torch = _torch()
+        self._check(layer, q)
+        rows, hq, qdt = self._queries(q, n_keys, row_pos0)
         mk, p, b = _mask_args(kind, mask_geometry)
-        out, odt = _attention_out(q, out_dtype)
-        lib = _lib.load()
-        with _on(q):
-            ws, ws_bytes, _held = _workspace(
-                lib.drt_op_attention_kv8_workspace_bytes(rows, hq, self.kv_heads, n_keys), q)
-            _lib.check(lib.drt_op_attention_kv8(
-                _ptr(q), qdt, data, self.head_stride, scales, rows, hq, self.kv_heads, n_keys,
-                row_pos0, mk, p, b, _ptr(out), odt, ws, ws_bytes, _stream(q)))
+        out, odt = _attention_out(torch, q, rows, hq, out_dtype)
+        need = _workspace_bytes("drt_op_attention_kv8_workspace_bytes", rows, hq, self.kv_heads,
+                                n_keys)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _launch(torch, _lib.load().drt_op_attention_kv8, self._index, q.data_ptr(), qdt,
+                self._data(layer), self.head_stride, self._scales(layer), rows, hq, self.kv_heads,
+                n_keys, row_pos0, mk, p, b, out.data_ptr(), odt,
+                None if ws is None else ws.data_ptr(), need)
         return out
 
     def select_blocks(self, layer: int, q, *, block_size: int, count: int, n_keys: int,
@@ -370,21 +386,19 @@ class PrefixKVCache:
         torch = _torch()
         if self.sums is None:
             raise ValueError("select_blocks needs a cache with block_sums=True")
-        _, _, sums = self._layer(layer, q)
-        rows, hq, qdt = self._queries(q)
-        self._keys(n_keys, rows, row_pos0)
+        self._check(layer, q)
+        rows, hq, qdt = self._queries(q, n_keys, row_pos0)
         _sparse_args(block_size, count)
         if sinks < 0 or local < 1 or sinks + local > count:
             raise ValueError("select_blocks needs sinks >= 0, local >= 1, sinks + local <= count")
         mk, p, b = _mask_args(kind, mask_geometry)
         blocks = torch.empty((rows, self.kv_heads, count), dtype=torch.int32, device=q.device)
-        lib = _lib.load()
-        with _on(q):
-            ws, ws_bytes, _held = _workspace(lib.drt_op_select_blocks_workspace_bytes(
-                rows, self.kv_heads, n_keys, block_size), q)
-            _lib.check(lib.drt_op_select_blocks(
-                _ptr(q), qdt, sums, self.tiles, rows, hq, self.kv_heads, n_keys, row_pos0, mk, p,
-                b, block_size, count, sinks, local, _ptr(blocks), ws, ws_bytes, _stream(q)))
+        need = _workspace_bytes("drt_op_select_blocks_workspace_bytes", rows, self.kv_heads,
+                                n_keys, block_size)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _launch(torch, _lib.load().drt_op_select_blocks, self._index, q.data_ptr(), qdt,
+                self._sums(layer), self.tiles, rows, hq, self.kv_heads, n_keys, row_pos0, mk, p, b,
+                block_size, count, sinks, local, blocks.data_ptr(), ws.data_ptr(), need)
         return blocks
 
     def sparse_attention(self, layer: int, q, blocks, *, block_size: int, n_keys: int,
@@ -395,34 +409,32 @@ class PrefixKVCache:
         An entry that is no larger than one before it in its list, or lies beyond the row's
         keys, is passed over (so ``-1`` is none); a row without any gives zeros."""
         torch = _torch()
-        data, scales, _ = self._layer(layer, q, blocks)
-        rows, hq, qdt = self._queries(q)
-        self._keys(n_keys, rows, row_pos0)
-        if (blocks.dtype != torch.int32 or blocks.dim() != 3
-                or blocks.shape[:2] != (rows, self.kv_heads)):
+        self._check(layer, q, blocks)
+        rows, hq, qdt = self._queries(q, n_keys, row_pos0)
+        if blocks.dtype is not torch.int32 or blocks.dim() != 3:
             raise ValueError("blocks must be int32 [rows, kv_heads, count]")
-        count = blocks.shape[2]
+        br, bh, count = blocks.shape
+        if br != rows or bh != self.kv_heads:
+            raise ValueError("blocks must be int32 [rows, kv_heads, count]")
         _sparse_args(block_size, count)
         mk, p, b = _mask_args(kind, mask_geometry)
-        out, odt = _attention_out(q, out_dtype)
-        lib = _lib.load()
-        with _on(q):
-            ws, ws_bytes, _held = _workspace(lib.drt_op_sparse_attention_workspace_bytes(
-                rows, hq, self.kv_heads, block_size, count), q)
-            _lib.check(lib.drt_op_sparse_attention(
-                _ptr(q), qdt, data, self.head_stride, self.kv_dtype, scales, rows, hq,
-                self.kv_heads, n_keys, row_pos0, mk, p, b, _ptr(blocks), block_size, count,
-                _ptr(out), odt, ws, ws_bytes, _stream(q)))
+        out, odt = _attention_out(torch, q, rows, hq, out_dtype)
+        need = _workspace_bytes("drt_op_sparse_attention_workspace_bytes", rows, hq, self.kv_heads,
+                                block_size, count)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _launch(torch, _lib.load().drt_op_sparse_attention, self._index, q.data_ptr(), qdt,
+                self._data(layer), self.head_stride, self.kv_dtype, self._scales(layer), rows, hq,
+                self.kv_heads, n_keys, row_pos0, mk, p, b, blocks.data_ptr(), block_size, count,
+                out.data_ptr(), odt, None if ws is None else ws.data_ptr(), need)
         return out
 
 
-def _attention_out(q, out_dtype):
-    torch = _torch()
+def _attention_out(torch, q, rows, hq, out_dtype):
     out_dtype = out_dtype or torch.float32
-    if out_dtype not in (torch.float32, torch.bfloat16):
+    if out_dtype is not torch.float32 and out_dtype is not torch.bfloat16:
         raise ValueError("attention out must be float32 or bfloat16")
-    out = torch.empty((q.shape[0], q.shape[1] * 128), dtype=out_dtype, device=q.device)
-    return out, _lib.F32 if out_dtype == torch.float32 else _lib.BF16
+    out = torch.empty((rows, hq * 128), dtype=out_dtype, device=q.device)
+    return out, _lib.F32 if out_dtype is torch.float32 else _lib.BF16
 
 
 def _sparse_args(block_size, count):
