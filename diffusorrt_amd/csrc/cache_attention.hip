@@ -1,0 +1,756 @@
+// GQA attention over the prefix cache for gfx950: over all of an 8-bit cache's keys (kv8.h), decode
+// blocks and prompts alike, and over listed blocks of either cache's.
+//
+// Queries of one K/V head are flattened to query vectors (row, head of the group) in tiles of 32, keys
+// come in tiles of 32, and a wave computes S^T = K Q^T and O^T += V^T P^T as 32x32x16 products, as
+// the attention over a whole 16-bit cache (attention.hip) does.
+// A wave loads a tile (8 KiB of codes, 16 KiB of 16-bit values) straight into registers, 16 bytes a
+// lane and load, and makes fp16 operands of codes there: no staging, no barrier in the loop. A tile's K
+// registers are loaded anew as soon as its scores are done, its V registers after its products.
+//
+// Scales. With K = 2^a k and V = 2^b v for a tile (k, v the codes), the base-2 exponent of a
+// weighted value is u = (k . q) * 2^a * c, c = log2(e) / sqrt(128), and
+//   o = sum p v 2^b / sum p,  p = 2^u.
+// The wave keeps p' = 2^(u + b - base): its sum against v needs no factor, and the normaliser
+// adds 2^-b of a tile's sum of p'. So a tile's scales cost a few operations a lane, not one a
+// score, and p' is largest where a tile's part of the result is: fp16 holds it to 2^-11 of its value
+// wherever it counts. The running base is raised when a tile's largest u + b exceeds it by more than
+// 8 (p' <= 2^8); any base gives the same quotient. p' is the one rounding ahead of the sums
+// (to the product's operand type); scores, base, normaliser and O are fp32. The normaliser adds p'
+// before that rounding: weights on a tile of tiny values may vanish in fp16 beside others, not in it.
+// Queries over 8 bits: fp16 as they are; bf16 ones are scaled by a power of two per query vector to a
+// largest magnitude in [1, 2) (exact: fp16 has three bits more; elements below 2^-14 of the
+// vector's largest lose some, at most 2^-25 of that largest).
+//
+// Listed blocks. A query tile is the 32 / G rows (G heads a group; 32 heads at a time above that) of
+// neighbours, and the tile's blocks are the union of its rows' lists, each with a bit per row: an
+// LDS bitmap, WIN blocks at a time, so a list is a set, whatever its order and repetitions.
+// Neighbouring queries mostly choose the same blocks: a block is then loaded and made operands once
+// for all of them, and every column of the products is in use (one wave per row, 16 columns of
+// which G are used: 2048 rows x 16 heads, 16 blocks of 64 of 32768 keys, 226 us; 64 here).
+#include "kv8.h"
+#include "launch.h"
+
+#include <cmath>
+
+using drt::AttnWhere;
+
+namespace {
+
+constexpr float CA_RESCALE_LOG2 = 8.f;
+// A base beyond this is rounded by more than 2^-4: p' = 2^(fma(s, a, off - base)) would then be off by
+// that, without bound; with the exponent rounded before the base is taken off it never passes 2^8.
+constexpr float CA_LARGE = 1048576.f;
+// The bytes' 128 leaves O with the running sum of weights, at the latest after so many tiles: its
+// share of the sum in fp32, which costs O precision, stays that of 1024 keys.
+constexpr int CA_FOLD = 32;
+constexpr int CA_QROW = 136;  // 16-bit elements per query vector in LDS (+ 16 bytes)
+constexpr int CA_WIN = 2048;  // blocks of one bitmap
+
+DRT_DEV float ca_max_xor32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// What a cache's element type means to the kernel: 0 = 8-bit, 1 = fp16, 2 = bf16.
+template <int DT> struct CacheT {
+  static constexpr int TILE = DT == 0 ? KV8_TILE : 2 * KV8_TILE, LOADS = DT == 0 ? 4 : 8;
+  typedef f16x8 vec;
+  static DRT_DEV f32x16 mma(vec a, vec b, f32x16 c) { return mfma_f16(a, b, c); }
+  static DRT_DEV _Float16 weight(float p) { return (_Float16)p; }
+};
+template <> struct CacheT<2> {
+  static constexpr int TILE = 2 * KV8_TILE, LOADS = 8;
+  typedef bf16x8 vec;
+  static DRT_DEV f32x16 mma(vec a, vec b, f32x16 c) { return mfma_bf16(a, b, c); }
+  static DRT_DEV __bf16 weight(float p) { return (__bf16)p; }
+};
+// Operand i of the eight of a tile's K or V from its registers.
+template <int DT, int N> DRT_DEV typename CacheT<DT>::vec ca_operand(const u32x4 (&r)[N], int i) {
+  if constexpr (DT == 0)
+    return kv8_to_f16(r[i >> 1][2 * (i & 1)], r[i >> 1][2 * (i & 1) + 1]);
+  else
+    return __builtin_bit_cast(typename CacheT<DT>::vec, r[i]);
+}
+
+// A tile's values (16 bits) that are not finite, taken out of its V registers: in their place
+// every query column that sees one's key gets infinity or NaN in that head dim, as p * V would be, and the
+// others nothing, where 0 * V would be NaN. An indicator product for each of the three.
+template <int DT>
+DRT_DEV void ca_values_apart(u32x4 (&vr)[8], int key0, int end, int lane, f32x16 (&o)[4]) {
+  typedef CacheT<DT> T;
+  typedef typename T::vec vec;
+  constexpr uint32_t EXP = DT == 1 ? 0x7c00u : 0x7f80u, ONE = DT == 1 ? 0x3c00u : 0x3f80u;
+  vec sees[2];  // 1 for the keys of this lane's that its column sees
+#pragma unroll
+  for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      sees[kh][e] = T::weight(key0 + mfma_row(kh * 8 + e, lane) < end ? 1.f : 0.f);
+#pragma unroll 1
+  for (int kind = 0; kind < 3; ++kind) {  // NaN, +infinity, -infinity
+    const float put = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
+#pragma unroll
+    for (int hb = 0; hb < 4; ++hb) {
+      f32x16 n = f32x16{};
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh) {
+        u32x4 w = vr[hb * 2 + kh];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t y = w[e];
+          uint32_t mark = 0u;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t z = (y >> (16 * h)) & 0xffffu;
+            const bool hit = kind == 0 ? (z & 0x7fffu) > EXP : kind == 1 ? z == EXP : z == (EXP | 0x8000u);
+            mark |= hit ? ONE << (16 * h) : 0u;
+          }
+          w[e] = mark;
+        }
+        n = T::mma(__builtin_bit_cast(vec, w), sees[kh], n);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[hb][r] = n[r] > 0.f ? o[hb][r] + put : o[hb][r];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t y = vr[i][e];
+      const uint32_t keep = ((y & EXP) == EXP ? 0u : 0xffffu) | ((y & (EXP << 16)) == EXP << 16 ? 0u : 0xffff0000u);
+      vr[i][e] = y & keep;
+    }
+}
+
+struct CaArgs {
+  const uint16_t* q;       // [rows][Hq][128]
+  const uint8_t* kv;       // this layer
+  int64_t head_stride;     // bytes
+  const float* scales;     // 8-bit
+  const int32_t* blocks;   // [rows][Hkv][count] (listed blocks)
+  int q_bf16, n_rows, Hq, Hkv, splits, tiles_per_split, count, block;
+  float c;                 // log2(e) / sqrt(128), times 2^24 over 8 bits
+  AttnWhere where;
+  void* out;               // [rows][Hq * 128], bf16 or fp32
+  float* o_part;           // [splits][rows][Hq][128] (not OUT)
+  float* ml_part;          // [splits][rows][Hq][2]
+  int out_bf16;
+};
+
+// QT query tiles a wave, QW waves over query tiles, KW waves over keys (wave kw takes key
+// tiles kw, kw + KW, ...; their parts meet in LDS at the end). OUT: one key range, the
+// result itself; otherwise a part for the combine. SPARSE: the listed blocks' keys.
+template <int DT, int QT, int QW, int KW, bool OUT, bool SPARSE>
+__global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArgs x) {
+  typedef CacheT<DT> T;
+  typedef typename T::vec vec;
+  constexpr int NW = QW * KW, THREADS = 64 * NW, NQ = 32 * QT * QW, TILE = T::TILE, LD = T::LOADS;
+  static_assert(!SPARSE || (QT == 1 && QW == 1), "a work-group has one union of lists");
+  constexpr int O_BYTES = QT * 16384;  // a wave's O
+  constexpr int Q_BYTES = NQ * CA_QROW * 2, OUT_BYTES = QW * 8192;
+  constexpr int ML_BYTES = QT * 512, MRG = KW > 1 ? (NW / 2) * (O_BYTES + ML_BYTES) : 0;
+  constexpr int LDS = Q_BYTES > MRG ? (Q_BYTES > OUT_BYTES ? Q_BYTES : OUT_BYTES)
+                                    : (MRG > OUT_BYTES ? MRG : OUT_BYTES);
+  __shared__ __align__(16) char smem[LDS];
+  __shared__ float2 qinfo[NQ];  // c times a query vector's power of two; -128 * 2^-24 its sum
+  __shared__ uint32_t bits[SPARSE ? CA_WIN : 1];  // rows that list a block of the window
+  __shared__ int2 list[SPARSE ? CA_WIN : 1];      // its blocks and their rows
+  __shared__ int tally[SPARSE ? NW + 1 : 1];
+  const int lane = threadIdx.x & 63, tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int qw = wave % QW, kw = wave / QW;
+  const AttnWhere& where = x.where;
+  const int G = x.Hq / x.Hkv, kvh = blockIdx.x % x.Hkv, split = blockIdx.x / x.Hkv;
+  // the last rows, which see the most keys, start first
+  const int group = (int)gridDim.y - 1 - (int)blockIdx.y;
+
+  // The (row, head) of query vector v of the work-group.
+  const int GC = SPARSE ? min(G, 32) : G, RPT = 32 / GC;  // (listed blocks) heads and rows of a tile
+  const int head0 = SPARSE ? (int)blockIdx.z * 32 : 0, row0 = SPARSE ? group * RPT : 0;
+  const int qt0 = SPARSE ? 0 : group * (QW * QT), n_qv = x.n_rows * G;
+  auto row_of = [&](int v) { return SPARSE ? row0 + v / GC : (qt0 * 32 + v) / G; };
+  auto head_of = [&](int v) {
+    return kvh * G + (SPARSE ? head0 + v % GC : (qt0 * 32 + v) % G);
+  };
+  auto exists = [&](int v) {
+    return SPARSE ? v < RPT * GC && row0 + v / GC < x.n_rows && head0 + v % GC < G
+                  : qt0 * 32 + v < n_qv;
+  };
+
+  // queries into LDS, 16 threads (eight elements each) a query vector
+#pragma unroll
+  for (int it0 = 0; it0 < NQ * 16; it0 += THREADS) {
+    const int v = (it0 + tid) >> 4, ch = tid & 15;
+    u32x4 raw = u32x4{0u, 0u, 0u, 0u};
+    if (exists(v)) raw = *(const u32x4*)(x.q + ((int64_t)row_of(v) * x.Hq + head_of(v)) * 128 + ch * 8);
+    float pw = 1.f, sum = 0.f;
+    if constexpr (DT == 0) {
+      if (x.q_bf16) {
+        uint32_t most = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          most = max(most, max((raw[e] << 16) & 0x7fffffffu, raw[e] & 0x7fff0000u));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
+        const int ex = most ? min(max((int)(most >> 23) - 127, -126), 126) : 0;
+        pw = __uint_as_float((uint32_t)(127 + ex) << 23);
+        const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          raw[e] = pack_half2((_Float16)(__uint_as_float(raw[e] << 16) * inv),
+                              (_Float16)(__uint_as_float(raw[e] & 0xffff0000u) * inv));
+      }
+      sum = kv8_add8(__builtin_bit_cast(f16x8, raw), 0.f);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    }
+    *(u32x4*)(smem + (v * CA_QROW + ch * 8) * 2) = raw;
+    if (ch == 0) qinfo[v] = make_float2(x.c * pw, -KV8_BIAS / KV8_POW * sum);
+  }
+  __syncthreads();
+
+  const int wv0 = qw * QT * 32;  // the wave's first query vector
+  const uint16_t* ql = (const uint16_t*)smem + (wv0 + (lane & 31)) * CA_QROW + 8 * (lane >> 5);
+  constexpr bool HOLD = QT == 1;  // the queries' operands in registers
+  vec qr[HOLD ? 8 : 1];
+  if (HOLD) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) qr[HOLD ? i : 0] = *(const vec*)(ql + 16 * i);
+  }
+  int q_end[QT];
+  float cq[QT], nq[QT], m_run[QT], l_run[QT], p_run[QT];
+  f32x16 o[QT][4];
+  const int last_row = x.n_rows - 1;
+#pragma unroll
+  for (int j = 0; j < QT; ++j) {
+    const int v = wv0 + j * 32 + (lane & 31);
+    q_end[j] = key_end_of(min(row_of(v), last_row), where);
+    cq[j] = qinfo[v].x;
+    nq[j] = qinfo[v].y;
+  }
+  auto reset = [&] {
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+      m_run[j] = -INFINITY;
+      l_run[j] = p_run[j] = 0.f;
+#pragma unroll
+      for (int hb = 0; hb < 4; ++hb) o[j][hb] = f32x16{};
+    }
+  };
+  reset();
+  // (ends never fall from row to row) keys every row of the wave sees, and any of them
+  const int end_row = min(SPARSE ? row0 + RPT - 1 : row_of(wv0 + QT * 32 - 1), last_row);
+  const int wave_full = key_end_of(min(row_of(wv0), last_row), where);
+  const int wave_end = key_end_of(end_row, where);
+  const uint32_t my_row = SPARSE ? 1u << ((lane & 31) / GC & 31) : 0u;  // (32 columns at most: see exists)
+  const uint32_t all_rows = SPARSE ? (uint32_t)((1ull << (end_row - row0 + 1)) - 1) : 0u;
+
+  const uint8_t* base = x.kv + kvh * x.head_stride + lane * 16;
+  // (scalar loads: a vector load's value would be waited for with the tile in flight)
+  const auto* sc = (const __attribute__((address_space(4))) float*)(uintptr_t)(
+      DT == 0 ? x.scales + kvh * (x.head_stride / TILE) * 2 : nullptr);
+  auto scales_of = [&](int t) { return make_float2(sc[2 * (int64_t)t], sc[2 * (int64_t)t + 1]); };
+  u32x4 kr[LD], vr[LD];
+  float2 st = make_float2(1.f, 1.f);
+  int fold = CA_FOLD;
+
+  // n tiles, the first at t with its rows; next(t, rows) steps to the wave's following tile.
+  // careful (16 bits): see below.
+  auto run = [&](int n, int t, uint32_t rows, bool careful, auto&& next) {
+    if (n <= 0) return;
+    {
+      const uint8_t* p = base + (int64_t)t * TILE;
+#pragma unroll
+      for (int i = 0; i < LD; ++i) kr[i] = *(const u32x4*)(p + i * 1024);
+#pragma unroll
+      for (int i = 0; i < LD; ++i) vr[i] = *(const u32x4*)(p + TILE / 2 + i * 1024);
+      if (DT == 0) st = scales_of(t);
+    }
+    for (int it = 0; it < n; ++it) {
+      const int key0 = t * 32;
+      const uint32_t seen = rows;
+      const float sk = st.x, sv = st.y;
+      if (it + 1 < n) next(t, rows);  // (the last tile's own again: loaded, not used)
+      const uint8_t* p = base + (int64_t)t * TILE;
+      f32x16 s[QT];
+#pragma unroll
+      for (int j = 0; j < QT; ++j) s[j] = f32x16{};
+      if (!HOLD) asm volatile("" ::: "memory");  // (read the queries here, tile by tile)
+      // products ahead of another wave's softmax: 75 -> 72 us for 2048 rows over 4096 keys
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const vec kf = ca_operand<DT>(kr, i);
+#pragma unroll
+        for (int j = 0; j < QT; ++j)
+          s[j] = T::mma(kf, HOLD ? qr[HOLD ? i : 0] : *(const vec*)(ql + j * 32 * CA_QROW + 16 * i), s[j]);
+      }
+#pragma unroll
+      for (int i = 0; i < LD; ++i) kr[i] = *(const u32x4*)(p + i * 1024);
+      __builtin_amdgcn_s_setprio(0);
+      asm volatile("" ::: "memory");  // (a scalar load among the reads of LDS would be waited for with them)
+      if (DT == 0) st = scales_of(t);
+      const bool bad = DT == 0 && !(sk + sv < INFINITY);  // a NaN tile: so is every row that sees it
+      const bool part = key0 + 32 > wave_full || (SPARSE && seen != all_rows);
+      if (part || bad) {
+#pragma unroll
+        for (int j = 0; j < QT; ++j) {
+          const int mine = SPARSE && !(seen & my_row) ? 0 : q_end[j];
+          if (bad && key0 < mine) {
+            l_run[j] = NAN;
+            m_run[j] = m_run[j] == -INFINITY ? 0.f : m_run[j];
+          }
+          const int end = bad ? 0 : mine;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[j][r] = key0 + mfma_row(r, lane) < end ? s[j][r] : -INFINITY;
+        }
+      }
+      const float lb = DT != 0 || bad ? 0.f : (float)((int)(__float_as_uint(sv) >> 23) - 127);  // sv = 2^lb
+      const float inv_sv = DT != 0 ? 1.f : bad ? 0.f : __uint_as_float((254u << 23) - __float_as_uint(sv));
+      vec pf[QT][2];
+#pragma unroll
+      for (int j = 0; j < QT; ++j) {
+        // (within the finite numbers above zero whatever the powers of two: no 0 * inf)
+        float a = DT != 0 ? cq[j] : bad ? 1.f : __builtin_amdgcn_fmed3f(sk * cq[j], 1e-37f, 3e38f);
+        float tmax = s[j][0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, s[j][r]);
+        const float off0 = DT != 0 ? 0.f : fmaf(nq[j], a, lb);
+        const float u = fmaf(ca_max_xor32(tmax), a, off0);  // -inf: no visible key in the tile
+        const bool up = u > m_run[j] + CA_RESCALE_LOG2;
+        if (__ballot(up) || (DT == 0 && fold == 1)) {
+          const float alpha = up ? __builtin_amdgcn_exp2f(m_run[j] - u) : 1.f;  // 0 from -inf
+          const float less = DT != 0 ? 0.f
+                                     : alpha * (-KV8_BIAS / KV8_POW) *
+                                           (p_run[j] + __shfl_xor(p_run[j], 32, 64));
+#pragma unroll
+          for (int hb = 0; hb < 4; ++hb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              o[j][hb][r] = DT == 0 ? fmaf(o[j][hb][r], alpha, less) : o[j][hb][r] * alpha;
+          l_run[j] *= alpha;
+          p_run[j] = 0.f;
+          m_run[j] = up ? u : m_run[j];
+        }
+        const float mb = m_run[j] == -INFINITY ? 0.f : m_run[j];
+        float off = off0 - mb;
+        if (__ballot(fabsf(mb) > CA_LARGE)) {  // exponents rounded as the base was
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[j][r] = fmaf(s[j][r], a, off0);
+          a = 1.f;
+          off = -mb;
+        }
+        float psum = 0.f;
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float w = __builtin_amdgcn_exp2f(fmaf(s[j][kh * 8 + e], a, off));
+            psum += w;
+            pf[j][kh][e] = T::weight(w);
+          }
+        if constexpr (DT == 0) p_run[j] = kv8_add8(pf[j][1], kv8_add8(pf[j][0], p_run[j]));
+        l_run[j] = fmaf(psum, inv_sv, l_run[j]);
+      }
+      fold = fold == 1 ? CA_FOLD : fold - 1;
+      if constexpr (DT != 0) {
+        if (careful && part) {
+          const int mine = SPARSE && !(seen & my_row) ? 0 : q_end[0];
+          ca_values_apart<DT>(vr, key0, mine, lane, o[0]);
+        }
+      }
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int hb = 0; hb < 4; ++hb)
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh) {
+          const vec vf = ca_operand<DT>(vr, hb * 2 + kh);
+#pragma unroll
+          for (int j = 0; j < QT; ++j) o[j][hb] = T::mma(vf, pf[j][kh], o[j][hb]);
+        }
+#pragma unroll
+      for (int i = 0; i < LD; ++i) vr[i] = *(const u32x4*)(p + TILE / 2 + i * 1024);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+
+  if constexpr (!SPARSE) {
+    const int n_tiles = (where.n_keys + 31) >> 5, t0 = split * x.tiles_per_split + kw;
+    const int t_end = !exists(wv0) ? 0
+                                   : min(min(n_tiles, (split + 1) * x.tiles_per_split), (wave_end + 31) >> 5);
+    run((t_end - t0 + KW - 1) / KW, t0, 0u, false, [&](int& t, uint32_t&) { t += KW; });
+  } else {
+    const int m = x.block >> 5, n_blocks = (int)(((int64_t)wave_end + x.block - 1) / x.block);
+    const int step_e = KW / m, step_r = KW % m;
+    // 16 bits: a V that is not finite makes 0 * V of a row that does not see it NaN too. Rows
+    // are looked at afterwards, and only if some are not finite is it all done again with care.
+    bool careful = false;
+    for (;;) {
+      for (int w0 = 0; w0 < n_blocks; w0 += CA_WIN) {
+        const int n_win = min(CA_WIN, n_blocks - w0);
+        __syncthreads();  // the window before has been read
+        for (int i = tid; i < n_win; i += THREADS) bits[i] = 0u;
+        __syncthreads();
+        const int n_entries = (end_row - row0 + 1) * x.count;
+        for (int i = tid; i < n_entries; i += THREADS) {
+          const int r = i / x.count;
+          const int b = x.blocks[((int64_t)(row0 + r) * x.Hkv + kvh) * x.count + (i - r * x.count)];
+          if (b >= w0 && b < w0 + n_win && (int64_t)b * x.block < key_end_of(row0 + r, where))
+            atomicOr(&bits[b - w0], 1u << r);
+        }
+        __syncthreads();
+        // the window's blocks in order: wave w finds those of its share, then all take their places
+        constexpr int SHARE = CA_WIN / NW;
+        int found = 0;
+        for (int i = wave * SHARE; i < min(n_win, (wave + 1) * SHARE); i += 64)
+          found += __popcll(__ballot(i + lane < n_win && bits[min(i + lane, CA_WIN - 1)] != 0u));
+        if (lane == 0) tally[wave] = found;
+        __syncthreads();
+        int at = 0, n_list = 0;
+        for (int w = 0; w < NW; ++w) {
+          at += w < wave ? tally[w] : 0;
+          n_list += tally[w];
+        }
+        for (int i = wave * SHARE; i < min(n_win, (wave + 1) * SHARE); i += 64) {
+          const uint32_t b = i + lane < n_win ? bits[min(i + lane, CA_WIN - 1)] : 0u;
+          const uint64_t hit = __ballot(b != 0u);
+          if (b) list[at + __popcll(hit & ((1ull << lane) - 1))] = make_int2(w0 + i + lane, (int)b);
+          at += __popcll(hit);
+        }
+        __syncthreads();
+        n_list = __builtin_amdgcn_readfirstlane(n_list);
+        if (n_list > 0) {
+          // tiles in all (of the last block those that the rows see), and this range's
+          const int last = __builtin_amdgcn_readfirstlane(list[n_list - 1].x);
+          const int64_t n = (int64_t)(n_list - 1) * m + min((int64_t)m, ((wave_end + 31) >> 5) - (int64_t)last * m);
+          const int j0 = (int)(n * split / x.splits) + kw, j1 = (int)(n * (split + 1) / x.splits);
+          int e = j0 / m, r = j0 - e * m;
+          auto here = [&](int& t, uint32_t& rows) {
+            const int2 b = list[min(e, n_list - 1)];
+            t = __builtin_amdgcn_readfirstlane(b.x) * m + r;
+            rows = (uint32_t)__builtin_amdgcn_readfirstlane(b.y);
+          };
+          int t = 0;
+          uint32_t rows = 0u;
+          if (j0 < j1) here(t, rows);
+          run((j1 - j0 + KW - 1) / KW, t, rows, careful, [&](int& t2, uint32_t& rows2) {
+            e += step_e;
+            r += step_r;
+            if (r >= m) {
+              r -= m;
+              ++e;
+            }
+            here(t2, rows2);
+          });
+        }
+      }
+      if (DT == 0 || careful) break;
+      bool odd = false;
+#pragma unroll
+      for (int hb = 0; hb < 4; ++hb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) odd = odd || !(fabsf(o[0][hb][r]) < INFINITY);
+      if (!__syncthreads_or(odd)) break;
+      careful = true;
+      reset();
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < QT; ++j) {
+    l_run[j] += __shfl_xor(l_run[j], 32, 64);
+    if (DT == 0) {
+      p_run[j] += __shfl_xor(p_run[j], 32, 64);
+#pragma unroll
+      for (int hb = 0; hb < 4; ++hb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[j][hb][r] = fmaf(o[j][hb][r], KV8_POW, -KV8_BIAS * p_run[j]);
+    }
+  }
+
+  // the key ways of a wave's queries in pairs
+  if (KW > 1) {
+#pragma unroll
+    for (int half = KW / 2; half > 0; half >>= 1) {
+      __syncthreads();  // the queries, or the round before, have been read
+      if (kw >= half && kw < 2 * half) {
+        char* d = smem + ((kw - half) * QW + qw) * (O_BYTES + ML_BYTES);
+#pragma unroll
+        for (int j = 0; j < QT; ++j) {
+#pragma unroll
+          for (int hb = 0; hb < 4; ++hb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              ((f32x4*)d)[(j * 16 + hb * 4 + r) * 64 + lane] =
+                  f32x4{o[j][hb][4 * r], o[j][hb][4 * r + 1], o[j][hb][4 * r + 2], o[j][hb][4 * r + 3]};
+          ((float2*)(d + O_BYTES))[j * 64 + lane] = make_float2(m_run[j], l_run[j]);
+        }
+      }
+      __syncthreads();
+      if (kw < half) {
+        const char* d = smem + (kw * QW + qw) * (O_BYTES + ML_BYTES);
+#pragma unroll
+        for (int j = 0; j < QT; ++j) {
+          const float2 ml = ((const float2*)(d + O_BYTES))[j * 64 + lane];
+          const float mm = fmaxf(m_run[j], ml.x);
+          const float w0 = m_run[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[j] - mm);
+          const float w1 = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mm);
+#pragma unroll
+          for (int hb = 0; hb < 4; ++hb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const f32x4 y = ((const f32x4*)d)[(j * 16 + hb * 4 + r) * 64 + lane];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                o[j][hb][4 * r + e] = fmaf(w1, y[e], w0 * o[j][hb][4 * r + e]);
+            }
+          l_run[j] = fmaf(w1, ml.y, w0 * l_run[j]);
+          m_run[j] = mm;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (kw > 0) return;  // (no barrier follows)
+  // Rows out: half a query tile's O^T (64 head dims) at a time through 8 KiB of the wave's own, as 16-byte
+  // pieces (query v, piece p at p ^ v: every bank in turn both ways), eight lanes a query vector.
+  f32x4* ot = (f32x4*)(smem + qw * 8192);
+#pragma unroll
+  for (int jh = 0; jh < 2 * QT; ++jh) {
+    const int j = jh >> 1, hf = jh & 1;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        ot[(lane & 31) * 16 + ((b * 8 + 2 * r + (lane >> 5)) ^ (lane & 15))] =
+            f32x4{o[j][2 * hf + b][4 * r], o[j][2 * hf + b][4 * r + 1], o[j][2 * hf + b][4 * r + 2],
+                  o[j][2 * hf + b][4 * r + 3]};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int v = (lane >> 3) + 8 * i, ch = lane & 7, wv = wv0 + j * 32 + v;
+      const float m = __shfl(m_run[j], v, 64), l = __shfl(l_run[j], v, 64);
+      f32x4 y0 = ot[v * 16 + ((2 * ch) ^ (v & 15))], y1 = ot[v * 16 + ((2 * ch + 1) ^ (v & 15))];
+      if (!exists(wv)) continue;
+      const int64_t rh = (int64_t)row_of(wv) * x.Hq + head_of(wv);
+      const int64_t at = rh * 128 + hf * 64 + ch * 8;
+      if (OUT) {
+        const float inv = SPARSE && l == 0.f ? 0.f : 1.f / l;  // no key: zeros
+        y0 *= inv;
+        y1 *= inv;
+        if (x.out_bf16) {
+          u32x4 w;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            w[e] = (uint32_t)float_to_bf16_bits(y0[2 * e]) |
+                   ((uint32_t)float_to_bf16_bits(y0[2 * e + 1]) << 16);
+            w[2 + e] = (uint32_t)float_to_bf16_bits(y1[2 * e]) |
+                       ((uint32_t)float_to_bf16_bits(y1[2 * e + 1]) << 16);
+          }
+          *(u32x4*)((uint16_t*)x.out + at) = w;
+        } else {
+          *(f32x4*)((float*)x.out + at) = y0;
+          *(f32x4*)((float*)x.out + at + 4) = y1;
+        }
+      } else {
+        const int64_t n = (int64_t)x.n_rows * x.Hq;
+        *(f32x4*)(x.o_part + split * n * 128 + at) = y0;
+        *(f32x4*)(x.o_part + split * n * 128 + at + 4) = y1;
+        if (hf == 0 && ch == 0) *(float2*)(x.ml_part + (split * n + rh) * 2) = make_float2(m, l);
+      }
+    }
+  }
+}
+
+// The key ranges of a (row, head) joined, one wave each: lane (sg, ch) adds head dims 8 ch .. + 8 of ranges sg,
+// sg + 4, ..., all of a batch's loads before their use, and the four groups meet by lane exchanges.
+// A row without a key gives zeros.
+__global__ __launch_bounds__(128) void part_combine_kernel(const float* __restrict__ o_part,
+                                                           const float* __restrict__ ml_part,
+                                                           int splits, int64_t n,
+                                                           void* __restrict__ out, int bf16) {
+  const int64_t id = blockIdx.x * (int64_t)2 + (threadIdx.x >> 6);
+  if (id >= n) return;
+  const int lane = threadIdx.x & 63, ch = lane & 15, sg = lane >> 4;
+  constexpr int SB = 4;
+  float m = -INFINITY, l = 0.f;
+  f32x4 a0 = f32x4{}, a1 = f32x4{};
+  for (int s0 = sg; s0 < splits; s0 += 4 * SB) {
+    float2 ml[SB];
+    f32x4 p0[SB], p1[SB];
+#pragma unroll
+    for (int j = 0; j < SB; ++j) {
+      const int64_t at = (int64_t)min(s0 + 4 * j, splits - 1) * n + id;
+      ml[j] = *(const float2*)(ml_part + at * 2);
+      p0[j] = *(const f32x4*)(o_part + at * 128 + 8 * ch);
+      p1[j] = *(const f32x4*)(o_part + at * 128 + 8 * ch + 4);
+    }
+    float mb = m;
+#pragma unroll
+    for (int j = 0; j < SB; ++j) {
+      if (s0 + 4 * j >= splits) ml[j] = make_float2(-INFINITY, 0.f);
+      mb = fmaxf(mb, ml[j].x);
+    }
+    const float sc = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mb);
+    a0 *= sc;
+    a1 *= sc;
+    l *= sc;
+#pragma unroll
+    for (int j = 0; j < SB; ++j) {
+      const float w = ml[j].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[j].x - mb);
+      a0 += w * p0[j];
+      a1 += w * p1[j];
+      l = fmaf(w, ml[j].y, l);
+    }
+    m = mb;
+  }
+  const float mm = fmaxf(fmaxf(m, __shfl_xor(m, 16, 64)), fmaxf(__shfl_xor(m, 32, 64), __shfl_xor(m, 48, 64)));
+  const float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm);
+  a0 *= w;
+  a1 *= w;
+  l *= w;
+#pragma unroll
+  for (int o = 16; o < 64; o <<= 1) {
+    l += __shfl_xor(l, o, 64);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a0[e] += __shfl_xor(a0[e], o, 64);
+      a1[e] += __shfl_xor(a1[e], o, 64);
+    }
+  }
+  if (sg) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  a0 *= inv;
+  a1 *= inv;
+  const int64_t at = id * 128 + 8 * ch;
+  if (bf16) {
+    u32x4 y;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      y[e] = (uint32_t)float_to_bf16_bits(a0[2 * e]) | ((uint32_t)float_to_bf16_bits(a0[2 * e + 1]) << 16);
+      y[2 + e] =
+          (uint32_t)float_to_bf16_bits(a1[2 * e]) | ((uint32_t)float_to_bf16_bits(a1[2 * e + 1]) << 16);
+    }
+    *(u32x4*)((uint16_t*)out + at) = y;
+  } else {
+    *(f32x4*)((float*)out + at) = a0;
+    *(f32x4*)((float*)out + at + 4) = a1;
+  }
+}
+
+}  // namespace
+
+namespace drt {
+
+void part_combine(const float* o_part, const float* ml_part, int splits, int64_t n, void* out,
+                  bool bf16, hipStream_t s) {
+  hipLaunchKernelGGL(part_combine_kernel, dim3((unsigned)((n + 1) / 2)), dim3(128), 0, s, o_part,
+                     ml_part, splits, n, out, (int)bf16);
+  DRT_HIP(hipGetLastError());
+}
+
+CachePlan plan_attention8(int n_rows, int Hq, int Hkv, int n_keys) {
+  CachePlan p;
+  const int64_t qtiles = ((int64_t)n_rows * (Hq / Hkv) + 31) / 32;
+  // Many queries: two query tiles a wave (a tile's codes made operands once for both), four key
+  // ways in a work-group of their own, so that work-groups are as many as can be (2048 rows x 16
+  // heads over 4096 keys: 72 us; two and one key ways, which need key ranges to fill the chip:
+  // 101, 110). Few: eight waves over the one, two or four query tiles.
+  p.wide = qtiles > 4;
+  p.qw = p.wide || qtiles == 1 ? 1 : qtiles == 2 ? 2 : 4;
+  const int kw = p.wide ? 4 : 8 / p.qw, per = p.wide ? 2 : p.qw;  // (query tiles of a work-group)
+  p.groups = (qtiles + per - 1) / per;
+  const int n_tiles = (int)(((int64_t)n_keys + 31) / 32);
+  const int64_t wgs = Hkv * p.groups;
+  int64_t splits = std::max<int64_t>(1, (p.wide ? 512 : 256) / wgs);
+  splits = std::min<int64_t>({splits, (n_tiles + kw - 1) / kw, 64});
+  p.tiles_per_split = (int)((n_tiles + splits - 1) / splits);
+  p.splits = (n_tiles + p.tiles_per_split - 1) / p.tiles_per_split;
+  return p;
+}
+
+CachePlan plan_sparse(int n_rows, int Hq, int Hkv, int count, int block) {
+  CachePlan p;
+  const int G = Hq / Hkv, rows = 32 / std::min(G, 32), heads = (G + 31) / 32;
+  p.groups = ((int64_t)n_rows + rows - 1) / rows;
+  // Few work-groups: as many key ranges as give every CU one (of a list's tiles, eight at least)
+  const int64_t wgs = p.groups * Hkv * heads, tiles = (int64_t)count * (block / 32);
+  p.wide = wgs >= 512;
+  p.splits = p.wide ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({256 / wgs, (tiles + 7) / 8, 64}));
+  return p;
+}
+
+size_t cache_part_bytes(const CachePlan& p, int n_rows, int Hq) {
+  return p.splits == 1 ? 0 : (size_t)p.splits * n_rows * Hq * 130 * 4;
+}
+
+static CaArgs args_of(KvType type, const void* q, bool q_bf16, const void* kv_layer,
+                      int64_t kv_head_stride, const float* scales, int n_rows, int Hq, int Hkv,
+                      const AttnWhere& where, const CachePlan& p, float* part, void* out,
+                      bool out_bf16) {
+  CaArgs a{};
+  a.q = (const uint16_t*)q;
+  a.kv = (const uint8_t*)kv_layer;
+  a.head_stride = type == KvType::I8 ? kv_head_stride : 2 * kv_head_stride;
+  a.scales = scales;
+  a.q_bf16 = q_bf16;
+  a.n_rows = n_rows;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.splits = p.splits;
+  a.tiles_per_split = p.tiles_per_split;
+  a.block = 32;
+  a.c = 1.44269504088896340736f / sqrtf(128.0f) * (type == KvType::I8 ? KV8_POW : 1.f);
+  a.where = where;
+  a.out = out;
+  a.o_part = part;
+  a.ml_part = part ? part + (size_t)p.splits * n_rows * Hq * 128 : nullptr;
+  a.out_bf16 = out_bf16;
+  return a;
+}
+
+#define DRT_CA(DT, QT, QW, KW, SPARSE)                                                            \
+  do {                                                                                            \
+    if (p.splits == 1)                                                                            \
+      hipLaunchKernelGGL((cache_attn_kernel<DT, QT, QW, KW, true, SPARSE>), grid, dim3(64 * QW * KW), 0, s, a); \
+    else                                                                                          \
+      hipLaunchKernelGGL((cache_attn_kernel<DT, QT, QW, KW, false, SPARSE>), grid, dim3(64 * QW * KW), 0, s, a); \
+  } while (0)
+
+void attention8(const void* q, bool q_bf16, const void* kv_layer, int64_t kv_head_stride,
+                const float* scales, int n_rows, int Hq, int Hkv, const AttnWhere& where,
+                const CachePlan& p, float* part, void* out, bool out_bf16, hipStream_t s) {
+  const CaArgs a = args_of(KvType::I8, q, q_bf16, kv_layer, kv_head_stride, scales, n_rows, Hq, Hkv,
+                           where, p, part, out, out_bf16);
+  const dim3 grid((unsigned)(p.splits * Hkv), (unsigned)p.groups);
+  if (p.wide) DRT_CA(0, 2, 1, 4, false);
+  else if (p.qw == 1) DRT_CA(0, 1, 1, 8, false);
+  else if (p.qw == 2) DRT_CA(0, 1, 2, 4, false);
+  else DRT_CA(0, 1, 4, 2, false);
+  DRT_HIP(hipGetLastError());
+  if (p.splits > 1) part_combine(part, a.ml_part, p.splits, (int64_t)n_rows * Hq, out, out_bf16, s);
+}
+
+void sparse_attention(KvType type, const void* q, bool q_bf16, const void* kv_layer,
+                      int64_t kv_head_stride, const float* scales, int n_rows, int Hq, int Hkv,
+                      const AttnWhere& where, const int32_t* blocks, int count, int block,
+                      const CachePlan& p, float* part, void* out, bool out_bf16, hipStream_t s) {
+  CaArgs a = args_of(type, q, q_bf16, kv_layer, kv_head_stride, scales, n_rows, Hq, Hkv, where, p,
+                     part, out, out_bf16);
+  a.blocks = blocks;
+  a.count = count;
+  a.block = block;
+  const dim3 grid((unsigned)(p.splits * Hkv), (unsigned)p.groups, (unsigned)((Hq / Hkv + 31) / 32));
+#define DRT_SP(DT)                                                                                \
+  do { if (p.wide) DRT_CA(DT, 1, 1, 4, true); else DRT_CA(DT, 1, 1, 8, true); } while (0)
+  if (type == KvType::I8) DRT_SP(0);
+  else if (type == KvType::F16) DRT_SP(1);
+  else DRT_SP(2);
+#undef DRT_SP
+  DRT_HIP(hipGetLastError());
+  if (p.splits > 1) part_combine(part, a.ml_part, p.splits, (int64_t)n_rows * Hq, out, out_bf16, s);
+}
+#undef DRT_CA
+
+}  // namespace drt

@@ -219,15 +219,19 @@ void kv_load(KvType type, const void* kv, int64_t head_stride, const float* scal
              int pos0, void* k, void* v, bool out_bf16, hipStream_t s);
 void kv_sums(bool bf16, const void* kv, int64_t head_stride, int Hkv, int pos0, int n, float* sums,
              hipStream_t s);
-struct Attn8Plan {
-  int qw = 1, kw = 8, qgroups = 1, splits = 1, tiles_per_split = 1;
-  bool wide = false;  // two query tiles a wave
+// How an attention over the cache is cut: key ranges (splits), whose parts are joined by a second
+// launch, and work-groups of query tiles.
+struct CachePlan {
+  int qw = 1, splits = 1, tiles_per_split = 1;
+  int64_t groups = 1;
+  bool wide = false;
 };
-Attn8Plan plan_attention8(int n_rows, int Hq, int Hkv, int n_keys);
-size_t attention8_part_bytes(const Attn8Plan& p, int n_rows, int Hq);
+CachePlan plan_attention8(int n_rows, int Hq, int Hkv, int n_keys);
+CachePlan plan_sparse(int n_rows, int Hq, int Hkv, int count, int block);
+size_t cache_part_bytes(const CachePlan& p, int n_rows, int Hq);
 void attention8(const void* q, bool q_bf16, const void* kv_layer, int64_t kv_head_stride,
                 const float* scales, int n_rows, int Hq, int Hkv, const AttnWhere& where,
-                const Attn8Plan& p, float* part, void* out, bool out_bf16, hipStream_t s);
+                const CachePlan& p, float* part, void* out, bool out_bf16, hipStream_t s);
 
 // Block-sparse attention over either cache. Blocks are `block` keys (a multiple of 32).
 struct SparseSel {
@@ -237,12 +241,10 @@ size_t select_blocks_bytes(int n_rows, int Hkv, int n_keys, int block);
 void select_blocks(const void* q, bool q_bf16, const float* sums, int64_t sums_head_stride,
                    int n_rows, int Hq, int Hkv, const AttnWhere& where, const SparseSel& sel,
                    void* workspace, int32_t* blocks, hipStream_t s);
-int sparse_splits(int n_rows, int Hq, int Hkv, int count, int block);
-size_t sparse_part_bytes(int n_rows, int Hq, int splits);
 void sparse_attention(KvType type, const void* q, bool q_bf16, const void* kv_layer,
                       int64_t kv_head_stride, const float* scales, int n_rows, int Hq, int Hkv,
                       const AttnWhere& where, const int32_t* blocks, int count, int block,
-                      int splits, float* part, void* out, bool out_bf16, hipStream_t s);
+                      const CachePlan& p, float* part, void* out, bool out_bf16, hipStream_t s);
 
 // Epilogues.
 // rot (optional): receives the XCD rotation of the launch (see probe_round_robin).

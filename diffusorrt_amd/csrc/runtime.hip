@@ -2855,7 +2855,7 @@ int32_t drt_op_kv_load(const void* cache, int64_t head_stride, int32_t kv_dtype,
 
 size_t drt_op_attention_kv8_workspace_bytes(int32_t rows, int32_t hq, int32_t hkv, int32_t n_keys) {
   if (rows <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || n_keys <= 0) return 0;
-  return attention8_part_bytes(plan_attention8(rows, hq, hkv, n_keys), rows, hq);
+  return cache_part_bytes(plan_attention8(rows, hq, hkv, n_keys), rows, hq);
 }
 
 int32_t drt_op_attention_kv8(const void* q, int32_t q_dtype, const void* cache, int64_t head_stride,
@@ -2872,11 +2872,11 @@ int32_t drt_op_attention_kv8(const void* q, int32_t q_dtype, const void* cache, 
     require_kv(cache, head_stride, scales, DRT_I8, n_keys, "attention_kv8");
     const bool qb = q_is_bf16(q_dtype, DRT_I8, q, "attention_kv8");
     require_out(out, out_dtype, "attention_kv8");
-    const Attn8Plan p = plan_attention8(rows, hq, hkv, n_keys);
-    require(p.qgroups <= 65535 && (int64_t)p.splits * hkv < (1ll << 31) &&
+    const CachePlan p = plan_attention8(rows, hq, hkv, n_keys);
+    require(p.groups <= 65535 && (int64_t)p.splits * hkv < (1ll << 31) &&
                 (int64_t)rows * (hq / hkv) < INT32_MAX - 512,
             "attention_kv8: too many rows for one call");
-    const size_t need = attention8_part_bytes(p, rows, hq);
+    const size_t need = cache_part_bytes(p, rows, hq);
     require(workspace_bytes >= need && (workspace || !need) && ((uintptr_t)workspace & 15) == 0,
             "attention_kv8 workspace too small or not 16-byte aligned");
     attention8(q, qb, cache, head_stride, scales, rows, hq, hkv, where, p,
@@ -2921,7 +2921,7 @@ int32_t drt_op_select_blocks(const void* q, int32_t q_dtype, const float* sums, 
 size_t drt_op_sparse_attention_workspace_bytes(int32_t rows, int32_t hq, int32_t hkv,
                                                int32_t block_size, int32_t count) {
   if (!sparse_shape_ok(rows, hq, hkv, block_size, count)) return 0;
-  return sparse_part_bytes(rows, hq, sparse_splits(rows, hq, hkv, count, block_size));
+  return cache_part_bytes(plan_sparse(rows, hq, hkv, count, block_size), rows, hq);
 }
 
 int32_t drt_op_sparse_attention(const void* q, int32_t q_dtype, const void* cache,
@@ -2940,12 +2940,14 @@ int32_t drt_op_sparse_attention(const void* q, int32_t q_dtype, const void* cach
     require_kv(cache, head_stride, scales, kv_dtype, n_keys, "sparse_attention");
     const bool qb = q_is_bf16(q_dtype, kv_dtype, q, "sparse_attention");
     require_out(out, out_dtype, "sparse_attention");
-    const int splits = sparse_splits(rows, hq, hkv, count, block_size);
-    const size_t need = sparse_part_bytes(rows, hq, splits);
+    const CachePlan p = plan_sparse(rows, hq, hkv, count, block_size);
+    require(p.groups <= 65535 && hq / hkv <= 65535 && (int64_t)p.splits * hkv < (1ll << 31),
+            "sparse_attention: too many rows for one call");
+    const size_t need = cache_part_bytes(p, rows, hq);
     require(workspace_bytes >= need && (workspace || !need) && ((uintptr_t)workspace & 15) == 0,
             "sparse_attention workspace too small or not 16-byte aligned");
     sparse_attention(type, q, qb, cache, head_stride, scales, rows, hq, hkv, where, blocks, count,
-                     block_size, splits, need ? (float*)workspace : nullptr, out,
+                     block_size, p, need ? (float*)workspace : nullptr, out,
                      out_dtype == DRT_BF16, as_stream(stream));
   });
 }

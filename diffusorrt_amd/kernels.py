@@ -406,8 +406,8 @@ class PrefixKVCache:
         """:meth:`attention` over the keys of ``blocks`` (int32 ``[rows, kv_heads, count]``, as
         :meth:`select_blocks` gives them or a caller's own) that the row sees.
 
-        An entry that is no larger than one before it in its list, or lies beyond the row's
-        keys, is passed over (so ``-1`` is none); a row without any gives zeros."""
+        A list is a set: its order and repetitions do not matter, entries beyond the row's keys
+        and negative ones are none; a row without any block gives zeros."""
         torch = _torch()
         self._check(layer, q, blocks)
         rows, hq, qdt = self._queries(q, n_keys, row_pos0)

@@ -341,9 +341,10 @@ int32_t drt_op_select_blocks(const void* q, int32_t q_dtype, const float* sums, 
                              int32_t mask_block_size, int32_t block_size, int32_t count,
                              int32_t sinks, int32_t local, int32_t* blocks, void* workspace,
                              size_t workspace_bytes, void* stream);
-/* drt_op_attention (or _kv8) over the listed blocks' keys only, blocks [rows, hkv, count] of any origin:
- * an entry that is no larger than one before it, or beyond the row's keys, is passed over; a row
- * without any is zeros. q: fp16 or bf16 over DRT_I8, else of the cache's type. */
+/* drt_op_attention (or _kv8) over the listed blocks' keys only, blocks [rows, hkv, count] of any
+ * origin: a list is a set (its order and repetitions do not matter), entries beyond the row's keys and
+ * negative ones are none, a row without any block is zeros. q: fp16 or bf16 over DRT_I8, else of the
+ * cache's type. */
 size_t drt_op_sparse_attention_workspace_bytes(int32_t rows, int32_t hq, int32_t hkv,
                                                int32_t block_size, int32_t count);
 int32_t drt_op_sparse_attention(const void* q, int32_t q_dtype, const void* cache,

@@ -106,12 +106,7 @@ def attention(q, k, v, ends, blocks=None, block: int = 0):
             kv = h // (hq // hkv)
             keys = np.arange(ends[r])
             if blocks is not None:
-                listed, top = [], -1
-                for b in blocks[r, kv]:
-                    if b > top:
-                        listed.append(b)
-                        top = b
-                keys = keys[np.isin(keys // block, listed)]
+                keys = keys[np.isin(keys // block, blocks[r, kv])]  # (a list is a set)
             if not len(keys):
                 continue
             s = k[keys, kv] @ q[r, h] * 128 ** -0.5

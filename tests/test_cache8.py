@@ -65,11 +65,11 @@ def test_select_takes_forced_blocks_then_scores_then_lower_blocks():
     assert got[2, 0].tolist() == [0, 2, 3, 7]  # 7 ties 2, 3 and 5: the lower two
 
 
-def test_an_entry_no_larger_than_one_before_counts_once():
+def test_a_list_is_a_set():
     rng = np.random.default_rng(4)
     q, k, v = rng.standard_normal((1, 1, 128)), *rng.standard_normal((2, 128, 1, 128))
     ends = np.array([100])
-    a = X.attention(q, k, v, ends, np.array([[[1, 1, 0, 3, 3, 2]]]), 32)[0]
+    a = X.attention(q, k, v, ends, np.array([[[3, 1, 1, -5, 3, 9]]]), 32)[0]
     b = X.attention(q, k, v, ends, np.array([[[1, 3]]]), 32)[0]
     assert np.array_equal(a, b)
     assert not X.attention(q, k, v, ends, np.array([[[-1, 4, 9]]]), 32)[0].any()
@@ -115,7 +115,7 @@ def _select(**kw):
 def _sparse(**kw):
     a = dict(q=P, qdt=_lib.F16, cache=P, stride=8192 * 4, dtype=_lib.I8, scales=P, rows=8, hq=4,
              hkv=2, n_keys=128, pos0=0, mask=_lib.MASK_D2F_HYBRID, prompt=0, block=32, blocks=P,
-             size=32, count=4, out=P, odt=_lib.F32, ws=P, ws_bytes=1 << 40, stream=None) | kw
+             size=32, count=64, out=P, odt=_lib.F32, ws=P, ws_bytes=1 << 40, stream=None) | kw
     return "drt_op_sparse_attention", list(a.values())
 
 
