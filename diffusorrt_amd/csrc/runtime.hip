@@ -2910,8 +2910,9 @@ int32_t drt_op_select_blocks(const void* q, int32_t q_dtype, const float* sums, 
                                      mask_block_size, "select_blocks");
     require(q_dtype == DRT_F16 || q_dtype == DRT_BF16, "select_blocks q must be F16 or BF16");
     require((n_keys + 31) / 32 <= sums_tiles, "select_blocks n_keys exceed the sums");
-    require(workspace && ((uintptr_t)workspace & 7) == 0 &&
-                workspace_bytes >= select_blocks_bytes(rows, hkv, n_keys, block_size),
+    require(((uintptr_t)q & 15) == 0, "select_blocks q must be 16-byte aligned");
+    const size_t need = select_blocks_bytes(rows, hkv, n_keys, block_size);
+    require((workspace || !need) && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= need,
             "select_blocks workspace too small or not 8-byte aligned");
     select_blocks(q, q_dtype == DRT_BF16, sums, sums_tiles * 128, rows, hq, hkv, where,
                   SparseSel{block_size, count, sinks, local}, workspace, blocks, as_stream(stream));

@@ -31,78 +31,100 @@ DRT_DEV uint64_t score_key(double x) {
   return b >> 63 ? ~b : b | (1ull << 63);
 }
 
-// Scores of 16 rows against 64 blocks of one K/V head: thread (b, r) holds block b of rows 4r ..
-// 4r + 3, the queries' and the blocks' sums meet in LDS in 64 bits, 32 head dims at a time.
-// Grid: (row group * chunks + chunk) * Hkv + head.
-constexpr int SEL_ROWS = 16, SEL_BLOCKS = 64, SEL_DIMS = 32;
-__global__ __launch_bounds__(256) void block_scores_kernel(
-    const uint16_t* __restrict__ q, int q_bf16, const float* __restrict__ sums,
-    int64_t sums_head_stride, int row0, int n_rows, int Hq, int Hkv, const AttnWhere where,
-    const SparseSel sel, int n_blocks, uint64_t* __restrict__ keys) {
-  const int kvh = blockIdx.x % Hkv, rest = blockIdx.x / Hkv;
-  const int chunks = (n_blocks + SEL_BLOCKS - 1) / SEL_BLOCKS;
-  const int chunk = rest % chunks, r0 = (rest / chunks) * SEL_ROWS;
-  const int G = Hq / Hkv, tid = threadIdx.x, m = sel.block >> 5;
-  // the last row of the group sees the most: blocks at or beyond its last `local` are never scored
-  const int rows = min(SEL_ROWS, n_rows - r0);
-  const int scored = (key_end_of(row0 + r0 + rows - 1, where) + sel.block - 1) / sel.block - sel.local;
-  const int b0 = chunk * SEL_BLOCKS;
-  if (b0 >= scored) return;
-  __shared__ double qs[SEL_ROWS][SEL_DIMS];
-  __shared__ double bs[SEL_DIMS][SEL_BLOCKS + 1];
-  const int lb = tid & 63, lr = (tid >> 6) * 4;
-  double acc[4] = {0.0, 0.0, 0.0, 0.0};
-  for (int d0 = 0; d0 < 128; d0 += SEL_DIMS) {
-    __syncthreads();
-    for (int i = tid; i < SEL_ROWS * SEL_DIMS; i += 256) {
-      const int r = i / SEL_DIMS, d = i % SEL_DIMS;
-      double s = 0.0;
-      if (r < rows) {
-        const uint16_t* p = q + ((int64_t)(row0 + r0 + r) * Hq + kvh * G) * 128 + d0 + d;
-        for (int g = 0; g < G; ++g) s += (double)q_value(p[g * 128], q_bf16);
-      }
-      qs[r][d] = s;
-    }
-    for (int i = tid; i < SEL_BLOCKS * SEL_DIMS; i += 256) {
-      const int b = i / SEL_DIMS, d = i % SEL_DIMS;
-      double s = 0.0;
-      if (b0 + b < scored) {
-        const float* p = sums + kvh * sums_head_stride + (int64_t)(b0 + b) * m * 128 + d0 + d;
-        for (int t = 0; t < m; ++t) s += (double)p[t * 128];
-      }
-      bs[d][b] = s;
-    }
-    __syncthreads();
-#pragma unroll 4
-    for (int d = 0; d < SEL_DIMS; ++d) {
-      const double x = bs[d][lb];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fma(qs[lr + e][d], x, acc[e]);
-    }
-  }
-  if (b0 + lb >= scored) return;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (lr + e < rows)
-      keys[((int64_t)(r0 + lr + e) * Hkv + kvh) * n_blocks + b0 + lb] = score_key(acc[e]);
+// Blocks a row sees.
+DRT_DEV int blocks_of(int row, const AttnWhere& where, int block) {
+  return (int)(((int64_t)key_end_of(row, where) + block - 1) / block);
 }
 
-// A row's choice for one K/V head, one wave: the need-th largest key by its bits from the
-// top (a candidate prefix stands when at least `need` keys reach it; when exactly `need` do, they are the choice),
-// then the blocks in ascending order. R: keys a lane holds, block 64 i + lane (0: read anew each time).
-template <int R>
-__global__ __launch_bounds__(256) void choose_blocks_kernel(const uint64_t* __restrict__ keys,
-                                                            int row0, int n_rows, int Hkv,
-                                                            const AttnWhere where,
-                                                            const SparseSel sel, int n_blocks,
-                                                            int32_t* __restrict__ blocks) {
+// Scores of 16 rows against 16 blocks at a time, as 16x16x4 products in 64 bits. The rows' queries,
+// the group's heads added up, meet in LDS; lane (i, g) then holds head dims 16 c + 4 g .. + 4
+// (c = 0..7) of row i, and of block i as they are in memory (64 bytes in a row of 16 blocks a load),
+// its tiles added up: a product takes one of them of each lane group, and leaves rows g, g + 4,
+// g + 8, g + 12 of block i. The 32 products of 16 x 16 scores take a SIMD 2048 cycles.
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+constexpr int SEL_QROW = 130;  // doubles of a row in LDS
+
+template <int THREADS>
+DRT_DEV void add_queries(const uint16_t* __restrict__ q, int q_bf16, int64_t row, int rows, int Hq,
+                         int G, int kvh, double* qs) {
+  constexpr int N = 2048 / THREADS;  // head dims a thread
+  const int r = threadIdx.x * N / 128, d = threadIdx.x * N % 128;
+  const uint16_t* p = q + ((row + min(r, rows - 1)) * Hq + kvh * G) * 128 + d;
+  double a[N] = {};
+#pragma unroll 4
+  for (int h = 0; h < G; ++h) {
+    uint32_t w[N / 2];
+    if constexpr (N == 8) {
+      const u32x4 y = *(const u32x4*)(p + h * 128);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = y[e];
+    } else {
+      const uint2 y = *(const uint2*)(p + h * 128);
+      w[0] = y.x;
+      w[1] = y.y;
+    }
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) {
+      a[2 * e] += (double)q_value((uint16_t)(w[e] & 0xffffu), q_bf16);
+      a[2 * e + 1] += (double)q_value((uint16_t)(w[e] >> 16), q_bf16);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) qs[r * SEL_QROW + d + e] = a[e];
+}
+
+// Blocks b0 .. + 16, b0 + step .. + 16, ... below b_end: put(block, row of the 16, key). ready()
+// is called once the first blocks are on their way, and returns with the queries in qs.
+template <typename Ready, typename Put>
+DRT_DEV void score_blocks(const float* __restrict__ sums, int b0, int step, int b_end, int m,
+                          const double* qs, Ready&& ready, Put&& put) {
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const float* base = sums + 4 * g;
+  f32x4 x[8];  // a block's first tile, loaded a step ahead
+  auto load = [&](int b) {
+    const float* p = base + (int64_t)min(b + i, b_end - 1) * m * 128;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) x[c] = *(const f32x4_e*)(p + 16 * c);
+  };
+  if (b0 < b_end) load(b0);
+  ready();
+  if (b0 >= b_end) return;
+  double a[32];
+#pragma unroll
+  for (int d = 0; d < 32; ++d) a[d] = qs[i * SEL_QROW + 16 * (d >> 2) + 4 * g + (d & 3)];
+  for (; b0 < b_end; b0 += step) {
+    double y[32];
+#pragma unroll
+    for (int d = 0; d < 32; ++d) y[d] = (double)x[d >> 2][d & 3];
+    const float* p = base + (int64_t)min(b0 + i, b_end - 1) * m * 128;
+    for (int t = 1; t < m; ++t) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) x[c] = *(const f32x4_e*)(p + (int64_t)t * 128 + 16 * c);
+#pragma unroll
+      for (int d = 0; d < 32; ++d) y[d] += (double)x[d >> 2][d & 3];
+    }
+    load(b0 + step);  // (behind the last: loaded, not used)
+    f64x4 acc = f64x4{}, acc1 = f64x4{};  // (two chains: a product waits for the one before it)
+#pragma unroll
+    for (int d = 0; d < 32; d += 2) {
+      acc = __builtin_amdgcn_mfma_f64_16x16x4f64(a[d], y[d], acc, 0, 0, 0);
+      acc1 = __builtin_amdgcn_mfma_f64_16x16x4f64(a[d + 1], y[d + 1], acc1, 0, 0, 0);
+    }
+    acc += acc1;
+    if (b0 + i < b_end) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) put(b0 + i, g + 4 * e, score_key(acc[e]));
+    }
+  }
+}
+
+// A row's choice for one K/V head, one wave: the need-th largest key by its bits from the top (a
+// candidate prefix stands when at least `need` keys reach it; when exactly `need` do, they are
+// the choice; the upper halves alone mostly decide it), then the blocks in ascending order.
+// key_at(b): the key of scored block b. R: keys a lane holds, block 64 i + lane (0: asked for anew each time).
+template <int R, typename KeyAt>
+DRT_DEV void choose_row(KeyAt&& key_at, int nb, const SparseSel& sel, int32_t* out) {
   const int lane = threadIdx.x & 63;
-  const int64_t id = blockIdx.x * (int64_t)4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (id >= (int64_t)n_rows * Hkv) return;
-  const int row = row0 + (int)(id / Hkv);
-  const uint64_t* mine = keys + id * n_blocks;
-  int32_t* out = blocks + ((int64_t)row0 * Hkv + id) * sel.count;
-  const int nb = (key_end_of(row, where) + sel.block - 1) / sel.block;  // blocks the row sees
   if (nb <= sel.count) {
     for (int i = lane; i < sel.count; i += 64) out[i] = i < nb ? i : -1;
     return;
@@ -113,7 +135,7 @@ __global__ __launch_bounds__(256) void choose_blocks_kernel(const uint64_t* __re
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int b = 64 * i + lane;
-    held[i] = b >= lo && b < hi ? mine[b] : 0ull;
+    held[i] = b >= lo && b < hi ? key_at(b) : 0ull;
   }
   // f(i, key of block 64 i + lane) for every i; 0, below every score's, where none is scored
   auto each = [&](auto&& f) {
@@ -123,13 +145,23 @@ __global__ __launch_bounds__(256) void choose_blocks_kernel(const uint64_t* __re
     } else {
       for (int i = 0; i < (nb + 63) / 64; ++i) {
         const int b = 64 * i + lane;
-        f(i, b >= lo && b < hi ? mine[b] : 0ull);
+        f(i, b >= lo && b < hi ? key_at(b) : 0ull);
       }
     }
   };
-  uint64_t cut = 0ull;  // the largest prefix that at least `need` keys reach
+  uint32_t upper = 0u;  // the largest prefix that at least `need` keys reach
   bool exact = need == 0;
-  for (int bit = 63; bit >= 0 && !exact; --bit) {
+  for (int bit = 31; bit >= 0 && !exact; --bit) {
+    const uint32_t want = upper | (1u << bit);
+    int n = 0;
+    each([&](int, uint64_t k) { n += __popcll(__ballot((uint32_t)(k >> 32) >= want)); });
+    if (n >= need) {
+      upper = want;
+      exact = n == need;
+    }
+  }
+  uint64_t cut = (uint64_t)upper << 32;
+  for (int bit = 31; bit >= 0 && !exact; --bit) {
     const uint64_t want = cut | (1ull << bit);
     int n = 0;
     each([&](int, uint64_t k) { n += __popcll(__ballot(k >= want)); });
@@ -157,44 +189,130 @@ __global__ __launch_bounds__(256) void choose_blocks_kernel(const uint64_t* __re
   });
 }
 
+struct SelArgs {
+  const uint16_t* q;   // [rows][Hq][128]
+  const float* sums;   // [Hkv][tiles][128]
+  int64_t sums_head_stride;
+  int q_bf16, row0, n_rows, Hq, Hkv, n_blocks, per;
+  AttnWhere where;
+  SparseSel sel;
+  uint64_t* keys;      // [n_rows][Hkv][n_blocks]
+  int32_t* blocks;     // [rows][Hkv][count]
+};
+
+// Both steps for 16 rows of one K/V head in a work-group of eight waves, the keys in LDS (RB rounds of 64
+// blocks). 1000 rows x 4 heads, 500 blocks: FUSED_US us; in two launches, with the keys in memory, 22 + 14.
+template <int RB>
+__global__ __launch_bounds__(512, 2) void select_kernel(const SelArgs x) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kvh = blockIdx.x % x.Hkv, r0 = blockIdx.x / x.Hkv * 16;
+  const int rows = min(16, x.n_rows - r0), G = x.Hq / x.Hkv;
+  __shared__ double qs[16 * SEL_QROW];
+  __shared__ uint64_t keys[16][RB * 64];
+  // the last row sees the most: blocks at or beyond its last `local` are never scored
+  const int nb_last = blocks_of(x.row0 + r0 + rows - 1, x.where, x.sel.block);
+  const int b_end = nb_last <= x.sel.count ? 0 : nb_last - x.sel.local;
+  score_blocks(x.sums + kvh * x.sums_head_stride, wave * 16, 128, b_end, x.sel.block >> 5, qs,
+               [&] {
+                 add_queries<512>(x.q, x.q_bf16, x.row0 + r0, rows, x.Hq, G, kvh, qs);
+                 __syncthreads();
+               },
+               [&](int b, int r, uint64_t k) { keys[r][b] = k; });
+  __syncthreads();
+  for (int r = wave; r < rows; r += 8) {
+    const int64_t row = x.row0 + r0 + r;
+    choose_row<RB>([&](int b) { return keys[r][b]; }, blocks_of((int)row, x.where, x.sel.block), x.sel,
+                   x.blocks + (row * x.Hkv + kvh) * x.sel.count);
+  }
+}
+
+// The scores alone: 16 rows against 64 * per blocks of one K/V head, four waves.
+__global__ __launch_bounds__(256, 2) void block_scores_kernel(const SelArgs x) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // work-group: (row tile * chunks + chunk) * Hkv + head
+  const int chunks = (x.n_blocks + 64 * x.per - 1) / (64 * x.per);
+  const int kvh = blockIdx.x % x.Hkv, rest = blockIdx.x / x.Hkv, chunk = rest % chunks;
+  const int r0 = rest / chunks * 16, rows = min(16, x.n_rows - r0), G = x.Hq / x.Hkv;
+  const int scored = blocks_of(x.row0 + r0 + rows - 1, x.where, x.sel.block) - x.sel.local;
+  if (chunk * x.per * 64 >= scored) return;
+  __shared__ double qs[16 * SEL_QROW];
+  const int b0 = (chunk * 4 + wave) * x.per * 16;
+  score_blocks(x.sums + kvh * x.sums_head_stride, b0, 16, min(scored, b0 + x.per * 16),
+               x.sel.block >> 5, qs,
+               [&] {
+                 add_queries<256>(x.q, x.q_bf16, x.row0 + r0, rows, x.Hq, G, kvh, qs);
+                 __syncthreads();
+               },
+               [&](int b, int r, uint64_t k) {
+                 if (r < rows) x.keys[((int64_t)(r0 + r) * x.Hkv + kvh) * x.n_blocks + b] = k;
+               });
+}
+
+template <int R> __global__ __launch_bounds__(256) void choose_blocks_kernel(const SelArgs x) {
+  const int64_t id = blockIdx.x * (int64_t)4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (id >= (int64_t)x.n_rows * x.Hkv) return;
+  const uint64_t* mine = x.keys + id * x.n_blocks;
+  choose_row<R>([&](int b) { return mine[b]; },
+                blocks_of(x.row0 + (int)(id / x.Hkv), x.where, x.sel.block), x.sel,
+                x.blocks + ((int64_t)x.row0 * x.Hkv + id) * x.sel.count);
+}
+
 // Rows whose scores one pass holds: 256 MiB of them at most.
 int select_rows(int n_rows, int Hkv, int n_blocks) {
   const int64_t most = ((int64_t)1 << 28) / ((int64_t)Hkv * n_blocks * 8);
-  return (int)std::min<int64_t>(n_rows, std::max<int64_t>(SEL_ROWS, most / SEL_ROWS * SEL_ROWS));
+  return (int)std::min<int64_t>(n_rows, std::max<int64_t>(16, most / 16 * 16));
 }
 
 }  // namespace
 
 namespace drt {
 
+// Both steps in one launch: work-groups of 16 rows and a K/V head that find half the CUs at
+// least something to do, and keys that fit LDS.
+static bool select_at_once(int n_rows, int Hkv, int n_blocks) {
+  return n_blocks <= 1024 && (int64_t)((n_rows + 15) / 16) * Hkv >= 128;
+}
+
 size_t select_blocks_bytes(int n_rows, int Hkv, int n_keys, int block) {
   const int nb = (int)(((int64_t)n_keys + block - 1) / block);
-  return (size_t)select_rows(n_rows, Hkv, nb) * Hkv * nb * 8;
+  return select_at_once(n_rows, Hkv, nb) ? 0 : (size_t)select_rows(n_rows, Hkv, nb) * Hkv * nb * 8;
 }
 
 void select_blocks(const void* q, bool q_bf16, const float* sums, int64_t sums_head_stride,
                    int n_rows, int Hq, int Hkv, const AttnWhere& where, const SparseSel& sel,
                    void* workspace, int32_t* blocks, hipStream_t s) {
   const int nb = (int)(((int64_t)where.n_keys + sel.block - 1) / sel.block);
+  SelArgs a{(const uint16_t*)q, sums, sums_head_stride, (int)q_bf16, 0, n_rows, Hq, Hkv, nb, 1, where,
+            sel, (uint64_t*)workspace, blocks};
+  if (select_at_once(n_rows, Hkv, nb)) {
+    const int64_t wgs = (int64_t)((n_rows + 15) / 16) * Hkv;
+    require(wgs < ((int64_t)1 << 31), "select_blocks: too many rows for one call");
+    const dim3 grid((unsigned)wgs);
+    if (nb <= 256) hipLaunchKernelGGL(select_kernel<4>, grid, dim3(512), 0, s, a);
+    else if (nb <= 512) hipLaunchKernelGGL(select_kernel<8>, grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL(select_kernel<16>, grid, dim3(512), 0, s, a);
+    DRT_HIP(hipGetLastError());
+    return;
+  }
   const int step = select_rows(n_rows, Hkv, nb);
-  const int64_t chunks = (nb + SEL_BLOCKS - 1) / SEL_BLOCKS;
   for (int r = 0; r < n_rows; r += step) {
-    const int rows = std::min(step, n_rows - r);
-    const int64_t grid = (rows + SEL_ROWS - 1) / SEL_ROWS * chunks * Hkv;
-    require(grid < ((int64_t)1 << 31), "select_blocks: too many blocks for one call");
-    if (nb > sel.count)
-      hipLaunchKernelGGL(block_scores_kernel, dim3((unsigned)grid), dim3(256), 0, s,
-                         (const uint16_t*)q, (int)q_bf16, sums, sums_head_stride, r, rows, Hq, Hkv,
-                         where, sel, nb, (uint64_t*)workspace);
-    const dim3 cgrid((unsigned)(((int64_t)rows * Hkv + 3) / 4));
-#define DRT_CHOOSE(R)                                                                            \
-  hipLaunchKernelGGL(choose_blocks_kernel<R>, cgrid, dim3(256), 0, s, (const uint64_t*)workspace, r, \
-                     rows, Hkv, where, sel, nb, blocks)
-    if (nb <= 256) DRT_CHOOSE(4);
-    else if (nb <= 1024) DRT_CHOOSE(16);
-    else if (nb <= 2048) DRT_CHOOSE(32);
-    else DRT_CHOOSE(0);
-#undef DRT_CHOOSE
+    a.row0 = r;
+    a.n_rows = std::min(step, n_rows - r);
+    const int64_t tiles = (a.n_rows + 15) / 16;
+    if (nb > sel.count) {
+      // 16 x 16 scores a wave: as few as leave no SIMD without a wave, four at most
+      a.per = (int)std::max<int64_t>(1, std::min<int64_t>(4, tiles * ((nb + 15) / 16) * Hkv / 1024));
+      const int64_t wgs = tiles * ((nb + 64 * a.per - 1) / (64 * a.per)) * Hkv;
+      require(wgs < ((int64_t)1 << 31), "select_blocks: too many blocks for one call");
+      hipLaunchKernelGGL(block_scores_kernel, dim3((unsigned)wgs), dim3(256), 0, s, a);
+    }
+    const dim3 grid((unsigned)(((int64_t)a.n_rows * Hkv + 3) / 4));
+    if (nb <= 256) hipLaunchKernelGGL(choose_blocks_kernel<4>, grid, dim3(256), 0, s, a);
+    else if (nb <= 512) hipLaunchKernelGGL(choose_blocks_kernel<8>, grid, dim3(256), 0, s, a);
+    else if (nb <= 1024) hipLaunchKernelGGL(choose_blocks_kernel<16>, grid, dim3(256), 0, s, a);
+    else if (nb <= 2048) hipLaunchKernelGGL(choose_blocks_kernel<32>, grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(choose_blocks_kernel<0>, grid, dim3(256), 0, s, a);
     DRT_HIP(hipGetLastError());
   }
 }

@@ -395,10 +395,11 @@ class PrefixKVCache:
         blocks = torch.empty((rows, self.kv_heads, count), dtype=torch.int32, device=q.device)
         need = _workspace_bytes("drt_op_select_blocks_workspace_bytes", rows, self.kv_heads,
                                 n_keys, block_size)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         _launch(torch, _lib.load().drt_op_select_blocks, self._index, q.data_ptr(), qdt,
                 self._sums(layer), self.tiles, rows, hq, self.kv_heads, n_keys, row_pos0, mk, p, b,
-                block_size, count, sinks, local, blocks.data_ptr(), ws.data_ptr(), need)
+                block_size, count, sinks, local, blocks.data_ptr(),
+                None if ws is None else ws.data_ptr(), need)
         return blocks
 
     def sparse_attention(self, layer: int, q, blocks, *, block_size: int, n_keys: int,

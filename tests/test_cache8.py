@@ -141,7 +141,7 @@ REFUSED = (
         {"qdt": _lib.I8}, {"rows": 0}, {"hq": 3}, {"n_keys": 0}, {"n_keys": 129}, {"pos0": -1},
         {"size": 0}, {"size": 48}, {"size": -32}, {"count": 0}, {"count": 1025}, {"sinks": -1},
         {"local": 0}, {"sinks": 3, "local": 2}, {"sinks": 2**31 - 1, "local": 2**31 - 1},
-        {"mask": 7}, {"block": 0}, {"ws": P + 4})]
+        {"mask": 7}, {"block": 0}, {"ws": P + 4}, {"q": P + 8})]
     + [_sparse(**kw) for kw in (
         {"q": None}, {"cache": None}, {"scales": None}, {"blocks": None}, {"out": None},
         {"ws": None}, {"ws_bytes": 8}, {"dtype": _lib.F32}, {"dtype": _lib.BF16},

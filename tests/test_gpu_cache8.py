@@ -356,6 +356,12 @@ def test_attention_over_more_8_bit_keys_than_4_gib_hold():
     (5, 2, 2, 40000, 39990, None, "f16", "i8", 32, 100, 0, 1),    # 1250
     (3, 2, 1, 70000, 69990, None, "f16", "f16", 32, 60, 0, 1),    # 2188
     (5, 2, 1, 640, 0, None, "f16", "i8", 32, 4, 2, 2),            # nothing left to score
+    # enough rows and heads for one launch: 47, 375 and 938 blocks, and none to score
+    (260, 8, 8, 3000, 2740, (0, 32), "bf16", "bf16", 64, 12, 1, 2),
+    (257, 16, 8, 12000, 5000, (2, 40), "f16", "i8", 32, 20, 0, 1),
+    (250, 8, 8, 30000, 29750, None, "f16", "i8", 32, 33, 3, 1),
+    (700, 4, 4, 700, 0, (0, 1), "f16", "i8", 32, 5, 0, 1),
+    (256, 8, 8, 100, 0, None, "f16", "i8", 32, 4, 0, 1),
 ])
 def test_select_blocks(rows, hq, hkv, n_keys, pos0, mask, qdt, dtype, block, count, sinks, local):
     _say("select", rows, hq, hkv, n_keys, pos0, mask, qdt, dtype, block, count, sinks, local)
@@ -372,11 +378,13 @@ def test_select_blocks(rows, hq, hkv, n_keys, pos0, mask, qdt, dtype, block, cou
     np.testing.assert_array_equal(got.cpu().numpy(), want)
 
 
-@pytest.mark.parametrize("n", [100, 700, 1500, 2500])  # (blocks: each of the kernel's forms)
-def test_select_blocks_with_equal_and_nan_scores(n):
+# (blocks and rows: each of the kernels' forms)
+@pytest.mark.parametrize("n,rows", [(100, 4), (400, 4), (700, 4), (1500, 4), (2500, 4), (100, 2048),
+                                    (400, 2048), (700, 2048)])
+def test_select_blocks_with_equal_and_nan_scores(n, rows):
     from diffusorrt_amd.kernels import PrefixKVCache
 
-    _say("select ties", n)
+    _say("select ties", n, rows)
     cache = PrefixKVCache(1, 1, 32 * n, dtype="f16", block_sums=True)
     rng = np.random.default_rng(n)
     sums = np.zeros((1, n, 128))
@@ -389,11 +397,11 @@ def test_select_blocks_with_equal_and_nan_scores(n):
     sums[0, rng.integers(0, n - 1, 5), 3] = -np.inf
     ends = X.key_ends(4, 32 * n, 0)
     cache.sums[0] = torch.from_numpy(sums).float().cuda()
-    got = cache.select_blocks(0, q.cuda(), block_size=32, count=20, n_keys=32 * n, row_pos0=0,
-                              kind="full")
+    got = cache.select_blocks(0, q.repeat(rows // 4, 1, 1).cuda(), block_size=32, count=20,
+                              n_keys=32 * n, row_pos0=0, kind="full")
     with np.errstate(invalid="ignore"):
         want = X.select_blocks(_np(q), sums, ends, block=32, count=20)
-    np.testing.assert_array_equal(got.cpu().numpy(), want)
+    np.testing.assert_array_equal(got.cpu().numpy(), np.tile(want, (rows // 4, 1, 1)))
 
 
 def test_select_never_hears_of_hidden_keys():
