@@ -149,12 +149,10 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   typedef typename T::vec vec;
   constexpr int NW = QW * KW, THREADS = 64 * NW, NQ = 32 * QT * QW, TILE = T::TILE, LD = T::LOADS;
   static_assert(!SPARSE || (QT == 1 && QW == 1), "a work-group has one union of lists");
-  constexpr int O_BYTES = QT * 16384;  // a wave's O
-  constexpr int Q_BYTES = NQ * CA_QROW * 2, OUT_BYTES = QW * 8192;
-  constexpr int ML_BYTES = QT * 512, MRG = KW > 1 ? (NW / 2) * (O_BYTES + ML_BYTES) : 0;
-  constexpr int LDS = Q_BYTES > MRG ? (Q_BYTES > OUT_BYTES ? Q_BYTES : OUT_BYTES)
-                                    : (MRG > OUT_BYTES ? MRG : OUT_BYTES);
-  __shared__ __align__(16) char smem[LDS];
+  // LDS: the queries, then halves (64 head dims) of every wave's O, 8 KiB a query tile
+  constexpr int Q_BYTES = NQ * CA_QROW * 2, HALF_BYTES = NW * QT * 8192;
+  __shared__ __align__(16) char smem[Q_BYTES > HALF_BYTES ? Q_BYTES : HALF_BYTES];
+  __shared__ float2 ml[KW][NQ];  // base and sum of every way
   __shared__ float2 qinfo[NQ];  // c times a query vector's power of two; -128 * 2^-24 its sum
   __shared__ uint32_t bits[SPARSE ? CA_WIN : 1];  // rows that list a block of the window
   __shared__ int2 list[SPARSE ? CA_WIN : 1];      // its blocks and their rows
@@ -180,57 +178,75 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
                   : qt0 * 32 + v < n_qv;
   };
 
-  // queries into LDS, 16 threads (eight elements each) a query vector
+  // the queries, 16 threads (eight elements each) a query vector, on their way
+  constexpr int QL = NQ * 16 / THREADS;
+  static_assert(QL * THREADS == NQ * 16, "whole rounds of the queries");
+  u32x4 qraw[QL];
 #pragma unroll
-  for (int it0 = 0; it0 < NQ * 16; it0 += THREADS) {
-    const int v = (it0 + tid) >> 4, ch = tid & 15;
-    u32x4 raw = u32x4{0u, 0u, 0u, 0u};
-    if (exists(v)) raw = *(const u32x4*)(x.q + ((int64_t)row_of(v) * x.Hq + head_of(v)) * 128 + ch * 8);
-    float pw = 1.f, sum = 0.f;
-    if constexpr (DT == 0) {
-      if (x.q_bf16) {
-        uint32_t most = 0u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          most = max(most, max((raw[e] << 16) & 0x7fffffffu, raw[e] & 0x7fff0000u));
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
-        const int ex = most ? min(max((int)(most >> 23) - 127, -126), 126) : 0;
-        pw = __uint_as_float((uint32_t)(127 + ex) << 23);
-        const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          raw[e] = pack_half2((_Float16)(__uint_as_float(raw[e] << 16) * inv),
-                              (_Float16)(__uint_as_float(raw[e] & 0xffff0000u) * inv));
-      }
-      sum = kv8_add8(__builtin_bit_cast(f16x8, raw), 0.f);
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    }
-    *(u32x4*)(smem + (v * CA_QROW + ch * 8) * 2) = raw;
-    if (ch == 0) qinfo[v] = make_float2(x.c * pw, -KV8_BIAS / KV8_POW * sum);
+  for (int it = 0; it < QL; ++it) {
+    const int v = (it * THREADS + tid) >> 4;
+    qraw[it] = u32x4{0u, 0u, 0u, 0u};
+    if (exists(v))
+      qraw[it] = *(const u32x4*)(x.q + ((int64_t)row_of(v) * x.Hq + head_of(v)) * 128 + (tid & 15) * 8);
   }
-  __syncthreads();
 
   const int wv0 = qw * QT * 32;  // the wave's first query vector
   const uint16_t* ql = (const uint16_t*)smem + (wv0 + (lane & 31)) * CA_QROW + 8 * (lane >> 5);
   constexpr bool HOLD = QT == 1;  // the queries' operands in registers
   vec qr[HOLD ? 8 : 1];
-  if (HOLD) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) qr[HOLD ? i : 0] = *(const vec*)(ql + 16 * i);
-  }
   int q_end[QT];
   float cq[QT], nq[QT], m_run[QT], l_run[QT], p_run[QT];
   f32x16 o[QT][4];
   const int last_row = x.n_rows - 1;
 #pragma unroll
-  for (int j = 0; j < QT; ++j) {
-    const int v = wv0 + j * 32 + (lane & 31);
-    q_end[j] = key_end_of(min(row_of(v), last_row), where);
-    cq[j] = qinfo[v].x;
-    nq[j] = qinfo[v].y;
-  }
+  for (int j = 0; j < QT; ++j)
+    q_end[j] = key_end_of(min(row_of(wv0 + j * 32 + (lane & 31)), last_row), where);
+  // Queries into LDS and from there to the waves. Called by every thread, once, with the
+  // first tile's loads under way.
+  auto stage = [&] {
+#pragma unroll
+    for (int it = 0; it < QL; ++it) {
+      const int v = (it * THREADS + tid) >> 4, ch = tid & 15;
+      u32x4 raw = qraw[it];
+      float pw = 1.f, sum = 0.f;
+      if constexpr (DT == 0) {
+        if (x.q_bf16) {
+          uint32_t most = 0u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            most = max(most, max((raw[e] << 16) & 0x7fffffffu, raw[e] & 0x7fff0000u));
+#pragma unroll
+          for (int d = 8; d > 0; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+          const int ex = most ? min(max((int)(most >> 23) - 127, -126), 126) : 0;
+          pw = __uint_as_float((uint32_t)(127 + ex) << 23);
+          const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            raw[e] = pack_half2((_Float16)(__uint_as_float(raw[e] << 16) * inv),
+                                (_Float16)(__uint_as_float(raw[e] & 0xffff0000u) * inv));
+        }
+        sum = kv8_add8(__builtin_bit_cast(f16x8, raw), 0.f);
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
+      }
+      *(u32x4*)(smem + (v * CA_QROW + ch * 8) * 2) = raw;
+      if (ch == 0) qinfo[v] = make_float2(x.c * pw, -KV8_BIAS / KV8_POW * sum);
+    }
+    // (a bare barrier: __syncthreads() would wait for the tile on its way)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    if (HOLD) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) qr[HOLD ? i : 0] = *(const vec*)(ql + 16 * i);
+    }
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+      const float2 y = qinfo[wv0 + j * 32 + (lane & 31)];
+      cq[j] = y.x;
+      nq[j] = y.y;
+    }
+  };
   auto reset = [&] {
 #pragma unroll
     for (int j = 0; j < QT; ++j) {
@@ -257,18 +273,18 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   float2 st = make_float2(1.f, 1.f);
   int fold = CA_FOLD;
 
-  // n tiles, the first at t with its rows; next(t, rows) steps to the wave's following tile.
-  // careful (16 bits): see below.
-  auto run = [&](int n, int t, uint32_t rows, bool careful, auto&& next) {
+  auto first = [&](int n, int t) {
     if (n <= 0) return;
-    {
-      const uint8_t* p = base + (int64_t)t * TILE;
+    const uint8_t* p = base + (int64_t)t * TILE;
 #pragma unroll
-      for (int i = 0; i < LD; ++i) kr[i] = *(const u32x4*)(p + i * 1024);
+    for (int i = 0; i < LD; ++i) kr[i] = *(const u32x4*)(p + i * 1024);
 #pragma unroll
-      for (int i = 0; i < LD; ++i) vr[i] = *(const u32x4*)(p + TILE / 2 + i * 1024);
-      if (DT == 0) st = scales_of(t);
-    }
+    for (int i = 0; i < LD; ++i) vr[i] = *(const u32x4*)(p + TILE / 2 + i * 1024);
+    if (DT == 0) st = scales_of(t);
+  };
+  // n tiles, the first (on its way) at t with its rows; next(t, rows) steps to the wave's following
+  // tile. careful (16 bits): see below.
+  auto run = [&](int n, int t, uint32_t rows, bool careful, auto&& next) {
     for (int it = 0; it < n; ++it) {
       const int key0 = t * 32;
       const uint32_t seen = rows;
@@ -381,13 +397,16 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
     const int n_tiles = (where.n_keys + 31) >> 5, t0 = split * x.tiles_per_split + kw;
     const int t_end = !exists(wv0) ? 0
                                    : min(min(n_tiles, (split + 1) * x.tiles_per_split), (wave_end + 31) >> 5);
-    run((t_end - t0 + KW - 1) / KW, t0, 0u, false, [&](int& t, uint32_t&) { t += KW; });
+    const int n = (t_end - t0 + KW - 1) / KW;
+    first(n, t0);
+    stage();
+    run(n, t0, 0u, false, [&](int& t, uint32_t&) { t += KW; });
   } else {
     const int m = x.block >> 5, n_blocks = (int)(((int64_t)wave_end + x.block - 1) / x.block);
     const int step_e = KW / m, step_r = KW % m;
     // 16 bits: a V that is not finite makes 0 * V of a row that does not see it NaN too. Rows
     // are looked at afterwards, and only if some are not finite is it all done again with care.
-    bool careful = false;
+    bool careful = false, staged = false;
     for (;;) {
       for (int w0 = 0; w0 < n_blocks; w0 += CA_WIN) {
         const int n_win = min(CA_WIN, n_blocks - w0);
@@ -422,30 +441,33 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
         }
         __syncthreads();
         n_list = __builtin_amdgcn_readfirstlane(n_list);
-        if (n_list > 0) {
-          // tiles in all (of the last block those that the rows see), and this range's
-          const int last = __builtin_amdgcn_readfirstlane(list[n_list - 1].x);
-          const int64_t n = (int64_t)(n_list - 1) * m + min((int64_t)m, ((wave_end + 31) >> 5) - (int64_t)last * m);
-          const int j0 = (int)(n * split / x.splits) + kw, j1 = (int)(n * (split + 1) / x.splits);
-          int e = j0 / m, r = j0 - e * m;
-          auto here = [&](int& t, uint32_t& rows) {
-            const int2 b = list[min(e, n_list - 1)];
-            t = __builtin_amdgcn_readfirstlane(b.x) * m + r;
-            rows = (uint32_t)__builtin_amdgcn_readfirstlane(b.y);
-          };
-          int t = 0;
-          uint32_t rows = 0u;
-          if (j0 < j1) here(t, rows);
-          run((j1 - j0 + KW - 1) / KW, t, rows, careful, [&](int& t2, uint32_t& rows2) {
-            e += step_e;
-            r += step_r;
-            if (r >= m) {
-              r -= m;
-              ++e;
-            }
-            here(t2, rows2);
-          });
-        }
+        // tiles in all (of the last block those that the rows see), and this wave's of this range
+        const int last = __builtin_amdgcn_readfirstlane(list[max(n_list - 1, 0)].x);
+        const int64_t n = n_list == 0 ? 0
+                                      : (int64_t)(n_list - 1) * m +
+                                            min((int64_t)m, ((wave_end + 31) >> 5) - (int64_t)last * m);
+        const int j0 = (int)(n * split / x.splits) + kw, j1 = (int)(n * (split + 1) / x.splits);
+        int e = j0 / m, r = j0 - e * m;
+        auto here = [&](int& t, uint32_t& rows) {
+          const int2 b = list[min(e, n_list - 1)];
+          t = __builtin_amdgcn_readfirstlane(b.x) * m + r;
+          rows = (uint32_t)__builtin_amdgcn_readfirstlane(b.y);
+        };
+        int t = 0;
+        uint32_t rows = 0u;
+        if (j0 < j1) here(t, rows);
+        first(j1 - j0, t);
+        if (!staged) stage();
+        staged = true;
+        run((j1 - j0 + KW - 1) / KW, t, rows, careful, [&](int& t2, uint32_t& rows2) {
+          e += step_e;
+          r += step_r;
+          if (r >= m) {
+            r -= m;
+            ++e;
+          }
+          here(t2, rows2);
+        });
       }
       if (DT == 0 || careful) break;
       bool odd = false;
@@ -470,85 +492,61 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
     }
   }
 
-  // the key ways of a wave's queries in pairs
-  if (KW > 1) {
+  // The key ways joined and rows out, half a head (64 head dims) at a time: every wave leaves its
+  // half in LDS as 16-byte pieces (query v, piece p at p ^ v: every bank in turn both ways), then
+  // eight threads a query vector add the ways' and write theirs, all waves taking part.
 #pragma unroll
-    for (int half = KW / 2; half > 0; half >>= 1) {
-      __syncthreads();  // the queries, or the round before, have been read
-      if (kw >= half && kw < 2 * half) {
-        char* d = smem + ((kw - half) * QW + qw) * (O_BYTES + ML_BYTES);
+  for (int hf = 0; hf < 2; ++hf) {
+    __syncthreads();  // the queries, or the first half, have been read
 #pragma unroll
-        for (int j = 0; j < QT; ++j) {
+    for (int j = 0; j < QT; ++j) {
+      f32x4* d = (f32x4*)(smem + ((kw * QW + qw) * QT + j) * 8192);
 #pragma unroll
-          for (int hb = 0; hb < 4; ++hb)
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              ((f32x4*)d)[(j * 16 + hb * 4 + r) * 64 + lane] =
-                  f32x4{o[j][hb][4 * r], o[j][hb][4 * r + 1], o[j][hb][4 * r + 2], o[j][hb][4 * r + 3]};
-          ((float2*)(d + O_BYTES))[j * 64 + lane] = make_float2(m_run[j], l_run[j]);
-        }
-      }
-      __syncthreads();
-      if (kw < half) {
-        const char* d = smem + (kw * QW + qw) * (O_BYTES + ML_BYTES);
-#pragma unroll
-        for (int j = 0; j < QT; ++j) {
-          const float2 ml = ((const float2*)(d + O_BYTES))[j * 64 + lane];
-          const float mm = fmaxf(m_run[j], ml.x);
-          const float w0 = m_run[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[j] - mm);
-          const float w1 = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mm);
-#pragma unroll
-          for (int hb = 0; hb < 4; ++hb)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const f32x4 y = ((const f32x4*)d)[(j * 16 + hb * 4 + r) * 64 + lane];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                o[j][hb][4 * r + e] = fmaf(w1, y[e], w0 * o[j][hb][4 * r + e]);
-            }
-          l_run[j] = fmaf(w1, ml.y, w0 * l_run[j]);
-          m_run[j] = mm;
-        }
-      }
+        for (int r = 0; r < 4; ++r)
+          d[(lane & 31) * 16 + ((b * 8 + 2 * r + (lane >> 5)) ^ (lane & 15))] =
+              f32x4{o[j][2 * hf + b][4 * r], o[j][2 * hf + b][4 * r + 1], o[j][2 * hf + b][4 * r + 2],
+                    o[j][2 * hf + b][4 * r + 3]};
+      if (hf == 0 && lane < 32) ml[kw][wv0 + j * 32 + lane] = make_float2(m_run[j], l_run[j]);
     }
-  }
-  __syncthreads();
-  if (kw > 0) return;  // (no barrier follows)
-  // Rows out: half a query tile's O^T (64 head dims) at a time through 8 KiB of the wave's own, as 16-byte
-  // pieces (query v, piece p at p ^ v: every bank in turn both ways), eight lanes a query vector.
-  f32x4* ot = (f32x4*)(smem + qw * 8192);
+    __syncthreads();
 #pragma unroll
-  for (int jh = 0; jh < 2 * QT; ++jh) {
-    const int j = jh >> 1, hf = jh & 1;
+    for (int it = 0; it < (NQ * 8 + THREADS - 1) / THREADS; ++it) {
+      const int v = (it * THREADS + tid) >> 3, ch = tid & 7;
+      if (v >= NQ || !exists(v)) continue;
+      float2 w[KW];
+      float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+      for (int k = 0; k < KW; ++k) {
+        w[k] = ml[k][v];
+        m = fmaxf(m, w[k].x);
+      }
+      f32x4 y0 = f32x4{}, y1 = f32x4{};
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        ot[(lane & 31) * 16 + ((b * 8 + 2 * r + (lane >> 5)) ^ (lane & 15))] =
-            f32x4{o[j][2 * hf + b][4 * r], o[j][2 * hf + b][4 * r + 1], o[j][2 * hf + b][4 * r + 2],
-                  o[j][2 * hf + b][4 * r + 3]};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int v = (lane >> 3) + 8 * i, ch = lane & 7, wv = wv0 + j * 32 + v;
-      const float m = __shfl(m_run[j], v, 64), l = __shfl(l_run[j], v, 64);
-      f32x4 y0 = ot[v * 16 + ((2 * ch) ^ (v & 15))], y1 = ot[v * 16 + ((2 * ch + 1) ^ (v & 15))];
-      if (!exists(wv)) continue;
-      const int64_t rh = (int64_t)row_of(wv) * x.Hq + head_of(wv);
+      for (int k = 0; k < KW; ++k) {
+        const f32x4* d = (const f32x4*)(smem + (k * QW * QT + (v >> 5)) * 8192) + (v & 31) * 16;
+        const float f = w[k].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w[k].x - m);
+        y0 += f * d[(2 * ch) ^ (v & 15)];
+        y1 += f * d[(2 * ch + 1) ^ (v & 15)];
+        l = fmaf(f, w[k].y, l);
+      }
+      const int64_t rh = (int64_t)row_of(v) * x.Hq + head_of(v);
       const int64_t at = rh * 128 + hf * 64 + ch * 8;
       if (OUT) {
         const float inv = SPARSE && l == 0.f ? 0.f : 1.f / l;  // no key: zeros
         y0 *= inv;
         y1 *= inv;
         if (x.out_bf16) {
-          u32x4 w;
+          u32x4 z;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            w[e] = (uint32_t)float_to_bf16_bits(y0[2 * e]) |
+            z[e] = (uint32_t)float_to_bf16_bits(y0[2 * e]) |
                    ((uint32_t)float_to_bf16_bits(y0[2 * e + 1]) << 16);
-            w[2 + e] = (uint32_t)float_to_bf16_bits(y1[2 * e]) |
+            z[2 + e] = (uint32_t)float_to_bf16_bits(y1[2 * e]) |
                        ((uint32_t)float_to_bf16_bits(y1[2 * e + 1]) << 16);
           }
-          *(u32x4*)((uint16_t*)x.out + at) = w;
+          *(u32x4*)((uint16_t*)x.out + at) = z;
         } else {
           *(f32x4*)((float*)x.out + at) = y0;
           *(f32x4*)((float*)x.out + at + 4) = y1;
