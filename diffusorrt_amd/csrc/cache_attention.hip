@@ -131,7 +131,7 @@ struct CaArgs {
   int64_t head_stride;     // bytes
   const float* scales;     // 8-bit
   const int32_t* blocks;   // [rows][Hkv][count] (listed blocks)
-  int q_bf16, n_rows, Hq, Hkv, splits, tiles_per_split, count, block;
+  int q_bf16, n_rows, Hq, Hkv, splits, count, block;
   float c;                 // log2(e) / sqrt(128), times 2^24 over 8 bits
   AttnWhere where;
   void* out;               // [rows][Hq * 128], bf16 or fp32
@@ -272,6 +272,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   u32x4 kr[LD], vr[LD];
   float2 st = make_float2(1.f, 1.f);
   int fold = CA_FOLD;
+  uint32_t heard = 0u;  // whether this lane's row lists any of the wave's tiles
 
   auto first = [&](int n, int t) {
     if (n <= 0) return;
@@ -310,11 +311,15 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
       asm volatile("" ::: "memory");  // (a scalar load among the reads of LDS would be waited for with them)
       if (DT == 0) st = scales_of(t);
       const bool bad = DT == 0 && !(sk + sv < INFINITY);  // a NaN tile: so is every row that sees it
+      // A row that does not list the tile's block weighs it nothing: by its exponent's offset where
+      // its end is not in the tile either. (A NaN score then still is one: see careful, heard.)
+      const bool hit = !SPARSE || (seen & my_row) != 0u;
+      if (SPARSE) heard |= seen & my_row;
       const bool part = key0 + 32 > wave_full || (SPARSE && seen != all_rows);
-      if (part || bad) {
+      if (key0 + 32 > wave_full || bad || (careful && part)) {
 #pragma unroll
         for (int j = 0; j < QT; ++j) {
-          const int mine = SPARSE && !(seen & my_row) ? 0 : q_end[j];
+          const int mine = hit ? q_end[j] : 0;
           if (bad && key0 < mine) {
             l_run[j] = NAN;
             m_run[j] = m_run[j] == -INFINITY ? 0.f : m_run[j];
@@ -335,7 +340,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
 #pragma unroll
         for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, s[j][r]);
         const float off0 = DT != 0 ? 0.f : fmaf(nq[j], a, lb);
-        const float u = fmaf(ca_max_xor32(tmax), a, off0);  // -inf: no visible key in the tile
+        const float u = hit ? fmaf(ca_max_xor32(tmax), a, off0) : -INFINITY;  // -inf: no visible key
         const bool up = u > m_run[j] + CA_RESCALE_LOG2;
         if (__ballot(up) || (DT == 0 && fold == 1)) {
           const float alpha = up ? __builtin_amdgcn_exp2f(m_run[j] - u) : 1.f;  // 0 from -inf
@@ -359,6 +364,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
           a = 1.f;
           off = -mb;
         }
+        if (SPARSE) off = hit ? off : -INFINITY;
         float psum = 0.f;
 #pragma unroll
         for (int kh = 0; kh < 2; ++kh)
@@ -374,7 +380,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
       fold = fold == 1 ? CA_FOLD : fold - 1;
       if constexpr (DT != 0) {
         if (careful && part) {
-          const int mine = SPARSE && !(seen & my_row) ? 0 : q_end[0];
+          const int mine = hit ? q_end[0] : 0;
           ca_values_apart<DT>(vr, key0, mine, lane, o[0]);
         }
       }
@@ -394,9 +400,9 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   };
 
   if constexpr (!SPARSE) {
-    const int n_tiles = (where.n_keys + 31) >> 5, t0 = split * x.tiles_per_split + kw;
-    const int t_end = !exists(wv0) ? 0
-                                   : min(min(n_tiles, (split + 1) * x.tiles_per_split), (wave_end + 31) >> 5);
+    const int64_t n_tiles = (where.n_keys + 31) >> 5;
+    const int t0 = (int)(n_tiles * split / x.splits) + kw;
+    const int t_end = !exists(wv0) ? 0 : min((int)(n_tiles * (split + 1) / x.splits), (wave_end + 31) >> 5);
     const int n = (t_end - t0 + KW - 1) / KW;
     first(n, t0);
     stage();
@@ -404,8 +410,9 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   } else {
     const int m = x.block >> 5, n_blocks = (int)(((int64_t)wave_end + x.block - 1) / x.block);
     const int step_e = KW / m, step_r = KW % m;
-    // 16 bits: a V that is not finite makes 0 * V of a row that does not see it NaN too. Rows
-    // are looked at afterwards, and only if some are not finite is it all done again with care.
+    // 16 bits: a V that is not finite makes 0 * V of a row that does not see it NaN too, and a K the
+    // score of one that does not list it. Rows are looked at afterwards, and only if some are not
+    // finite is it all done again with care.
     bool careful = false, staged = false;
     for (;;) {
       for (int w0 = 0; w0 < n_blocks; w0 += CA_WIN) {
@@ -484,6 +491,11 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   for (int j = 0; j < QT; ++j) {
     l_run[j] += __shfl_xor(l_run[j], 32, 64);
     if (DT == 0) {
+      if (SPARSE && !heard) {  // (a NaN query's scores of tiles that it does not list)
+        l_run[j] = p_run[j] = 0.f;
+#pragma unroll
+        for (int hb = 0; hb < 4; ++hb) o[j][hb] = f32x16{};
+      }
       p_run[j] += __shfl_xor(p_run[j], 32, 64);
 #pragma unroll
       for (int hb = 0; hb < 4; ++hb)
@@ -662,9 +674,7 @@ CachePlan plan_attention8(int n_rows, int Hq, int Hkv, int n_keys) {
   const int n_tiles = (int)(((int64_t)n_keys + 31) / 32);
   const int64_t wgs = Hkv * p.groups;
   int64_t splits = std::max<int64_t>(1, (p.wide ? 512 : 256) / wgs);
-  splits = std::min<int64_t>({splits, (n_tiles + kw - 1) / kw, 64});
-  p.tiles_per_split = (int)((n_tiles + splits - 1) / splits);
-  p.splits = (n_tiles + p.tiles_per_split - 1) / p.tiles_per_split;
+  p.splits = (int)std::min<int64_t>({splits, (n_tiles + kw - 1) / kw, 64});
   return p;
 }
 
@@ -697,7 +707,6 @@ static CaArgs args_of(KvType type, const void* q, bool q_bf16, const void* kv_la
   a.Hq = Hq;
   a.Hkv = Hkv;
   a.splits = p.splits;
-  a.tiles_per_split = p.tiles_per_split;
   a.block = 32;
   a.c = 1.44269504088896340736f / sqrtf(128.0f) * (type == KvType::I8 ? KV8_POW : 1.f);
   a.where = where;

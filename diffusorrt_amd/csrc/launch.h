@@ -222,7 +222,7 @@ void kv_sums(bool bf16, const void* kv, int64_t head_stride, int Hkv, int pos0, 
 // How an attention over the cache is cut: key ranges (splits), whose parts are joined by a second
 // launch, and work-groups of query tiles.
 struct CachePlan {
-  int qw = 1, splits = 1, tiles_per_split = 1;
+  int qw = 1, splits = 1;
   int64_t groups = 1;
   bool wide = false;
 };
