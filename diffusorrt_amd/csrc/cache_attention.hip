@@ -272,7 +272,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   u32x4 kr[LD], vr[LD];
   float2 st = make_float2(1.f, 1.f);
   int fold = CA_FOLD;
-  uint32_t heard = 0u;  // whether this lane's row lists any of the wave's tiles
+  uint32_t heard = 0u;  // whether this lane's row sees any of the wave's tiles
 
   auto first = [&](int n, int t) {
     if (n <= 0) return;
@@ -314,7 +314,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
       // A row that does not list the tile's block weighs it nothing: by its exponent's offset where
       // its end is not in the tile either. (A NaN score then still is one: see careful, heard.)
       const bool hit = !SPARSE || (seen & my_row) != 0u;
-      if (SPARSE) heard |= seen & my_row;
+      if (SPARSE) heard |= key0 < q_end[0] ? seen & my_row : 0u;
       const bool part = key0 + 32 > wave_full || (SPARSE && seen != all_rows);
       if (key0 + 32 > wave_full || bad || (careful && part)) {
 #pragma unroll
@@ -424,8 +424,8 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
         for (int i = tid; i < n_entries; i += THREADS) {
           const int r = i / x.count;
           const int b = x.blocks[((int64_t)(row0 + r) * x.Hkv + kvh) * x.count + (i - r * x.count)];
-          if (b >= w0 && b < w0 + n_win && (int64_t)b * x.block < key_end_of(row0 + r, where))
-            atomicOr(&bits[b - w0], 1u << r);
+          // (one beyond its row's keys only: its tiles are masked key by key)
+          if (b >= w0 && b < w0 + n_win) atomicOr(&bits[b - w0], 1u << r);
         }
         __syncthreads();
         // the window's blocks in order: wave w finds those of its share, then all take their places
@@ -491,7 +491,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   for (int j = 0; j < QT; ++j) {
     l_run[j] += __shfl_xor(l_run[j], 32, 64);
     if (DT == 0) {
-      if (SPARSE && !heard) {  // (a NaN query's scores of tiles that it does not list)
+      if (SPARSE && !heard) {  // (a NaN query's scores of tiles that its row does not see)
         l_run[j] = p_run[j] = 0.f;
 #pragma unroll
         for (int hb = 0; hb < 4; ++hb) o[j][hb] = f32x16{};

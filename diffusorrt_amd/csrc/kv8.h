@@ -54,6 +54,7 @@ DRT_DEV int key_end_of(int row, const drt::AttnWhere& w) {
   if (!w.masked) return w.n_keys;
   const int p = w.row_pos0 + row;
   if (p < w.prompt_len) return min(w.n_keys, w.prompt_len);
-  const int64_t end = w.prompt_len + ((int64_t)(p - w.prompt_len) / w.block + 1) * w.block;
+  const uint32_t mine = (uint32_t)(p - w.prompt_len) / (uint32_t)w.block;
+  const int64_t end = w.prompt_len + ((int64_t)mine + 1) * w.block;
   return (int)min((int64_t)w.n_keys, end);
 }
