@@ -674,7 +674,9 @@ CachePlan plan_attention8(int n_rows, int Hq, int Hkv, int n_keys) {
   const int n_tiles = (int)(((int64_t)n_keys + 31) / 32);
   const int64_t wgs = Hkv * p.groups;
   int64_t splits = std::max<int64_t>(1, (p.wide ? 512 : 256) / wgs);
-  p.splits = (int)std::min<int64_t>({splits, (n_tiles + kw - 1) / kw, 64});
+  // (Three tiles a wave cost less than the second launch: one row x 28 heads over 768 keys 7.8 us, 8.3
+  // with key ranges, over 1024 8.7 and 8.3; 32 rows x 16 heads over 384 keys 8.4 and 9.0.)
+  p.splits = n_tiles <= 3 * kw ? 1 : (int)std::min<int64_t>({splits, (n_tiles + kw - 1) / kw, 64});
   return p;
 }
 
@@ -686,7 +688,11 @@ CachePlan plan_sparse(int n_rows, int Hq, int Hkv, int count, int block) {
   // 28 heads, 16 blocks of 64: 12.4 us; of eight 13.3, of 16 16.2)
   const int64_t wgs = p.groups * Hkv * heads, tiles = (int64_t)count * (block / 32);
   p.wide = wgs >= 512;
-  p.splits = p.wide ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({256 / wgs, (tiles + 3) / 4, 64}));
+  // (As few as 16 tiles of a tile's rows cost less than the second launch: one row x 28 heads, 8 blocks of
+  // 64 9.4 us, with key ranges 10.1; 16 blocks 11.2 and 10.2.)
+  p.splits = p.wide || tiles * std::min(n_rows, rows) <= 16
+                 ? 1
+                 : (int)std::max<int64_t>(1, std::min<int64_t>({256 / wgs, (tiles + 3) / 4, 64}));
   return p;
 }
 
