@@ -24,10 +24,10 @@
 //
 // Listed blocks. A query tile is the 32 / G rows (G heads a group; 32 heads at a time above that) of
 // neighbours, and the tile's blocks are the union of its rows' lists, each with a bit per row: an
-// LDS bitmap, WIN blocks at a time, so a list is a set, whatever its order and repetitions.
+// LDS bitmap, CA_WIN blocks at a time, so a list is a set, whatever its order and repetitions.
 // Neighbouring queries mostly choose the same blocks: a block is then loaded and made operands once
 // for all of them, and every column of the products is in use (one wave per row, 16 columns of
-// which G are used: 2048 rows x 16 heads, 16 blocks of 64 of 32768 keys, 226 us; 64 here).
+// which G are used: 2048 rows x 16 heads, 16 blocks of 64 of 32768 keys, 226 us; 57 here).
 #include "kv8.h"
 #include "launch.h"
 
@@ -218,7 +218,8 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
 #pragma unroll
           for (int d = 8; d > 0; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
           const int ex = most ? min(max((int)(most >> 23) - 127, -126), 126) : 0;
-          pw = __uint_as_float((uint32_t)(127 + ex) << 23);
+          // (beyond 2^80 the scores are further apart than fp32 tells, and would overflow)
+          pw = __uint_as_float((uint32_t)(127 + min(ex, 80)) << 23);
           const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
 #pragma unroll
           for (int e = 0; e < 4; ++e)

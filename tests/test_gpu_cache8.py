@@ -246,7 +246,7 @@ def test_tiles_of_very_different_scales(rows, sparse):
                torch.float32)
 
 
-@pytest.mark.parametrize("qsize", [1e-38, 1e-20, 1e20])
+@pytest.mark.parametrize("qsize", [1e-38, 1e-20, 1e20, 5e37])
 def test_bf16_queries_of_any_size(qsize):
     _say("bf16 q *", qsize)
     gen = torch.Generator().manual_seed(12)
@@ -312,6 +312,54 @@ def test_nan_reaches_the_rows_that_see_it_only(dtype):
             assert torch.equal(nan, want)
             if dtype == "i8" or where == "k":  # (a NaN of V in 16 bits is one head dim's)
                 assert torch.equal(whole, want)
+
+
+@pytest.mark.parametrize("dtype", ["i8", "f16", "bf16"])
+def test_values_that_are_not_finite_stay_with_the_rows_that_list_them(dtype):
+    """16 neighbouring rows, which the kernel takes together, list the 16 subsets of four blocks. V
+    of block 1 has infinities and a NaN, K of block 3 a NaN; row 16 on lists them all."""
+    from diffusorrt_amd.kernels import PrefixKVCache
+
+    _say("not finite", dtype)
+    gen = torch.Generator().manual_seed(17)
+    cache = PrefixKVCache(1, 1, 128, dtype=dtype)
+    k, v = _kv(gen, 128, 1)
+    clean = v.clone(), k.clone()
+    v[40, 0, 3], v[41, 0, 4], v[63, 0, 5] = float("inf"), -float("inf"), float("nan")
+    k[100, 0, 7] = float("nan")
+    cache.store(0, k.cuda(), v.cuda(), 0)
+    blocks = np.full((32, 1, 4), -1, np.int32)
+    for r in range(32):
+        mine = [b for b in range(4) if r >= 16 or r >> b & 1]
+        blocks[r, 0, :len(mine)] = mine
+    q = torch.randn((32, 2, 128), generator=gen).to(TDT.get(dtype, torch.float16))
+    q[0, 1, 0] = float("nan")  # (row 0 lists nothing: zeros)
+    got = cache.sparse_attention(0, q.cuda(), torch.from_numpy(blocks).cuda(), block_size=32,
+                                 n_keys=128, row_pos0=0, kind="full")
+    got = _np(got).reshape(32, 2, 128)
+    if dtype == "i8":
+        ref = X.Cache8(1, 128)
+        ref.store(clean[1].numpy(), clean[0].numpy(), 0)
+        k8, v8 = ref.values
+    else:
+        k8, v8 = (_np(x.to(TDT[dtype])) for x in (clean[1], clean[0]))
+    ends = X.key_ends(32, 128, 0)
+    qn = np.nan_to_num(_np(q))
+    out, weight = X.attention(qn, k8, v8, ends, blocks, 32)
+    bound = X.attention_bound(qn, k8, v8, ends, weight, HALF[dtype], 128,
+                              scales8=_scales(cache, 0))
+    for r in range(32):
+        lists = set(blocks[r, 0].tolist())
+        if 3 in lists or (dtype == "i8" and 1 in lists):
+            assert np.isnan(got[r]).all(), r
+            continue
+        ok = np.ones(128, bool)
+        if 1 in lists:
+            assert (got[r, :, 3] == np.inf).all() and (got[r, :, 4] == -np.inf).all()
+            assert np.isnan(got[r, :, 5]).all()
+            ok[3:6] = False
+        assert (np.abs(got[r] - out[r]) <= bound[r] * 1.001)[:, ok].all(), r
+    assert not got[0].any()
 
 
 def test_attention_over_more_8_bit_keys_than_4_gib_hold():
@@ -429,6 +477,9 @@ def test_select_never_hears_of_hidden_keys():
     (70, 4, 2, 70, 0, (0, 32), "f16", "f32", 64, 3),
     (45, 40, 2, 300, 255, (7, 5), "f16", "f32", 32, 6),       # 20 heads a group
     (600, 8, 4, 600, 0, (0, 1), "f16", "bf16", 32, 4),        # one range, causal
+    (5, 4, 1, 70000, 69995, None, "f16", "f32", 32, 40),      # more blocks than a bitmap holds
+    (1100, 2, 1, 1100, 0, None, "bf16", "bf16", 32, 3),       # 16 rows a tile, four ways
+    (40, 1, 1, 900, 860, (3, 7), "f16", "f32", 64, 5),        # one head a group: 32 rows a tile
 ])
 def test_sparse_attention(dtype, rows, hq, hkv, n_keys, pos0, mask, qdt, odt, block, count):
     if dtype != "i8":
