@@ -47,7 +47,7 @@ constexpr int SEL_QROW = 130;  // doubles of a row in LDS
 template <int THREADS>
 DRT_DEV void add_queries(const uint16_t* __restrict__ q, int q_bf16, int64_t row, int rows, int Hq,
                          int G, int kvh, double* qs) {
-  constexpr int N = 2048 / THREADS;  // head dims a thread
+  constexpr int N = 2048 / THREADS;  // head dims a thread (8 or 2)
   const int r = threadIdx.x * N / 128, d = threadIdx.x * N % 128;
   const uint16_t* p = q + ((row + min(r, rows - 1)) * Hq + kvh * G) * 128 + d;
   double a[N] = {};
@@ -59,9 +59,7 @@ DRT_DEV void add_queries(const uint16_t* __restrict__ q, int q_bf16, int64_t row
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = y[e];
     } else {
-      const uint2 y = *(const uint2*)(p + h * 128);
-      w[0] = y.x;
-      w[1] = y.y;
+      w[0] = *(const uint32_t*)(p + h * 128);
     }
 #pragma unroll
     for (int e = 0; e < N / 2; ++e) {
@@ -89,9 +87,7 @@ DRT_DEV void score_blocks(const float* __restrict__ sums, int b0, int step, int 
   if (b0 < b_end) load(b0);
   ready();
   if (b0 >= b_end) return;
-  double a[32];
-#pragma unroll
-  for (int d = 0; d < 32; ++d) a[d] = qs[i * SEL_QROW + 16 * (d >> 2) + 4 * g + (d & 3)];
+  const double* a = qs + i * SEL_QROW + 4 * g;
   for (; b0 < b_end; b0 += step) {
     double y[32];
 #pragma unroll
@@ -104,11 +100,13 @@ DRT_DEV void score_blocks(const float* __restrict__ sums, int b0, int step, int 
       for (int d = 0; d < 32; ++d) y[d] += (double)x[d >> 2][d & 3];
     }
     load(b0 + step);  // (behind the last: loaded, not used)
+    asm volatile("" ::: "memory");  // (the queries are read block by block: no registers for them all)
     f64x4 acc = f64x4{}, acc1 = f64x4{};  // (two chains: a product waits for the one before it)
 #pragma unroll
     for (int d = 0; d < 32; d += 2) {
-      acc = __builtin_amdgcn_mfma_f64_16x16x4f64(a[d], y[d], acc, 0, 0, 0);
-      acc1 = __builtin_amdgcn_mfma_f64_16x16x4f64(a[d + 1], y[d + 1], acc1, 0, 0, 0);
+      const double* e = a + 16 * (d >> 2) + (d & 3);
+      acc = __builtin_amdgcn_mfma_f64_16x16x4f64(e[0], y[d], acc, 0, 0, 0);
+      acc1 = __builtin_amdgcn_mfma_f64_16x16x4f64(e[1], y[d + 1], acc1, 0, 0, 0);
     }
     acc += acc1;
     if (b0 + i < b_end) {
@@ -200,10 +198,10 @@ struct SelArgs {
   int32_t* blocks;     // [rows][Hkv][count]
 };
 
-// Both steps for 16 rows of one K/V head in a work-group of eight waves, the keys in LDS (RB rounds of 64
+// Both steps for 16 rows of one K/V head in a work-group of 16 waves, the keys in LDS (RB rounds of 64
 // blocks). 1000 rows x 4 heads, 500 blocks: FUSED_US us; in two launches, with the keys in memory, 22 + 14.
 template <int RB>
-__global__ __launch_bounds__(512, 2) void select_kernel(const SelArgs x) {
+__global__ __launch_bounds__(1024, 4) void select_kernel(const SelArgs x) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = blockIdx.x % x.Hkv, r0 = blockIdx.x / x.Hkv * 16;
@@ -213,16 +211,16 @@ __global__ __launch_bounds__(512, 2) void select_kernel(const SelArgs x) {
   // the last row sees the most: blocks at or beyond its last `local` are never scored
   const int nb_last = blocks_of(x.row0 + r0 + rows - 1, x.where, x.sel.block);
   const int b_end = nb_last <= x.sel.count ? 0 : nb_last - x.sel.local;
-  score_blocks(x.sums + kvh * x.sums_head_stride, wave * 16, 128, b_end, x.sel.block >> 5, qs,
+  score_blocks(x.sums + kvh * x.sums_head_stride, wave * 16, 256, b_end, x.sel.block >> 5, qs,
                [&] {
-                 add_queries<512>(x.q, x.q_bf16, x.row0 + r0, rows, x.Hq, G, kvh, qs);
+                 add_queries<1024>(x.q, x.q_bf16, x.row0 + r0, rows, x.Hq, G, kvh, qs);
                  __syncthreads();
                },
                [&](int b, int r, uint64_t k) { keys[r][b] = k; });
   __syncthreads();
-  for (int r = wave; r < rows; r += 8) {
-    const int64_t row = x.row0 + r0 + r;
-    choose_row<RB>([&](int b) { return keys[r][b]; }, blocks_of((int)row, x.where, x.sel.block), x.sel,
+  if (wave < rows) {
+    const int64_t row = x.row0 + r0 + wave;
+    choose_row<RB>([&](int b) { return keys[wave][b]; }, blocks_of((int)row, x.where, x.sel.block), x.sel,
                    x.blocks + (row * x.Hkv + kvh) * x.sel.count);
   }
 }
@@ -289,9 +287,9 @@ void select_blocks(const void* q, bool q_bf16, const float* sums, int64_t sums_h
     const int64_t wgs = (int64_t)((n_rows + 15) / 16) * Hkv;
     require(wgs < ((int64_t)1 << 31), "select_blocks: too many rows for one call");
     const dim3 grid((unsigned)wgs);
-    if (nb <= 256) hipLaunchKernelGGL(select_kernel<4>, grid, dim3(512), 0, s, a);
-    else if (nb <= 512) hipLaunchKernelGGL(select_kernel<8>, grid, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL(select_kernel<16>, grid, dim3(512), 0, s, a);
+    if (nb <= 256) hipLaunchKernelGGL(select_kernel<4>, grid, dim3(1024), 0, s, a);
+    else if (nb <= 512) hipLaunchKernelGGL(select_kernel<8>, grid, dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL(select_kernel<16>, grid, dim3(1024), 0, s, a);
     DRT_HIP(hipGetLastError());
     return;
   }
