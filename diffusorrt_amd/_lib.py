@@ -129,7 +129,7 @@ SIGNATURES = {
     "drt_op_lm_head_score": (_I32, [_VP, _VP, _VP, _I32, _I32, _I32, _VP, C.c_float, _U64, _I32,
                                     _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
     "drt_op_kv8_store": (_I32, [_VP, _VP, _I32, _I32, _I32, _I32, _VP, _I64, _VP, _VP, _VP]),
-    "drt_op_kv_sums": (_I32, [_VP, _I64, _I32, _I32, _I32, _I32, _VP, _VP]),
+    "drt_op_kv16_store": (_I32, [_VP, _VP, _I32, _I32, _I32, _I32, _VP, _I64, _I32, _VP, _VP]),
     "drt_op_kv_load": (_I32, [_VP, _I64, _I32, _VP, _I32, _I32, _I32, _VP, _VP, _I32, _VP]),
     "drt_op_attention_kv8_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32]),
     "drt_op_attention_kv8": (_I32, [_VP, _I32, _VP, _I64, _VP, _I32, _I32, _I32, _I32, _I32,

@@ -171,18 +171,87 @@ __global__ __launch_bounds__(256) void kv_load_kernel(const uint8_t* __restrict_
   }
 }
 
-// The keys of a 16-bit tile added up, in 64 bits and rounded once (an 8-bit tile's sums are
-// the store's own). One 128-thread work-group per (tile, head), thread = head dim.
-template <int DT>
-__global__ __launch_bounds__(128) void kv_sums_kernel(const uint8_t* __restrict__ kv,
-                                                      int64_t head_stride_bytes, int t0,
-                                                      float* __restrict__ sums) {
-  const int t = t0 + blockIdx.x, h = blockIdx.y, hd = threadIdx.x;
-  const uint8_t* tile = kv + h * head_stride_bytes + (int64_t)t * 2 * KV8_TILE;
-  double s = 0.0;
+// Rows into a 16-bit cache, as kv_pack_kernel (attention.hip) writes them, and the touched tiles' keys added
+// up, the rows that stay among them, in 64 bits and rounded once. One 256-thread work-group per
+// (tile, head): thread (kk, c) has head dims 8 c .. + 8 of keys kk and kk + 16; of V the eight keys that share 16 bytes.
+template <typename T> DRT_DEV T kv16_of(float f);
+template <> DRT_DEV _Float16 kv16_of<_Float16>(float f) { return (_Float16)f; }
+template <> DRT_DEV __bf16 kv16_of<__bf16>(float f) { return (__bf16)f; }
+
+template <typename T, bool SRC_BF16>
+__global__ __launch_bounds__(256) void kv16_store_kernel(const void* __restrict__ k_src,
+                                                         const void* __restrict__ v_src, int n,
+                                                         int Hkv, int pos0, T* __restrict__ kv,
+                                                         int64_t kv_head_stride,
+                                                         float* __restrict__ sums) {
+  const int t = (pos0 >> 5) + blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
+  const int64_t row_t = (int64_t)32 * t - pos0;  // source row of the tile's key 0 (may be negative)
+  T* tile = kv + h * kv_head_stride + (int64_t)t * KV8_TILE;
+  const int64_t stride = (int64_t)Hkv * 128;
+  __shared__ double part[4][128];
+  auto valid = [&](int kk) { return row_t + kk >= 0 && row_t + kk < n; };
+  auto at = [&](int kk) { return (row_t + kk) * stride + h * 128; };
+  double sum[8] = {};
 #pragma unroll
-  for (int kk = 0; kk < 32; ++kk) s += (double)kv_value<DT>(tile, kv16_k_at(kk, hd), 1.f);
-  sums[(h * (head_stride_bytes / (2 * KV8_TILE)) + t) * 128 + hd] = (float)s;
+  for (int i = 0; i < 2; ++i) {
+    const int kk = (tid >> 4) + 16 * i, c = tid & 15;
+    T o[8];
+    if (valid(kk)) {
+      if (SRC_BF16) {
+        const u32x4 w = *(const u32x4_e*)((const uint16_t*)k_src + at(kk) + 8 * c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o[2 * e] = kv16_of<T>(bf16_bits_to_float(w[e] & 0xffffu));
+          o[2 * e + 1] = kv16_of<T>(bf16_bits_to_float(w[e] >> 16));
+        }
+      } else {
+        const float* p = (const float*)k_src + at(kk) + 8 * c;
+        const f32x4 a = *(const f32x4_e*)p, b = *(const f32x4_e*)(p + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o[e] = kv16_of<T>(a[e]);
+          o[4 + e] = kv16_of<T>(b[e]);
+        }
+      }
+      *(u32x4*)(tile + (c * 32 + kk) * 8) = __builtin_bit_cast(u32x4, o);
+    } else {
+      __builtin_memcpy(o, tile + (c * 32 + kk) * 8, 16);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] += (double)(float)o[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {  // the four keys of this wave's lanes
+    sum[e] += __shfl_xor(sum[e], 16, 64);
+    sum[e] += __shfl_xor(sum[e], 32, 64);
+    if ((tid & 63) < 16) part[tid >> 6][8 * (tid & 15) + e] = sum[e];
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int it = tid + 256 * i, hd = it & 127, kh = it >> 8, hh = (it >> 7) & 1;
+    T o[8];
+    bool all = true;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {  // slot j holds key 16 kh + 4 hh + (j & 3) + 8 (j >> 2)
+      const int kk = 16 * kh + 4 * hh + (j & 3) + 8 * (j >> 2);
+      all = all && valid(kk);
+      const int64_t s = at(valid(kk) ? kk : (int)-row_t) + hd;  // (source row 0: never stored)
+      o[j] = kv16_of<T>(SRC_BF16 ? bf16_bits_to_float(((const uint16_t*)v_src)[s])
+                                 : ((const float*)v_src)[s]);
+    }
+    T* dst = tile + 4096 + ((((hd >> 5) * 2 + kh) * 2 + hh) * 32 + (hd & 31)) * 8;
+    if (all) {
+      *(u32x4*)dst = __builtin_bit_cast(u32x4, o);
+    } else {  // the tile's other keys stay as they are
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (valid(16 * kh + 4 * hh + (j & 3) + 8 * (j >> 2))) dst[j] = o[j];
+    }
+  }
+  __syncthreads();
+  if (tid < 128)
+    sums[(h * (kv_head_stride / KV8_TILE) + t) * 128 + tid] =
+        (float)((part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]));
 }
 
 unsigned tiles_of(int pos0, int n) { return (unsigned)(((int64_t)pos0 + n - 1) / 32 - pos0 / 32 + 1); }
@@ -219,15 +288,18 @@ void kv_load(KvType type, const void* kv, int64_t head_stride, const float* scal
   DRT_HIP(hipGetLastError());
 }
 
-void kv_sums(bool bf16, const void* kv, int64_t head_stride, int Hkv, int pos0, int n, float* sums,
-             hipStream_t s) {
+void kv16_store(bool kv_bf16, const void* k, const void* v, bool src_bf16, int n, int Hkv, int pos0,
+                void* kv, int64_t head_stride, float* sums, hipStream_t s) {
   const dim3 grid(tiles_of(pos0, n), (unsigned)Hkv);
-  if (bf16)
-    hipLaunchKernelGGL(kv_sums_kernel<2>, grid, dim3(128), 0, s, (const uint8_t*)kv,
-                       2 * head_stride, pos0 / 32, sums);
-  else
-    hipLaunchKernelGGL(kv_sums_kernel<1>, grid, dim3(128), 0, s, (const uint8_t*)kv,
-                       2 * head_stride, pos0 / 32, sums);
+#define DRT_KV16(T, B)                                                                        \
+  hipLaunchKernelGGL((kv16_store_kernel<T, B>), grid, dim3(256), 0, s, k, v, n, Hkv, pos0,    \
+                     (T*)kv, head_stride, sums)
+  if (kv_bf16) {
+    if (src_bf16) DRT_KV16(__bf16, true); else DRT_KV16(__bf16, false);
+  } else {
+    if (src_bf16) DRT_KV16(_Float16, true); else DRT_KV16(_Float16, false);
+  }
+#undef DRT_KV16
   DRT_HIP(hipGetLastError());
 }
 

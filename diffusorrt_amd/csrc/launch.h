@@ -217,8 +217,8 @@ void kv8_store(const void* k, const void* v, bool src_bf16, int n, int Hkv, int 
                int64_t head_stride, float* scales, float* sums, hipStream_t s);
 void kv_load(KvType type, const void* kv, int64_t head_stride, const float* scales, int n, int Hkv,
              int pos0, void* k, void* v, bool out_bf16, hipStream_t s);
-void kv_sums(bool bf16, const void* kv, int64_t head_stride, int Hkv, int pos0, int n, float* sums,
-             hipStream_t s);
+void kv16_store(bool kv_bf16, const void* k, const void* v, bool src_bf16, int n, int Hkv, int pos0,
+                void* kv, int64_t head_stride, float* sums, hipStream_t s);
 // How an attention over the cache is cut: key ranges (splits), whose parts are joined by a second
 // launch, and work-groups of query tiles.
 struct CachePlan {

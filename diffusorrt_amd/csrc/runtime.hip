@@ -2829,13 +2829,17 @@ int32_t drt_op_kv8_store(const void* k, const void* v, int32_t src_dtype, int32_
   });
 }
 
-int32_t drt_op_kv_sums(const void* cache, int64_t head_stride, int32_t kv_dtype, int32_t n,
-                       int32_t hkv, int32_t pos0, float* sums, void* stream) {
+int32_t drt_op_kv16_store(const void* k, const void* v, int32_t src_dtype, int32_t n, int32_t hkv,
+                          int32_t pos0, void* cache, int64_t head_stride, int32_t kv_dtype,
+                          float* sums, void* stream) {
   return guarded([&] {
-    require(cache && sums && n > 0 && hkv > 0 && hkv <= 65535 && pos0 >= 0, "bad kv_sums arguments");
-    require(kv_dtype == DRT_F16 || kv_dtype == DRT_BF16, "kv_sums cache must be F16 or BF16");
-    require_kv(cache, head_stride, nullptr, kv_dtype, (int64_t)pos0 + n, "kv_sums");
-    kv_sums(kv_dtype == DRT_BF16, cache, head_stride, hkv, pos0, n, sums, as_stream(stream));
+    require(k && v && cache && sums && n > 0 && hkv > 0 && hkv <= 65535 && pos0 >= 0,
+            "bad kv16_store arguments");
+    require(src_dtype == DRT_F32 || src_dtype == DRT_BF16, "kv16_store source must be F32 or BF16");
+    require(kv_dtype == DRT_F16 || kv_dtype == DRT_BF16, "kv16_store cache must be F16 or BF16");
+    require_kv(cache, head_stride, nullptr, kv_dtype, (int64_t)pos0 + n, "kv16_store");
+    kv16_store(kv_dtype == DRT_BF16, k, v, src_dtype == DRT_BF16, n, hkv, pos0, cache, head_stride,
+               sums, as_stream(stream));
   });
 }
 

@@ -300,10 +300,8 @@ class PrefixKVCache:
                 _launch(torch, lib.drt_op_kv8_store, self._index, k.data_ptr(), v.data_ptr(), src,
                         n, self.kv_heads, pos0, data, self.head_stride, self._scales(layer), sums)
             else:
-                _launch(torch, lib.drt_op_kv_pack, self._index, k.data_ptr(), v.data_ptr(), src,
-                        n, self.kv_heads, pos0, data, self.head_stride, self.kv_dtype)
-                _launch(torch, lib.drt_op_kv_sums, self._index, data, self.head_stride,
-                        self.kv_dtype, n, self.kv_heads, pos0, sums)
+                _launch(torch, lib.drt_op_kv16_store, self._index, k.data_ptr(), v.data_ptr(), src,
+                        n, self.kv_heads, pos0, data, self.head_stride, self.kv_dtype, sums)
             self.length = max(self.length, pos0 + n)
             return
         layer_view = self.data[layer]

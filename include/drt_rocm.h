@@ -308,9 +308,10 @@ int32_t drt_op_lm_head_score(const void* qw, const void* sb, const void* wb, int
 int32_t drt_op_kv8_store(const void* k, const void* v, int32_t src_dtype, int32_t n, int32_t hkv,
                          int32_t pos0, void* cache, int64_t head_stride, float* scales, float* sums,
                          void* stream);
-/* The same sums for the tiles of positions pos0..pos0+n-1 of a 16-bit cache (drt_op_kv_pack). */
-int32_t drt_op_kv_sums(const void* cache, int64_t head_stride, int32_t kv_dtype, int32_t n,
-                       int32_t hkv, int32_t pos0, float* sums, void* stream);
+/* drt_op_kv_pack that keeps a 16-bit cache's sums with it. */
+int32_t drt_op_kv16_store(const void* k, const void* v, int32_t src_dtype, int32_t n, int32_t hkv,
+                          int32_t pos0, void* cache, int64_t head_stride, int32_t kv_dtype,
+                          float* sums, void* stream);
 /* Rows of a cache of any type (DRT_I8, DRT_F16, DRT_BF16; scales for DRT_I8) as values:
  * k, v [n, hkv, 128] of out_dtype (DRT_F32 or DRT_BF16). */
 int32_t drt_op_kv_load(const void* cache, int64_t head_stride, int32_t kv_dtype, const float* scales,
@@ -332,7 +333,7 @@ int32_t drt_op_attention_kv8(const void* q, int32_t q_dtype, const void* cache, 
  * of those between, the ones whose keys' sum has the largest product with the sum of the head
  * group's queries (in 64 bits; equal ones: the lower block; a NaN is the largest). Blocks ascend in
  * blocks [rows, hkv, count]; a row that sees fewer lists them all, then -1. sums: [hkv][sums_tiles][128] of
- * drt_op_kv8_store or drt_op_kv_sums. Neither call's overlapping ones may share a workspace. */
+ * drt_op_kv8_store or drt_op_kv16_store. Neither call's overlapping ones may share a workspace. */
 size_t drt_op_select_blocks_workspace_bytes(int32_t rows, int32_t hkv, int32_t n_keys,
                                             int32_t block_size);
 int32_t drt_op_select_blocks(const void* q, int32_t q_dtype, const float* sums, int64_t sums_tiles,

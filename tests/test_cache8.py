@@ -86,10 +86,10 @@ def _store(**kw):
     return "drt_op_kv8_store", list(a.values())
 
 
-def _sums(**kw):
-    a = dict(cache=P, stride=8192 * 4, dtype=_lib.F16, n=32, hkv=2, pos0=0, sums=P,
-             stream=None) | kw
-    return "drt_op_kv_sums", list(a.values())
+def _store16(**kw):
+    a = dict(k=P, v=P, src=_lib.F32, n=32, hkv=2, pos0=0, cache=P, stride=8192 * 4,
+             dtype=_lib.F16, sums=P, stream=None) | kw
+    return "drt_op_kv16_store", list(a.values())
 
 
 def _load(**kw):
@@ -125,8 +125,10 @@ REFUSED = (
         {"n": -1}, {"hkv": 0}, {"hkv": 70000}, {"pos0": -1}, {"pos0": 97}, {"n": 129},
         {"pos0": 2**31 - 1}, {"stride": 8192 * 4 + 1}, {"stride": 0}, {"cache": P + 8},
         {"scales": P + 4})]
-    + [_sums(**kw) for kw in (
-        {"cache": None}, {"sums": None}, {"dtype": _lib.I8}, {"n": 0}, {"pos0": 97}, {"pos0": -1})]
+    + [_store16(**kw) for kw in (
+        {"k": None}, {"v": None}, {"cache": None}, {"sums": None}, {"dtype": _lib.I8}, {"n": 0},
+        {"src": _lib.F16}, {"hkv": 0}, {"hkv": 70000}, {"pos0": 97}, {"pos0": -1},
+        {"stride": 8192 * 4 - 8}, {"cache": P + 8})]
     + [_load(**kw) for kw in (
         {"cache": None}, {"k": None}, {"v": None}, {"scales": None}, {"dtype": _lib.F32},
         {"out": _lib.F16}, {"n": 0}, {"pos0": 97}, {"k": P + 4})]
