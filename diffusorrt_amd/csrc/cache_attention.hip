@@ -27,7 +27,15 @@
 // LDS bitmap, CA_WIN blocks at a time, so a list is a set, whatever its order and repetitions.
 // Neighbouring queries mostly choose the same blocks: a block is then loaded and made operands once
 // for all of them, and every column of the products is in use (one wave per row, 16 columns of
-// which G are used: 2048 rows x 16 heads, 16 blocks of 64 of 32768 keys, 226 us; 57 here).
+// which G are used: 2048 rows x 16 heads, 16 blocks of 64 of 32768 keys, 226 us; 56 here).
+//
+// Bound. A long cache's codes (32 rows x 16 heads over 131072 keys x 8 heads, 268 MB: 56 us, 4.8
+// TB/s, what a large copy reaches). Many rows: the instructions of the softmax and of making
+// operands, 62 % of the VALU's time beside 40 % of the matrix units' (2048 rows x 16 heads over 4096
+// keys under the mask: 62 us, 0.83 PFLOP/s). A block of 32 rows x 16 heads over 8224 keys: 12.9 us, of
+// which 7 are there without any tile (launch, queries, the ways' meeting, parts out), and
+// part_combine_kernel's 4. Three waves a SIMD spill; a larger window of blocks in LDS for two (60 us
+// for 57), weights' sums by other chains or by dot products did not pay.
 #include "kv8.h"
 #include "launch.h"
 
@@ -75,8 +83,8 @@ template <int DT, int N> DRT_DEV typename CacheT<DT>::vec ca_operand(const u32x4
 }
 
 // A tile's values (16 bits) that are not finite, taken out of its V registers: in their place
-// every query column that sees one's key gets infinity or NaN in that head dim, as p * V would be, and the
-// others nothing, where 0 * V would be NaN. An indicator product for each of the three.
+// every query column that sees one's key gets infinity or NaN in that head dim, as p * V would be,
+// and the others nothing, where 0 * V would be NaN. An indicator product for each of the three.
 template <int DT>
 DRT_DEV void ca_values_apart(u32x4 (&vr)[8], int key0, int end, int lane, f32x16 (&o)[4]) {
   typedef CacheT<DT> T;
@@ -104,7 +112,9 @@ DRT_DEV void ca_values_apart(u32x4 (&vr)[8], int key0, int end, int lane, f32x16
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t z = (y >> (16 * h)) & 0xffffu;
-            const bool hit = kind == 0 ? (z & 0x7fffu) > EXP : kind == 1 ? z == EXP : z == (EXP | 0x8000u);
+            const bool hit = kind == 0   ? (z & 0x7fffu) > EXP
+                             : kind == 1 ? z == EXP
+                                         : z == (EXP | 0x8000u);
             mark |= hit ? ONE << (16 * h) : 0u;
           }
           w[e] = mark;
@@ -120,7 +130,8 @@ DRT_DEV void ca_values_apart(u32x4 (&vr)[8], int key0, int end, int lane, f32x16
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t y = vr[i][e];
-      const uint32_t keep = ((y & EXP) == EXP ? 0u : 0xffffu) | ((y & (EXP << 16)) == EXP << 16 ? 0u : 0xffff0000u);
+      const uint32_t keep = ((y & EXP) == EXP ? 0u : 0xffffu) |
+                            ((y & (EXP << 16)) == EXP << 16 ? 0u : 0xffff0000u);
       vr[i][e] = y & keep;
     }
 }
@@ -262,7 +273,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   const int end_row = min(SPARSE ? row0 + RPT - 1 : row_of(wv0 + QT * 32 - 1), last_row);
   const int wave_full = key_end_of(min(row_of(wv0), last_row), where);
   const int wave_end = key_end_of(end_row, where);
-  const uint32_t my_row = SPARSE ? 1u << ((lane & 31) / GC & 31) : 0u;  // (32 columns at most: see exists)
+  const uint32_t my_row = SPARSE ? 1u << ((lane & 31) / GC & 31) : 0u;
   const uint32_t all_rows = SPARSE ? (uint32_t)((1ull << (end_row - row0 + 1)) - 1) : 0u;
 
   const uint8_t* base = x.kv + kvh * x.head_stride + lane * 16;
@@ -304,12 +315,14 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
         const vec kf = ca_operand<DT>(kr, i);
 #pragma unroll
         for (int j = 0; j < QT; ++j)
-          s[j] = T::mma(kf, HOLD ? qr[HOLD ? i : 0] : *(const vec*)(ql + j * 32 * CA_QROW + 16 * i), s[j]);
+          s[j] = T::mma(
+              kf, HOLD ? qr[HOLD ? i : 0] : *(const vec*)(ql + j * 32 * CA_QROW + 16 * i), s[j]);
       }
 #pragma unroll
       for (int i = 0; i < LD; ++i) kr[i] = *(const u32x4*)(p + i * 1024);
       __builtin_amdgcn_s_setprio(0);
-      asm volatile("" ::: "memory");  // (a scalar load among the reads of LDS would be waited for with them)
+      // (a scalar load among the reads of LDS would be waited for with them)
+      asm volatile("" ::: "memory");
       if (DT == 0) st = scales_of(t);
       const bool bad = DT == 0 && !(sk + sv < INFINITY);  // a NaN tile: so is every row that sees it
       // A row that does not list the tile's block weighs it nothing: by its exponent's offset where
@@ -330,8 +343,9 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
           for (int r = 0; r < 16; ++r) s[j][r] = key0 + mfma_row(r, lane) < end ? s[j][r] : -INFINITY;
         }
       }
-      const float lb = DT != 0 || bad ? 0.f : (float)((int)(__float_as_uint(sv) >> 23) - 127);  // sv = 2^lb
-      const float inv_sv = DT != 0 ? 1.f : bad ? 0.f : __uint_as_float((254u << 23) - __float_as_uint(sv));
+      const uint32_t vb = __float_as_uint(sv);  // sv = 2^lb
+      const float lb = DT != 0 || bad ? 0.f : (float)((int)(vb >> 23) - 127);
+      const float inv_sv = DT != 0 ? 1.f : bad ? 0.f : __uint_as_float((254u << 23) - vb);
       vec pf[QT][2];
 #pragma unroll
       for (int j = 0; j < QT; ++j) {
@@ -403,7 +417,8 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   if constexpr (!SPARSE) {
     const int64_t n_tiles = (where.n_keys + 31) >> 5;
     const int t0 = (int)(n_tiles * split / x.splits) + kw;
-    const int t_end = !exists(wv0) ? 0 : min((int)(n_tiles * (split + 1) / x.splits), (wave_end + 31) >> 5);
+    const int t_end = !exists(wv0) ? 0
+                                   : min((int)(n_tiles * (split + 1) / x.splits), (wave_end + 31) >> 5);
     const int n = (t_end - t0 + KW - 1) / KW;
     first(n, t0);
     stage();
@@ -574,9 +589,10 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   }
 }
 
-// The key ranges of a (row, head) joined, one wave each: lane (sg, ch) adds head dims 8 ch .. + 8 of ranges sg,
-// sg + 4, ..., all of a batch's loads before their use, and the four groups meet by lane exchanges.
-// A row without a key gives zeros.
+// The key ranges of a (row, head) joined, one wave each: lane (sg, ch) adds head dims 8 ch .. + 8 of
+// ranges sg, sg + 4, ..., all of a batch's loads before their use, and the four groups meet by lane
+// exchanges. A row without a key gives zeros. Bound by its launch and one round of loads: 32 rows x 16
+// heads, 32 ranges (8.5 MB, of L2) 4.0 us, nine rows x 28 heads 2.5; batches of eight no faster.
 __global__ __launch_bounds__(128) void part_combine_kernel(const float* __restrict__ o_part,
                                                            const float* __restrict__ ml_part,
                                                            int splits, int64_t n,
@@ -616,7 +632,8 @@ __global__ __launch_bounds__(128) void part_combine_kernel(const float* __restri
     }
     m = mb;
   }
-  const float mm = fmaxf(fmaxf(m, __shfl_xor(m, 16, 64)), fmaxf(__shfl_xor(m, 32, 64), __shfl_xor(m, 48, 64)));
+  const float mm = fmaxf(fmaxf(m, __shfl_xor(m, 16, 64)),
+                         fmaxf(__shfl_xor(m, 32, 64), __shfl_xor(m, 48, 64)));
   const float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm);
   a0 *= w;
   a1 *= w;
@@ -639,9 +656,10 @@ __global__ __launch_bounds__(128) void part_combine_kernel(const float* __restri
     u32x4 y;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      y[e] = (uint32_t)float_to_bf16_bits(a0[2 * e]) | ((uint32_t)float_to_bf16_bits(a0[2 * e + 1]) << 16);
-      y[2 + e] =
-          (uint32_t)float_to_bf16_bits(a1[2 * e]) | ((uint32_t)float_to_bf16_bits(a1[2 * e + 1]) << 16);
+      y[e] = (uint32_t)float_to_bf16_bits(a0[2 * e]) |
+             ((uint32_t)float_to_bf16_bits(a0[2 * e + 1]) << 16);
+      y[2 + e] = (uint32_t)float_to_bf16_bits(a1[2 * e]) |
+                 ((uint32_t)float_to_bf16_bits(a1[2 * e + 1]) << 16);
     }
     *(u32x4*)((uint16_t*)out + at) = y;
   } else {
@@ -666,8 +684,9 @@ CachePlan plan_attention8(int n_rows, int Hq, int Hkv, int n_keys) {
   const int64_t qtiles = ((int64_t)n_rows * (Hq / Hkv) + 31) / 32;
   // Many queries: two query tiles a wave (a tile's codes made operands once for both), four key
   // ways in a work-group of their own, so that work-groups are as many as can be (2048 rows x 16
-  // heads over 4096 keys: 72 us; two and one key ways, which need key ranges to fill the chip:
-  // 101, 110). Few: eight waves over the one, two or four query tiles.
+  // heads over 4096 keys: 72 us at that step; two and one key ways, which need key ranges to fill the
+  // chip: 101, 110). Few: eight waves over the one, two or four query tiles (two tiles a wave: 32 rows
+  // over 8224 keys 18 us for 12.6, over 131072 keys 66 for 57; a wave waits on what it holds).
   p.wide = qtiles > 4;
   p.qw = p.wide || qtiles == 1 ? 1 : qtiles == 2 ? 2 : 4;
   const int kw = p.wide ? 4 : 8 / p.qw, per = p.wide ? 2 : p.qw;  // (query tiles of a work-group)
@@ -685,12 +704,12 @@ CachePlan plan_sparse(int n_rows, int Hq, int Hkv, int count, int block) {
   CachePlan p;
   const int G = Hq / Hkv, rows = 32 / std::min(G, 32), heads = (G + 31) / 32;
   p.groups = ((int64_t)n_rows + rows - 1) / rows;
-  // Few work-groups: as many key ranges as give every CU one, of four of a list's tiles at least (9 rows x
-  // 28 heads, 16 blocks of 64: 12.4 us; of eight 13.3, of 16 16.2)
+  // Few work-groups: as many key ranges as give every CU one, of four of a list's tiles at least (9
+  // rows x 28 heads, 16 blocks of 64: 12.4 us; of eight 13.3, of 16 16.2)
   const int64_t wgs = p.groups * Hkv * heads, tiles = (int64_t)count * (block / 32);
   p.wide = wgs >= 512;
-  // (As few as 16 tiles of a tile's rows cost less than the second launch: one row x 28 heads, 8 blocks of
-  // 64 9.4 us, with key ranges 10.1; 16 blocks 11.2 and 10.2.)
+  // (As few as 16 tiles of a tile's rows cost less than the second launch: one row x 28 heads, 8
+  // blocks of 64 9.4 us, with key ranges 10.1; 16 blocks 11.2 and 10.2.)
   p.splits = p.wide || tiles * std::min(n_rows, rows) <= 16
                  ? 1
                  : (int)std::max<int64_t>(1, std::min<int64_t>({256 / wgs, (tiles + 3) / 4, 64}));
@@ -725,12 +744,13 @@ static CaArgs args_of(KvType type, const void* q, bool q_bf16, const void* kv_la
   return a;
 }
 
+#define DRT_CA1(DT, QT, QW, KW, OUT, SPARSE)                                                      \
+  hipLaunchKernelGGL((cache_attn_kernel<DT, QT, QW, KW, OUT, SPARSE>), grid, dim3(64 * QW * KW), 0, \
+                     s, a)
 #define DRT_CA(DT, QT, QW, KW, SPARSE)                                                            \
   do {                                                                                            \
-    if (p.splits == 1)                                                                            \
-      hipLaunchKernelGGL((cache_attn_kernel<DT, QT, QW, KW, true, SPARSE>), grid, dim3(64 * QW * KW), 0, s, a); \
-    else                                                                                          \
-      hipLaunchKernelGGL((cache_attn_kernel<DT, QT, QW, KW, false, SPARSE>), grid, dim3(64 * QW * KW), 0, s, a); \
+    if (p.splits == 1) DRT_CA1(DT, QT, QW, KW, true, SPARSE);                                     \
+    else DRT_CA1(DT, QT, QW, KW, false, SPARSE);                                                  \
   } while (0)
 
 void attention8(const void* q, bool q_bf16, const void* kv_layer, int64_t kv_head_stride,
@@ -767,5 +787,6 @@ void sparse_attention(KvType type, const void* q, bool q_bf16, const void* kv_la
   if (p.splits > 1) part_combine(part, a.ml_part, p.splits, (int64_t)n_rows * Hq, out, out_bf16, s);
 }
 #undef DRT_CA
+#undef DRT_CA1
 
 }  // namespace drt

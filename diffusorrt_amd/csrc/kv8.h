@@ -32,8 +32,9 @@ DRT_DEV int kv8_v_at(int kk, int hd) {
 // anyway, and 128 times the sum of x is taken off in fp32 (x the query: once per query vector; x the
 // weights: one running sum). The exact fp16 c (1024 + b, less 1152) takes twice the instructions.
 DRT_DEV f16x8 kv8_to_f16(uint32_t lo, uint32_t hi) {
-  const u32x4 r = {__builtin_amdgcn_perm(lo, lo, 0x0c050c04u), __builtin_amdgcn_perm(lo, lo, 0x0c070c06u),
-                   __builtin_amdgcn_perm(hi, hi, 0x0c050c04u), __builtin_amdgcn_perm(hi, hi, 0x0c070c06u)};
+  const u32x4 r = {
+      __builtin_amdgcn_perm(lo, lo, 0x0c050c04u), __builtin_amdgcn_perm(lo, lo, 0x0c070c06u),
+      __builtin_amdgcn_perm(hi, hi, 0x0c050c04u), __builtin_amdgcn_perm(hi, hi, 0x0c070c06u)};
   return __builtin_bit_cast(f16x8, r);
 }
 constexpr float KV8_POW = 16777216.f;  // 2^24

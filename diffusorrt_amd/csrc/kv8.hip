@@ -8,13 +8,17 @@ namespace {
 // One 256-thread work-group per (tile, K/V head); thread t holds 16 head dims of key t / 8, of K
 // and of V: the new rows from their source, the tile's other rows as they read. The largest
 // magnitudes choose the powers of two (a comparison of bits, in which NaN and infinities are
-// the largest), every value is rounded once (x / scale is exact), and the codes meet in LDS, from where the
-// tile leaves in 16-byte pieces.
+// the largest), every value is rounded once (x / scale is exact), and the codes meet in LDS, from
+// where the tile leaves in 16-byte pieces.
 //   e = the least integer >= -40 with max <= 127 * 2^e;  code = rint(x * 2^-e)
 // A power of two, not max / 127: a tile that is stored to again is quantized anew from
-// what it reads as, which with these scales is one more rounding only when e rises, each time to half
-// the resolution or less, so any number of stores stays within one step of what they wrote
+// what it reads as, which with these scales is one more rounding only when e rises, each time to
+// half the resolution or less, so any number of stores stays within one step of what they wrote
 // (1/2 + 1/4 + ...); and x / scale never falls on the wrong side of a rounding.
+// Bound: the rows read and the codes written (131072 bf16 rows x 8 heads: 805 MB in 207 us, 3.9 of
+// a copy's 4.7 TB/s; 2000 fp32 rows x 4 heads 7.0 us); of a block of 32 rows, 5.5 us, the chain of a
+// launch, the loads, two barriers and the stores. A work-group has a tile alone: its scale
+// needs every row of it, and no other work-group's.
 template <bool SRC_BF16>
 __global__ __launch_bounds__(256) void kv8_store_kernel(
     const void* __restrict__ k_src, const void* __restrict__ v_src, int n, int Hkv, int pos0,
@@ -111,7 +115,9 @@ __global__ __launch_bounds__(256) void kv8_store_kernel(
 }
 
 // Rows [pos0, pos0 + n) of a cache back as [n][Hkv][128] values. One 256-thread work-group
-// per (tile, head), which reads the tile whole.
+// per (tile, head), which reads the tile whole: 16-byte pieces by way of LDS, whose few rows of a
+// ragged end cost no launch of their own. Bound as the store is: 32 rows x 8 heads 3.1 us, a launch;
+// 2000 x 4 heads to fp32 4.3 us, 10.2 MB.
 // DT: 0 = 8-bit, 1 = fp16, 2 = bf16.
 DRT_DEV int kv16_k_at(int kk, int hd) { return ((hd >> 3) * 32 + kk) * 8 + (hd & 7); }
 DRT_DEV int kv16_v_at(int kk, int hd) {
@@ -171,9 +177,11 @@ __global__ __launch_bounds__(256) void kv_load_kernel(const uint8_t* __restrict_
   }
 }
 
-// Rows into a 16-bit cache, as kv_pack_kernel (attention.hip) writes them, and the touched tiles' keys added
-// up, the rows that stay among them, in 64 bits and rounded once. One 256-thread work-group per
-// (tile, head): thread (kk, c) has head dims 8 c .. + 8 of keys kk and kk + 16; of V the eight keys that share 16 bytes.
+// Rows into a 16-bit cache, as kv_pack_kernel (attention.hip) writes them, and the touched tiles'
+// keys added up, the rows that stay among them, in 64 bits and rounded once. One 256-thread
+// work-group per (tile, head): thread (kk, c) has head dims 8 c .. + 8 of keys kk and kk + 16; of V
+// the eight keys that share 16 bytes. One launch for both: 9 rows x 4 heads 4.3 us, all latency (a
+// sum kernel behind the store 3.4 + 1.7, and the gap between them).
 template <typename T> DRT_DEV T kv16_of(float f);
 template <> DRT_DEV _Float16 kv16_of<_Float16>(float f) { return (_Float16)f; }
 template <> DRT_DEV __bf16 kv16_of<__bf16>(float f) { return (__bf16)f; }

@@ -1,8 +1,8 @@
 // Which blocks of keys each query row reads in a block-sparse attention (cache_attention.hip).
 //
 // Blocks are `block` keys (whole tiles of 32) of a K/V head. A row's blocks for a K/V head are
-// its first `sinks`, its last `local` (the last one it sees among them) and, of those between, the ones with
-// the largest
+// its first `sinks`, its last `local` (the last one it sees among them) and, of those between, the
+// ones with the largest
 //   score(row, b) = (sum of the head group's queries of the row) . (sum of the block's keys)
 // - up to a factor, the mean product of the group's queries with the block's keys. Every scored block
 // is seen whole: the last block, which the mask may cut, is taken without a score, so that
@@ -100,7 +100,7 @@ DRT_DEV void score_blocks(const float* __restrict__ sums, int b0, int step, int 
       for (int d = 0; d < 32; ++d) y[d] += (double)x[d >> 2][d & 3];
     }
     load(b0 + step);  // (behind the last: loaded, not used)
-    asm volatile("" ::: "memory");  // (the queries are read block by block: no registers for them all)
+    asm volatile("" ::: "memory");  // (queries read block by block: no registers for them all)
     f64x4 acc = f64x4{}, acc1 = f64x4{};  // (two chains: a product waits for the one before it)
 #pragma unroll
     for (int d = 0; d < 32; d += 2) {
@@ -119,7 +119,9 @@ DRT_DEV void score_blocks(const float* __restrict__ sums, int b0, int step, int 
 // A row's choice for one K/V head, one wave: the need-th largest key by its bits from the top (a
 // candidate prefix stands when at least `need` keys reach it; when exactly `need` do, they are
 // the choice; the upper halves alone mostly decide it), then the blocks in ascending order.
-// key_at(b): the key of scored block b. R: keys a lane holds, block 64 i + lane (0: asked for anew each time).
+// key_at(b): the key of scored block b. R: keys a lane holds, block 64 i + lane (0: asked for anew
+// each time). A bit costs each of the wave's rounds a comparison and a count: 1000 rows x 4 heads of
+// 500 blocks 14 us as a launch of its own, of it half the loads' and the launch's latency.
 template <int R, typename KeyAt>
 DRT_DEV void choose_row(KeyAt&& key_at, int nb, const SparseSel& sel, int32_t* out) {
   const int lane = threadIdx.x & 63;
@@ -198,11 +200,13 @@ struct SelArgs {
   int32_t* blocks;     // [rows][Hkv][count]
 };
 
-// Both steps for 16 rows of one K/V head in a work-group of 16 waves, the keys in LDS (RB rounds of 64
-// blocks). 1000 rows x 4 heads, 500 blocks: FUSED_US us; in two launches, with the keys in memory, 22 + 14.
+// Both steps for 16 rows of one K/V head in a work-group of 16 waves, the keys in LDS (RB rounds of
+// 64 blocks). 1000 rows x 4 heads, 500 blocks: 23.8 us; in two launches, with the keys in memory,
+// 22 + 14. Bound: a work-group's chain (queries, scores, barrier, the choice's bits one after the
+// other), of 252 work-groups on as many CUs at once; the 1 MB of sums is read from L2 and
+// the products would take 7 us.
 template <int RB>
 __global__ __launch_bounds__(1024, 4) void select_kernel(const SelArgs x) {
-  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = blockIdx.x % x.Hkv, r0 = blockIdx.x / x.Hkv * 16;
   const int rows = min(16, x.n_rows - r0), G = x.Hq / x.Hkv;
@@ -225,7 +229,9 @@ __global__ __launch_bounds__(1024, 4) void select_kernel(const SelArgs x) {
   }
 }
 
-// The scores alone: 16 rows against 64 * per blocks of one K/V head, four waves.
+// The scores alone: 16 rows against 64 * per blocks of one K/V head, four waves. For few rows: those
+// of a block find 128 work-groups here, 16 above (32 rows x 8 heads over 512 blocks 6.7 us, and
+// 6.7 for the choice; at once 26).
 __global__ __launch_bounds__(256, 2) void block_scores_kernel(const SelArgs x) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // work-group: (row tile * chunks + chunk) * Hkv + head

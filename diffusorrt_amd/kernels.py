@@ -202,13 +202,15 @@ class PrefixKVCache:
     head): 32-key tiles of 8192 elements (K block then V block) in the MFMA
     operand order of the attention kernel. Unwritten slots stay zero.
 
-    ``dtype`` is ``"f16"``, ``"bf16"`` or ``"i8"``: whole numbers of [-127, 127] times
-    one power of two for each tile's K and V (``scales [layers, kv_heads, tiles, 2]``), half the
-    bytes of a 16-bit cache. A store into an ``"i8"`` cache quantizes each tile it touches as a whole, from
+    ``dtype`` is ``"f16"``, ``"bf16"`` or ``"i8"``: whole numbers of [-127, 127] times one power
+    of two for each tile's K and V (``scales [layers, kv_heads, tiles, 2]``), half the bytes of a
+    16-bit cache. A store into an ``"i8"`` cache quantizes each tile it touches as a whole, from
     the rows it keeps (as they read) and the new ones, to the least power of two >= 2^-40 that
-    holds them: a value is off by at most half of it (max / 127 to 2 max / 127), a row that later stores
-    of its tile went past by less than one of the last scale. A tile with a value that is not finite, or beyond
-    127 * 2^40, reads as NaN until every row of it is stored anew.
+    holds them: a value is off by at most half of it (max / 127 to 2 max / 127), a row that later
+    stores of its tile went past by less than one of the last scale. A tile with a value that is
+    not finite, or beyond 127 * 2^40, reads as NaN until one store writes all 32 rows of it, or
+    :meth:`clear`; so does a tile that keeps rows of an earlier sequence take their size into its
+    scale. Clear an ``"i8"`` cache, or one with ``block_sums``, before another sequence.
 
     ``block_sums=True`` keeps the sum of each tile's keys (``sums [layers, kv_heads, tiles,
     128]``) up to date, which :meth:`select_blocks` scores blocks by."""
@@ -241,6 +243,15 @@ class PrefixKVCache:
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.data, self.scales, self.sums)
                    if t is not None)
+
+    def clear(self) -> None:
+        """Forget every row: the cache as it was made."""
+        self.data.fill_(128 if self.scales is not None else 0)
+        if self.scales is not None:
+            self.scales.fill_(1.0)
+        if self.sums is not None:
+            self.sums.fill_(0.0)
+        self.length = 0
 
     def _check(self, layer, *tensors):
         """The layer, and where the tensors of a call are."""
@@ -378,9 +389,10 @@ class PrefixKVCache:
         keys ``[0, n_keys)``: int32 ``[rows, kv_heads, count]``, ascending.
 
         They are the first ``sinks`` and the last ``local`` blocks that the row sees and, of
-        those between, the ones whose keys' sum has the largest product with the sum of
-        the row's queries of the head's group (compared in 64 bits; equal ones: the lower block). A row that sees no
-        more than ``count`` blocks lists them all, then ``-1``. Needs ``block_sums=True``."""
+        those between, the ones whose keys' sum has the largest product with the sum of the
+        row's queries of the head's group (compared in 64 bits; equal ones: the lower block). A
+        row that sees no more than ``count`` blocks lists them all, then ``-1``. Needs
+        ``block_sums=True``."""
         torch = _torch()
         if self.sums is None:
             raise ValueError("select_blocks needs a cache with block_sums=True")

@@ -299,12 +299,13 @@ int32_t drt_op_lm_head_score(const void* qw, const void* sb, const void* wb, int
  * byte is a code + 128, a value code * scale, with scales [hkv][head_stride / 8192][2] fp32 (a
  * tile's K and V), powers of two. For a tile's K, and for its V: scale = the least power of two >=
  * 2^-40 with max|x| <= 127 * scale, code = x / scale rounded to nearest, ties to even. A tile with
- * a value that is not finite, or beyond 127 * 2^40, reads as NaN as a whole. Codes start as 128,
- * scales as 1. Caches are 16-byte aligned and head strides whole tiles. */
+ * a value that is not finite, or beyond 127 * 2^40, reads as NaN as a whole (and keeps doing so
+ * until one store writes all of its rows). Codes start as 128, scales as 1. Caches are 16-byte
+ * aligned and head strides whole tiles. */
 
 /* Rows k, v ([n, hkv, 128] fp32 or bf16) to positions pos0..pos0+n-1. A tile is quantized as a
- * whole from the rows it keeps, as they read, and the new ones. sums: NULL or [hkv][head_stride / 8192][128]
- * fp32, which receive each touched tile's keys added up. */
+ * whole from the rows it keeps, as they read, and the new ones. sums: NULL or
+ * [hkv][head_stride / 8192][128] fp32, which receive each touched tile's keys added up. */
 int32_t drt_op_kv8_store(const void* k, const void* v, int32_t src_dtype, int32_t n, int32_t hkv,
                          int32_t pos0, void* cache, int64_t head_stride, float* scales, float* sums,
                          void* stream);
@@ -317,8 +318,8 @@ int32_t drt_op_kv16_store(const void* k, const void* v, int32_t src_dtype, int32
 int32_t drt_op_kv_load(const void* cache, int64_t head_stride, int32_t kv_dtype, const float* scales,
                        int32_t n, int32_t hkv, int32_t pos0, void* k, void* v, int32_t out_dtype,
                        void* stream);
-/* drt_op_attention over an 8-bit cache; q fp16 or bf16 (q_dtype), row_pos0 >= 0. Calls that overlap must
- * not share a workspace (it may be NULL where 0 bytes are asked for). */
+/* drt_op_attention over an 8-bit cache; q fp16 or bf16 (q_dtype), row_pos0 >= 0. Calls that overlap
+ * must not share a workspace (it may be NULL where 0 bytes are asked for). */
 size_t drt_op_attention_kv8_workspace_bytes(int32_t rows, int32_t hq, int32_t hkv, int32_t n_keys);
 int32_t drt_op_attention_kv8(const void* q, int32_t q_dtype, const void* cache, int64_t head_stride,
                              const float* scales, int32_t rows, int32_t hq, int32_t hkv,
@@ -332,8 +333,9 @@ int32_t drt_op_attention_kv8(const void* q, int32_t q_dtype, const void* cache, 
  * lists `count` (1..1024) of the blocks the row sees: the first `sinks`, the last `local` (>= 1) and,
  * of those between, the ones whose keys' sum has the largest product with the sum of the head
  * group's queries (in 64 bits; equal ones: the lower block; a NaN is the largest). Blocks ascend in
- * blocks [rows, hkv, count]; a row that sees fewer lists them all, then -1. sums: [hkv][sums_tiles][128] of
- * drt_op_kv8_store or drt_op_kv16_store. Neither call's overlapping ones may share a workspace. */
+ * blocks [rows, hkv, count]; a row that sees fewer lists them all, then -1. sums:
+ * [hkv][sums_tiles][128] of drt_op_kv8_store or drt_op_kv16_store. Neither call's overlapping ones
+ * may share a workspace. */
 size_t drt_op_select_blocks_workspace_bytes(int32_t rows, int32_t hkv, int32_t n_keys,
                                             int32_t block_size);
 int32_t drt_op_select_blocks(const void* q, int32_t q_dtype, const float* sums, int64_t sums_tiles,

@@ -188,6 +188,25 @@ def test_a_host_tensor_is_refused():
                                 kind="full")
 
 
+@pytest.mark.parametrize("dtype", ["i8", "f16", "bf16"])
+def test_clear_is_a_new_cache(dtype):
+    from diffusorrt_amd.kernels import PrefixKVCache
+
+    new, used = (PrefixKVCache(2, 3, 64, dtype=dtype, device="cpu", block_sums=True)
+                 for _ in range(2))
+    used.data.fill_(7)
+    used.sums.fill_(float("nan"))
+    if used.scales is not None:
+        used.scales.fill_(float("nan"))
+    used.length = 40
+    used.clear()
+    assert used.length == 0 and used.kv_dtype == new.kv_dtype
+    for name in ("data", "scales", "sums"):
+        a, b = getattr(new, name), getattr(used, name)
+        assert (a is None) == (b is None)
+        assert a is None or (a.dtype == b.dtype and torch.equal(a, b))
+
+
 def test_an_8_bit_cache_is_half_the_bytes():
     from diffusorrt_amd.kernels import PrefixKVCache
 

@@ -134,6 +134,25 @@ def test_store_at_the_ends_of_the_scales_and_beyond():
     assert bool((cache.load(0, 32 * t, 32)[0] == 1).all())
 
 
+def test_a_cleared_cache_serves_another_sequence():
+    """Large and NaN rows of the sequence before have no part in the next one's scales."""
+    from diffusorrt_amd.kernels import PrefixKVCache
+
+    _say("clear")
+    gen = torch.Generator().manual_seed(31)
+    cache, ref = PrefixKVCache(2, 2, 96, dtype="i8", block_sums=True), X.Cache8(2, 96)
+    k, v = _kv(gen, 96, 2, 1000.0)
+    k[70] = float("nan")
+    cache.store(1, k.cuda(), v.cuda(), 0)
+    assert bool(torch.isnan(cache.scales).any())
+    cache.clear()
+    k, v = _kv(gen, 70, 2, 1.0)
+    for at, n in ((0, 40), (40, 1), (41, 29)):
+        cache.store(1, k[at:at + n].cuda(), v[at:at + n].cuda(), at)
+        ref.store(_np(k[at:at + n]), _np(v[at:at + n]), at)
+    _same_as(cache, 1, ref)
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_load_and_sums_of_a_16_bit_cache(dtype):
     from diffusorrt_amd.kernels import PrefixKVCache
