@@ -15,10 +15,15 @@ namespace {
 // what it reads as, which with these scales is one more rounding only when e rises, each time to
 // half the resolution or less, so any number of stores stays within one step of what they wrote
 // (1/2 + 1/4 + ...); and x / scale never falls on the wrong side of a rounding.
-// Bound: the rows read and the codes written (131072 bf16 rows x 8 heads: 805 MB in 207 us, 3.9 of
-// a copy's 4.7 TB/s; 2000 fp32 rows x 4 heads 7.0 us); of a block of 32 rows, 5.5 us, the chain of a
+// Bound: the rows read and the codes written (131072 bf16 rows x 8 heads: 805 MB in 154 us, 5.2 TB/s,
+// 168 with sums; 2000 fp32 rows x 4 heads 5.8 us); of a block of 32 rows, 4.2 us, the chain of a
 // launch, the loads, two barriers and the stores. A work-group has a tile alone: its scale
-// needs every row of it, and no other work-group's.
+// needs every row of it, and no other work-group's. Codes cross LDS as words: byte by byte, and
+// with every head dim's sum exchanged by itself, 222 us with sums, and 5.7 for the block.
+// Where byte `at` of the tile is in LDS: 16-byte pieces change places within 256 bytes, so that
+// the threads' words, 256 and 1024 bytes apart, meet more banks.
+DRT_DEV int kv8_lds(int at) { return at ^ (((at >> 8) & 3) << 4) ^ (((at >> 10) & 3) << 6); }
+
 template <bool SRC_BF16>
 __global__ __launch_bounds__(256) void kv8_store_kernel(
     const void* __restrict__ k_src, const void* __restrict__ v_src, int n, int Hkv, int pos0,
@@ -63,10 +68,15 @@ __global__ __launch_bounds__(256) void kv8_store_kernel(
   } else {  // a row that stays
     const float sk = sc[0], sv = sc[1];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      x[0][e] = sk * (float)((int)tile[kv8_k_at(kk, d0 + e)] - 128);
-      x[1][e] = sv * (float)((int)tile[kv8_v_at(kk, d0 + e)] - 128);
+    for (int h = 0; h < 2; ++h) {  // eight head dims of K are eight bytes in a row
+      const uint2 w = *(const uint2*)(tile + kv8_k_at(kk, d0 + 8 * h));
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[0][8 * h + e] = sk * (float)((int)(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xffu) - 128);
     }
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      x[1][e] = sv * (float)((int)tile[kv8_v_at(kk, d0 + e)] - 128);
   }
   uint32_t m[2] = {0u, 0u};
 #pragma unroll
@@ -79,35 +89,78 @@ __global__ __launch_bounds__(256) void kv8_store_kernel(
   }
   __syncthreads();  // (also: every row that stays has been read)
   float scale[2];
+  uint32_t y[2][4];  // the thread's codes + 128, as bytes
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     const uint32_t b = max(max(most[w][0], most[w][1]), max(most[w][2], most[w][3]));
     // 127 = 1.984375 * 2^6
     const int e = max(KV8_MIN_EXP, (int)(b >> 23) - 133 + ((b & 0x7fffffu) > 0x7e0000u ? 1 : 0));
     const bool fits = e <= KV8_MAX_EXP;
-    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    const float inv = __uint_as_float((uint32_t)(127 - min(e, KV8_MAX_EXP)) << 23);
     scale[w] = fits ? __uint_as_float((uint32_t)(127 + e) << 23) : __uint_as_float(0x7fc00000u);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int c = fits ? (int)rintf(x[w][i] * inv) : 0;
-      codes[w ? kv8_v_at(kk, d0 + i) : kv8_k_at(kk, d0 + i)] = (uint8_t)(c + 128);
-      x[w][i] = (float)c;
+    for (int q = 0; q < 4; ++q) {
+      uint32_t z = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)  // (a whole number before its conversion)
+        z = __builtin_amdgcn_cvt_pk_u8_f32(rintf(x[w][4 * q + i] * inv) + 128.f, i, z);
+      y[w][q] = fits ? z : 0x80808080u;
     }
   }
-  if (sums) {  // whole numbers below 2^12: exact in any order
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      int s = (int)x[0][i];  // the eight keys of this wave (lanes 8 apart)
-      s += __shfl_xor(s, 8, 64);
-      s += __shfl_xor(s, 16, 64);
-      s += __shfl_xor(s, 32, 64);
-      if ((tid & 63) < 8) part[tid >> 6][d0 + i] = s;
+  for (int h = 0; h < 2; ++h)
+    *(uint2*)(codes + kv8_lds(kv8_k_at(kk, d0 + 8 * h))) = make_uint2(y[0][2 * h], y[0][2 * h + 1]);
+  // V has four keys in a row: the threads of four neighbouring ones (lanes 8 and 16 apart) exchange
+  // their words, until thread kk & 3 = r has head dims 4 r .. + 4 of all four, and turn the bytes.
+  const int b0 = tid & 8, b1 = tid & 16, r = (tid >> 3) & 3;
+  {
+    const uint32_t s0 = (uint32_t)__shfl_xor((int)(b0 ? y[1][0] : y[1][1]), 8, 64);
+    const uint32_t s1 = (uint32_t)__shfl_xor((int)(b0 ? y[1][2] : y[1][3]), 8, 64);
+    const uint32_t u0 = b0 ? s0 : y[1][0], u1 = b0 ? y[1][1] : s0;  // dims 4 (r & 1) of keys 0, 1
+    const uint32_t v0 = b0 ? s1 : y[1][2], v1 = b0 ? y[1][3] : s1;  // dims 8 + 4 (r & 1)
+    const uint32_t t0 = (uint32_t)__shfl_xor((int)(b1 ? u0 : v0), 16, 64);
+    const uint32_t t1 = (uint32_t)__shfl_xor((int)(b1 ? u1 : v1), 16, 64);
+    const uint32_t k0 = b1 ? t0 : u0, k1 = b1 ? t1 : u1, k2 = b1 ? v0 : t0, k3 = b1 ? v1 : t1;
+    const uint32_t lo01 = __builtin_amdgcn_perm(k1, k0, 0x05010400u);  // dims 0, 1 of keys 0, 1
+    const uint32_t hi01 = __builtin_amdgcn_perm(k1, k0, 0x07030602u);  // dims 2, 3
+    const uint32_t lo23 = __builtin_amdgcn_perm(k3, k2, 0x05010400u);
+    const uint32_t hi23 = __builtin_amdgcn_perm(k3, k2, 0x07030602u);
+    const uint32_t z[4] = {__builtin_amdgcn_perm(lo23, lo01, 0x05040100u),
+                           __builtin_amdgcn_perm(lo23, lo01, 0x07060302u),
+                           __builtin_amdgcn_perm(hi23, hi01, 0x05040100u),
+                           __builtin_amdgcn_perm(hi23, hi01, 0x07060302u)};
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *(uint32_t*)(codes + kv8_lds(kv8_v_at(kk & ~3, d0 + 4 * r + c))) = z[c];
+  }
+  if (sums) {  // whole numbers: exact in any order
+    // two head dims a word (4 q + o and 4 q + o + 2 in word 2 q + o), the eight keys of the wave added
+    // up; each exchange leaves a lane half of the words
+    uint32_t a[8];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      a[2 * q] = y[0][q] & 0x00ff00ffu;
+      a[2 * q + 1] = (y[0][q] >> 8) & 0x00ff00ffu;
     }
+#pragma unroll
+    for (int n = 4; n > 0; n >>= 1) {
+      const int bit = 32 / n;  // lanes 8, 16, 32 apart
+      const bool up = tid & bit;
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const uint32_t give = up ? a[i] : a[i + n], keep = up ? a[i + n] : a[i];
+        a[i] = keep + (uint32_t)__shfl_xor((int)give, bit, 64);
+      }
+    }
+    const int i = (tid & 8 ? 4 : 0) + (tid & 16 ? 2 : 0) + (tid & 32 ? 1 : 0);
+    int* to = part[tid >> 6] + d0 + 4 * (i >> 1) + (i & 1);
+    to[0] = (int)(a[0] & 0xffffu) - 8 * 128;
+    to[2] = (int)(a[0] >> 16) - 8 * 128;
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    *(u32x4*)(tile + (tid + 256 * i) * 16) = *(const u32x4*)(codes + (tid + 256 * i) * 16);
+    *(u32x4*)(tile + (tid + 256 * i) * 16) = *(const u32x4*)(codes + kv8_lds((tid + 256 * i) * 16));
   if (tid < 2) sc[tid] = tid ? scale[1] : scale[0];
   if (sums && tid < 128)
     sums[(h * tiles + t) * 128 + tid] =
