@@ -257,9 +257,11 @@ class PrefixKVCache:
         """The layer, and where the tensors of a call are."""
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer must be in [0, {self.layers})")
+        if self._index < 0:
+            raise ValueError("the cache must be on a GPU")
         for t in tensors:
-            if t.get_device() != self._index or self._index < 0:
-                raise ValueError("tensors must be on the cache's device, a GPU")
+            if t.get_device() != self._index:
+                raise ValueError("tensors must be on the cache's device")
             if not t.is_contiguous():
                 raise ValueError("the cache's calls take contiguous tensors")
 
@@ -295,17 +297,22 @@ class PrefixKVCache:
     def store(self, layer: int, k, v, pos0: int) -> None:
         """Write ``k/v [n, Hkv, 128]`` (fp32 or bf16) at positions ``pos0..pos0+n-1``."""
         torch = _torch()
-        _require_cuda(k, v)
-        n = k.shape[0]
-        if k.shape != v.shape or k.shape[1:] != (self.kv_heads, 128):
+        tiled = self.scales is not None or self.sums is not None
+        if tiled:
+            self._check(layer, k, v)
+        else:
+            _require_cuda(k, v)
+        shape = k.shape
+        n = shape[0]
+        if shape != v.shape or shape[1:] != (self.kv_heads, 128):
             raise ValueError("store takes k, v of shape [n, kv_heads, 128]")
         if pos0 < 0 or pos0 + n > self.capacity:
             raise ValueError("store positions exceed the cache capacity")
-        if k.dtype not in (torch.float32, torch.bfloat16) or v.dtype != k.dtype:
+        dtype = k.dtype
+        if dtype not in (torch.float32, torch.bfloat16) or v.dtype != dtype:
             raise ValueError("store takes fp32 or bf16 k/v")
-        src = _lib.BF16 if k.dtype == torch.bfloat16 else _lib.F32
-        if self.scales is not None or self.sums is not None:
-            self._check(layer, k, v)
+        src = _lib.BF16 if dtype is torch.bfloat16 else _lib.F32
+        if tiled:
             lib, data, sums = _lib.load(), self._data(layer), self._sums(layer)
             if self.scales is not None:
                 _launch(torch, lib.drt_op_kv8_store, self._index, k.data_ptr(), v.data_ptr(), src,
@@ -330,7 +337,7 @@ class PrefixKVCache:
             raise ValueError("load gives float32 or bfloat16")
         if n < 1 or pos0 < 0 or pos0 + n > self.capacity:
             raise ValueError("load positions outside the cache")
-        self._check(layer, self.data)
+        self._check(layer)
         k = torch.empty((n, self.kv_heads, 128), dtype=out_dtype, device=self.data.device)
         v = torch.empty_like(k)
         _launch(torch, _lib.load().drt_op_kv_load, self._index, self._data(layer),
