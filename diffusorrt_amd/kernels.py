@@ -474,7 +474,7 @@ def _mask_args(kind, mask_geometry):
             p, b = int(mask_geometry["prompt_len"]), int(mask_geometry["block_size"])
         else:
             p, b = (int(v) for v in mask_geometry)
-        if p < 0 or b < 1:
+        if not (0 <= p <= _I32_MAX and 1 <= b <= _I32_MAX):
             raise ValueError("bad d2f_hybrid mask geometry")
         return _lib.MASK_D2F_HYBRID, p, b
     raise ValueError(f"unsupported attention mask kind: {kind}")

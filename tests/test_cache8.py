@@ -188,6 +188,16 @@ def test_a_host_tensor_is_refused():
                                 kind="full")
 
 
+@pytest.mark.parametrize("geometry", [(-1, 32), (0, 0), (2**31, 32), (0, 2**31), (2**32, 32),
+                                      (0, 2**32 + 32)])
+def test_mask_geometry_beyond_32_bits_is_refused(geometry):
+    from diffusorrt_amd.kernels import _mask_args
+
+    with pytest.raises(ValueError):
+        _mask_args("d2f_hybrid", geometry)
+    assert _mask_args("d2f_hybrid", (2**31 - 1, 2**31 - 1))[1:] == (2**31 - 1, 2**31 - 1)
+
+
 @pytest.mark.parametrize("dtype", ["i8", "f16", "bf16"])
 def test_clear_is_a_new_cache(dtype):
     from diffusorrt_amd.kernels import PrefixKVCache
