@@ -414,17 +414,20 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
     __builtin_amdgcn_s_setprio(0);
   };
 
+  // Where range k of n tiles begins. (Below 2^26 tiles, up to 64 ranges: 32 bits hold the product, and
+  // a division of 64 would take as long as a tile.)
+  auto share = [&](int n, int k) { return (int)((uint32_t)n * (uint32_t)k / (uint32_t)x.splits); };
   if constexpr (!SPARSE) {
-    const int64_t n_tiles = (where.n_keys + 31) >> 5;
-    const int t0 = (int)(n_tiles * split / x.splits) + kw;
-    const int t_end = !exists(wv0) ? 0
-                                   : min((int)(n_tiles * (split + 1) / x.splits), (wave_end + 31) >> 5);
+    const int n_tiles = (where.n_keys + 31) >> 5;
+    const int t0 = share(n_tiles, split) + kw;
+    const int t_end = !exists(wv0) ? 0 : min(share(n_tiles, split + 1), (wave_end + 31) >> 5);
     const int n = (t_end - t0 + KW - 1) / KW;
     first(n, t0);
     stage();
     run(n, t0, 0u, false, [&](int& t, uint32_t&) { t += KW; });
   } else {
-    const int m = x.block >> 5, n_blocks = (int)(((int64_t)wave_end + x.block - 1) / x.block);
+    const int m = x.block >> 5;
+    const int n_blocks = (int)((uint32_t)(wave_end - 1) / (uint32_t)x.block) + 1;
     const int step_e = KW / m, step_r = KW % m;
     // 16 bits: a V that is not finite makes 0 * V of a row that does not see it NaN too, and a K the
     // score of one that does not list it. Rows are looked at afterwards, and only if some are not
@@ -466,10 +469,8 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
         n_list = __builtin_amdgcn_readfirstlane(n_list);
         // tiles in all (of the last block those that the rows see), and this wave's of this range
         const int last = __builtin_amdgcn_readfirstlane(list[max(n_list - 1, 0)].x);
-        const int64_t n = n_list == 0 ? 0
-                                      : (int64_t)(n_list - 1) * m +
-                                            min((int64_t)m, ((wave_end + 31) >> 5) - (int64_t)last * m);
-        const int j0 = (int)(n * split / x.splits) + kw, j1 = (int)(n * (split + 1) / x.splits);
+        const int n = n_list == 0 ? 0 : (n_list - 1) * m + min(m, ((wave_end + 31) >> 5) - last * m);
+        const int j0 = share(n, split) + kw, j1 = share(n, split + 1);
         int e = j0 / m, r = j0 - e * m;
         auto here = [&](int& t, uint32_t& rows) {
           const int2 b = list[min(e, n_list - 1)];

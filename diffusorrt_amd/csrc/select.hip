@@ -31,9 +31,29 @@ DRT_DEV uint64_t score_key(double x) {
   return b >> 63 ? ~b : b | (1ull << 63);
 }
 
-// Blocks a row sees.
+// Blocks a row sees (one at least).
 DRT_DEV int blocks_of(int row, const AttnWhere& where, int block) {
-  return (int)(((int64_t)key_end_of(row, where) + block - 1) / block);
+  return (int)((uint32_t)(key_end_of(row, where) - 1) / (uint32_t)block) + 1;
+}
+
+// The largest of the wave's values, by lane moves within 16 lanes, then from row to row.
+DRT_DEV uint32_t wave_most(uint32_t x) {
+#define DRT_STEP(CTRL) \
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, false))
+  DRT_STEP(0x111);  // from 1, 2, 4, 8 lanes below
+  DRT_STEP(0x112);
+  DRT_STEP(0x114);
+  DRT_STEP(0x118);
+  DRT_STEP(0x142);  // lane 15 of a row to the next row, lane 31 to the upper half
+  DRT_STEP(0x143);
+#undef DRT_STEP
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+
+// Set bits of a mask below this lane.
+DRT_DEV int bits_below(uint64_t mask) {
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                        __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
 }
 
 // Scores of 16 rows against 16 blocks at a time, as 16x16x4 products in 64 bits. The rows' queries,
@@ -116,12 +136,13 @@ DRT_DEV void score_blocks(const float* __restrict__ sums, int b0, int step, int 
   }
 }
 
-// A row's choice for one K/V head, one wave: the need-th largest key by its bits from the top (a
-// candidate prefix stands when at least `need` keys reach it; when exactly `need` do, they are
-// the choice; the upper halves alone mostly decide it), then the blocks in ascending order.
+// A row's choice for one K/V head, one wave: a cut that exactly `need` keys reach, then the blocks in
+// ascending order. The cut lies between one that enough keys reach (first an exponent below the
+// largest key, where that of scores mostly is, then two, four, ...) and one that too few do, and is
+// found by halving; the upper halves of the keys alone mostly decide it, in about ten steps. Where
+// equal keys leave none, the least key of the choice, found bit by bit.
 // key_at(b): the key of scored block b. R: keys a lane holds, block 64 i + lane (0: asked for anew
-// each time). A bit costs each of the wave's rounds a comparison and a count: 1000 rows x 4 heads of
-// 500 blocks 14 us as a launch of its own, of it half the loads' and the launch's latency.
+// each time). A step costs each of the wave's rounds a comparison and a count.
 template <int R, typename KeyAt>
 DRT_DEV void choose_row(KeyAt&& key_at, int nb, const SparseSel& sel, int32_t* out) {
   const int lane = threadIdx.x & 63;
@@ -149,16 +170,42 @@ DRT_DEV void choose_row(KeyAt&& key_at, int nb, const SparseSel& sel, int32_t* o
       }
     }
   };
-  uint32_t upper = 0u;  // the largest prefix that at least `need` keys reach
-  bool exact = need == 0;
-  for (int bit = 31; bit >= 0 && !exact; --bit) {
-    const uint32_t want = upper | (1u << bit);
+  auto reach = [&](uint32_t want) {
     int n = 0;
-    each([&](int, uint64_t k) { n += __popcll(__ballot((uint32_t)(k >> 32) >= want)); });
+    each([&](int, uint64_t k) { n += (int)__popcll(__ballot((uint32_t)(k >> 32) >= want)); });
+    return n;
+  };
+  uint32_t upper = 0u;  // the largest that at least `need` keys' upper halves reach
+  bool exact = need == 0;
+  if (!exact) {
+    uint32_t most = 0u;
+    each([&](int, uint64_t k) { most = max(most, (uint32_t)(k >> 32)); });
+    most = wave_most(most);
+    // (no key's upper half is past `most`: that one may be ~0u, a NaN's, and is tried as it is)
+    uint32_t high = most, down = 1u << 20;
+    int n = reach(most);
     if (n >= need) {
-      upper = want;
-      exact = n == need;
+      upper = most;
+    } else {
+      for (;;) {
+        upper = most > down ? most - down : 0u;
+        n = upper ? reach(upper) : need + 1;  // (0: reached by all, those without a score too)
+        if (n >= need) break;
+        high = upper;
+        down = down < 1u << 31 ? down << 1 : ~0u;
+      }
+      while (n != need && high - upper > 1u) {
+        const uint32_t mid = upper + (high - upper) / 2;
+        const int k = reach(mid);
+        if (k >= need) {
+          upper = mid;
+          n = k;
+        } else {
+          high = mid;
+        }
+      }
     }
+    exact = n == need;
   }
   uint64_t cut = (uint64_t)upper << 32;
   for (int bit = 31; bit >= 0 && !exact; --bit) {
@@ -175,16 +222,15 @@ DRT_DEV void choose_row(KeyAt&& key_at, int nb, const SparseSel& sel, int32_t* o
   int ties = need;
   each([&](int, uint64_t k) { ties -= __popcll(__ballot(k > cut)); });
   int at = 0;
-  const uint64_t below = (1ull << lane) - 1;
   each([&](int i, uint64_t k) {
     const int b = 64 * i + lane;
     const bool scored = b >= lo && b < hi;
     const uint64_t tied = __ballot(scored && k == cut);
     bool take = scored ? k > cut : b < nb;
-    if (scored && k == cut) take = (int)__popcll(tied & below) < ties;
+    if (scored && k == cut) take = bits_below(tied) < ties;
     ties -= min(ties, (int)__popcll(tied));
     const uint64_t mask = __ballot(take);
-    if (take) out[at + __popcll(mask & below)] = b;
+    if (take) out[at + bits_below(mask)] = b;
     at += __popcll(mask);
   });
 }
@@ -201,10 +247,11 @@ struct SelArgs {
 };
 
 // Both steps for 16 rows of one K/V head in a work-group of 16 waves, the keys in LDS (RB rounds of
-// 64 blocks). 1000 rows x 4 heads, 500 blocks: 23.8 us; in two launches, with the keys in memory,
-// 22 + 14. Bound: a work-group's chain (queries, scores, barrier, the choice's bits one after the
-// other), of 252 work-groups on as many CUs at once; the 1 MB of sums is read from L2 and
-// the products would take 7 us.
+// 64 blocks). 1000 rows x 4 heads, 500 blocks: 22.3 us (23.8 with the choice's bits one after the other
+// and divisions of 64 bits); in two launches, with the keys in memory, 22 + 14. Bound: a
+// work-group's chain (queries, scores, barrier, the choice), of 252 work-groups on as many CUs at
+// once; the 1 MB of sums is read from L2 and the products would take 7 us. Many more rows: L2, which
+// every 16 rows read all sums from (2048 rows x 8 heads, 512 blocks of two tiles: 96 us, products 29).
 template <int RB>
 __global__ __launch_bounds__(1024, 4) void select_kernel(const SelArgs x) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
