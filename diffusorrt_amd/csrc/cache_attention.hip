@@ -61,6 +61,31 @@ DRT_DEV float ca_max_xor32(float v) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// A value of the lane 1, 2, then 7 - i of eight, 15 - i of sixteen places away: four steps join 16 lanes.
+template <int STEP> DRT_DEV uint32_t ca_of_16(uint32_t x) {
+  constexpr int CTRL = STEP == 0 ? 0xb1 : STEP == 1 ? 0x4e : STEP == 2 ? 0x141 : 0x140;
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, true);
+}
+DRT_DEV uint32_t ca_max16(uint32_t x) {
+  x = max(x, ca_of_16<0>(x));
+  x = max(x, ca_of_16<1>(x));
+  x = max(x, ca_of_16<2>(x));
+  return max(x, ca_of_16<3>(x));
+}
+DRT_DEV float ca_sum16(float x) {
+  x += __uint_as_float(ca_of_16<0>(__float_as_uint(x)));
+  x += __uint_as_float(ca_of_16<1>(__float_as_uint(x)));
+  x += __uint_as_float(ca_of_16<2>(__float_as_uint(x)));
+  return x + __uint_as_float(ca_of_16<3>(__float_as_uint(x)));
+}
+
+// A barrier for LDS: __syncthreads() would wait for the loads on their way too.
+DRT_DEV void ca_lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // What a cache's element type means to the kernel: 0 = 8-bit, 1 = fp16, 2 = bf16.
 template <int DT> struct CacheT {
   static constexpr int TILE = DT == 0 ? KV8_TILE : 2 * KV8_TILE, LOADS = DT == 0 ? 4 : 8;
@@ -189,6 +214,16 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
                   : qt0 * 32 + v < n_qv;
   };
 
+  // the tile's lists, their first entries on their way
+  const int end_row = min(SPARSE ? row0 + RPT - 1 : 0, x.n_rows - 1);
+  const int n_entries = SPARSE ? (end_row - row0 + 1) * x.count : 0;
+  auto entry = [&](int i, int& r) {
+    r = (int)((uint32_t)i / (uint32_t)x.count);
+    return x.blocks[((int64_t)(row0 + r) * x.Hkv + kvh) * x.count + (i - r * x.count)];
+  };
+  int entry0 = -1, entry0_row = 0;
+  if (SPARSE && tid < n_entries) entry0 = entry(tid, entry0_row);
+
   // the queries, 16 threads (eight elements each) a query vector, on their way
   constexpr int QL = NQ * 16 / THREADS;
   static_assert(QL * THREADS == NQ * 16, "whole rounds of the queries");
@@ -226,8 +261,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             most = max(most, max((raw[e] << 16) & 0x7fffffffu, raw[e] & 0x7fff0000u));
-#pragma unroll
-          for (int d = 8; d > 0; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+          most = ca_max16(most);
           const int ex = most ? min(max((int)(most >> 23) - 127, -126), 126) : 0;
           // (beyond 2^80 the scores are further apart than fp32 tells, and would overflow)
           pw = __uint_as_float((uint32_t)(127 + min(ex, 80)) << 23);
@@ -237,17 +271,12 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
             raw[e] = pack_half2((_Float16)(__uint_as_float(raw[e] << 16) * inv),
                                 (_Float16)(__uint_as_float(raw[e] & 0xffff0000u) * inv));
         }
-        sum = kv8_add8(__builtin_bit_cast(f16x8, raw), 0.f);
-#pragma unroll
-        for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
+        sum = ca_sum16(kv8_add8(__builtin_bit_cast(f16x8, raw), 0.f));
       }
       *(u32x4*)(smem + (v * CA_QROW + ch * 8) * 2) = raw;
       if (ch == 0) qinfo[v] = make_float2(x.c * pw, -KV8_BIAS / KV8_POW * sum);
     }
-    // (a bare barrier: __syncthreads() would wait for the tile on its way)
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    ca_lds_barrier();
     if (HOLD) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) qr[HOLD ? i : 0] = *(const vec*)(ql + 16 * i);
@@ -270,9 +299,9 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   };
   reset();
   // (ends never fall from row to row) keys every row of the wave sees, and any of them
-  const int end_row = min(SPARSE ? row0 + RPT - 1 : row_of(wv0 + QT * 32 - 1), last_row);
   const int wave_full = key_end_of(min(row_of(wv0), last_row), where);
-  const int wave_end = key_end_of(end_row, where);
+  const int wave_end =
+      key_end_of(SPARSE ? end_row : min(row_of(wv0 + QT * 32 - 1), last_row), where);
   const uint32_t my_row = SPARSE ? 1u << ((lane & 31) / GC & 31) : 0u;
   const uint32_t all_rows = SPARSE ? (uint32_t)((1ull << (end_row - row0 + 1)) - 1) : 0u;
 
@@ -436,36 +465,38 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
     for (;;) {
       for (int w0 = 0; w0 < n_blocks; w0 += CA_WIN) {
         const int n_win = min(CA_WIN, n_blocks - w0);
-        __syncthreads();  // the window before has been read
+        if (w0 || careful) ca_lds_barrier();  // the window before has been read
         for (int i = tid; i < n_win; i += THREADS) bits[i] = 0u;
-        __syncthreads();
-        const int n_entries = (end_row - row0 + 1) * x.count;
+        ca_lds_barrier();
         for (int i = tid; i < n_entries; i += THREADS) {
-          const int r = i / x.count;
-          const int b = x.blocks[((int64_t)(row0 + r) * x.Hkv + kvh) * x.count + (i - r * x.count)];
+          int r = entry0_row;
+          const int b = i == tid ? entry0 : entry(i, r);
           // (one beyond its row's keys only: its tiles are masked key by key)
           if (b >= w0 && b < w0 + n_win) atomicOr(&bits[b - w0], 1u << r);
         }
-        __syncthreads();
+        ca_lds_barrier();
         // the window's blocks in order: wave w finds those of its share, then all take their places
-        constexpr int SHARE = CA_WIN / NW;
-        int found = 0;
-        for (int i = wave * SHARE; i < min(n_win, (wave + 1) * SHARE); i += 64)
-          found += __popcll(__ballot(i + lane < n_win && bits[min(i + lane, CA_WIN - 1)] != 0u));
+        const int part_of = (n_win + 64 * NW - 1) / (64 * NW) * 64, i0 = wave * part_of;
+        auto rows_of = [&](int i) { return i + lane < n_win ? bits[min(i + lane, CA_WIN - 1)] : 0u; };
+        const uint32_t rows0 = rows_of(i0);
+        int found = (int)__popcll(__ballot(rows0 != 0u));
+        for (int i = i0 + 64; i < min(n_win, i0 + part_of); i += 64)
+          found += (int)__popcll(__ballot(rows_of(i) != 0u));
         if (lane == 0) tally[wave] = found;
-        __syncthreads();
+        ca_lds_barrier();
         int at = 0, n_list = 0;
+#pragma unroll
         for (int w = 0; w < NW; ++w) {
           at += w < wave ? tally[w] : 0;
           n_list += tally[w];
         }
-        for (int i = wave * SHARE; i < min(n_win, (wave + 1) * SHARE); i += 64) {
-          const uint32_t b = i + lane < n_win ? bits[min(i + lane, CA_WIN - 1)] : 0u;
+        for (int i = i0; i < min(n_win, i0 + part_of); i += 64) {
+          const uint32_t b = i == i0 ? rows0 : rows_of(i);
           const uint64_t hit = __ballot(b != 0u);
           if (b) list[at + __popcll(hit & ((1ull << lane) - 1))] = make_int2(w0 + i + lane, (int)b);
           at += __popcll(hit);
         }
-        __syncthreads();
+        ca_lds_barrier();
         n_list = __builtin_amdgcn_readfirstlane(n_list);
         // tiles in all (of the last block those that the rows see), and this wave's of this range
         const int last = __builtin_amdgcn_readfirstlane(list[max(n_list - 1, 0)].x);
