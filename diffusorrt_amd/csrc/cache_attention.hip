@@ -185,9 +185,12 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   typedef typename T::vec vec;
   constexpr int NW = QW * KW, THREADS = 64 * NW, NQ = 32 * QT * QW, TILE = T::TILE, LD = T::LOADS;
   static_assert(!SPARSE || (QT == 1 && QW == 1), "a work-group has one union of lists");
-  // LDS: the queries, then halves (64 head dims) of every wave's O, 8 KiB a query tile
-  constexpr int Q_BYTES = NQ * CA_QROW * 2, HALF_BYTES = NW * QT * 8192;
-  __shared__ __align__(16) char smem[Q_BYTES > HALF_BYTES ? Q_BYTES : HALF_BYTES];
+  // LDS: the queries, then halves (64 head dims) of every wave's O, one after the other: the first is
+  // on its way to memory under the second (32 rows over 8224 keys 12.3 us; all at once 12.7). One
+  // query tile has little to write: all at once (one row over 8192 keys 6.4 us; halves 6.9).
+  constexpr int PASSES = KW == 8 && !SPARSE ? 1 : 2, PIECES = 32 / PASSES, WAVE_O = 32 * PIECES * 16;
+  constexpr int Q_BYTES = NQ * CA_QROW * 2, O_BYTES = NW * QT * WAVE_O;
+  __shared__ __align__(16) char smem[Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
   __shared__ float2 ml[KW][NQ];  // base and sum of every way
   __shared__ float2 qinfo[NQ];  // c times a query vector's power of two; -128 * 2^-24 its sum
   __shared__ uint32_t bits[SPARSE ? CA_WIN : 1];  // rows that list a block of the window
@@ -552,28 +555,30 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
     }
   }
 
-  // The key ways joined and rows out, half a head (64 head dims) at a time: every wave leaves its
-  // half in LDS as 16-byte pieces (query v, piece p at p ^ v: every bank in turn both ways), then
-  // eight threads a query vector add the ways' and write theirs, all waves taking part.
+  // The key ways joined and rows out: every wave leaves its O, or half of it, in LDS as 16-byte
+  // pieces (query v, piece p at p ^ v: every bank in turn both ways), then threads with eight head
+  // dims of a query vector add the ways' and write theirs, all waves taking part.
+  constexpr int CH = PIECES / 2;
 #pragma unroll
-  for (int hf = 0; hf < 2; ++hf) {
+  for (int hf = 0; hf < PASSES; ++hf) {
     __syncthreads();  // the queries, or the first half, have been read
 #pragma unroll
     for (int j = 0; j < QT; ++j) {
-      f32x4* d = (f32x4*)(smem + ((kw * QW + qw) * QT + j) * 8192);
+      f32x4* d = (f32x4*)(smem + ((kw * QW + qw) * QT + j) * WAVE_O);
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < 4 / PASSES; ++b) {
+        const f32x16& y = o[j][hf * (4 / PASSES) + b];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          d[(lane & 31) * 16 + ((b * 8 + 2 * r + (lane >> 5)) ^ (lane & 15))] =
-              f32x4{o[j][2 * hf + b][4 * r], o[j][2 * hf + b][4 * r + 1], o[j][2 * hf + b][4 * r + 2],
-                    o[j][2 * hf + b][4 * r + 3]};
+          d[(lane & 31) * PIECES + ((b * 8 + 2 * r + (lane >> 5)) ^ (lane & 15))] =
+              f32x4{y[4 * r], y[4 * r + 1], y[4 * r + 2], y[4 * r + 3]};
+      }
       if (hf == 0 && lane < 32) ml[kw][wv0 + j * 32 + lane] = make_float2(m_run[j], l_run[j]);
     }
     __syncthreads();
 #pragma unroll
-    for (int it = 0; it < (NQ * 8 + THREADS - 1) / THREADS; ++it) {
-      const int v = (it * THREADS + tid) >> 3, ch = tid & 7;
+    for (int it = 0; it < (NQ * CH + THREADS - 1) / THREADS; ++it) {
+      const int v = (it * THREADS + tid) / CH, ch = tid % CH;
       if (v >= NQ || !exists(v)) continue;
       float2 w[KW];
       float m = -INFINITY, l = 0.f;
@@ -585,7 +590,8 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
       f32x4 y0 = f32x4{}, y1 = f32x4{};
 #pragma unroll
       for (int k = 0; k < KW; ++k) {
-        const f32x4* d = (const f32x4*)(smem + (k * QW * QT + (v >> 5)) * 8192) + (v & 31) * 16;
+        const f32x4* d =
+            (const f32x4*)(smem + (k * QW * QT + (v >> 5)) * WAVE_O) + (v & 31) * PIECES;
         const float f = w[k].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w[k].x - m);
         y0 += f * d[(2 * ch) ^ (v & 15)];
         y1 += f * d[(2 * ch + 1) ^ (v & 15)];
