@@ -27,13 +27,13 @@
 // LDS bitmap, CA_WIN blocks at a time, so a list is a set, whatever its order and repetitions.
 // Neighbouring queries mostly choose the same blocks: a block is then loaded and made operands once
 // for all of them, and every column of the products is in use (one wave per row, 16 columns of
-// which G are used: 2048 rows x 16 heads, 16 blocks of 64 of 32768 keys, 226 us; 56 here).
+// which G are used: 2048 rows x 16 heads, 16 blocks of 64 of 32768 keys, 226 us; 52 here).
 //
 // Bound. A long cache's codes (32 rows x 16 heads over 131072 keys x 8 heads, 268 MB: 56 us, 4.8
 // TB/s, what a large copy reaches). Many rows: the instructions of the softmax and of making
 // operands, 62 % of the VALU's time beside 40 % of the matrix units' (2048 rows x 16 heads over 4096
-// keys under the mask: 62 us, 0.83 PFLOP/s). A block of 32 rows x 16 heads over 8224 keys: 12.9 us, of
-// which 7 are there without any tile (launch, queries, the ways' meeting, parts out), and
+// keys under the mask: 62 us, 0.83 PFLOP/s). A block of 32 rows x 16 heads over 8224 keys: 11.8 us, of
+// which 6 to 7 are there without any tile (launch, queries, the ways' meeting, parts out), and
 // part_combine_kernel's 4. Three waves a SIMD spill; a larger window of blocks in LDS for two (60 us
 // for 57), weights' sums by other chains or by dot products did not pay.
 #include "kv8.h"
@@ -61,7 +61,8 @@ DRT_DEV float ca_max_xor32(float v) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// A value of the lane 1, 2, then 7 - i of eight, 15 - i of sixteen places away: four steps join 16 lanes.
+// The value of another lane: one away, two away, the mirror image in eight, in sixteen. The four steps
+// join 16 lanes.
 template <int STEP> DRT_DEV uint32_t ca_of_16(uint32_t x) {
   constexpr int CTRL = STEP == 0 ? 0xb1 : STEP == 1 ? 0x4e : STEP == 2 ? 0x141 : 0x140;
   return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, true);

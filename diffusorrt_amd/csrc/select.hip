@@ -247,7 +247,7 @@ struct SelArgs {
 };
 
 // Both steps for 16 rows of one K/V head in a work-group of 16 waves, the keys in LDS (RB rounds of
-// 64 blocks). 1000 rows x 4 heads, 500 blocks: 22.3 us (23.8 with the choice's bits one after the other
+// 64 blocks). 1000 rows x 4 heads, 500 blocks: 22.1 us (23.8 with the choice's bits one after the other
 // and divisions of 64 bits); in two launches, with the keys in memory, 22 + 14. Bound: a
 // work-group's chain (queries, scores, barrier, the choice), of 252 work-groups on as many CUs at
 // once; the 1 MB of sums is read from L2 and the products would take 7 us. Many more rows: L2, which
@@ -271,14 +271,15 @@ __global__ __launch_bounds__(1024, 4) void select_kernel(const SelArgs x) {
   __syncthreads();
   if (wave < rows) {
     const int64_t row = x.row0 + r0 + wave;
-    choose_row<RB>([&](int b) { return keys[wave][b]; }, blocks_of((int)row, x.where, x.sel.block), x.sel,
+    choose_row<RB>([&](int b) { return keys[wave][b]; },
+                   blocks_of((int)row, x.where, x.sel.block), x.sel,
                    x.blocks + (row * x.Hkv + kvh) * x.sel.count);
   }
 }
 
 // The scores alone: 16 rows against 64 * per blocks of one K/V head, four waves. For few rows: those
-// of a block find 128 work-groups here, 16 above (32 rows x 8 heads over 512 blocks 6.7 us, and
-// 6.7 for the choice; at once 26).
+// of a block find 128 work-groups here, 16 above (32 rows x 8 heads over 512 blocks 6.6 us, and
+// 5.9 for the choice; at once 24).
 __global__ __launch_bounds__(256, 2) void block_scores_kernel(const SelArgs x) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // work-group: (row tile * chunks + chunk) * Hkv + head
@@ -320,9 +321,11 @@ int select_rows(int n_rows, int Hkv, int n_blocks) {
 namespace drt {
 
 // Both steps in one launch: work-groups of 16 rows and a K/V head that find half the CUs at
-// least something to do, and keys that fit LDS.
+// least something to do, and keys that fit LDS; or so few blocks that one work-group's time for them
+// is less than a second launch's (a call of 32 rows x 8 heads, blocks of 64: 128 of them 9.8 us, in
+// two launches 12.2; 256 of them 14.7 and 12.3).
 static bool select_at_once(int n_rows, int Hkv, int n_blocks) {
-  return n_blocks <= 1024 && (int64_t)((n_rows + 15) / 16) * Hkv >= 128;
+  return n_blocks <= 128 || (n_blocks <= 1024 && (int64_t)((n_rows + 15) / 16) * Hkv >= 128);
 }
 
 size_t select_blocks_bytes(int n_rows, int Hkv, int n_keys, int block) {
@@ -340,7 +343,8 @@ void select_blocks(const void* q, bool q_bf16, const float* sums, int64_t sums_h
     const int64_t wgs = (int64_t)((n_rows + 15) / 16) * Hkv;
     require(wgs < ((int64_t)1 << 31), "select_blocks: too many rows for one call");
     const dim3 grid((unsigned)wgs);
-    if (nb <= 256) hipLaunchKernelGGL(select_kernel<4>, grid, dim3(1024), 0, s, a);
+    if (nb <= 128) hipLaunchKernelGGL(select_kernel<2>, grid, dim3(1024), 0, s, a);
+    else if (nb <= 256) hipLaunchKernelGGL(select_kernel<4>, grid, dim3(1024), 0, s, a);
     else if (nb <= 512) hipLaunchKernelGGL(select_kernel<8>, grid, dim3(1024), 0, s, a);
     else hipLaunchKernelGGL(select_kernel<16>, grid, dim3(1024), 0, s, a);
     DRT_HIP(hipGetLastError());

@@ -139,7 +139,8 @@ REFUSED = (
         {"mask": 2}, {"block": 0}, {"prompt": -1}, {"q": P + 2}, {"out": P + 8}, {"ws": P + 8},
         {"rows": 2**30, "ws_bytes": 1 << 60})]
     + [_select(**kw) for kw in (
-        {"q": None}, {"sums": None}, {"blocks": None}, {"ws": None}, {"ws_bytes": 8},
+        {"q": None}, {"sums": None}, {"blocks": None},
+        {"n_keys": 8192, "tiles": 256, "ws": None}, {"n_keys": 8192, "tiles": 256, "ws_bytes": 8},
         {"qdt": _lib.I8}, {"rows": 0}, {"hq": 3}, {"n_keys": 0}, {"n_keys": 129}, {"pos0": -1},
         {"size": 0}, {"size": 48}, {"size": -32}, {"count": 0}, {"count": 1025}, {"sinks": -1},
         {"local": 0}, {"sinks": 3, "local": 2}, {"sinks": 2**31 - 1, "local": 2**31 - 1},

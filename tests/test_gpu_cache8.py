@@ -429,6 +429,10 @@ def test_attention_over_more_8_bit_keys_than_4_gib_hold():
     (250, 8, 8, 30000, 29750, None, "f16", "i8", 32, 33, 3, 1),
     (700, 4, 4, 700, 0, (0, 1), "f16", "i8", 32, 5, 0, 1),
     (256, 8, 8, 100, 0, None, "f16", "i8", 32, 4, 0, 1),
+    # as many blocks as one launch takes for few rows, and one more
+    (3, 7, 1, 4096, 4090, None, "f16", "f16", 32, 9, 1, 2),
+    (19, 4, 2, 4097, 4000, (5, 9), "bf16", "i8", 32, 9, 1, 2),
+    (2, 4, 2, 12288, 12000, None, "f16", "i8", 96, 40, 0, 3),
 ])
 def test_select_blocks(rows, hq, hkv, n_keys, pos0, mask, qdt, dtype, block, count, sinks, local):
     _say("select", rows, hq, hkv, n_keys, pos0, mask, qdt, dtype, block, count, sinks, local)
