@@ -177,29 +177,28 @@ struct CaArgs {
   int out_bf16;
 };
 
-// QT query tiles a wave, QW waves over query tiles, KW waves over keys (wave kw takes key
-// tiles kw, kw + KW, ...; their parts meet in LDS at the end). OUT: one key range, the
-// result itself; otherwise a part for the combine. SPARSE: the listed blocks' keys.
-template <int DT, int QT, int QW, int KW, bool OUT, bool SPARSE>
-__global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArgs x) {
+// QT query tiles, KW waves over keys (wave kw takes key tiles kw, kw + KW, ...; their parts meet in LDS
+// at the end). OUT: one key range, the result itself; otherwise a part for the combine.
+// SPARSE: the listed blocks' keys.
+template <int DT, int QT, int KW, bool OUT, bool SPARSE>
+__global__ __launch_bounds__(64 * KW, 2) void cache_attn_kernel(const CaArgs x) {
   typedef CacheT<DT> T;
   typedef typename T::vec vec;
-  constexpr int NW = QW * KW, THREADS = 64 * NW, NQ = 32 * QT * QW, TILE = T::TILE, LD = T::LOADS;
-  static_assert(!SPARSE || (QT == 1 && QW == 1), "a work-group has one union of lists");
+  constexpr int THREADS = 64 * KW, NQ = 32 * QT, TILE = T::TILE, LD = T::LOADS;
+  static_assert(!SPARSE || QT == 1, "a work-group has one union of lists");
   // LDS: the queries, then halves (64 head dims) of every wave's O, one after the other: the first is
   // on its way to memory under the second (32 rows over 8224 keys 12.3 us; all at once 12.7). One
   // query tile has little to write: all at once (one row over 8192 keys 6.4 us; halves 6.9).
   constexpr int PASSES = KW == 8 && !SPARSE ? 1 : 2, PIECES = 32 / PASSES, WAVE_O = 32 * PIECES * 16;
-  constexpr int Q_BYTES = NQ * CA_QROW * 2, O_BYTES = NW * QT * WAVE_O;
+  constexpr int Q_BYTES = NQ * CA_QROW * 2, O_BYTES = KW * QT * WAVE_O;
   __shared__ __align__(16) char smem[Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
   __shared__ float2 ml[KW][NQ];  // base and sum of every way
   __shared__ float2 qinfo[NQ];  // c times a query vector's power of two; -128 * 2^-24 its sum
   __shared__ uint32_t bits[SPARSE ? CA_WIN : 1];  // rows that list a block of the window
   __shared__ int2 list[SPARSE ? CA_WIN : 1];      // its blocks and their rows
-  __shared__ int tally[SPARSE ? NW + 1 : 1];
+  __shared__ int tally[SPARSE ? KW : 1];
   const int lane = threadIdx.x & 63, tid = threadIdx.x;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int qw = wave % QW, kw = wave / QW;
+  const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const AttnWhere& where = x.where;
   const int G = x.Hq / x.Hkv, kvh = blockIdx.x % x.Hkv, split = blockIdx.x / x.Hkv;
   // the last rows, which see the most keys, start first
@@ -208,7 +207,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   // The (row, head) of query vector v of the work-group.
   const int GC = SPARSE ? min(G, 32) : G, RPT = 32 / GC;  // (listed blocks) heads and rows of a tile
   const int head0 = SPARSE ? (int)blockIdx.z * 32 : 0, row0 = SPARSE ? group * RPT : 0;
-  const int qt0 = SPARSE ? 0 : group * (QW * QT), n_qv = x.n_rows * G;
+  const int qt0 = SPARSE ? 0 : group * QT, n_qv = x.n_rows * G;
   auto row_of = [&](int v) { return SPARSE ? row0 + v / GC : (qt0 * 32 + v) / G; };
   auto head_of = [&](int v) {
     return kvh * G + (SPARSE ? head0 + v % GC : (qt0 * 32 + v) % G);
@@ -240,8 +239,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
       qraw[it] = *(const u32x4*)(x.q + ((int64_t)row_of(v) * x.Hq + head_of(v)) * 128 + (tid & 15) * 8);
   }
 
-  const int wv0 = qw * QT * 32;  // the wave's first query vector
-  const uint16_t* ql = (const uint16_t*)smem + (wv0 + (lane & 31)) * CA_QROW + 8 * (lane >> 5);
+  const uint16_t* ql = (const uint16_t*)smem + (lane & 31) * CA_QROW + 8 * (lane >> 5);
   constexpr bool HOLD = QT == 1 && DT == 0;  // the queries' operands in registers (16 bits: too many)
   vec qr[HOLD ? 8 : 1];
   int q_end[QT];
@@ -250,7 +248,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   const int last_row = x.n_rows - 1;
 #pragma unroll
   for (int j = 0; j < QT; ++j)
-    q_end[j] = key_end_of(min(row_of(wv0 + j * 32 + (lane & 31)), last_row), where);
+    q_end[j] = key_end_of(min(row_of(j * 32 + (lane & 31)), last_row), where);
   // Queries into LDS and from there to the waves. Called by every thread, once, with the
   // first tile's loads under way.
   auto stage = [&] {
@@ -287,7 +285,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
     }
 #pragma unroll
     for (int j = 0; j < QT; ++j) {
-      const float2 y = qinfo[wv0 + j * 32 + (lane & 31)];
+      const float2 y = qinfo[j * 32 + (lane & 31)];
       cq[j] = y.x;
       nq[j] = y.y;
     }
@@ -302,10 +300,9 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
     }
   };
   reset();
-  // (ends never fall from row to row) keys every row of the wave sees, and any of them
-  const int wave_full = key_end_of(min(row_of(wv0), last_row), where);
-  const int wave_end =
-      key_end_of(SPARSE ? end_row : min(row_of(wv0 + QT * 32 - 1), last_row), where);
+  // (ends never fall from row to row) keys that every row of the work-group sees, and any of them
+  const int full_end = key_end_of(min(row_of(0), last_row), where);
+  const int any_end = key_end_of(SPARSE ? end_row : min(row_of(QT * 32 - 1), last_row), where);
   const uint32_t my_row = SPARSE ? 1u << ((lane & 31) / GC & 31) : 0u;
   const uint32_t all_rows = SPARSE ? (uint32_t)((1ull << (end_row - row0 + 1)) - 1) : 0u;
 
@@ -362,8 +359,8 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
       // its end is not in the tile either. (A NaN score then still is one: see careful, heard.)
       const bool hit = !SPARSE || (seen & my_row) != 0u;
       if (SPARSE) heard |= key0 < q_end[0] ? seen & my_row : 0u;
-      const bool part = key0 + 32 > wave_full || (SPARSE && seen != all_rows);
-      if (key0 + 32 > wave_full || bad || (careful && part)) {
+      const bool part = key0 + 32 > full_end || (SPARSE && seen != all_rows);
+      if (key0 + 32 > full_end || bad || (careful && part)) {
 #pragma unroll
         for (int j = 0; j < QT; ++j) {
           const int mine = hit ? q_end[j] : 0;
@@ -453,14 +450,14 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
   if constexpr (!SPARSE) {
     const int n_tiles = (where.n_keys + 31) >> 5;
     const int t0 = share(n_tiles, split) + kw;
-    const int t_end = !exists(wv0) ? 0 : min(share(n_tiles, split + 1), (wave_end + 31) >> 5);
+    const int t_end = min(share(n_tiles, split + 1), (any_end + 31) >> 5);
     const int n = (t_end - t0 + KW - 1) / KW;
     first(n, t0);
     stage();
     run(n, t0, 0u, false, [&](int& t, uint32_t&) { t += KW; });
   } else {
     const int m = x.block >> 5;
-    const int n_blocks = (int)((uint32_t)(wave_end - 1) / (uint32_t)x.block) + 1;
+    const int n_blocks = (int)((uint32_t)(any_end - 1) / (uint32_t)x.block) + 1;
     const int step_e = KW / m, step_r = KW % m;
     // 16 bits: a V that is not finite makes 0 * V of a row that does not see it NaN too, and a K the
     // score of one that does not list it. Rows are looked at afterwards, and only if some are not
@@ -480,18 +477,18 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
         }
         ca_lds_barrier();
         // the window's blocks in order: wave w finds those of its share, then all take their places
-        const int part_of = (n_win + 64 * NW - 1) / (64 * NW) * 64, i0 = wave * part_of;
+        const int part_of = (n_win + 64 * KW - 1) / (64 * KW) * 64, i0 = kw * part_of;
         auto rows_of = [&](int i) { return i + lane < n_win ? bits[min(i + lane, CA_WIN - 1)] : 0u; };
         const uint32_t rows0 = rows_of(i0);
         int found = (int)__popcll(__ballot(rows0 != 0u));
         for (int i = i0 + 64; i < min(n_win, i0 + part_of); i += 64)
           found += (int)__popcll(__ballot(rows_of(i) != 0u));
-        if (lane == 0) tally[wave] = found;
+        if (lane == 0) tally[kw] = found;
         ca_lds_barrier();
         int at = 0, n_list = 0;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          at += w < wave ? tally[w] : 0;
+        for (int w = 0; w < KW; ++w) {
+          at += w < kw ? tally[w] : 0;
           n_list += tally[w];
         }
         for (int i = i0; i < min(n_win, i0 + part_of); i += 64) {
@@ -504,7 +501,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
         n_list = __builtin_amdgcn_readfirstlane(n_list);
         // tiles in all (of the last block those that the rows see), and this wave's of this range
         const int last = __builtin_amdgcn_readfirstlane(list[max(n_list - 1, 0)].x);
-        const int n = n_list == 0 ? 0 : (n_list - 1) * m + min(m, ((wave_end + 31) >> 5) - last * m);
+        const int n = n_list == 0 ? 0 : (n_list - 1) * m + min(m, ((any_end + 31) >> 5) - last * m);
         const int j0 = share(n, split) + kw, j1 = share(n, split + 1);
         int e = j0 / m, r = j0 - e * m;
         auto here = [&](int& t, uint32_t& rows) {
@@ -565,7 +562,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
     __syncthreads();  // the queries, or the first half, have been read
 #pragma unroll
     for (int j = 0; j < QT; ++j) {
-      f32x4* d = (f32x4*)(smem + ((kw * QW + qw) * QT + j) * WAVE_O);
+      f32x4* d = (f32x4*)(smem + (kw * QT + j) * WAVE_O);
 #pragma unroll
       for (int b = 0; b < 4 / PASSES; ++b) {
         const f32x16& y = o[j][hf * (4 / PASSES) + b];
@@ -574,7 +571,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
           d[(lane & 31) * PIECES + ((b * 8 + 2 * r + (lane >> 5)) ^ (lane & 15))] =
               f32x4{y[4 * r], y[4 * r + 1], y[4 * r + 2], y[4 * r + 3]};
       }
-      if (hf == 0 && lane < 32) ml[kw][wv0 + j * 32 + lane] = make_float2(m_run[j], l_run[j]);
+      if (hf == 0 && lane < 32) ml[kw][j * 32 + lane] = make_float2(m_run[j], l_run[j]);
     }
     __syncthreads();
 #pragma unroll
@@ -592,7 +589,7 @@ __global__ __launch_bounds__(64 * QW * KW, 2) void cache_attn_kernel(const CaArg
 #pragma unroll
       for (int k = 0; k < KW; ++k) {
         const f32x4* d =
-            (const f32x4*)(smem + (k * QW * QT + (v >> 5)) * WAVE_O) + (v & 31) * PIECES;
+            (const f32x4*)(smem + (k * QT + (v >> 5)) * WAVE_O) + (v & 31) * PIECES;
         const float f = w[k].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w[k].x - m);
         y0 += f * d[(2 * ch) ^ (v & 15)];
         y1 += f * d[(2 * ch + 1) ^ (v & 15)];
@@ -721,21 +718,31 @@ void part_combine(const float* o_part, const float* ml_part, int splits, int64_t
 CachePlan plan_attention8(int n_rows, int Hq, int Hkv, int n_keys) {
   CachePlan p;
   const int64_t qtiles = ((int64_t)n_rows * (Hq / Hkv) + 31) / 32;
-  // Many queries: two query tiles a wave (a tile's codes made operands once for both), four key
-  // ways in a work-group of their own, so that work-groups are as many as can be (2048 rows x 16
-  // heads over 4096 keys: 72 us at that step; two and one key ways, which need key ranges to fill the
-  // chip: 101, 110). Few: eight waves over the one, two or four query tiles (two tiles a wave: 32 rows
-  // over 8224 keys 18 us for 12.6, over 131072 keys 66 for 57; a wave waits on what it holds).
-  p.wide = qtiles > 4;
-  p.qw = p.wide || qtiles == 1 ? 1 : qtiles == 2 ? 2 : 4;
-  const int kw = p.wide ? 4 : 8 / p.qw, per = p.wide ? 2 : p.qw;  // (query tiles of a work-group)
-  p.groups = (qtiles + per - 1) / per;
   const int n_tiles = (int)(((int64_t)n_keys + 31) / 32);
-  const int64_t wgs = Hkv * p.groups;
-  int64_t splits = std::max<int64_t>(1, (p.wide ? 512 : 256) / wgs);
-  // (Three tiles a wave cost less than the second launch: one row x 28 heads over 768 keys 7.8 us, 8.3
-  // with key ranges, over 1024 8.7 and 8.3; 32 rows x 16 heads over 384 keys 8.4 and 9.0.)
-  p.splits = n_tiles <= 3 * kw ? 1 : (int)std::min<int64_t>({splits, (n_tiles + kw - 1) / kw, 64});
+  // Many queries: two query tiles a wave (a tile's codes made operands once for both), four key ways,
+  // where that makes work-groups for three in four of the 512 places (2048 rows x 16 heads over 4096
+  // keys 79 us, one query tile and eight ways 88; 1000 rows 52 and 44). Otherwise one query tile and
+  // eight ways: the least time a work-group (64 rows over 8224 keys: 13 us; four query tiles a
+  // work-group and two ways, which read a tile once for all four, 19; over 131072 keys 91 and 95).
+  p.groups = (qtiles + 1) / 2;
+  p.wide = Hkv * p.groups >= 384;
+  if (p.wide) return p;
+  p.groups = qtiles;
+  // Key ranges by what a call takes, in us: its rounds of 256 work-groups, 2.5 and 0.6 a tile of a wave
+  // each; a second launch 4 (one row x 28 heads over 1337 keys: 9.3 a call in one launch, 13.8 in two, in
+  // a graph 9.0 and 7.8; over 2048 11.2 and 13.6, 10.8 and 7.9), and the parts, written and read.
+  const int64_t wgs = Hkv * qtiles;
+  const float part_us = (float)n_rows * (float)Hq * (2 * 130 * 4 / 4.5e6f);
+  float best = INFINITY;
+  const int most = std::min(64, (n_tiles + 7) / 8);
+  for (int s = 1; s <= most; ++s) {
+    const float us = (float)((wgs * s + 255) / 256) * (2.5f + 0.6f * (float)((n_tiles + 8 * s - 1) / (8 * s))) +
+                     (s > 1 ? 4.f + part_us * (float)s : 0.f);
+    if (us < best) {
+      best = us;
+      p.splits = s;
+    }
+  }
   return p;
 }
 
@@ -783,13 +790,12 @@ static CaArgs args_of(KvType type, const void* q, bool q_bf16, const void* kv_la
   return a;
 }
 
-#define DRT_CA1(DT, QT, QW, KW, OUT, SPARSE)                                                      \
-  hipLaunchKernelGGL((cache_attn_kernel<DT, QT, QW, KW, OUT, SPARSE>), grid, dim3(64 * QW * KW), 0, \
-                     s, a)
-#define DRT_CA(DT, QT, QW, KW, SPARSE)                                                            \
+#define DRT_CA1(DT, QT, KW, OUT, SPARSE) \
+  hipLaunchKernelGGL((cache_attn_kernel<DT, QT, KW, OUT, SPARSE>), grid, dim3(64 * KW), 0, s, a)
+#define DRT_CA(DT, QT, KW, SPARSE)                                                                \
   do {                                                                                            \
-    if (p.splits == 1) DRT_CA1(DT, QT, QW, KW, true, SPARSE);                                     \
-    else DRT_CA1(DT, QT, QW, KW, false, SPARSE);                                                  \
+    if (p.splits == 1) DRT_CA1(DT, QT, KW, true, SPARSE);                                         \
+    else DRT_CA1(DT, QT, KW, false, SPARSE);                                                      \
   } while (0)
 
 void attention8(const void* q, bool q_bf16, const void* kv_layer, int64_t kv_head_stride,
@@ -798,10 +804,8 @@ void attention8(const void* q, bool q_bf16, const void* kv_layer, int64_t kv_hea
   const CaArgs a = args_of(KvType::I8, q, q_bf16, kv_layer, kv_head_stride, scales, n_rows, Hq, Hkv,
                            where, p, part, out, out_bf16);
   const dim3 grid((unsigned)(p.splits * Hkv), (unsigned)p.groups);
-  if (p.wide) DRT_CA(0, 2, 1, 4, false);
-  else if (p.qw == 1) DRT_CA(0, 1, 1, 8, false);
-  else if (p.qw == 2) DRT_CA(0, 1, 2, 4, false);
-  else DRT_CA(0, 1, 4, 2, false);
+  if (p.wide) DRT_CA1(0, 2, 4, true, false);
+  else DRT_CA(0, 1, 8, false);
   DRT_HIP(hipGetLastError());
   if (p.splits > 1) part_combine(part, a.ml_part, p.splits, (int64_t)n_rows * Hq, out, out_bf16, s);
 }
@@ -817,7 +821,7 @@ void sparse_attention(KvType type, const void* q, bool q_bf16, const void* kv_la
   a.block = block;
   const dim3 grid((unsigned)(p.splits * Hkv), (unsigned)p.groups, (unsigned)((Hq / Hkv + 31) / 32));
 #define DRT_SP(DT)                                                                                \
-  do { if (p.wide) DRT_CA(DT, 1, 1, 4, true); else DRT_CA(DT, 1, 1, 8, true); } while (0)
+  do { if (p.wide) DRT_CA1(DT, 1, 4, true, true); else DRT_CA(DT, 1, 8, true); } while (0)
   if (type == KvType::I8) DRT_SP(0);
   else if (type == KvType::F16) DRT_SP(1);
   else DRT_SP(2);

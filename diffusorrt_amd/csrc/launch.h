@@ -222,7 +222,7 @@ void kv16_store(bool kv_bf16, const void* k, const void* v, bool src_bf16, int n
 // How an attention over the cache is cut: key ranges (splits), whose parts are joined by a second
 // launch, and work-groups of query tiles.
 struct CachePlan {
-  int qw = 1, splits = 1;
+  int splits = 1;
   int64_t groups = 1;
   bool wide = false;
 };
