@@ -32,9 +32,9 @@
 // Bound. A long cache's codes (32 rows x 16 heads over 131072 keys x 8 heads, 268 MB: 56 us, 4.8
 // TB/s, what a large copy reaches). Many rows: the instructions of the softmax and of making
 // operands, 62 % of the VALU's time beside 40 % of the matrix units' (2048 rows x 16 heads over 4096
-// keys under the mask: 62 us, 0.83 PFLOP/s). A block of 32 rows x 16 heads over 8224 keys: 11.8 us, of
-// which 6 to 7 are there without any tile (launch, queries, the ways' meeting, parts out), and
-// part_combine_kernel's 4. Three waves a SIMD spill; a larger window of blocks in LDS for two (60 us
+// keys under the mask: 62 us, 0.83 PFLOP/s). A block of 32 rows x 16 heads over 8224 keys: 11.3 us with
+// its combine, in a graph, of which about 7 are there without any tile (launches, queries, the ways'
+// meeting, parts out and in). Three waves a SIMD spill; a larger window of blocks in LDS for two (60 us
 // for 57), weights' sums by other chains or by dot products did not pay.
 #include "kv8.h"
 #include "launch.h"
@@ -754,9 +754,9 @@ CachePlan plan_sparse(int n_rows, int Hq, int Hkv, int count, int block) {
   // rows x 28 heads, 16 blocks of 64: 12.4 us; of eight 13.3, of 16 16.2)
   const int64_t wgs = p.groups * Hkv * heads, tiles = (int64_t)count * (block / 32);
   p.wide = wgs >= 512;
-  // (As few as 16 tiles of a tile's rows cost less than the second launch: one row x 28 heads, 8
-  // blocks of 64 9.4 us, with key ranges 10.1; 16 blocks 11.2 and 10.2.)
-  p.splits = p.wide || tiles * std::min(n_rows, rows) <= 16
+  // (32 tiles of a tile's rows at most cost less than the second launch: one row x 28 heads, 16 blocks
+  // of 64 10.5 us a call, with key ranges 14.1; in a graph 10.1 and 9.2.)
+  p.splits = p.wide || tiles * std::min(n_rows, rows) <= 32
                  ? 1
                  : (int)std::max<int64_t>(1, std::min<int64_t>({256 / wgs, (tiles + 3) / 4, 64}));
   return p;
