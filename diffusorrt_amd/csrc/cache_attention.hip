@@ -736,8 +736,9 @@ CachePlan plan_attention8(int n_rows, int Hq, int Hkv, int n_keys) {
   float best = INFINITY;
   const int most = std::min(64, (n_tiles + 7) / 8);
   for (int s = 1; s <= most; ++s) {
-    const float us = (float)((wgs * s + 255) / 256) * (2.5f + 0.6f * (float)((n_tiles + 8 * s - 1) / (8 * s))) +
-                     (s > 1 ? 4.f + part_us * (float)s : 0.f);
+    const float rounds = (float)((wgs * s + 255) / 256);
+    const float tiles = (float)((n_tiles + 8 * s - 1) / (8 * s));
+    const float us = rounds * (2.5f + 0.6f * tiles) + (s > 1 ? 4.f + part_us * (float)s : 0.f);
     if (us < best) {
       best = us;
       p.splits = s;
