@@ -754,7 +754,9 @@ CachePlan plan_sparse(int n_rows, int Hq, int Hkv, int count, int block) {
   // Few work-groups: as many key ranges as give every CU one, of four of a list's tiles at least (9
   // rows x 28 heads, 16 blocks of 64: 12.4 us; of eight 13.3, of 16 16.2)
   const int64_t wgs = p.groups * Hkv * heads, tiles = (int64_t)count * (block / 32);
-  p.wide = wgs >= 512;
+  // More than the CUs: four waves a work-group, two of which share a CU (1000 rows x 16 heads, 16 blocks of
+  // 64 of 32768 keys: 28.7 us; eight waves, in two rounds, 36.5).
+  p.wide = wgs > 256;
   // (32 tiles of a tile's rows at most cost less than the second launch: one row x 28 heads, 16 blocks
   // of 64 10.5 us a call, with key ranges 14.1; in a graph 10.1 and 9.2.)
   p.splits = p.wide || tiles * std::min(n_rows, rows) <= 32
