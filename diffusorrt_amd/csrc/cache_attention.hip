@@ -728,9 +728,10 @@ CachePlan plan_attention8(int n_rows, int Hq, int Hkv, int n_keys) {
   p.wide = Hkv * p.groups >= 384;
   if (p.wide) return p;
   p.groups = qtiles;
-  // Key ranges by what a call takes, in us: its rounds of 256 work-groups, 2.5 and 0.6 a tile of a wave
-  // each; a second launch 4 (one row x 28 heads over 1337 keys: 9.3 a call in one launch, 13.8 in two, in
-  // a graph 9.0 and 7.8; over 2048 11.2 and 13.6, 10.8 and 7.9), and the parts, written and read.
+  // Key ranges by what a call takes, in us: its rounds of 256 work-groups, 2.5 and 0.6 a tile of a
+  // wave each; a second launch 4 (one row x 28 heads over 1337 keys: 9.3 a call in one launch, 13.8 in
+  // two, in a graph 9.0 and 7.8; over 2048 11.2 and 13.6, 10.8 and 7.9), and the parts, written and
+  // read.
   const int64_t wgs = Hkv * qtiles;
   const float part_us = (float)n_rows * (float)Hq * (2 * 130 * 4 / 4.5e6f);
   float best = INFINITY;
@@ -754,8 +755,8 @@ CachePlan plan_sparse(int n_rows, int Hq, int Hkv, int count, int block) {
   // Few work-groups: as many key ranges as give every CU one, of four of a list's tiles at least (9
   // rows x 28 heads, 16 blocks of 64: 12.4 us; of eight 13.3, of 16 16.2)
   const int64_t wgs = p.groups * Hkv * heads, tiles = (int64_t)count * (block / 32);
-  // More than the CUs: four waves a work-group, two of which share a CU (1000 rows x 16 heads, 16 blocks of
-  // 64 of 32768 keys: 28.7 us; eight waves, in two rounds, 36.5).
+  // More than the CUs: four waves a work-group, two of which share a CU (1000 rows x 16 heads, 16
+  // blocks of 64 of 32768 keys: 28.7 us; eight waves, in two rounds, 36.5).
   p.wide = wgs > 256;
   // (32 tiles of a tile's rows at most cost less than the second launch: one row x 28 heads, 16 blocks
   // of 64 10.5 us a call, with key ranges 14.1; in a graph 10.1 and 9.2.)
