@@ -652,7 +652,10 @@ __global__ __launch_bounds__(128) void part_combine_kernel(const float* __restri
     float mb = m;
 #pragma unroll
     for (int j = 0; j < SB; ++j) {
-      if (s0 + 4 * j >= splits) ml[j] = make_float2(-INFINITY, 0.f);
+      if (s0 + 4 * j >= splits) {  // (the last range's again: 0 * infinity would be NaN)
+        ml[j] = make_float2(-INFINITY, 0.f);
+        p0[j] = p1[j] = f32x4{};
+      }
       mb = fmaxf(mb, ml[j].x);
     }
     const float sc = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mb);
