@@ -134,6 +134,9 @@ def attention_bound(q, k, v, ends, weight, p_half: float, n_keys: int, *, q_bf16
       which a product rounds at most once a key and a fold once more (a tile's sum of weights: 32
       times), 2 n_keys times in all;
     - bf16 queries that are scaled to fp16 lose at most 2^-25 of the vector's largest each.
+
+    From a few thousand keys on this is wider than a tile's part of the result (8224 keys: 0.020,
+    results 0.018): it holds, but tells little there. :func:`attention_limit` does.
     """
     q = np.abs(np.asarray(q, np.float64))
     k, v = np.abs(np.nan_to_num(k)), np.abs(np.nan_to_num(v))
@@ -146,3 +149,75 @@ def attention_bound(q, k, v, ends, weight, p_half: float, n_keys: int, *, q_bf16
     rel = p_half + 2 * e + (n_keys / 32 + 64) * 2.0 ** -24
     floor = n_keys * 2.0 ** -24 * v.max() + (2 * n_keys + 4) * 2.0 ** -24 * 255 * scales8[1]
     return rel[..., None] * weight + floor
+
+
+def attention_terms(q, k, v, ends, scales=None, blocks=None, block: int = 0):
+    """:func:`attention` with what :func:`attention_limit` is made of, for each (row, head):
+
+    - out, weight ``[rows, hq, 128]`` as :func:`attention`;
+    - keys: how many it attends to; score: the largest sum of |q| (|k| + 128 K scales) / sqrt(128)
+      of one; kside: the largest sum of |k| + 128 K scales;
+    - most: the largest p |code| scale (8 bits) or p |v|, at its largest |code| or |v|;
+    - span: the sum of p 255 V scales (8 bits), 0 otherwise;
+    - tiles ``[rows, hq, tiles]``: what each tile of keys has of the weights' sum (1).
+
+    scales: ``[hkv, tiles, 2]`` of an 8-bit cache."""
+    q = np.asarray(q, np.float64)
+    rows, hq, _ = q.shape
+    n, hkv, _ = k.shape
+    g, pad = hq // hkv, -n % TILE
+    t = {"out": np.zeros((rows, hq, 128)), "weight": np.zeros((rows, hq, 128)),
+         "tiles": np.zeros((rows, hq, (n + pad) // TILE))}
+    t |= {name: np.zeros((rows, hq)) for name in ("keys", "score", "kside", "most", "span")}
+    key = np.arange(n)
+    for h in range(hkv):
+        seen = key[None] < np.asarray(ends)[:, None]
+        if blocks is not None:
+            hit = np.zeros((rows, -(-n // block)), bool)
+            r, at = np.nonzero((blocks[:, h] >= 0) & (blocks[:, h] < hit.shape[1]))
+            hit[r, blocks[r, h, at]] = True
+            seen = seen & hit[:, key // block]
+        sk, sv = np.zeros((2, n)) if scales is None else \
+            np.repeat(scales[h], TILE, 0)[:n].T
+        kk, vv = k[:, h], v[:, h]
+        kabs = np.abs(kk) + 128 * sk[:, None]
+        for j in range(g):
+            i = h * g + j
+            s = np.where(seen, q[:, i] @ kk.T * 128 ** -0.5, -np.inf)
+            top = s.max(1)
+            p = np.where(seen, np.exp(s - np.where(np.isfinite(top), top, 0)[:, None]), 0.0)
+            p /= np.maximum(p.sum(1), 1e-300)[:, None]
+            t["out"][:, i], t["weight"][:, i] = p @ vv, p @ np.abs(vv)
+            t["keys"][:, i] = seen.sum(1)
+            t["score"][:, i] = np.where(seen, np.abs(q[:, i]) @ kabs.T * 128 ** -0.5, 0).max(1)
+            t["kside"][:, i] = np.where(seen, kabs.sum(1), 0).max(1)
+            t["most"][:, i] = (p * (127 * sv)).max(1) if scales is not None else \
+                p.max(1) * np.abs(vv).max()
+            t["span"][:, i] = 255 * (p @ sv)
+            t["tiles"][:, i] = np.pad(p, ((0, 0), (0, pad))).reshape(rows, -1, TILE).sum(2)
+    return t
+
+
+def attention_limit(q, t, p_half: float, n_keys: int, ranges: int, *, q_bf16_scaled=False):
+    """:func:`attention_bound` by what each (row, head) attends to: no more than the roundings can
+    add up to there, so that a tile or a block left out passes it. ranges: the call's key ranges.
+
+    - A wave has every fourth tile at most of a range, and no keys but the row's own weigh more than
+      zero: ``keys`` of a wave below. What it sums is rounded once a key, the weights' sum of 8
+      bits as often, both once more a tile (a fold, or a change of base), and joined with the other
+      waves' and ranges' (64 roundings and 64 more at most). As every rounding is at most
+      half a step of a partial sum of magnitudes, and the waves' sums of magnitudes add up to the
+      row's, that is so many times 2^-24 of ``weight`` or, over 8 bits, of ``span``.
+    - A weight is rounded to the product's type: ``p_half`` of it, or 2^-25 of a unit that is no
+      more than the largest of its wave: ``most`` for each key.
+    - Scores as in attention_bound, with the sums of one key's magnitudes for those of the
+      largest of every head dim."""
+    q = np.abs(np.asarray(q, np.float64))
+    e = 130 * 2.0 ** -24 * t["score"]
+    if q_bf16_scaled:
+        e = e + 128 ** -0.5 * 2.0 ** -25 * q.max(-1) * t["kside"]
+    wave = np.minimum(t["keys"], TILE * ((-(-n_keys // TILE)) // (4 * ranges) + 2))
+    steps = (2 * wave + 2 * (wave / TILE + 1) + 128) * 2.0 ** -24
+    rel = p_half + 2 * e + steps
+    floor = t["keys"] * 2.0 ** -25 * t["most"] + steps * t["span"]
+    return rel[..., None] * t["weight"] + floor[..., None]
