@@ -238,3 +238,119 @@ def test_listed_blocks_of_rows(i, dtype):
     kh, vh, scales = _held(k, v, dtype)
     t = X.attention_terms(q.double().numpy(), kh, vh, ends, scales, lists, block)
     _within(got, t, _limit(q, t, dtype, n, _listed_ranges(i), TDT[odt]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["dense", "i8", "f16", "bf16"])
+def test_many_rows_over_tiles_of_very_different_scales(form):
+    """V tiles from 1e-9 to 1e9 and zero, K tiles zero and large, over the many-row kernels (416
+    work-groups of two query tiles; 800 of a list's)."""
+    rows, hq, hkv, n = 400, 64, 32, 32 * 12
+    _say("scale spread", form)
+    dtype = "i8" if form == "dense" else form
+    rng = np.random.default_rng(5)
+    q = torch.from_numpy(rng.standard_normal((rows, hq, 128), np.float32)).to(
+        TDT[dtype] if dtype != "i8" else torch.float16) * 3
+    k, v = (torch.from_numpy(rng.standard_normal((n, hkv, 128), np.float32)) for _ in range(2))
+    sizes = [0.0, 1e-9, 1.0, 1e9, 0.0, 1e-6, 1e3, 0.0, 1e-9, 1e-3, 1e-7, 0.0]
+    for at, s in enumerate(sizes):
+        v[32 * at:32 * at + 32] *= s if dtype != "f16" else min(s, 1e3)
+    k[64:128] = 0.0
+    k[320:] *= 30.0
+    cache = _cache(k, v, dtype)
+    kh, vh, scales = _held(k, v, dtype)
+    for n_keys in (32, 64, 96, 352, n):
+        ends = X.key_ends(rows, n_keys, 0)
+        lists = None if form == "dense" else \
+            np.tile(np.arange(n_keys // 32, dtype=np.int32), (rows, hkv, 1))
+        got = _call(cache, q, n_keys, 0, None, torch.float32, lists, 32)
+        t = X.attention_terms(q.double().numpy(), kh[:n_keys], vh[:n_keys], ends,
+                              None if scales is None else scales[:, :n_keys // 32], lists, 32)
+        _within(got, t, _limit(q, t, dtype, n_keys, 1, torch.float32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("form", ["dense", "i8", "f16", "bf16"])
+def test_nan_among_many_rows_reaches_those_that_see_it(form, where):
+    """Blocks of 32 rows under the mask: a NaN key or value in block 2 reaches rows 64 and on, a NaN
+    query its own head; what is not finite behind n_keys reaches none. The other rows keep their
+    results."""
+    rows, hq, hkv, n = 416, 64, 32, 448
+    n_keys = 416
+    _say("nan", form, where)
+    dtype = "i8" if form == "dense" else form
+    rng = np.random.default_rng(13)
+    q = torch.from_numpy(rng.standard_normal((rows, hq, 128), np.float32)).to(
+        TDT[dtype] if dtype != "i8" else torch.bfloat16)
+    k, v = (torch.from_numpy(rng.standard_normal((n, hkv, 128), np.float32)) for _ in range(2))
+    held = _held(k, v, dtype)
+    (k if where == "k" else v)[70, :, 5] = float("nan")
+    k[n_keys:], v[n_keys:] = float("nan"), float("inf")
+    q_nan = q.clone()
+    q_nan[3, 1, 0] = float("nan")
+    lists = None if form == "dense" else \
+        np.tile(np.arange(n_keys // 32, dtype=np.int32), (rows, hkv, 1))
+    got = _call(_cache(k, v, dtype), q_nan, n_keys, 0, (0, 32), torch.float32, lists, 32)
+    want = np.zeros((rows, hq), bool)
+    want[64:] = True
+    want[3, 1] = True
+    np.testing.assert_array_equal(np.isnan(got).any(2), want)
+    if dtype == "i8" or where == "k":  # (a NaN of V in 16 bits is one head dim's)
+        np.testing.assert_array_equal(np.isnan(got).all(2), want)
+    else:
+        assert np.isfinite(got[64:, :, :5]).all() and np.isfinite(got[64:, :, 6:]).all()
+    ends = X.key_ends(rows, n_keys, 0, (0, 32))
+    some = np.r_[0:3, 4:64]
+    t = X.attention_terms(q.double().numpy()[some], held[0][:n_keys], held[1][:n_keys], ends[some],
+                          None if held[2] is None else held[2][:, :n_keys // 32],
+                          None if lists is None else lists[some], 32)
+    _within(got[some], t, _limit(q[some], t, dtype, n_keys, 1, torch.float32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,hq,hkv,blocks", [
+    (600, 32, 16, 20),    # four waves a work-group
+    (40, 8, 4, 20),       # eight, key ranges
+    (6, 8, 4, 2200),      # two windows of blocks, key ranges
+    (520, 16, 1, 2200),   # two windows, four waves
+])
+def test_values_that_are_not_finite_among_lists(dtype, rows, hq, hkv, blocks):
+    """Neighbouring rows, every third of which lists two blocks (of each window, if there are two)
+    with infinities and a NaN in V and every fifth one with a NaN in K; the others keep theirs."""
+    _say("not finite", dtype, rows, hq, hkv, blocks)
+    n, count = 32 * blocks, 12
+    rng = np.random.default_rng(blocks + rows)
+    q = torch.from_numpy(rng.standard_normal((rows, hq, 128), np.float32)).to(TDT[dtype])
+    k, v = (torch.from_numpy(rng.standard_normal((n, hkv, 128), np.float32)) for _ in range(2))
+    kh, vh, _ = _held(k, v, dtype)
+    odd, nan = (1, blocks - 2), blocks - 4
+    for b in odd:
+        v[32 * b + 9, :, 3], v[32 * b + 30, :, 4] = float("inf"), -float("inf")
+        v[32 * b + 17, :, 5] = float("nan")
+    k[32 * nan + 11, :, 7] = float("nan")
+    free = np.setdiff1d(np.arange(blocks), (*odd, nan))
+    lists = np.full((rows, hkv, count), -1, np.int32)
+    for r in range(rows):
+        for h in range(hkv):
+            lists[r, h, :9] = rng.choice(free, 9, replace=False)
+            if r % 3 == 0:
+                lists[r, h, 9:11] = odd
+            if r % 5 == 0:
+                lists[r, h, 11] = nan
+    got = _call(_cache(k, v, dtype), q, n, 0, None, torch.float32, lists, 32)
+    ends = X.key_ends(rows, n, 0)
+    r = np.arange(rows)
+    assert np.isnan(got[r % 5 == 0]).all()
+    mine = got[(r % 3 == 0) & (r % 5 != 0)]
+    assert (mine[..., 3] == np.inf).all() and (mine[..., 4] == -np.inf).all()
+    assert np.isnan(mine[..., 5]).all()
+    some = np.unique(np.linspace(0, rows - 1, 64).astype(int))
+    t = X.attention_terms(q[some].double().numpy(), kh, vh, ends[some], None, lists[some], 32)
+    tol = _limit(q[some], t, dtype, n, _ranges("drt_op_sparse_attention_workspace_bytes", rows, hq,
+                                               hkv, 32, count), torch.float32)
+    off = ~(np.abs(got[some] - t["out"]) <= tol)
+    off[some % 5 == 0] = False
+    off[some % 3 == 0, :, 3:6] = False
+    assert not off.any(), np.argwhere(off)[:5]
