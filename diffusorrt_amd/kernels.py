@@ -194,6 +194,17 @@ def _launch(torch, fn, index, *args):
         _lib.check(status)
 
 
+def _cache_dtype(dtype) -> int:
+    """The code of a cache's type; what is no name of one is refused, never another type's cache."""
+    code = {"f16": _lib.F16, "bf16": _lib.BF16, "i8": _lib.I8,
+            # (other names that fp16 has always gone by here)
+            None: _lib.F16, "fp16": _lib.F16, "float16": _lib.F16,
+            _torch().float16: _lib.F16}.get(dtype)
+    if code is None:
+        raise ValueError(f"a cache's dtype is 'f16', 'bf16' or 'i8', not {dtype!r}")
+    return code
+
+
 class PrefixKVCache:
     """Tiled K/V cache for ``layers`` layers on one device.
 
@@ -202,15 +213,16 @@ class PrefixKVCache:
     head): 32-key tiles of 8192 elements (K block then V block) in the MFMA
     operand order of the attention kernel. Unwritten slots stay zero.
 
-    ``dtype`` is ``"f16"``, ``"bf16"`` or ``"i8"``: whole numbers of [-127, 127] times one power
-    of two for each tile's K and V (``scales [layers, kv_heads, tiles, 2]``), half the bytes of a
-    16-bit cache. A store into an ``"i8"`` cache quantizes each tile it touches as a whole, from
-    the rows it keeps (as they read) and the new ones, to the least power of two >= 2^-40 that
-    holds them: a value is off by at most half of it (max / 127 to 2 max / 127), a row that later
-    stores of its tile went past by less than one of the last scale. A tile with a value that is
-    not finite, or beyond 127 * 2^40, reads as NaN until one store writes all 32 rows of it, or
-    :meth:`clear`; so does a tile that keeps rows of an earlier sequence take their size into its
-    scale. Clear an ``"i8"`` cache, or one with ``block_sums``, before another sequence.
+    ``dtype`` is ``"f16"``, ``"bf16"`` or ``"i8"``; another is a ValueError. ``"i8"``: whole numbers
+    of [-127, 127] times one power of two for each tile's K and V (``scales [layers, kv_heads,
+    tiles, 2]``), half the bytes of a 16-bit cache. A store into an ``"i8"`` cache quantizes each
+    tile it touches as a whole, from the rows it keeps (as they read) and the new ones, to the least
+    power of two >= 2^-40 that holds them: a value is off by at most half of it (max / 127 to
+    2 max / 127), a row that later stores of its tile went past by less than one of the last scale.
+    A tile with a value that is not finite, or beyond 127 * 2^40, reads as NaN until one store
+    writes all 32 rows of it, or :meth:`clear`; so does a tile that keeps rows of an earlier
+    sequence take their size into its scale. Clear an ``"i8"`` cache, or one with ``block_sums``,
+    before another sequence.
 
     ``block_sums=True`` keeps the sum of each tile's keys (``sums [layers, kv_heads, tiles,
     128]``) up to date, which :meth:`select_blocks` scores blocks by."""
@@ -222,16 +234,16 @@ class PrefixKVCache:
         self.tiles = (int(capacity) + 31) // 32
         self.capacity = self.tiles * 32
         self.head_stride = self.tiles * KV_TILE_ELEMS
-        self.kv_dtype = {"bf16": _lib.BF16, "i8": _lib.I8}.get(dtype, _lib.F16)
+        self.kv_dtype = _cache_dtype(dtype)
         shape = (self.layers, self.kv_heads, self.head_stride)
         device = device or "cuda"
         self.scales = self.sums = None
-        if dtype == "i8":  # a byte is a code + 128
+        if self.kv_dtype == _lib.I8:  # a byte is a code + 128
             self.data = torch.full(shape, 128, dtype=torch.uint8, device=device)
             self.scales = torch.ones((*shape[:2], self.tiles, 2), dtype=torch.float32,
                                      device=device)
         else:
-            self.data = torch.zeros(shape, dtype=torch.bfloat16 if dtype == "bf16"
+            self.data = torch.zeros(shape, dtype=torch.bfloat16 if self.kv_dtype == _lib.BF16
                                     else torch.float16, device=device)
         if block_sums:
             self.sums = torch.zeros((*shape[:2], self.tiles, 128), dtype=torch.float32,
@@ -486,7 +498,12 @@ def attention(q, k, v, *, head_dim: int, kind: str, mask_geometry=None, q_positi
 
     ``q_positions`` (absolute positions of the q rows) must be contiguous; by
     default q rows are the last ``rq`` positions of the ``rk`` keys. The output
-    dtype follows ``q`` like the reference's ``.astype(out_dtype)``."""
+    dtype follows ``q`` like the reference's ``.astype(out_dtype)``.
+
+    ``kv_dtype`` is the cache's: ``"bf16"``, ``"f16"`` or ``"i8"``. Queries are rounded to a
+    16-bit cache's own type; over ``"i8"`` bf16 and fp16 ones stay as they are and others are
+    rounded to fp16. Beyond 65504 a query in fp16 is an infinity and its row NaN: larger ones are
+    for bf16."""
     torch = _torch()
     if head_dim != 128:
         raise ValueError("attention head_dim must be 128")

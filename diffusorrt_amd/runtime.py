@@ -119,6 +119,8 @@ class Runtime:
 
         if device != "rocm":
             raise ValueError(f"this runtime serves device='rocm', not {device!r}")
+        if kv_dtype == "i8":
+            raise ValueError("a session's cache is 'f16' or 'bf16' (8 bits: PrefixKVCache)")
         if not torch.cuda.is_available():
             raise RuntimeError("the rocm runtime needs a visible AMD GPU")
         lib = _lib.load()
