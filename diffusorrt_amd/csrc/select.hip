@@ -310,7 +310,8 @@ template <int R> __global__ __launch_bounds__(256) void choose_blocks_kernel(con
                 x.blocks + ((int64_t)x.row0 * x.Hkv + id) * x.sel.count);
 }
 
-// Rows whose scores one pass holds: 256 MiB of them at most.
+// Rows whose scores one pass holds: 256 MiB of keys, or those of 16 rows where these are more (which
+// share what a pass reads of the sums; a quarter of the sums' bytes at most).
 int select_rows(int n_rows, int Hkv, int n_blocks) {
   const int64_t most = ((int64_t)1 << 28) / ((int64_t)Hkv * n_blocks * 8);
   return (int)std::min<int64_t>(n_rows, std::max<int64_t>(16, most / 16 * 16));

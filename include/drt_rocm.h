@@ -334,8 +334,9 @@ int32_t drt_op_attention_kv8(const void* q, int32_t q_dtype, const void* cache, 
  * of those between, the ones whose keys' sum has the largest product with the sum of the head
  * group's queries (in 64 bits; equal ones: the lower block; a NaN is the largest). Blocks ascend in
  * blocks [rows, hkv, count]; a row that sees fewer lists them all, then -1. sums:
- * [hkv][sums_tiles][128] of drt_op_kv8_store or drt_op_kv16_store. Neither call's overlapping ones
- * may share a workspace. */
+ * [hkv][sums_tiles][128] of drt_op_kv8_store or drt_op_kv16_store. The workspace is 256 MiB at most, or
+ * 16 rows of 8 bytes a block and K/V head where those are more. Neither call's overlapping ones may
+ * share a workspace. */
 size_t drt_op_select_blocks_workspace_bytes(int32_t rows, int32_t hkv, int32_t n_keys,
                                             int32_t block_size);
 int32_t drt_op_select_blocks(const void* q, int32_t q_dtype, const float* sums, int64_t sums_tiles,
