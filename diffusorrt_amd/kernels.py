@@ -222,7 +222,9 @@ class PrefixKVCache:
     A tile with a value that is not finite, or beyond 127 * 2^40, reads as NaN until one store
     writes all 32 rows of it, or :meth:`clear`; so does a tile that keeps rows of an earlier
     sequence take their size into its scale. Clear an ``"i8"`` cache, or one with ``block_sums``,
-    before another sequence.
+    before another sequence. Stores into such a cache read and write whole tiles: two that touch
+    one tile, be it other rows of it, must not overlap in time (order them by an event where they
+    are on two streams); stores into a plain 16-bit cache may.
 
     ``block_sums=True`` keeps the sum of each tile's keys (``sums [layers, kv_heads, tiles,
     128]``) up to date, which :meth:`select_blocks` scores blocks by."""

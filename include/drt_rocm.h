@@ -304,12 +304,15 @@ int32_t drt_op_lm_head_score(const void* qw, const void* sb, const void* wb, int
  * aligned and head strides whole tiles. */
 
 /* Rows k, v ([n, hkv, 128] fp32 or bf16) to positions pos0..pos0+n-1. A tile is quantized as a
- * whole from the rows it keeps, as they read, and the new ones. sums: NULL or
+ * whole from the rows it keeps, as they read, and the new ones: stores of different rows of one tile
+ * must not overlap in time (drt_op_kv_pack's may), as on two streams without an event between
+ * them; stores of different tiles, heads or layers may. sums: NULL or
  * [hkv][head_stride / 8192][128] fp32, which receive each touched tile's keys added up. */
 int32_t drt_op_kv8_store(const void* k, const void* v, int32_t src_dtype, int32_t n, int32_t hkv,
                          int32_t pos0, void* cache, int64_t head_stride, float* scales, float* sums,
                          void* stream);
-/* drt_op_kv_pack that keeps a 16-bit cache's sums with it. */
+/* drt_op_kv_pack that keeps a 16-bit cache's sums with it. The sums are of all of a tile's rows: here
+ * too stores of different rows of one tile must not overlap in time. */
 int32_t drt_op_kv16_store(const void* k, const void* v, int32_t src_dtype, int32_t n, int32_t hkv,
                           int32_t pos0, void* cache, int64_t head_stride, int32_t kv_dtype,
                           float* sums, void* stream);
