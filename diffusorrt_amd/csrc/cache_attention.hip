@@ -29,13 +29,16 @@
 // for all of them, and every column of the products is in use (one wave per row, 16 columns of
 // which G are used: 2048 rows x 16 heads, 16 blocks of 64 of 32768 keys, 226 us; 52 here).
 //
-// Bound. A long cache's codes (32 rows x 16 heads over 131072 keys x 8 heads, 268 MB: 56 us, 4.8
+// Bound. A long cache's codes (32 rows x 16 heads over 131072 keys x 8 heads, 268 MB: 57 us, 4.7
 // TB/s, what a large copy reaches). Many rows: the instructions of the softmax and of making
-// operands, 62 % of the VALU's time beside 40 % of the matrix units' (2048 rows x 16 heads over 4096
-// keys under the mask: 62 us, 0.83 PFLOP/s). A block of 32 rows x 16 heads over 8224 keys: 11.3 us with
-// its combine, in a graph, of which about 7 are there without any tile (launches, queries, the ways'
-// meeting, parts out and in). Three waves a SIMD spill; a larger window of blocks in LDS for two (60 us
-// for 57), weights' sums by other chains or by dot products did not pay.
+// operands, by the counters 52 % of all cycles on the VALU and 33 % on the matrix units, which two
+// waves a SIMD overlap little (2048 rows x 16 heads over 4096 keys under the mask: 62 us, 0.83 PFLOP/s;
+// over 32768 506 us, 1.05). Many rows over lists: 46 and 21 %, and between them the wait for tiles, one
+// a wave under way (2048 rows x 16 heads, 16 blocks of 64: 463 MB asked of L2, of which 168 miss). A
+// block of 32 rows x 16 heads over 8224 keys: 11.5 us with its combine, in a graph, of which about 7
+// are there without any tile (launches, queries, the ways' meeting, parts out and in). Three waves a
+// SIMD spill; a larger window of blocks in LDS for two (60 us for 57), weights' sums by other chains or
+// by dot products did not pay.
 #include "kv8.h"
 #include "launch.h"
 
@@ -98,6 +101,8 @@ template <> struct CacheT<2> {
   static constexpr int TILE = 2 * KV8_TILE, LOADS = 8;
   typedef bf16x8 vec;
   static DRT_DEV f32x16 mma(vec a, vec b, f32x16 c) { return mfma_bf16(a, b, c); }
+  // (bf16 as the values are, and as the attention over all of a bf16 cache has them: the product has one
+  // type. Results are off by 1.9 to 2.2 * 10^-3 in all where fp16 weights leave 1.7, a bf16 result's own.)
   static DRT_DEV __bf16 weight(float p) { return (__bf16)p; }
 };
 // Operand i of the eight of a tile's K or V from its registers.
@@ -725,7 +730,7 @@ CachePlan plan_attention8(int n_rows, int Hq, int Hkv, int n_keys) {
   // Many queries: two query tiles a wave (a tile's codes made operands once for both), four key ways,
   // where that makes work-groups for three in four of the 512 places (2048 rows x 16 heads over 4096
   // keys 79 us, one query tile and eight ways 88; 1000 rows 52 and 44). Otherwise one query tile and
-  // eight ways: the least time a work-group (64 rows over 8224 keys: 13 us; four query tiles a
+  // eight ways: the least time a work-group (64 rows over 8224 keys: 14 us; four query tiles a
   // work-group and two ways, which read a tile once for all four, 19; over 131072 keys 91 and 95).
   p.groups = (qtiles + 1) / 2;
   p.wide = Hkv * p.groups >= 384;

@@ -7,8 +7,9 @@
 // - up to a factor, the mean product of the group's queries with the block's keys. Every scored block
 // is seen whole: the last block, which the mask may cut, is taken without a score, so that
 // no key behind the mask has a say. Equal scores: the lower block. The score is
-// a 64-bit sum: of 11-bit queries and 24-bit sums of keys it is all but exact, and the
-// choice does not depend on the order of addition.
+// a 64-bit sum in a fixed order, from 24-bit sums of a tile's keys (exact over 8 bits, rounded once
+// over 16): blocks whose scores are apart by more than some 2^-46 of the magnitudes added up
+// are told apart, whatever the order.
 #include "kv8.h"
 #include "launch.h"
 
@@ -278,8 +279,8 @@ __global__ __launch_bounds__(1024, 4) void select_kernel(const SelArgs x) {
 }
 
 // The scores alone: 16 rows against 64 * per blocks of one K/V head, four waves. For few rows: those
-// of a block find 128 work-groups here, 16 above (32 rows x 8 heads over 512 blocks 6.6 us, and
-// 5.9 for the choice; at once 24).
+// of a block find 128 work-groups here, 16 above (32 rows x 8 heads over 512 blocks 6.7 us, and
+// 5.7 for the choice, 12.4 a call; at once 24).
 __global__ __launch_bounds__(256, 2) void block_scores_kernel(const SelArgs x) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // work-group: (row tile * chunks + chunk) * Hkv + head
