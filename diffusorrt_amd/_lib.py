@@ -84,6 +84,18 @@ class Metrics(C.Structure):
                 ("prof_launches", C.c_int64 * 4)]
 
 
+class Rotary(C.Structure):
+    _fields_ = [("freq", C.c_void_p), ("dim", C.c_int32), ("interleaved", C.c_int32),
+                ("magnitude", C.c_float)]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in (
+        "rows", "appendable", "hq", "hkv", "page_size", "pages", "mask_kind", "mask_block_size",
+        "n_small", "n_large", "n_joins", "n_tiles", "slots", "reserved")] + \
+        [(n, C.c_int64) for n in ("small", "large", "joins", "tiles", "table", "words")]
+
+
 _VP, _I32, _I64, _U64, _SZ = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_size_t
 _PI32, _PF64, _PF32 = C.POINTER(C.c_int32), C.POINTER(C.c_double), C.POINTER(C.c_float)
 
@@ -141,6 +153,16 @@ SIGNATURES = {
     "drt_op_sparse_attention": (_I32, [_VP, _I32, _VP, _I64, _I32, _VP, _I32, _I32, _I32, _I32,
                                        _I32, _I32, _I32, _I32, _VP, _I32, _I32, _VP, _I32, _VP,
                                        _SZ, _VP]),
+    "drt_op_rotate": (_I32, [_VP, _I64, _I64, _I32, _I32, _I32, _I32, C.POINTER(Rotary), _VP, _I32,
+                             _I32, _VP, _I64, _I64, _VP]),
+    "drt_paged_plan": (_I32, [_VP, _I32, _I32, _VP, _VP, _VP, _VP, _I32, _I32, _I32, _I32, _I32,
+                              _I32, _VP, _I64, C.POINTER(PagedBatch)]),
+    "drt_op_paged_append": (_I32, [C.POINTER(PagedBatch), _VP, _VP, _I64, _I64, _VP, _I64, _I64,
+                                   _VP, _I64, _I64, _I32, C.POINTER(Rotary), _VP, _I32, _VP, _VP]),
+    "drt_op_paged_load": (_I32, [C.POINTER(PagedBatch), _VP, _VP, _I32, _VP, _VP, _VP]),
+    "drt_op_paged_attention_workspace_bytes": (_SZ, [C.POINTER(PagedBatch)]),
+    "drt_op_paged_attention": (_I32, [C.POINTER(PagedBatch), _VP, _VP, _VP, _I32, _VP, _I32, _VP,
+                                      _SZ, _VP]),
 }
 
 _lib = None

@@ -246,6 +246,47 @@ void sparse_attention(KvType type, const void* q, bool q_bf16, const void* kv_la
                       const AttnWhere& where, const int32_t* blocks, int count, int block,
                       const CachePlan& p, float* part, void* out, bool out_bf16, hipStream_t s);
 
+// Rotary positions (rotary.hip).
+struct RotaryTurns {
+  const uint64_t* freq = nullptr;  // [dim / 2], 2^64 of a turn a position
+  float magnitude = 1.f;
+  int dim = 0;                     // the elements of a head that are turned (0: none)
+  bool half = true;                // pairs (i, i + dim / 2); else (2 i, 2 i + 1)
+};
+// type, here and below: 0 fp32, 1 fp16, 2 bf16. Strides in elements.
+struct RotateCall {
+  const void* x;
+  void* y;
+  int64_t x_row, x_head, y_row, y_head;
+  const int32_t* positions;  // null: pos0 + row
+  int type, pos0, rows, heads, hd, inverse;
+  RotaryTurns rotary;
+};
+void rotate(const RotateCall& r, hipStream_t s);
+
+// The paged cache (paged_plan.h).
+struct AppendCall {
+  const void *q, *k, *v;  // q may be null
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  int type, cache_bf16, n_tiles, hq, hkv, tpp;
+  const void* tiles;
+  void *cache, *q_out;
+  RotaryTurns rotary;
+};
+void paged_append(const AppendCall& c, hipStream_t s);
+void paged_load(const void* tiles, int n_tiles, const void* cache, int hkv, int tpp, void* k, void* v,
+                hipStream_t s);
+struct PagedAttnCall {
+  const void *q, *cache;
+  const int32_t* list;  // the batch's, on the device
+  int n_small, n_large, n_joins, slots;
+  int64_t small, large, joins, table;
+  int cache_bf16, hq, hkv, tpp, masked, block, out_type;
+  void *out, *workspace;
+};
+size_t paged_part_bytes(int slots, int hkv);
+void paged_attention(const PagedAttnCall& c, hipStream_t s);
+
 // Epilogues.
 // rot (optional): receives the XCD rotation of the launch (see probe_round_robin).
 // ss_out (optional, M <= 32): per-32-column partial sums of squares of the rows,

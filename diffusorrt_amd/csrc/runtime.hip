@@ -31,6 +31,7 @@
 #include "fused.h"
 #include "launch.h"
 #include "op_blocks.h"
+#include "paged_plan.h"
 
 namespace drt {
 
@@ -2954,6 +2955,214 @@ int32_t drt_op_sparse_attention(const void* q, int32_t q_dtype, const void* cach
     sparse_attention(type, q, qb, cache, head_stride, scales, rows, hq, hkv, where, blocks, count,
                      block_size, p, need ? (float*)workspace : nullptr, out,
                      out_dtype == DRT_BF16, as_stream(stream));
+  });
+}
+
+}  // extern "C"
+
+namespace {
+
+int elem_type(int32_t dtype, const char* what) {
+  require(dtype == DRT_F32 || dtype == DRT_F16 || dtype == DRT_BF16,
+          std::string(what) + " takes F32, F16 or BF16");
+  return dtype == DRT_F32 ? 0 : dtype == DRT_F16 ? 1 : 2;
+}
+
+RotaryTurns turns_of(const drt_rotary* r, int hd, const char* what) {
+  RotaryTurns t;
+  if (!r) return t;
+  require(r->freq && ((uintptr_t)r->freq & 7) == 0 && r->dim >= 2 && r->dim % 2 == 0 && r->dim <= hd,
+          std::string(what) + ": bad rotary (dim is even and no more than the head's elements)");
+  t.freq = (const uint64_t*)r->freq;
+  t.magnitude = r->magnitude;
+  t.dim = r->dim;
+  t.half = !r->interleaved;
+  return t;
+}
+
+void require_batch(const drt_paged_batch* b, const int32_t* list, const void* cache, int32_t kv_dtype,
+                   const char* what) {
+  const std::string op(what);
+  require(b && list && b->rows > 0 && b->words > 0 && ((uintptr_t)list & 15) == 0,
+          op + " needs a planned batch and its list, 16-byte aligned, on the device");
+  require(cache && ((uintptr_t)cache & 15) == 0, op + " cache must be 16-byte aligned");
+  require(kv_dtype == DRT_F16 || kv_dtype == DRT_BF16, op + " cache must be F16 or BF16");
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t drt_op_rotate(const void* x, int64_t x_row_stride, int64_t x_head_stride, int32_t dtype,
+                      int32_t rows, int32_t heads, int32_t hd, const drt_rotary* rotary,
+                      const int32_t* positions, int32_t pos0, int32_t inverse, void* y,
+                      int64_t y_row_stride, int64_t y_head_stride, void* stream) {
+  return guarded([&] {
+    require(x && y && rows > 0 && heads > 0 && hd > 0 && rotary, "bad rotate arguments");
+    RotateCall r{};
+    r.type = elem_type(dtype, "rotate");
+    const uintptr_t align = r.type == 0 ? 3 : 1;
+    require((((uintptr_t)x | (uintptr_t)y) & align) == 0 && ((uintptr_t)positions & 3) == 0,
+            "rotate: unaligned tensors");
+    r.rotary = turns_of(rotary, hd, "rotate");
+    r.x = x;
+    r.y = y;
+    r.x_row = x_row_stride;
+    r.x_head = x_head_stride;
+    r.y_row = y_row_stride;
+    r.y_head = y_head_stride;
+    r.positions = positions;
+    r.pos0 = pos0;
+    r.rows = rows;
+    r.heads = heads;
+    r.hd = hd;
+    r.inverse = inverse != 0;
+    rotate(r, as_stream(stream));
+  });
+}
+
+int32_t drt_paged_plan(const int32_t* table, int32_t width, int32_t seqs, const int32_t* rows,
+                       const int32_t* keys, const int32_t* pos0, const int32_t* prompt_len,
+                       int32_t page_size, int32_t pages, int32_t hq, int32_t hkv, int32_t mask_kind,
+                       int32_t mask_block_size, int32_t* list, int64_t list_words,
+                       drt_paged_batch* batch) {
+  return guarded([&] {
+    require(batch, "paged_plan needs a batch to fill in");
+    require(mask_kind == DRT_MASK_BIDIRECTIONAL || mask_kind == DRT_MASK_D2F_HYBRID,
+            "paged_plan mask kind must be bidirectional or d2f_hybrid");
+    PagedBatchArgs a;
+    a.seqs = seqs;
+    a.width = width;
+    a.table = table;
+    a.rows = rows;
+    a.keys = keys;
+    a.pos0 = pos0;
+    a.prompt_len = prompt_len;
+    a.page_size = page_size;
+    a.pages = pages;
+    a.hq = hq;
+    a.hkv = hkv;
+    a.masked = mask_kind == DRT_MASK_D2F_HYBRID;
+    a.block = mask_block_size;
+    const std::string wrong = paged_check(a);
+    require(wrong.empty(), wrong);
+    static thread_local std::vector<int32_t> words;
+    const PagedPlanInfo p = paged_plan(a, words);
+    require((int64_t)std::max({p.n_small, p.n_large, p.n_joins, p.n_tiles}) * hkv <= INT32_MAX,
+            "too many rows for one batch");
+    *batch = drt_paged_batch{};
+    batch->rows = p.rows;
+    batch->appendable = p.appendable;
+    batch->hq = hq;
+    batch->hkv = hkv;
+    batch->page_size = page_size;
+    batch->pages = pages;
+    batch->mask_kind = mask_kind;
+    batch->mask_block_size = std::max(1, mask_block_size);
+    batch->n_small = p.n_small;
+    batch->n_large = p.n_large;
+    batch->n_joins = p.n_joins;
+    batch->n_tiles = p.n_tiles;
+    batch->slots = p.slots;
+    batch->small = p.small;
+    batch->large = p.large;
+    batch->joins = p.joins;
+    batch->tiles = p.tiles;
+    batch->table = p.table;
+    batch->words = p.words;
+    if (list && list_words >= p.words)
+      std::memcpy(list, words.data(), (size_t)p.words * sizeof(int32_t));
+  });
+}
+
+int32_t drt_op_paged_append(const drt_paged_batch* batch, const int32_t* list, const void* k,
+                            int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                            int64_t v_row_stride, int64_t v_head_stride, const void* q,
+                            int64_t q_row_stride, int64_t q_head_stride, int32_t src_dtype,
+                            const drt_rotary* rotary, void* cache, int32_t kv_dtype, void* q_out,
+                            void* stream) {
+  return guarded([&] {
+    require_batch(batch, list, cache, kv_dtype, "paged_append");
+    require(k && v && (!q || q_out), "bad paged_append arguments");
+    require(batch->appendable,
+            "paged_append: a row lies behind its sequence's keys, or two sequences' in one tile");
+    AppendCall c{};
+    c.type = elem_type(src_dtype, "paged_append");
+    const uintptr_t align = c.type == 0 ? 3 : 1;
+    require((((uintptr_t)k | (uintptr_t)v | (uintptr_t)q) & align) == 0 && ((uintptr_t)q_out & 15) == 0,
+            "paged_append: unaligned tensors");
+    c.rotary = turns_of(rotary, 128, "paged_append");
+    require(c.rotary.dim % 16 == 0, "paged_append: rotary dim must be a multiple of 16");
+    c.q = q;
+    c.k = k;
+    c.v = v;
+    c.q_row = q_row_stride;
+    c.q_head = q_head_stride;
+    c.k_row = k_row_stride;
+    c.k_head = k_head_stride;
+    c.v_row = v_row_stride;
+    c.v_head = v_head_stride;
+    c.cache_bf16 = kv_dtype == DRT_BF16;
+    c.n_tiles = batch->n_tiles;
+    c.hq = batch->hq;
+    c.hkv = batch->hkv;
+    c.tpp = batch->page_size / 32;
+    c.tiles = list + batch->tiles;
+    c.cache = cache;
+    c.q_out = q_out;
+    paged_append(c, as_stream(stream));
+  });
+}
+
+int32_t drt_op_paged_load(const drt_paged_batch* batch, const int32_t* list, const void* cache,
+                          int32_t kv_dtype, void* k, void* v, void* stream) {
+  return guarded([&] {
+    require_batch(batch, list, cache, kv_dtype, "paged_load");
+    require(k && v && (((uintptr_t)k | (uintptr_t)v) & 15) == 0,
+            "paged_load k, v must be 16-byte aligned");
+    require(batch->appendable,
+            "paged_load: a row lies behind its sequence's keys, or two sequences' in one tile");
+    paged_load(list + batch->tiles, batch->n_tiles, cache, batch->hkv, batch->page_size / 32, k, v,
+               as_stream(stream));
+  });
+}
+
+size_t drt_op_paged_attention_workspace_bytes(const drt_paged_batch* batch) {
+  return batch && batch->slots > 0 ? paged_part_bytes(batch->slots, batch->hkv) : 0;
+}
+
+int32_t drt_op_paged_attention(const drt_paged_batch* batch, const int32_t* list, const void* q,
+                               const void* cache, int32_t kv_dtype, void* out, int32_t out_dtype,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    require_batch(batch, list, cache, kv_dtype, "paged_attention");
+    require(q && out && ((uintptr_t)q & 15) == 0, "paged_attention q must be 16-byte aligned");
+    require_out(out, out_dtype, "paged_attention");
+    const size_t need = drt_op_paged_attention_workspace_bytes(batch);
+    require(workspace_bytes >= need && (workspace || !need) && ((uintptr_t)workspace & 15) == 0,
+            "paged_attention workspace too small or not 16-byte aligned");
+    PagedAttnCall c{};
+    c.q = q;
+    c.cache = cache;
+    c.list = list;
+    c.n_small = batch->n_small;
+    c.n_large = batch->n_large;
+    c.n_joins = batch->n_joins;
+    c.slots = batch->slots;
+    c.small = batch->small;
+    c.large = batch->large;
+    c.joins = batch->joins;
+    c.table = batch->table;
+    c.cache_bf16 = kv_dtype == DRT_BF16;
+    c.hq = batch->hq;
+    c.hkv = batch->hkv;
+    c.tpp = batch->page_size / 32;
+    c.masked = batch->mask_kind == DRT_MASK_D2F_HYBRID;
+    c.block = batch->mask_block_size;
+    c.out_type = out_dtype == DRT_BF16 ? 2 : 0;
+    c.out = out;
+    c.workspace = need ? workspace : nullptr;
+    paged_attention(c, as_stream(stream));
   });
 }
 

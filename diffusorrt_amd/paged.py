@@ -1,0 +1,260 @@
+"""A K/V cache in pages that many sequences share: :class:`PagedKVCache`.
+
+:class:`.kernels.PrefixKVCache` holds one sequence, its keys one after the other; here a pool of
+pages holds any number, each a list of pages that the caller keeps. Two sequences may list the
+same page (a prefix in common).
+"""
+from __future__ import annotations
+
+import numpy as np
+
+from . import _lib
+from .kernels import KV_TILE_ELEMS, _attention_out, _cache_dtype, _launch, _mask_args, _torch
+from .rotary import _type_code
+
+_I32_MAX = 2**31 - 1
+
+
+def _whole_numbers(values, what):
+    """int32 numpy of a list, an array or a host tensor of whole numbers."""
+    torch = _torch()
+    if isinstance(values, torch.Tensor):
+        if values.is_cuda:
+            raise ValueError(f"{what} must be on the host")
+        values = values.numpy()
+    a = np.asarray(values)
+    if a.size == 0:
+        a = a.astype(np.int32)
+    if a.dtype.kind not in "iu":
+        raise ValueError(f"{what} must be whole numbers")
+    if a.size and (a.min() < -1 or a.max() > _I32_MAX):
+        raise ValueError(f"{what} must be whole numbers of 32 bits")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
+def _table(pages):
+    """int32 [seqs, width], -1 behind a list's end."""
+    if isinstance(pages, (list, tuple)):
+        lists = [_whole_numbers(p, "pages") for p in pages]
+        if any(p.ndim != 1 for p in lists):
+            raise ValueError("pages must be a list of page numbers for each sequence")
+        out = np.full((len(lists), max([1] + [p.size for p in lists])), -1, dtype=np.int32)
+        for row, p in zip(out, lists):
+            row[:p.size] = p
+        return out
+    out = _whole_numbers(pages, "pages")
+    if out.ndim != 2:
+        raise ValueError("pages must be [sequences, width]")
+    return out
+
+
+class PagedBatch:
+    """New rows of several sequences, as :meth:`PagedKVCache.batch` plans them: made once a step,
+    it serves ``append``, ``attention`` and ``load`` of every layer, on any stream. Keep it as long
+    as a captured graph that used it is replayed."""
+
+    def __init__(self, cache, table, keys, rows, heads, positions, kind, mask_geometry):
+        torch = _torch()
+        table = _table(table)
+        keys, rows = _whole_numbers(keys, "keys"), _whole_numbers(rows, "rows")
+        seqs = table.shape[0]
+        if keys.shape != (seqs,) or rows.shape != (seqs,):
+            raise ValueError("a batch takes pages, keys and rows of each sequence")
+        pos0 = keys - rows if positions is None else _whole_numbers(positions, "positions")
+        if pos0.shape != (seqs,):
+            raise ValueError("positions are the first row's of each sequence")
+        prompt = None
+        if kind == "causal":
+            if mask_geometry is not None:
+                raise ValueError("mask geometry is only consumed by the d2f_hybrid kind")
+            mask, block = _lib.MASK_D2F_HYBRID, 1
+        else:
+            if kind == "d2f_hybrid" and mask_geometry is not None and \
+                    not isinstance(mask_geometry, dict):
+                first, block = mask_geometry
+                if not isinstance(first, int):  # a prompt's length for each sequence
+                    prompt = _whole_numbers(first, "prompt lengths")
+                    if prompt.shape != (seqs,):
+                        raise ValueError("prompt lengths are one for each sequence")
+                    mask_geometry = (0, block)
+            mask, length, block = _mask_args(kind, mask_geometry)
+            if prompt is None and length:
+                prompt = np.full(seqs, length, dtype=np.int32)
+        self.kind = kind
+        self.info = _lib.PagedBatch()
+        self._geometry = cache._geometry
+        self._index = cache._index
+        lib = _lib.load()
+
+        def plan(out):
+            _lib.check(lib.drt_paged_plan(
+                table.ctypes.data, table.shape[1], seqs, rows.ctypes.data, keys.ctypes.data,
+                pos0.ctypes.data, None if prompt is None else prompt.ctypes.data, cache.page_size,
+                cache.pages, int(heads), cache.kv_heads, mask, block,
+                None if out is None else out.data_ptr(), 0 if out is None else out.numel(),
+                self.info))
+
+        on_gpu = self._index >= 0
+        host = torch.empty(1024 + 2 * table.size, dtype=torch.int32, pin_memory=on_gpu)
+        plan(host)
+        if self.info.words > host.numel():
+            host = torch.empty(self.info.words, dtype=torch.int32, pin_memory=on_gpu)
+            plan(host)
+        host = host[:self.info.words]
+        if not on_gpu:
+            self._list = host
+            return
+        with torch.cuda.device(self._index):
+            self._list = host.to(cache.data.device, non_blocking=True)
+            self._ready = torch.cuda.Event()
+            self._ready.record()
+            self._stream = torch._C._cuda_getCurrentRawStream(self._index)
+
+    @property
+    def rows(self) -> int:
+        """The rows of all sequences: what q, k and v have."""
+        return self.info.rows
+
+    @property
+    def heads(self) -> int:
+        return self.info.hq
+
+    def _here(self, torch) -> int:
+        """The list's address, for the current stream."""
+        if torch._C._cuda_getCurrentRawStream(self._index) != self._stream:
+            # (while a stream is captured its other work is done: capturing began with a wait)
+            if not torch.cuda.is_current_stream_capturing():
+                stream = torch.cuda.current_stream(self._index)
+                stream.wait_event(self._ready)
+                self._list.record_stream(stream)
+        return self._list.data_ptr()
+
+
+class PagedKVCache:
+    """Keys and values of ``layers`` layers in ``pages`` pages of ``page_size`` keys (a power of
+    two from 32 on) and ``kv_heads`` heads of 128, on one device; ``dtype`` is ``"f16"`` or
+    ``"bf16"``. Pages hold the 32-key tiles of :class:`.kernels.PrefixKVCache`.
+
+    Which pages a sequence has, and in which order, is the caller's: :meth:`batch` takes the
+    lists. A page may be given to another sequence without clearing it."""
+
+    def __init__(self, layers: int, kv_heads: int, pages: int, *, page_size: int = 64,
+                 dtype="f16", device=None):
+        torch = _torch()
+        self.layers, self.kv_heads, self.pages = int(layers), int(kv_heads), int(pages)
+        self.page_size = int(page_size)
+        if self.layers < 1 or self.kv_heads < 1 or self.pages < 1:
+            raise ValueError("a paged cache has a layer, a K/V head and a page at least")
+        if self.page_size < 32 or self.page_size & (self.page_size - 1):
+            raise ValueError("page_size must be a power of two from 32 on")
+        if self.pages * self.kv_heads * (self.page_size // 32) > _I32_MAX:
+            raise ValueError("a layer has at most 2^31 - 1 tiles of 32 keys and one head")
+        self.kv_dtype = _cache_dtype(dtype)
+        if self.kv_dtype == _lib.I8:
+            raise ValueError("a paged cache's dtype is 'f16' or 'bf16'")
+        self.dtype = torch.bfloat16 if self.kv_dtype == _lib.BF16 else torch.float16
+        self.data = torch.zeros((self.layers, self.pages, self.kv_heads,
+                                 self.page_size // 32 * KV_TILE_ELEMS), dtype=self.dtype,
+                                device=device or "cuda")
+        self._index = self.data.get_device()
+        self._geometry = (self.kv_heads, self.pages, self.page_size, self._index)
+
+    @property
+    def nbytes(self) -> int:
+        return self.data.numel() * 2
+
+    def batch(self, pages, keys, rows, *, heads: int, positions=None, kind: str = "causal",
+              mask_geometry=None) -> PagedBatch:
+        """The plan of a step of several sequences.
+
+        For each sequence: ``pages``, its page numbers in order (a list each, or int32
+        ``[sequences, width]`` on the host); ``keys``, how many keys it has, this step's with
+        them; ``rows``, how many rows are new. The rows of all sequences come one sequence's
+        behind the other's; they are a sequence's last positions, or ``positions`` says where the
+        first is. ``heads`` is the number of query heads.
+
+        ``kind``: ``"full"`` (every key of the sequence), ``"causal"`` (those up to the row's
+        position) or ``"d2f_hybrid"`` with ``mask_geometry`` (prompt length, block size): the
+        prompt, then whole blocks up to the row's own; the prompt length a number or one for each
+        sequence."""
+        return PagedBatch(self, pages, keys, rows, heads, positions, kind, mask_geometry)
+
+    def _check(self, layer, batch):
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer must be in [0, {self.layers})")
+        if self._index < 0:
+            raise ValueError("the cache must be on a GPU")
+        if not isinstance(batch, PagedBatch) or batch._geometry != self._geometry:
+            raise ValueError("the batch was planned for another cache")
+
+    def _layer(self, layer):
+        return self.data.data_ptr() + layer * self.data.stride(0) * 2
+
+    def _source(self, t, shape, what):
+        if t.shape != shape or t.get_device() != self._index or t.stride(2) != 1:
+            raise ValueError(f"{what} must be {list(shape)} on the cache's device, a head's elements "
+                             "side by side")
+
+    def append(self, layer: int, k, v, batch: PagedBatch, *, rotary=None, q=None):
+        """Write the batch's ``k, v [rows, kv_heads, 128]`` (fp32, fp16 or bf16, views of a fused
+        projection as they are) into its sequences' pages.
+
+        ``rotary`` (a :class:`.rotary.RotaryPositions` of a multiple of 16 elements): keys are
+        turned by their positions on the way, and so is ``q [rows, heads, 128]`` where given,
+        which comes back in the cache's type, ready for :meth:`attention`. Each value is rounded
+        once. Raises ValueError where two sequences of the batch have rows in one tile of a page,
+        or a row lies behind its sequence's keys."""
+        torch = _torch()
+        self._check(layer, batch)
+        info = batch.info
+        shape = (info.rows, self.kv_heads, 128)
+        self._source(k, shape, "append's k")
+        self._source(v, shape, "append's v")
+        code = _type_code(k.dtype)
+        if code is None or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+            raise ValueError("append takes k, v and q of one type: float32, float16 or bfloat16")
+        if rotary is not None and (rotary.dim > 128 or rotary.dim % 16 or
+                                   rotary._index != self._index):
+            raise ValueError("append's rotary must turn a multiple of 16 elements, 128 at most, "
+                             "on the cache's device")
+        out = None
+        if q is not None:
+            self._source(q, (info.rows, info.hq, 128), "append's q")
+            out = torch.empty(q.shape, dtype=self.dtype, device=q.device)
+        at = batch._here(torch)
+        _launch(torch, _lib.load().drt_op_paged_append, self._index, info, at, k.data_ptr(),
+                k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                None if q is None else q.data_ptr(), 0 if q is None else q.stride(0),
+                0 if q is None else q.stride(1), code, None if rotary is None else rotary._args,
+                self._layer(layer), self.kv_dtype, None if out is None else out.data_ptr())
+        return out
+
+    def load(self, layer: int, batch: PagedBatch):
+        """``(k, v) [rows, kv_heads, 128]`` of the batch's rows as the cache holds them."""
+        torch = _torch()
+        self._check(layer, batch)
+        k = torch.empty((batch.info.rows, self.kv_heads, 128), dtype=self.dtype,
+                        device=self.data.device)
+        v = torch.empty_like(k)
+        _launch(torch, _lib.load().drt_op_paged_load, self._index, batch.info, batch._here(torch),
+                self._layer(layer), self.kv_dtype, k.data_ptr(), v.data_ptr())
+        return k, v
+
+    def attention(self, layer: int, q, batch: PagedBatch, *, out_dtype=None):
+        """Attention of the batch's ``q [rows, heads, 128]`` (the cache's type) over the keys that
+        each row sees: ``[rows, heads * 128]`` in fp32 or bf16. A row without any gives zeros."""
+        torch = _torch()
+        self._check(layer, batch)
+        info = batch.info
+        if q.dim() != 3 or q.shape != (info.rows, info.hq, 128) or q.dtype != self.dtype or \
+                q.get_device() != self._index or not q.is_contiguous():
+            raise ValueError(f"q must be contiguous [{info.rows}, {info.hq}, 128] of the cache's "
+                             "type and device")
+        out, odt = _attention_out(torch, q, info.rows, info.hq, out_dtype)
+        lib = _lib.load()
+        need = lib.drt_op_paged_attention_workspace_bytes(info)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _launch(torch, lib.drt_op_paged_attention, self._index, info, batch._here(torch),
+                q.data_ptr(), self._layer(layer), self.kv_dtype, out.data_ptr(), odt,
+                None if ws is None else ws.data_ptr(), need)
+        return out

@@ -1,0 +1,204 @@
+"""Rotary positions of any form the models' configurations name: :class:`RotaryPositions`.
+
+:func:`.kernels.rope` takes fp32 rows and tables of the caller's (the reference's seam); here the
+frequencies are kept and the angles made where they are used, for any 32-bit position.
+"""
+from __future__ import annotations
+
+import math
+from fractions import Fraction
+
+from . import _lib
+from .kernels import _launch, _torch
+
+_I32_MIN, _I32_MAX = -2**31, 2**31 - 1
+_TWO_PI = 2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
+_LAYOUTS = ("half", "interleaved")
+_SCALING_FIELDS = {
+    "linear": {"factor"},
+    "ntk": {"factor"},
+    "yarn": {"factor", "original_max_position_embeddings", "beta_fast", "beta_slow",
+             "attention_factor"},
+}
+
+
+def _number(scaling, key, default=None):
+    value = scaling.get(key, default)
+    if isinstance(value, bool) or not isinstance(value, (int, float)) or \
+            not math.isfinite(value) or value <= 0:
+        raise ValueError(f"rope scaling needs a positive {key}")
+    return float(value)
+
+
+def rotary_frequencies(dim: int, theta: float = 1e6, scaling=None):
+    """``(frequencies, magnitude)``: radians a position of each of ``dim / 2`` pairs, and what
+    cosine and sine are multiplied by.
+
+    ``theta ** (-2 i / dim)``, or scaled for positions beyond those a model was trained on
+    (``scaling``, a configuration's ``rope_scaling``: ``rope_type`` or ``type``, and ``factor`` s):
+
+    * ``linear``: divided by s;
+    * ``ntk``: a base of ``theta * s ** (dim / (dim - 2))``, which leaves the first pair as it is
+      and divides the last by s;
+    * ``yarn``: pair i makes r = original_max_position_embeddings * f / 2 pi turns over the
+      original positions; f stays where r >= beta_fast (32), is divided by s where r <= beta_slow
+      (1), and lies between the two in proportion to r (arXiv 2309.00071, 3.2). The magnitude is
+      ``attention_factor``, by default 0.1 ln s + 1.
+    """
+    if isinstance(dim, bool) or not isinstance(dim, int) or dim < 2 or dim % 2:
+        raise ValueError("rotary dim must be an even number from 2 on")
+    theta = float(theta)
+    if not (math.isfinite(theta) and theta > 0):
+        raise ValueError("rotary theta must be positive")
+    plain = [theta ** (-2.0 * i / dim) for i in range(dim // 2)]
+    if scaling is None:
+        return plain, 1.0
+    if not isinstance(scaling, dict):
+        raise ValueError("rope scaling must be a dictionary")
+    kind = scaling.get("rope_type", scaling.get("type"))
+    if kind not in _SCALING_FIELDS:
+        raise ValueError(f"rope scaling type must be one of {sorted(_SCALING_FIELDS)}, not {kind!r}")
+    if set(scaling) - {"rope_type", "type"} - _SCALING_FIELDS[kind]:
+        raise ValueError("rope scaling contains unsupported fields")
+    factor = _number(scaling, "factor")
+    if kind == "linear":
+        return [f / factor for f in plain], 1.0
+    if kind == "ntk":
+        if dim < 4:
+            raise ValueError("ntk scaling needs two pairs at least")
+        base = theta * factor ** (dim / (dim - 2))
+        return [base ** (-2.0 * i / dim) for i in range(dim // 2)], 1.0
+    original = _number(scaling, "original_max_position_embeddings")
+    fast, slow = _number(scaling, "beta_fast", 32.0), _number(scaling, "beta_slow", 1.0)
+    if fast <= slow:
+        raise ValueError("yarn scaling needs beta_fast > beta_slow")
+    out = []
+    for f in plain:
+        turns = original * f / (2 * math.pi)
+        keep = min(1.0, max(0.0, (turns - slow) / (fast - slow)))
+        out.append(f * (keep + (1.0 - keep) / factor))
+    return out, _number(scaling, "attention_factor", 0.1 * math.log(factor) + 1.0)
+
+
+def _turns(f: float) -> int:
+    """2^64 of a turn a position, whole turns taken off, as a signed 64-bit number."""
+    u = round(Fraction(f) * 2**64 / _TWO_PI) % 2**64
+    return u - 2**64 if u >= 2**63 else u
+
+
+def _apart(t) -> bool:
+    """Whether no two elements of a tensor share a place."""
+    reach = 0
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if stride <= reach:
+            return False
+        reach += stride * (size - 1)
+    return True
+
+
+def _span(t):
+    """The bytes [first, last) that a tensor lies in."""
+    n = 1 + sum(s * (k - 1) for s, k in zip(t.stride(), t.shape))
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def _same_places(a, b) -> bool:
+    return a.data_ptr() == b.data_ptr() and all(
+        x == y or n == 1 for x, y, n in zip(a.stride(), b.stride(), a.shape))
+
+
+_TYPES = {}
+
+
+def _type_code(dtype):
+    if not _TYPES:
+        torch = _torch()
+        _TYPES.update({torch.float32: _lib.F32, torch.float16: _lib.F16,
+                       torch.bfloat16: _lib.BF16})
+    return _TYPES.get(dtype)
+
+
+class RotaryPositions:
+    """The rotation of the first ``dim`` elements of heads by their rows' positions.
+
+    ``layout``: ``"half"`` pairs elements ``(i, i + dim / 2)``, ``"interleaved"``
+    ``(2 i, 2 i + 1)``. ``theta`` and ``scaling`` as in :func:`rotary_frequencies`; or
+    ``frequencies``, ``dim / 2`` radians a position of any other form, and ``magnitude``. The
+    frequencies are kept as 64-bit fractions of a turn on ``device`` (the current GPU): an angle is
+    right to 2^-31 of a turn at any position of 32 bits, cosine and sine to 2^-22."""
+
+    def __init__(self, dim: int = 128, *, theta: float = 1e6, layout: str = "half", scaling=None,
+                 frequencies=None, magnitude=None, device=None):
+        torch = _torch()
+        if layout not in _LAYOUTS:
+            raise ValueError(f"rotary layout is 'half' or 'interleaved', not {layout!r}")
+        if frequencies is None:
+            if magnitude is not None:
+                raise ValueError("magnitude comes with frequencies of the caller's own")
+            self.frequencies, self.magnitude = rotary_frequencies(dim, theta, scaling)
+        else:
+            if scaling is not None:
+                raise ValueError("rotary takes either scaling or frequencies")
+            self.frequencies = [float(f) for f in frequencies]
+            if isinstance(dim, bool) or not isinstance(dim, int) or dim < 2 or \
+                    2 * len(self.frequencies) != dim or \
+                    not all(math.isfinite(f) for f in self.frequencies):
+                raise ValueError("rotary frequencies must be dim / 2 finite numbers")
+            self.magnitude = 1.0 if magnitude is None else float(magnitude)
+            if not math.isfinite(self.magnitude):
+                raise ValueError("rotary magnitude must be finite")
+        self.dim, self.layout = dim, layout
+        self.turns = torch.tensor([_turns(f) for f in self.frequencies], dtype=torch.int64,
+                                  device=device or "cuda")
+        self._index = self.turns.get_device()
+        self._args = _lib.Rotary(self.turns.data_ptr(), dim, int(layout == "interleaved"),
+                                 self.magnitude)
+
+    def rotate(self, x, positions, *, inverse: bool = False, out=None):
+        """``x [rows, heads, head_dim]`` (fp32, fp16 or bf16; any strides between rows and heads)
+        with row r turned by ``positions[r]`` (int32 on the device, or a number: the first row's,
+        the others one further each); elements from ``dim`` on as they are. ``inverse`` turns the
+        other way, which is also the rotation's gradient: that of ``x`` from that of the result.
+
+        ``out``: a tensor of x's shape and type, ``x`` itself or memory apart from it. Computed in
+        fp32, rounded once."""
+        torch = _torch()
+        if self._index < 0:
+            raise ValueError("the rotary's frequencies must be on a GPU")
+        if x.dim() != 3 or x.shape[2] < self.dim:
+            raise ValueError(f"rotate takes x [rows, heads, head_dim >= {self.dim}]")
+        code = _type_code(x.dtype)
+        if code is None:
+            raise ValueError("rotate takes float32, float16 or bfloat16")
+        rows, heads, hd = x.shape
+        if x.get_device() != self._index:
+            raise ValueError("x must be on the frequencies' device")
+        if x.stride(2) != 1 and hd > 1:
+            raise ValueError("a head's elements must be side by side")
+        if isinstance(positions, torch.Tensor):
+            if positions.dtype is not torch.int32 or positions.shape != (rows,) or \
+                    not positions.is_contiguous() or positions.get_device() != self._index:
+                raise ValueError("positions must be int32 [rows] on x's device, or a number")
+            at, pos0 = positions.data_ptr(), 0
+        else:
+            if isinstance(positions, bool) or not isinstance(positions, int):
+                raise ValueError("positions must be int32 [rows] on x's device, or a number")
+            at, pos0 = None, positions
+            if not (_I32_MIN <= pos0 and pos0 + rows - 1 <= _I32_MAX):
+                raise ValueError("positions must be of 32 bits")
+        if out is None:
+            out = torch.empty((rows, heads, hd), dtype=x.dtype, device=x.device)
+        else:
+            if out.shape != x.shape or out.dtype != x.dtype or out.get_device() != self._index or \
+                    (out.stride(2) != 1 and hd > 1) or not _apart(out):
+                raise ValueError("out must be a tensor of x's shape, type and device, its elements "
+                                 "apart and a head's side by side")
+            if x.numel() and not _same_places(x, out):
+                (a, b), (c, d) = _span(x), _span(out)
+                if a < d and c < b:
+                    raise ValueError("out must be x itself or memory apart from it")
+        if x.numel():
+            _launch(torch, _lib.load().drt_op_rotate, self._index, x.data_ptr(), x.stride(0),
+                    x.stride(1), code, rows, heads, hd, self._args, at, pos0, int(bool(inverse)),
+                    out.data_ptr(), out.stride(0), out.stride(1))
+        return out

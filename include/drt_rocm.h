@@ -362,6 +362,74 @@ int32_t drt_op_sparse_attention(const void* q, int32_t q_dtype, const void* cach
                                 int32_t count, void* out, int32_t out_dtype, void* workspace,
                                 size_t workspace_bytes, void* stream);
 
+/* ---- rotary positions (no counterpart in the reference beyond drt_op_rope) ----
+ * Element pairs of a head turned by position * frequency: pairs (i, i + dim / 2) of its first dim
+ * elements, or (2 i, 2 i + 1) (interleaved); a turned pair (a, b) is magnitude * (a cos t - b sin t,
+ * b cos t + a sin t). freq [dim / 2] uint64 on the device: a pair's turns a position in 2^-64, round(2^64 f
+ * / 2 pi) mod 2^64, so that an angle is right to 2^-31 of a turn at any 32-bit position. */
+typedef struct drt_rotary {
+  const void* freq;
+  int32_t dim;          /* even, <= the head's elements */
+  int32_t interleaved;
+  float magnitude;      /* what cosine and sine are multiplied by: 1 but for some scaled forms */
+} drt_rotary;
+/* x [rows, heads, hd] of dtype (DRT_F32, DRT_F16, DRT_BF16) to y, the same type and shape, elements
+ * beyond dim as they are; strides in elements, a head's elements side by side. y may be x (the same
+ * strides) and must not overlap it otherwise. Row r is at positions[r] (int32 [rows] on the device) or,
+ * with positions NULL, at pos0 + r; negative positions turn backwards, as inverse != 0 does. */
+int32_t drt_op_rotate(const void* x, int64_t x_row_stride, int64_t x_head_stride, int32_t dtype,
+                      int32_t rows, int32_t heads, int32_t hd, const drt_rotary* rotary,
+                      const int32_t* positions, int32_t pos0, int32_t inverse, void* y,
+                      int64_t y_row_stride, int64_t y_head_stride, void* stream);
+
+/* ---- the paged cache (no counterpart in the reference) ----
+ * A layer is `pages` pages of page_size keys (a power of two from 32 on) of hkv heads: tile i of head h in
+ * page g is the 16 KiB tile (g * hkv + h) * (page_size / 32) + i, 32 keys as drt_op_kv_pack lays them
+ * out. A batch is new rows of several sequences: sequence s has rows[s] of them, one sequence's behind the
+ * other's, row i at position pos0[s] + i, keys[s] keys in all (new ones with them), and its keys
+ * [j * page_size, ...) in page table[s * width + j]. Row at position p attends to keys [0, keys[s]), or
+ * under DRT_MASK_D2F_HYBRID to those before the end of its own block (prompt_len[s], or 0 where prompt_len
+ * is NULL; mask_block_size 1 and prompt length 0: the keys up to p). */
+typedef struct drt_paged_batch {
+  int32_t rows;        /* of all sequences */
+  int32_t appendable;  /* every row inside its sequence's keys, none in a tile of another's rows */
+  int32_t hq, hkv, page_size, pages, mask_kind, mask_block_size;
+  int32_t n_small, n_large, n_joins, n_tiles, slots, reserved;
+  int64_t small, large, joins, tiles, table;  /* where they begin in the list, in words */
+  int64_t words;       /* of the list */
+} drt_paged_batch;
+/* Checks a batch given by host arrays and fills *batch in; where list_words >= batch->words its work list
+ * goes to `list` (host), which the caller copies to the device. One list serves every layer's calls (and
+ * any number of them at once) as long as the batch stays as it is. A page outside the cache, or one
+ * missing, is DRT_INVALID_ARGUMENT. */
+int32_t drt_paged_plan(const int32_t* table, int32_t width, int32_t seqs, const int32_t* rows,
+                       const int32_t* keys, const int32_t* pos0, const int32_t* prompt_len,
+                       int32_t page_size, int32_t pages, int32_t hq, int32_t hkv, int32_t mask_kind,
+                       int32_t mask_block_size, int32_t* list, int64_t list_words,
+                       drt_paged_batch* batch);
+/* The batch's k, v [rows, hkv, 128] (src_dtype DRT_F32, DRT_F16 or DRT_BF16; strides in elements) into
+ * their places in one layer's cache (kv_dtype DRT_F16 or DRT_BF16), keys turned by their positions on
+ * the way where rotary is given (dim <= 128, a multiple of 16). q [rows, hq, 128], where given, is turned
+ * alike into q_out [rows, hq, 128] of kv_dtype. list: the plan's, on the device. Other rows of a tile
+ * stay as they are, so calls that write different rows may overlap in time. */
+int32_t drt_op_paged_append(const drt_paged_batch* batch, const int32_t* list, const void* k,
+                            int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                            int64_t v_row_stride, int64_t v_head_stride, const void* q,
+                            int64_t q_row_stride, int64_t q_head_stride, int32_t src_dtype,
+                            const drt_rotary* rotary, void* cache, int32_t kv_dtype, void* q_out,
+                            void* stream);
+/* The batch's rows as the cache holds them: k, v [rows, hkv, 128] of kv_dtype. */
+int32_t drt_op_paged_load(const drt_paged_batch* batch, const int32_t* list, const void* cache,
+                          int32_t kv_dtype, void* k, void* v, void* stream);
+/* Attention of q [rows, hq, 128] of kv_dtype over the batch's keys: out [rows, hq * 128] of out_dtype
+ * (DRT_F32 or DRT_BF16). A row without any key gives zeros; what the pages hold behind a sequence's last
+ * key, or a row does not see, has no part, be it NaN. Calls that overlap must not share a workspace (it
+ * may be NULL where 0 bytes are asked for). */
+size_t drt_op_paged_attention_workspace_bytes(const drt_paged_batch* batch);
+int32_t drt_op_paged_attention(const drt_paged_batch* batch, const int32_t* list, const void* q,
+                               const void* cache, int32_t kv_dtype, void* out, int32_t out_dtype,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
