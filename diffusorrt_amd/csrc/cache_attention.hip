@@ -336,8 +336,19 @@ __global__ __launch_bounds__(64 * KW, 2) void cache_attn_kernel(const CaArgs x) 
       fold = fold == 1 ? CA_FOLD : fold - 1;
       if constexpr (DT != 0) {
         if (careful && part) {
-          const int mine = hit ? q_end[0] : 0;
-          ca_values_apart<DT>(vr, key0, mine, lane, o[0]);
+          int mine[QT];
+#pragma unroll
+          for (int j = 0; j < QT; ++j) mine[j] = hit ? q_end[j] : 0;
+#pragma unroll
+          for (int hb = 0; hb < 4; ++hb) {
+            f32x16* at[QT];
+#pragma unroll
+            for (int j = 0; j < QT; ++j) at[j] = &o[j][hb];
+            u32x4 two[2] = {vr[2 * hb], vr[2 * hb + 1]};
+            ca_values_apart<DT, QT>(two, key0, mine, lane, at);
+            vr[2 * hb] = two[0];
+            vr[2 * hb + 1] = two[1];
+          }
         }
       }
       __builtin_amdgcn_s_setprio(1);

@@ -46,51 +46,56 @@ template <int DT, int N> DRT_DEV typename CacheT<DT>::vec ca_operand(const u32x4
     return __builtin_bit_cast(typename CacheT<DT>::vec, r[i]);
 }
 
-// A tile's values (16 bits) that are not finite, taken out of its V registers: in their place
-// every query column that sees one's key gets infinity or NaN in that head dim, as p * V would be,
-// and the others nothing, where 0 * V would be NaN. An indicator product for each of the three.
-template <int DT>
-DRT_DEV void ca_values_apart(u32x4 (&vr)[8], int key0, int end, int lane, f32x16 (&o)[4]) {
+// The values (16 bits) of a tile's 32 head dims in a lane's two operands that are not finite, taken out of
+// them: in their place every query column that sees one's key gets infinity or NaN in that head dim, as
+// p * V would be, and the others nothing, where 0 * V would be NaN. An indicator product for each of the
+// three. QT query tiles; o[j] is their O of these head dims, end[j] the keys their columns see.
+template <int DT, int QT>
+DRT_DEV void ca_values_apart(u32x4 (&vr)[2], int key0, const int (&end)[QT], int lane,
+                             f32x16* const (&o)[QT]) {
   typedef CacheT<DT> T;
   typedef typename T::vec vec;
   constexpr uint32_t EXP = DT == 1 ? 0x7c00u : 0x7f80u, ONE = DT == 1 ? 0x3c00u : 0x3f80u;
-  vec sees[2];  // 1 for the keys of this lane's that its column sees
-#pragma unroll
-  for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      sees[kh][e] = T::weight(key0 + mfma_row(kh * 8 + e, lane) < end ? 1.f : 0.f);
 #pragma unroll 1
   for (int kind = 0; kind < 3; ++kind) {  // NaN, +infinity, -infinity
     const float put = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
+    vec marks[2];
 #pragma unroll
-    for (int hb = 0; hb < 4; ++hb) {
+    for (int kh = 0; kh < 2; ++kh) {
+      u32x4 w = vr[kh];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t y = w[e];
+        uint32_t mark = 0u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t z = (y >> (16 * h)) & 0xffffu;
+          const bool hit = kind == 0   ? (z & 0x7fffu) > EXP
+                           : kind == 1 ? z == EXP
+                                       : z == (EXP | 0x8000u);
+          mark |= hit ? ONE << (16 * h) : 0u;
+        }
+        w[e] = mark;
+      }
+      marks[kh] = __builtin_bit_cast(vec, w);
+    }
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
       f32x16 n = f32x16{};
 #pragma unroll
       for (int kh = 0; kh < 2; ++kh) {
-        u32x4 w = vr[hb * 2 + kh];
+        vec sees;  // 1 for the keys of this lane's that its column sees
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t y = w[e];
-          uint32_t mark = 0u;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t z = (y >> (16 * h)) & 0xffffu;
-            const bool hit = kind == 0   ? (z & 0x7fffu) > EXP
-                             : kind == 1 ? z == EXP
-                                         : z == (EXP | 0x8000u);
-            mark |= hit ? ONE << (16 * h) : 0u;
-          }
-          w[e] = mark;
-        }
-        n = T::mma(__builtin_bit_cast(vec, w), sees[kh], n);
+        for (int e = 0; e < 8; ++e)
+          sees[e] = T::weight(key0 + mfma_row(kh * 8 + e, lane) < end[j] ? 1.f : 0.f);
+        n = T::mma(marks[kh], sees, n);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[hb][r] = n[r] > 0.f ? o[hb][r] + put : o[hb][r];
+      for (int r = 0; r < 16; ++r) (*o[j])[r] = n[r] > 0.f ? (*o[j])[r] + put : (*o[j])[r];
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t y = vr[i][e];

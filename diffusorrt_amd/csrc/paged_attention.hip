@@ -26,6 +26,7 @@ struct PaArgs {
   const uint16_t* q;    // [rows][hq][128]
   const uint8_t* cache; // this layer
   const PagedPiece* pieces;
+  const int32_t* first;  // a work-group's first piece
   const int32_t* table;  // a page's first tile of head 0
   int hq, hkv, tpp, masked, block;
   float c;               // log2(e) / sqrt(128)
@@ -49,6 +50,8 @@ DRT_DEV PagedPiece pa_piece(const PagedPiece* pieces, int i) {
   y.tile1 = p[7];
   y.slot = p[8];
   y.table = p[9];
+  y.last = p[10];
+  y.wide_log2 = p[11];
   return y;
 }
 
@@ -61,19 +64,45 @@ DRT_DEV int pa_key_end(const PaArgs& x, const PagedPiece& y, int row) {
   return (int)min((int64_t)y.keys, y.prompt_len + ((int64_t)mine + 1) * x.block);
 }
 
-// Whether any of a tile's V (16 bits) in this lane's registers is not finite.
-template <int CT> DRT_DEV bool pa_any_not_finite(const u32x4 (&vr)[8]) {
-  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-  u16x2 most = {0, 0};
+// c + the sum of eight weights as the products have them (so that the quotient of a few large weights is
+// not off by their roundings: a row that one key takes gets that key's value itself).
+DRT_DEV float pa_add8(const f16x8 p, float c) { return kv8_add8(p, c); }
+DRT_DEV float pa_add8(const bf16x8 p, float c) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+  const u32x4 w = __builtin_bit_cast(u32x4, p);
+  const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3];
+  c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w0), one, c, false);
+  c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w1), one, c, false);
+  c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w2), one, c, false);
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w3), one, c, false);
+}
+
+// The products of a tile's 32 head dims of V (two operands) with the weights of QT query tiles. part: keys
+// that not every row sees are among the tile's, or lie behind the sequence's last, and may be anything.
+template <int CT, int QT>
+DRT_DEV void pa_values(u32x4 v0, u32x4 v1, const typename CacheT<CT>::vec (&pf)[QT][2], bool part, int key0,
+                       const int (&end)[QT], int lane, f32x16* const (&o)[QT]) {
+  typedef CacheT<CT> T;
+  typedef typename T::vec vec;
+  u32x4 vr[2] = {v0, v1};
+  if (part) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 most = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t w = vr[i][e] & 0x7fff7fffu;
-      most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w));
-    }
-  constexpr unsigned short EXP = CT == 1 ? 0x7c00 : 0x7f80;
-  return most[0] >= EXP || most[1] >= EXP;
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t w = vr[i][e] & 0x7fff7fffu;
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w));
+      }
+    constexpr unsigned short EXP = CT == 1 ? 0x7c00 : 0x7f80;
+    if (__ballot(most[0] >= EXP || most[1] >= EXP)) ca_values_apart<CT, QT>(vr, key0, end, lane, o);
+  }
+#pragma unroll
+  for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+    for (int j = 0; j < QT; ++j) *o[j] = T::mma(__builtin_bit_cast(vec, vr[kh]), pf[j][kh], *o[j]);
 }
 
 DRT_DEV void pa_store8(const PaArgs& x, int64_t at, f32x4 y0, f32x4 y1) {
@@ -93,42 +122,44 @@ DRT_DEV void pa_store8(const PaArgs& x, int64_t at, f32x4 y0, f32x4 y1) {
   }
 }
 
-// Units of 32 query vectors: KW waves over keys (wave kw takes tiles kw, kw + KW, ... of the piece; they
-// meet in LDS at the end), a tile straight from memory into registers.
-template <int CT, int KW>
-__global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(const PaArgs x) {
+// Units of 32 or 64 query vectors (`wide` waves of 32 side by side) and the other waves over keys: way
+// kw takes tiles kw, kw + ways, ... of the piece, straight from memory into registers. Waves of one way
+// load the same tiles at the same time, the second from the first's lines. The ways meet in LDS at the
+// end.
+constexpr int PS_WAVES = 8;
+template <int CT>
+__global__ __launch_bounds__(64 * PS_WAVES, 2) void paged_attn_kernel(const PaArgs x) {
   typedef CacheT<CT> T;
   typedef typename T::vec vec;
-  constexpr int THREADS = 64 * KW, PIECES = 32, WAVE_O = 32 * PIECES * 16;
-  constexpr int Q_BYTES = 32 * PA_QROW * 2, O_BYTES = KW * WAVE_O;
-  __shared__ __align__(16) char smem[Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
-  __shared__ float2 ml[KW][32];
+  constexpr int PIECES = 32, WAVE_O = 32 * PIECES * 16;
+  __shared__ __align__(16) char smem[PS_WAVES * WAVE_O];
+  __shared__ float2 ml[PS_WAVES][32];
   const int lane = threadIdx.x & 63, tid = threadIdx.x;
-  const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = (int)(blockIdx.x % (uint32_t)x.hkv), G = x.hq / x.hkv;
+  // (a work-group has one piece here)
   const PagedPiece pc = pa_piece(x.pieces, (int)(blockIdx.x / (uint32_t)x.hkv));
-  const int vecs = min(32, pc.rows * G - pc.vec0);
-  auto row_of = [&](int v) { return (pc.vec0 + v) / G; };
+  const int wide = 1 << pc.wide_log2, ways = PS_WAVES >> pc.wide_log2;
+  const int kw = wave >> pc.wide_log2, qw = wave & (wide - 1);
+  const int vecs = min(32 * wide, pc.rows * G - pc.vec0);
+  auto row_of = [&](int v) { return (int)((uint32_t)(pc.vec0 + v) / (uint32_t)G); };
   auto offset_of = [&](int v) {  // of query vector v's head in q and out
     const int row = row_of(v);
     return ((int64_t)(pc.row0 + row) * x.hq + kvh * G + (pc.vec0 + v - row * G)) * 128;
   };
 
-  constexpr int QL = 512 / THREADS;
-  static_assert(QL * THREADS == 512, "whole rounds of the queries");
-  u32x4 qraw[QL];
+  // the queries (behind the last query vector it again: not used), 32 query vectors a round
+  u32x4 qraw[2];
 #pragma unroll
-  for (int it = 0; it < QL; ++it) {
-    const int v = (it * THREADS + tid) >> 4;
-    qraw[it] = u32x4{0u, 0u, 0u, 0u};
-    if (v < vecs) qraw[it] = *(const u32x4*)(x.q + offset_of(v) + (tid & 15) * 8);
-  }
+  for (int it = 0; it < 2; ++it)
+    if (it < wide)
+      qraw[it] = *(const u32x4*)(x.q + offset_of(min(32 * it + (tid >> 4), vecs - 1)) + (tid & 15) * 8);
 
   // this wave's tiles: lane l holds the tile number in the layer of its (64 i + l)-th
-  const int n = (pc.tile1 - pc.tile0 - kw + KW - 1) / KW;
+  const int n = (pc.tile1 - pc.tile0 - kw + ways - 1) >> (3 - pc.wide_log2);
   const int sh = __builtin_ctz(x.tpp);
   auto numbers = [&](int i) {
-    const int t = min(pc.tile0 + kw + KW * (i + lane), pc.tile1 - 1);
+    const int t = min(pc.tile0 + kw + ways * (i + lane), pc.tile1 - 1);
     return x.table[pc.table + (t >> sh)] + kvh * x.tpp + (t & (x.tpp - 1));
   };
   int held = n > 0 ? numbers(0) : 0;
@@ -143,24 +174,27 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(const PaArgs x) 
 #pragma unroll
     for (int i = 0; i < 8; ++i) vr[i] = *(const u32x4*)(p + PA_TILE / 2 + i * 1024);
   }
-  const int q_end = pa_key_end(x, pc, row_of(min(lane & 31, vecs - 1)));
-  // (ends never fall from row to row) keys that every row of the unit sees
-  const int full_end = pa_key_end(x, pc, row_of(0));
+  const int q_end[1] = {pa_key_end(x, pc, row_of(min(32 * qw + (lane & 31), vecs - 1)))};
+  // (ends never fall from row to row) keys that every row of the wave sees
+  const int full_end = pa_key_end(x, pc, row_of(min(32 * qw, vecs - 1)));
 #pragma unroll
-  for (int it = 0; it < QL; ++it)
-    *(u32x4*)(smem + (((it * THREADS + tid) >> 4) * PA_QROW + (tid & 15) * 8) * 2) = qraw[it];
+  for (int it = 0; it < 2; ++it)
+    if (it < wide)
+      *(u32x4*)(smem + ((32 * it + (tid >> 4)) * PA_QROW + (tid & 15) * 8) * 2) = qraw[it];
   ca_lds_barrier();
-  const uint16_t* ql = (const uint16_t*)smem + (lane & 31) * PA_QROW + 8 * (lane >> 5);
+  const uint16_t* ql = (const uint16_t*)smem + (32 * qw + (lane & 31)) * PA_QROW + 8 * (lane >> 5);
   vec qr[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) qr[i] = *(const vec*)(ql + 16 * i);
 
   float m_run = -INFINITY, l_run = 0.f;
+  float base = 0.f;     // m_run, or 0 before any key
+  float scale = x.c;    // 1 where the base is large: the scores are then scaled as it was
   f32x16 o[4];
 #pragma unroll
   for (int hb = 0; hb < 4; ++hb) o[hb] = f32x16{};
   for (int it = 0; it < n; ++it) {
-    const int key0 = (pc.tile0 + kw + KW * it) * 32;
+    const int key0 = (pc.tile0 + kw + ways * it) * 32;
     const int next = min(it + 1, n - 1);  // (the last tile's own again: loaded, not used)
     if ((next & 63) == 0 && next) held = numbers(next);
     const uint8_t* p = tile_at(next);
@@ -172,7 +206,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(const PaArgs x) 
     const bool part = key0 + 32 > full_end;
     if (part) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = key0 + mfma_row(r, lane) < q_end ? s[r] : -INFINITY;
+      for (int r = 0; r < 16; ++r) s[r] = key0 + mfma_row(r, lane) < q_end[0] ? s[r] : -INFINITY;
     }
     float tmax = s[0];
 #pragma unroll
@@ -185,75 +219,64 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(const PaArgs x) 
       for (int hb = 0; hb < 4; ++hb) o[hb] *= alpha;
       l_run *= alpha;
       m_run = up ? u : m_run;
+      base = up ? u : base;
+      scale = __ballot(fabsf(base) > CA_LARGE) ? 1.f : x.c;
     }
-    const float mb = m_run == -INFINITY ? 0.f : m_run;
-    float a = x.c;
-    if (__ballot(fabsf(mb) > CA_LARGE)) {  // exponents rounded as the base was
+    if (scale == 1.f) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= a;
-      a = 1.f;
+      for (int r = 0; r < 16; ++r) s[r] *= x.c;
     }
-    float psum = 0.f;
-    vec pf[2];
+    vec pf[1][2];
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float w = __builtin_amdgcn_exp2f(fmaf(s[kh * 8 + e], a, -mb));
-        psum += w;
-        pf[kh][e] = T::weight(w);
-      }
-    l_run += psum;
-    // What lies behind the sequence's last key, or is not for every row, may be anything
-    if (part && __ballot(pa_any_not_finite<CT>(vr))) ca_values_apart<CT>(vr, key0, q_end, lane, o);
+      for (int e = 0; e < 8; ++e)
+        pf[0][kh][e] = T::weight(__builtin_amdgcn_exp2f(fmaf(s[kh * 8 + e], scale, -base)));
+    l_run = pa_add8(pf[0][1], pa_add8(pf[0][0], l_run));
 #pragma unroll
-    for (int hb = 0; hb < 4; ++hb)
-#pragma unroll
-      for (int kh = 0; kh < 2; ++kh) o[hb] = T::mma(ca_operand<CT>(vr, hb * 2 + kh), pf[kh], o[hb]);
+    for (int hb = 0; hb < 4; ++hb) {
+      f32x16* const at[1] = {&o[hb]};
+      pa_values<CT, 1>(vr[2 * hb], vr[2 * hb + 1], pf, part, key0, q_end, lane, at);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) vr[i] = *(const u32x4*)(p + PA_TILE / 2 + i * 1024);
   }
   l_run += __shfl_xor(l_run, 32, 64);
 
-  // The key ways joined: every wave leaves its O in LDS as 16-byte pieces (query v, piece p at p ^ v:
-  // every bank in turn both ways), then threads with eight head dims of a query vector add the ways'.
+  // The ways joined: every wave leaves its O in LDS as 16-byte pieces (query v, piece p at p ^ v: every
+  // bank in turn both ways), then threads with eight head dims of a query vector add the ways'.
   __syncthreads();  // the queries have been read
   {
-    f32x4* d = (f32x4*)(smem + kw * WAVE_O);
+    f32x4* d = (f32x4*)(smem + wave * WAVE_O);
 #pragma unroll
     for (int b = 0; b < 4; ++b)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         d[(lane & 31) * PIECES + ((b * 8 + 2 * r + (lane >> 5)) ^ (lane & 15))] =
             f32x4{o[b][4 * r], o[b][4 * r + 1], o[b][4 * r + 2], o[b][4 * r + 3]};
-    if (lane < 32) ml[kw][lane] = make_float2(m_run, l_run);
+    if (lane < 32) ml[wave][lane] = make_float2(m_run, l_run);
   }
   __syncthreads();
-#pragma unroll
-  for (int it = 0; it < QL; ++it) {
-    const int v = (it * THREADS + tid) >> 4, ch = tid & 15;
-    if (v >= vecs) continue;
-    float2 w[KW];
+  const int v = tid >> 4, ch = tid & 15;
+  for (int it = 0; it < wide; ++it) {
+    if (32 * it + v >= vecs) break;
     float m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int k = 0; k < KW; ++k) {
-      w[k] = ml[k][v];
-      m = fmaxf(m, w[k].x);
-    }
+    for (int k = it; k < PS_WAVES; k += wide) m = fmaxf(m, ml[k][v].x);
     f32x4 y0 = f32x4{}, y1 = f32x4{};
-#pragma unroll
-    for (int k = 0; k < KW; ++k) {
+#pragma unroll 2
+    for (int k = it; k < PS_WAVES; k += wide) {
       const f32x4* d = (const f32x4*)(smem + k * WAVE_O) + v * PIECES;
-      const float f = w[k].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w[k].x - m);
+      const float2 w = ml[k][v];
+      const float f = w.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.x - m);
       y0 += f * d[(2 * ch) ^ (v & 15)];
       y1 += f * d[(2 * ch + 1) ^ (v & 15)];
-      l = fmaf(f, w[k].y, l);
+      l = fmaf(f, w.y, l);
     }
     if (pc.slot < 0) {
       const float inv = pc.tile1 == 0 ? 0.f : 1.f / l;  // (no key: zeros)
-      pa_store8(x, offset_of(v) + ch * 8, y0 * inv, y1 * inv);
+      pa_store8(x, offset_of(32 * it + v) + ch * 8, y0 * inv, y1 * inv);
     } else {
-      const int64_t at = ((int64_t)pc.slot * x.hkv + kvh) * 32 + v;
+      const int64_t at = ((int64_t)(pc.slot + it) * x.hkv + kvh) * 32 + v;
       *(f32x4*)(x.o_part + at * 128 + ch * 8) = y0;
       *(f32x4*)(x.o_part + at * 128 + ch * 8 + 4) = y1;
       if (ch == 0) *(float2*)(x.ml_part + at * 2) = make_float2(m, l);
@@ -261,24 +284,286 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(const PaArgs x) 
   }
 }
 
-// The parts of a unit joined, a wave for each query vector: lane (sg, ch) adds head dims 8 ch .. + 8 of
-// parts sg, sg + 4, ..., all of a batch's loads before their use, and the four groups meet by lane
-// exchanges.
+// Units of 256 query vectors: four waves of 64 (two tiles of 32, for both of which a tile's operands are
+// read once) for each of two key ways, which take turns at the tiles. Tiles come by direct-to-LDS
+// loads, the next while this is worked on, queries lie in LDS for all of it.
+constexpr int PL_HELD = 4;  // steps of 16 head dims whose queries are in registers
+constexpr int PL_Q = 256, PL_WAYS = 2;
+template <int CT>
+__device__ __forceinline__ void pa_large(const PaArgs& x) {
+  typedef CacheT<CT> T;
+  typedef typename T::vec vec;
+  __shared__ __align__(16) uint16_t q_lds[PL_Q * PA_QROW];
+  // separate arrays: the compiler knows the slot being read is not one being filled
+  __shared__ __align__(1024) char ring0[PL_WAYS * PA_TILE];
+  __shared__ __align__(1024) char ring1[PL_WAYS * PA_TILE];
+  __shared__ float2 ml[PL_Q];
+  const int lane = threadIdx.x & 63, tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qw = wave & 3, way = wave >> 2;
+  const int kvh = (int)(blockIdx.x % (uint32_t)x.hkv), G = x.hq / x.hkv;
+  for (int at = x.first[blockIdx.x / (uint32_t)x.hkv];; ++at) {
+  const PagedPiece pc = pa_piece(x.pieces, at);
+  const int vecs = min(PL_Q, pc.rows * G - pc.vec0);
+  auto row_of = [&](int v) { return (int)((uint32_t)(pc.vec0 + v) / (uint32_t)G); };
+  auto offset_of = [&](int v) {
+    const int row = row_of(v);
+    return ((int64_t)(pc.row0 + row) * x.hq + kvh * G + (pc.vec0 + v - row * G)) * 128;
+  };
+
+  // this key way's tiles
+  const int n_it = (pc.tile1 - pc.tile0 + PL_WAYS - 1) / PL_WAYS;       // of the work-group
+  const int n = (pc.tile1 - pc.tile0 - way + PL_WAYS - 1) / PL_WAYS;    // of the way
+  const int sh = __builtin_ctz(x.tpp);
+  auto numbers = [&](int i) {
+    const int t = min(pc.tile0 + way + PL_WAYS * (i + lane), pc.tile1 - 1);
+    return x.table[pc.table + (t >> sh)] + kvh * x.tpp + (t & (x.tpp - 1));
+  };
+  int held = n > 0 ? numbers(0) : 0;
+  auto issue = [&](int i, char* dst) {  // this wave's quarter of the way's tile i
+    if (i >= n) return;
+    if ((i & 63) == 0 && i) held = numbers(i);
+    const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(x.cache + (int64_t)__builtin_amdgcn_readlane(held, i & 63) * PA_TILE), 0, PA_TILE,
+        0x00020000);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          src, (__attribute__((address_space(3))) void*)(dst + way * PA_TILE + (qw * 4 + k) * 1024), 16,
+          (uint32_t)((qw * 4 + k) * 1024 + lane * 16), 0, 0, 0);
+  };
+  issue(0, ring0);
+  u32x4 qraw[8];  // (behind the last query vector it again: not used)
+#pragma unroll
+  for (int it = 0; it < 8; ++it)
+    qraw[it] = *(const u32x4*)(x.q + offset_of(min((it * 512 + tid) >> 4, vecs - 1)) + (tid & 15) * 8);
+#pragma unroll
+  for (int it = 0; it < 8; ++it)
+    *(u32x4*)(q_lds + ((it * 512 + tid) >> 4) * PA_QROW + (tid & 15) * 8) = qraw[it];
+  const uint16_t* ql = q_lds + (qw * 64 + (lane & 31)) * PA_QROW + 8 * (lane >> 5);
+  int q_end[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    q_end[j] = pa_key_end(x, pc, row_of(min(qw * 64 + 32 * j + (lane & 31), vecs - 1)));
+  // (ends never fall from row to row) keys that every row of the wave sees, and any of them
+  const int full_end = pa_key_end(x, pc, row_of(min(qw * 64, vecs - 1)));
+  const int wave_end = qw * 64 < vecs ? pa_key_end(x, pc, row_of(min(qw * 64 + 63, vecs - 1))) : 0;
+
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+  f32x16 o[2][4];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int hb = 0; hb < 4; ++hb) o[j][hb] = f32x16{};
+
+  f32x16 s[2];
+  vec pf[2][2];
+  float base[2] = {0.f, 0.f};  // m_run, or 0 before any key
+  float scale = x.c;           // 1 where a base is large: the scores are then scaled as it was
+  auto weights = [&] {         // of both query tiles, from their scores
+    float u[2];
+    bool up[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float tmax = s[j][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, s[j][r]);
+      u[j] = ca_max_xor32(tmax) * x.c;  // -inf: no visible key
+      up[j] = u[j] > m_run[j] + CA_RESCALE_LOG2;
+    }
+    if (__ballot(up[0] || up[1])) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float alpha = up[j] ? __builtin_amdgcn_exp2f(m_run[j] - u[j]) : 1.f;  // 0 from -inf
+#pragma unroll
+        for (int hb = 0; hb < 4; ++hb) o[j][hb] *= alpha;
+        l_run[j] *= alpha;
+        m_run[j] = up[j] ? u[j] : m_run[j];
+        base[j] = up[j] ? u[j] : base[j];
+      }
+      scale = __ballot(fmaxf(fabsf(base[0]), fabsf(base[1])) > CA_LARGE) ? 1.f : x.c;
+    }
+    if (scale == 1.f) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[j][r] *= x.c;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          pf[j][kh][e] =
+              T::weight(__builtin_amdgcn_exp2f(fmaf(s[j][kh * 8 + e], scale, -base[j])));
+      l_run[j] = pa_add8(pf[j][1], pa_add8(pf[j][0], l_run[j]));
+    }
+  };
+  // A step is a tile of each way. ANY: one that not every row sees whole; the others' steps have half of
+  // the queries in registers.
+  vec qr[2][PL_HELD];
+  auto step = [&](int i, const char* here, char* next, auto any) {
+    constexpr bool ANY = decltype(any)::value;
+    const int key0 = (pc.tile0 + way + PL_WAYS * i) * 32;
+    const bool mine = ANY ? i < n && key0 < wave_end : wave_end > 0;
+    const bool part = ANY && key0 + 32 > full_end;
+    const uint16_t* kt = (const uint16_t*)(here + way * PA_TILE) + lane * 8;
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): its tile is here
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (i + 1 < n_it) issue(i + 1, next);
+    if (mine) {
+      s[0] = s[1] = f32x16{};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const vec kf = *(const vec*)(kt + e * 512);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          s[j] = T::mma(kf, !ANY && e < PL_HELD ? qr[j][e < PL_HELD ? e : 0]
+                                                : *(const vec*)(ql + j * 32 * PA_QROW + 16 * e),
+                        s[j]);
+      }
+      if (part) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[j][r] = key0 + mfma_row(r, lane) < q_end[j] ? s[j][r] : -INFINITY;
+      }
+      weights();
+#pragma unroll
+      for (int hb = 0; hb < 4; ++hb) {
+        f32x16* const at[2] = {&o[0][hb], &o[1][hb]};
+        pa_values<CT, 2>(*(const u32x4*)(kt + 4096 + hb * 1024),
+                         *(const u32x4*)(kt + 4096 + hb * 1024 + 512), pf, part, key0, q_end, lane, at);
+      }
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave is done reading the slot
+  };
+  __syncthreads();  // the queries are in LDS
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int e = 0; e < PL_HELD; ++e) qr[j][e] = *(const vec*)(ql + j * 32 * PA_QROW + 16 * e);
+  // (a whole number of both rings' steps) tiles that every row of the unit sees, of both ways
+  const int whole = min(pa_key_end(x, pc, row_of(0)) >> 5, pc.tile1) - pc.tile0;
+  const int n_whole = max(whole, 0) / PL_WAYS & ~1;
+  int it = 0;
+  for (; it < n_whole; it += 2) {
+    step(it, ring0, ring1, std::false_type{});
+    step(it + 1, ring1, ring0, std::false_type{});
+  }
+  for (; it < n_it; it += 2) {
+    step(it, ring0, ring1, std::true_type{});
+    if (it + 1 >= n_it) break;
+    step(it + 1, ring1, ring0, std::true_type{});
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) l_run[j] += __shfl_xor(l_run[j], 32, 64);
+
+  // The second way's part to the first, which has the same queries in the same registers, 32 head dims
+  // of both query tiles at a time; the first way's waves write theirs out, eight head dims a lane.
+  char* const mine = (qw & 2 ? ring1 : ring0) + (qw & 1) * PA_TILE;  // 16 KiB
+  float f0[2], f1[2];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    __syncthreads();  // the ring, or the first half, has been read
+    if (way) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const f32x16& y = o[j][2 * half + b];
+            *(f32x4*)(mine + ((j * 2 + b) * 4 + r) * 1024 + lane * 16) =
+                f32x4{y[4 * r], y[4 * r + 1], y[4 * r + 2], y[4 * r + 3]};
+          }
+        if (half == 0 && lane < 32) ml[qw * 64 + j * 32 + lane] = make_float2(m_run[j], l_run[j]);
+      }
+    }
+    __syncthreads();
+    if (!way) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int v = qw * 64 + j * 32 + (lane & 31);
+        if (half == 0) {
+          const float2 z = ml[v];
+          const float m = fmaxf(m_run[j], z.x);
+          f0[j] = m_run[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[j] - m);
+          f1[j] = z.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(z.x - m);
+          m_run[j] = m;
+          l_run[j] = f0[j] * l_run[j] + f1[j] * z.y;
+        }
+        const float inv = pc.slot >= 0 ? 1.f : pc.tile1 == 0 ? 0.f : 1.f / l_run[j];  // (no key: zeros)
+        const bool there = v < vecs;
+        const int64_t part = ((int64_t)(pc.slot + (v >> 5)) * x.hkv + kvh) * 32 + (v & 31);
+        const int64_t out = there ? offset_of(v) : 0;
+        if (half == 0 && pc.slot >= 0 && there && lane < 32)
+          *(float2*)(x.ml_part + part * 2) = make_float2(m_run[j], l_run[j]);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; r += 2) {
+            // dims 8 r + 4 (lane / 32) + 0..3 and 8 (r + 1) + ... become 8 (r + lane / 32) + 0..7
+            f32x4 y[2];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const f32x16& z = o[j][2 * half + b];
+              y[g] = f32x4{z[4 * (r + g)], z[4 * (r + g) + 1], z[4 * (r + g) + 2], z[4 * (r + g) + 3]} *
+                         f0[j] +
+                     *(const f32x4*)(mine + ((j * 2 + b) * 4 + r + g) * 1024 + lane * 16) * f1[j];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(y[0][e]),
+                                                              __float_as_uint(y[1][e]), false, false);
+              y[0][e] = __uint_as_float(w[0]);
+              y[1][e] = __uint_as_float(w[1]);
+            }
+            const int hd = 64 * half + 32 * b + 8 * (r + (lane >> 5));
+            if (!there) continue;
+            if (pc.slot < 0) {
+              pa_store8(x, out + hd, y[0] * inv, y[1] * inv);
+            } else {
+              *(f32x4*)(x.o_part + part * 128 + hd) = y[0];
+              *(f32x4*)(x.o_part + part * 128 + hd + 4) = y[1];
+            }
+          }
+      }
+    }
+  }
+  if (pc.last) return;
+  __syncthreads();  // the next part's queries and tiles go where this one's O was
+  }
+}
+// (the buffer resource type is not known to the host pass: the body is a device function)
+template <int CT> __global__ __launch_bounds__(512, 2) void paged_attn_large_kernel(const PaArgs x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  pa_large<CT>(x);
+#endif
+}
+
+// The parts of a unit joined: WIDE, a wave for each query vector, lane (sg, ch) adding head dims 8 ch ..
+// + 8 of parts sg, sg + 4, ...; the four groups meet by lane exchanges. Otherwise sixteen lanes for each,
+// four query vectors a wave. All loads of a batch of parts are on their way before their use.
+template <bool WIDE>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PaArgs x, const PagedJoin* joins) {
   const int kvh = (int)(blockIdx.x % (uint32_t)x.hkv), G = x.hq / x.hkv;
   const PagedJoin y = joins[blockIdx.x / (uint32_t)x.hkv];
-  const int v = (int)blockIdx.y * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, ch = lane & 15, sg = WIDE ? lane >> 4 : 0;
+  const int v = WIDE ? (int)blockIdx.y * 4 + (threadIdx.x >> 6) : (int)blockIdx.y * 16 + (threadIdx.x >> 4);
   if (v >= y.vecs) return;
-  const int lane = threadIdx.x & 63, ch = lane & 15, sg = lane >> 4;
-  constexpr int SB = 4;
+  constexpr int SB = 4, STEP = WIDE ? 4 : 1;
   float m = -INFINITY, l = 0.f;
   f32x4 a0 = f32x4{}, a1 = f32x4{};
-  for (int s0 = sg; s0 < y.parts; s0 += 4 * SB) {
+  for (int s0 = sg; s0 < y.parts; s0 += STEP * SB) {
     float2 ml[SB];
     f32x4 p0[SB], p1[SB];
 #pragma unroll
     for (int j = 0; j < SB; ++j) {
-      const int64_t slot = y.slot + (int64_t)y.step * min(s0 + 4 * j, y.parts - 1);
+      const int64_t slot = y.slot + (int64_t)y.step * min(s0 + STEP * j, y.parts - 1);
       const int64_t at = (slot * x.hkv + kvh) * 32 + v;
       ml[j] = *(const float2*)(x.ml_part + at * 2);
       p0[j] = *(const f32x4*)(x.o_part + at * 128 + 8 * ch);
@@ -287,7 +572,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PaArgs x, const P
     float mb = m;
 #pragma unroll
     for (int j = 0; j < SB; ++j) {
-      if (s0 + 4 * j >= y.parts) {  // (the last part's again: 0 * infinity would be NaN)
+      if (s0 + STEP * j >= y.parts) {  // (the last part's again: 0 * infinity would be NaN)
         ml[j] = make_float2(-INFINITY, 0.f);
         p0[j] = p1[j] = f32x4{};
       }
@@ -306,22 +591,24 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PaArgs x, const P
     }
     m = mb;
   }
-  const float mm = fmaxf(fmaxf(m, __shfl_xor(m, 16, 64)),
-                         fmaxf(__shfl_xor(m, 32, 64), __shfl_xor(m, 48, 64)));
-  const float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm);
-  a0 *= w;
-  a1 *= w;
-  l *= w;
+  if (WIDE) {
+    const float mm = fmaxf(fmaxf(m, __shfl_xor(m, 16, 64)),
+                           fmaxf(__shfl_xor(m, 32, 64), __shfl_xor(m, 48, 64)));
+    const float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm);
+    a0 *= w;
+    a1 *= w;
+    l *= w;
 #pragma unroll
-  for (int o = 16; o < 64; o <<= 1) {
-    l += __shfl_xor(l, o, 64);
+    for (int o = 16; o < 64; o <<= 1) {
+      l += __shfl_xor(l, o, 64);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      a0[e] += __shfl_xor(a0[e], o, 64);
-      a1[e] += __shfl_xor(a1[e], o, 64);
+      for (int e = 0; e < 4; ++e) {
+        a0[e] += __shfl_xor(a0[e], o, 64);
+        a1[e] += __shfl_xor(a1[e], o, 64);
+      }
     }
+    if (sg) return;
   }
-  if (sg) return;
   const float inv = 1.f / l;  // (a unit that is cut has keys)
   const int row = (y.vec0 + v) / G;
   const int64_t at = ((int64_t)(y.row0 + row) * x.hq + kvh * G + (y.vec0 + v - row * G)) * 128 + 8 * ch;
@@ -352,13 +639,25 @@ void paged_attention(const PagedAttnCall& c, hipStream_t s) {
   if (c.n_small) {
     a.pieces = (const PagedPiece*)(c.list + c.small);
     const dim3 grid((unsigned)c.n_small * (unsigned)c.hkv);
-    if (c.cache_bf16) hipLaunchKernelGGL((paged_attn_kernel<2, 8>), grid, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((paged_attn_kernel<1, 8>), grid, dim3(512), 0, s, a);
+    if (c.cache_bf16) hipLaunchKernelGGL(paged_attn_kernel<2>, grid, dim3(64 * PS_WAVES), 0, s, a);
+    else hipLaunchKernelGGL(paged_attn_kernel<1>, grid, dim3(64 * PS_WAVES), 0, s, a);
+    DRT_HIP(hipGetLastError());
+  }
+  if (c.n_large) {
+    a.pieces = (const PagedPiece*)(c.list + c.large);
+    a.first = c.list + c.first_large;
+    const dim3 grid((unsigned)c.n_large * (unsigned)c.hkv);
+    if (c.cache_bf16) hipLaunchKernelGGL(paged_attn_large_kernel<2>, grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL(paged_attn_large_kernel<1>, grid, dim3(512), 0, s, a);
     DRT_HIP(hipGetLastError());
   }
   if (c.n_joins) {
-    hipLaunchKernelGGL(paged_join_kernel, dim3((unsigned)c.n_joins * (unsigned)c.hkv, 8), dim3(256), 0,
-                       s, a, (const PagedJoin*)(c.list + c.joins));
+    // Few query vectors of many parts by a wave each, many of few by a quarter.
+    const bool wide = c.slots > 4 * c.n_joins || (int64_t)c.n_joins * c.hkv < 64;
+    const unsigned n = (unsigned)c.n_joins * (unsigned)c.hkv;
+    const PagedJoin* joins = (const PagedJoin*)(c.list + c.joins);
+    if (wide) hipLaunchKernelGGL(paged_join_kernel<true>, dim3(n, 8), dim3(256), 0, s, a, joins);
+    else hipLaunchKernelGGL(paged_join_kernel<false>, dim3(n, 2), dim3(256), 0, s, a, joins);
     DRT_HIP(hipGetLastError());
   }
 }

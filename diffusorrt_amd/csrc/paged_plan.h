@@ -14,8 +14,9 @@
 
 namespace drt {
 
-// A work-group's part of an attention: up to `vecs` query vectors (row * G + head of the group, G = hq
-// / hkv) of one sequence over tiles [tile0, tile1) of its keys. Read by scalar loads: 64 bytes.
+// A part of an attention: a unit of query vectors (row * G + head of the group, G = hq / hkv) of one
+// sequence over tiles [tile0, tile1) of its keys. A work-group does some that follow one another: the
+// last of them says so. Read by scalar loads: 64 bytes.
 struct PagedPiece {
   int32_t row0, rows;        // the sequence's rows in the batch
   int32_t pos0, keys, prompt_len;
@@ -23,7 +24,9 @@ struct PagedPiece {
   int32_t tile0, tile1;
   int32_t slot;              // where its part goes (32 query vectors a slot); < 0: the whole unit
   int32_t table;             // the sequence's first page in the list
-  int32_t unused[6];
+  int32_t last;              // a work-group's last
+  int32_t wide_log2;         // (small kernel) its unit is of 32 << wide_log2 query vectors (0 or 1)
+  int32_t unused[4];
 };
 // 32 query vectors of a unit whose keys are split: their parts are in slots slot, slot + step, ...
 struct PagedJoin {
@@ -49,14 +52,14 @@ struct PagedBatchArgs {
 struct PagedPlanInfo {
   // appendable: every row lies inside its sequence's keys, and none in the tile of another sequence's
   int32_t rows = 0, appendable = 1;
+  // work-groups of a K/V head for each kernel, with where each one's parts begin in `small` / `large`
   int32_t n_small = 0, n_large = 0, n_joins = 0, n_tiles = 0, slots = 0;
-  int64_t small = 0, large = 0, joins = 0, tiles = 0, table = 0, words = 0;
+  int64_t small = 0, large = 0, first_small = 0, first_large = 0;
+  int64_t joins = 0, tiles = 0, table = 0, words = 0;
 };
 
-constexpr int PAGED_VECS = 32;      // query vectors of a unit of the small kernel
-constexpr int PAGED_VECS_L = 256;   // ... of the large one
-// Sequences of up to so many query vectors a K/V head go to the small kernel.
-constexpr int PAGED_SMALL = INT32_MAX;
+// Query vectors of a unit: of the small kernel, 32 or 64, and of the large one.
+constexpr int PAGED_VECS = 32, PAGED_VECS_L = 256;
 constexpr int PAGED_CUS = 256;
 
 // The number of keys that the row at position p sees, always the first ones.
@@ -102,43 +105,111 @@ namespace paged_detail {
 struct Unit {
   int seq, vec0, vecs;
   int64_t tiles;
-  int parts;
 };
 
-// How a kernel's units are cut along their keys: the parts of each. Times in us: `fixed` a part, `tile`
-// 32 keys of one, `join` for the second launch, `part` a part's 32 query vectors written and read;
-// `at_once` work-groups run side by side.
+// Times in us. A part: `fixed` (its queries in, its result out) and `tile` for 32 keys, alone on its CU;
+// `join`: the second launch that a cut needs.
 struct Costs {
-  double fixed, tile, join, part;
-  int at_once;
+  double fixed, tile, join;
 };
-inline void cut(std::vector<Unit>& units, int hkv, const Costs& c) {
+// The part [tile0, tile1) of unit `unit` for work-group `group`.
+struct Share {
+  int unit, group;
+  int64_t tile0, tile1;
+};
+// Units in their order as the shares of work-groups of equal time, `groups` of them at most. A share ends
+// inside a unit where it must; not within the time of a part's fixed cost of the unit's ends, where the cut
+// would cost what it saves.
+inline std::vector<Share> cut(const std::vector<Unit>& units, int groups, const Costs& c) {
+  std::vector<Share> out;
+  double left = 0.;
+  for (const Unit& u : units) left += c.fixed + c.tile * (double)u.tiles;
+  int group = 0;
+  const int64_t least = std::max<int64_t>(1, (int64_t)(c.fixed / c.tile));  // tiles worth a cut
+  double mine = 0., quota = left / groups;
+  for (int i = 0; i < (int)units.size(); ++i) {
+    int64_t at = 0;
+    const int64_t tiles = units[i].tiles;
+    for (;;) {
+      int64_t n = tiles - at;
+      const double room = quota - mine - c.fixed;
+      bool full = false;
+      if (group + 1 < groups && room < c.tile * (double)n) {  // it does not all fit
+        full = true;
+        int64_t fit = room > 0. ? (int64_t)(room / c.tile) : 0;
+        if (n - fit < least) fit = n;
+        if (fit < least) fit = 0;
+        if (fit == 0 && mine == 0.) fit = std::min(n, least);
+        n = fit;
+      }
+      if (n > 0 || (tiles == 0 && !full)) {
+        out.push_back(Share{i, group, at, at + n});
+        mine += c.fixed + c.tile * (double)n;
+        at += n;
+      }
+      if (full) {
+        left -= mine;
+        ++group;
+        mine = 0.;
+        // (what is left, evenly; a unit cut here begins once more)
+        quota = (left + (at > 0 && at < tiles ? c.fixed : 0.)) / (groups - group);
+        if (at > 0 && at < tiles) left += c.fixed;
+      }
+      if (at >= tiles && (tiles > 0 || n > 0 || !full)) break;
+    }
+  }
+  return out;
+}
+
+// The time of work-groups, `slots` of them at once, the longest first; parts: (tiles, how many).
+inline double makespan(std::vector<std::pair<int64_t, int64_t>>& parts, int slots, const Costs& c) {
+  std::sort(parts.begin(), parts.end(), std::greater<std::pair<int64_t, int64_t>>());
+  // rounds, each as long as its longest; or all of it evenly and the longest behind
+  double rounds = 0., sum = 0.;
+  int64_t room = 0;
+  for (const auto& y : parts) {
+    const double us = c.fixed + c.tile * (double)y.first;
+    sum += us * (double)y.second;
+    const int64_t n = y.second - room;
+    room = room > y.second ? room - y.second : 0;
+    if (n > 0) {
+      const int64_t r = (n + slots - 1) / slots;
+      rounds += us * (double)r;
+      room = r * slots - n;
+    }
+  }
+  const double longest = c.fixed + c.tile * (double)parts[0].first;
+  return std::max(longest, std::min(rounds, sum / slots + longest));
+}
+
+// The longest part, in tiles, of units that are cut into equal ones, each a work-group of its own, by the
+// least time of all. all_us: what reading the keys of all sequences once takes; the nearer the
+// work-groups' own time comes to that, the more they wait for one another.
+inline int64_t part_length(const std::vector<Unit>& units, int hkv, double all_us, const Costs& c) {
+  std::vector<std::pair<int64_t, int64_t>> parts;
   int64_t most = 0;
   for (const Unit& u : units) most = std::max(most, u.tiles);
-  if (most < 2) return;
   double best = -1.;
-  int64_t best_len = most;
-  // lengths of a part from whole units down, each about a fifth shorter than the last
-  for (int64_t len = most; len >= 1; len = std::min(len - 1, len * 4 / 5)) {
-    double longest = 0., sum = 0.;
-    int64_t extra = 0;
+  int64_t best_len = std::max<int64_t>(1, most);
+  for (int64_t len = best_len; len >= 1; len = std::min(len - 1, len * 4 / 5)) {
+    parts.clear();
+    int64_t cuts = 0, most_cuts = 0;
     for (const Unit& u : units) {
       const int64_t n = std::max<int64_t>(1, (u.tiles + len - 1) / len);
-      if (n > 256) { sum = -1.; break; }
-      const double one = c.fixed + c.tile * (double)((u.tiles + n - 1) / n);
-      longest = std::max(longest, one);
-      sum += one * (double)n;
-      if (n > 1) extra += n * ((u.vecs + 31) / 32);
+      parts.emplace_back((u.tiles + n - 1) / n, n * hkv);
+      cuts += n > 1 ? n * ((u.vecs + 31) / 32) : 0;
+      most_cuts = std::max(most_cuts, n);
     }
-    if (sum < 0.) break;
-    const double us = std::max(longest, sum * hkv / c.at_once) +
-                      (extra ? c.join + c.part * (double)extra * hkv : 0.);
+    if (most_cuts > 128) break;
+    const double own = makespan(parts, PAGED_CUS, c), all = c.fixed + all_us;
+    const double us = std::sqrt(std::sqrt(own * own * own * own + all * all * all * all)) +
+                      (cuts ? c.join + 0.008 * (double)(cuts * hkv) : 0.);
     if (best < 0. || us < best) {
       best = us;
       best_len = len;
     }
   }
-  for (Unit& u : units) u.parts = (int)std::max<int64_t>(1, (u.tiles + best_len - 1) / best_len);
+  return best_len;
 }
 
 }  // namespace paged_detail
@@ -154,19 +225,39 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
   std::vector<PagedTile> tiles;
   std::vector<int32_t> written;  // the tiles' numbers, to find two rows in one place
   int64_t n_table = 0;
+  // Sequences of many query vectors: by the large kernel where the others' is estimated to take longer. A
+  // tile of 256 query vectors is 0.88 us there and 1.32 in four units of 64; beginning, end and balance
+  // are 48 and 6 (2048 rows x 16 heads: over 16384 keys 267 us and 335, over 2048 57 and 38).
+  double work = 0.;  // tiles of 256 query vectors, of a CU
+  int64_t n64 = 0;
+  const auto unit_tiles = [&](int s, int64_t last_vec) {
+    const int64_t end = paged_key_end(a.pos0[s] + last_vec / G, a.keys[s], a.masked != 0,
+                                      a.prompt_len ? a.prompt_len[s] : 0, a.block);
+    return (end + 31) / 32;
+  };
+  for (int s = 0; s < a.seqs; ++s) {
+    const int64_t vecs = (int64_t)a.rows[s] * G;
+    n64 += (vecs + 63) / 64 * a.hkv;
+    if (vecs < PAGED_VECS_L) continue;
+    const int64_t n = (vecs + PAGED_VECS_L - 1) / PAGED_VECS_L;
+    work += 0.5 * (double)(n * (unit_tiles(s, 0) + unit_tiles(s, vecs - 1))) * a.hkv / PAGED_CUS;
+  }
+  const bool many = 0.88 * work + 48. < 1.32 * work + 6.;
+  // Units of 64 (whose tiles are read for 32 query vectors twice, by waves side by side) where they fill
+  // the chip: a chunk of 500 rows x 16 heads over 4097 keys beside 31 tokens 56 us, of 32 67; 512 rows
+  // over 16384 alone 148 and 92.
+  const int small_vecs = n64 >= 192 ? 2 * PAGED_VECS : PAGED_VECS;
   for (int s = 0; s < a.seqs; ++s) {
     row0[s] = p.rows;
     p.rows += a.rows[s];
     table0[s] = n_table;
     n_table += (a.keys[s] + (int64_t)a.page_size - 1) / a.page_size;
     const int64_t vecs = (int64_t)a.rows[s] * G;
-    const bool large = vecs > PAGED_SMALL;
-    const int step = large ? PAGED_VECS_L : PAGED_VECS;
+    const bool large = many && vecs >= PAGED_VECS_L;
+    const int step = large ? PAGED_VECS_L : small_vecs;
     for (int64_t v = 0; v < vecs; v += step) {
       const int n = (int)std::min<int64_t>(step, vecs - v);
-      const int64_t end = paged_key_end(a.pos0[s] + (v + n - 1) / G, a.keys[s], a.masked != 0,
-                                        a.prompt_len ? a.prompt_len[s] : 0, a.block);
-      units[large].push_back(Unit{s, (int)v, n, (end + 31) / 32, 1});
+      units[large].push_back(Unit{s, (int)v, n, unit_tiles(s, v + n - 1)});
     }
     // the tiles that rows inside the sequence's keys lie in
     const int32_t* pg = a.table + (int64_t)s * a.width;
@@ -190,15 +281,58 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
   std::sort(written.begin(), written.end());
   if (std::adjacent_find(written.begin(), written.end()) != written.end()) p.appendable = 0;
 
-  cut(units[0], a.hkv, Costs{3.0, 0.055, 4.0, 0.004, PAGED_CUS});
-  cut(units[1], a.hkv, Costs{4.0, 0.9, 4.0, 0.004, PAGED_CUS});
   std::vector<PagedPiece> pieces[2];
+  std::vector<int32_t> first[2];
   std::vector<PagedJoin> joins;
   int slot = 0;
   for (int k = 0; k < 2; ++k) {
-    for (const Unit& u : units[k]) {
-      const int s = u.seq, subs = (u.vecs + 31) / 32;
-      for (int i = 0; i < u.parts; ++i) {
+    if (units[k].empty()) continue;
+    std::vector<Share> shares;
+    if (k == 0) {
+      std::stable_sort(units[0].begin(), units[0].end(),
+                       [](const Unit& x, const Unit& y) { return x.tiles > y.tiles; });
+      int64_t all = 0;  // (units of one sequence follow one another, the longest first)
+      std::vector<int64_t> read(a.seqs, 0);
+      for (const Unit& u : units[0]) read[u.seq] = std::max(read[u.seq], u.tiles);
+      for (int64_t n : read) all += n;
+      const int64_t len = part_length(units[0], a.hkv, 0.0031 * (double)(all * a.hkv),
+                                      Costs{3.5, 0.2, 5.5});
+      int group = 0;
+      for (int i = 0; i < (int)units[0].size(); ++i) {
+        const int64_t tiles = units[0][i].tiles, n = std::max<int64_t>(1, (tiles + len - 1) / len);
+        for (int64_t j = 0; j < n; ++j)
+          shares.push_back(Share{i, group++, tiles * j / n, tiles * (j + 1) / n});
+      }
+    } else {
+      // whole units, or equal shares of all: by the time of either
+      const Costs c{12., 0.875, 25.};
+      const int groups = std::max(1, PAGED_CUS / a.hkv);
+      std::vector<std::pair<int64_t, int64_t>> len;
+      double sum = 0.;
+      for (const Unit& u : units[1]) {
+        len.emplace_back(u.tiles, a.hkv);
+        sum += c.fixed + c.tile * (double)u.tiles;
+      }
+      const double whole = makespan(len, PAGED_CUS, c);
+      const double parts = 8. * (double)(units[1].size() + groups) * a.hkv;  // (at most) written and read
+      if (whole <= sum / groups + c.fixed + c.join + 0.009 * parts) {
+        std::stable_sort(units[1].begin(), units[1].end(),
+                         [](const Unit& x, const Unit& y) { return x.tiles > y.tiles; });
+        for (int i = 0; i < (int)units[1].size(); ++i) shares.push_back(Share{i, i, 0, units[1][i].tiles});
+      } else {
+        shares = cut(units[1], groups, c);
+      }
+    }
+    for (size_t i = 0; i < shares.size();) {
+      size_t j = i;
+      while (j < shares.size() && shares[j].unit == shares[i].unit) ++j;
+      const Unit& u = units[k][shares[i].unit];
+      const int s = u.seq, subs = (u.vecs + 31) / 32, parts = (int)(j - i), slot0 = slot;
+      for (; i < j; ++i) {
+        if (i == 0 || shares[i].group != shares[i - 1].group) {
+          if (i) pieces[k].back().last = 1;
+          first[k].push_back((int32_t)pieces[k].size());
+        }
         PagedPiece y{};
         y.row0 = row0[s];
         y.rows = a.rows[s];
@@ -206,32 +340,29 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
         y.keys = a.keys[s];
         y.prompt_len = a.prompt_len ? a.prompt_len[s] : 0;
         y.vec0 = u.vec0;
-        y.tile0 = (int)(u.tiles * i / u.parts);
-        y.tile1 = (int)(u.tiles * (i + 1) / u.parts);
-        y.slot = u.parts > 1 ? slot + i * subs : -1;
+        y.tile0 = (int)shares[i].tile0;
+        y.tile1 = (int)shares[i].tile1;
+        y.slot = parts > 1 ? slot : -1;
         y.table = (int)table0[s];
+        y.wide_log2 = u.vecs > PAGED_VECS;
         pieces[k].push_back(y);
+        if (parts > 1) slot += subs;
       }
-      if (u.parts == 1) continue;
-      for (int j = 0; j < subs; ++j) {
+      for (int q = 0; parts > 1 && q < subs; ++q) {
         PagedJoin y{};
         y.row0 = row0[s];
-        y.vec0 = u.vec0 + 32 * j;
-        y.vecs = std::min(32, u.vecs - 32 * j);
-        y.slot = slot + j;
+        y.vec0 = u.vec0 + 32 * q;
+        y.vecs = std::min(32, u.vecs - 32 * q);
+        y.slot = slot0 + q;
         y.step = subs;
-        y.parts = u.parts;
+        y.parts = parts;
         joins.push_back(y);
       }
-      slot += subs * u.parts;
     }
-    // the longest first (parts of one length keep their order: neighbours read the same keys)
-    std::stable_sort(pieces[k].begin(), pieces[k].end(), [](const PagedPiece& x, const PagedPiece& y) {
-      return x.tile1 - x.tile0 > y.tile1 - y.tile0;
-    });
+    pieces[k].back().last = 1;
   }
-  p.n_small = (int)pieces[0].size();
-  p.n_large = (int)pieces[1].size();
+  p.n_small = (int)first[0].size();
+  p.n_large = (int)first[1].size();
   p.n_joins = (int)joins.size();
   p.n_tiles = (int)tiles.size();
   p.slots = slot;
@@ -244,6 +375,9 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
   };
   p.small = put(pieces[0].data(), pieces[0].size() * 16);
   p.large = put(pieces[1].data(), pieces[1].size() * 16);
+  p.first_small = put(first[0].data(), first[0].size());
+  p.first_large = put(first[1].data(), first[1].size());
+  out.resize((out.size() + 15) / 16 * 16);
   p.joins = put(joins.data(), joins.size() * 8);
   p.tiles = put(tiles.data(), tiles.size() * 8);
   p.table = (int64_t)out.size();

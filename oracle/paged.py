@@ -63,12 +63,12 @@ def attention(q, k, v, ends, kind="f16", out="f32"):
     """(o, bound) [rows, heads, 128] of q [rows, heads, 128] over k, v [keys, kv_heads, 128] (what the
     cache holds), row r over its first ends[r] keys; no key: zeros.
 
-    The bound counts, relative to the weighted sum of |v|: the weights' rounding to the cache's type
-    `kind`; a score's fp32 sum (130 roundings of its products' magnitudes), twice, for it is in the
-    weights' sum too; the exponent's argument, power and the sums in fp32 (2^-18: the argument is
-    rounded to 2^-24 of up to 2^5 once the base is off; the rest are single roundings in chains of a
-    few dozen). Weights of fp16 below its smallest normal one are off by 2^-25 each of at least one
-    whole weight in the sum. Then the result's rounding to `out`."""
+    The bound counts what changes a weight alike above and below the fraction, so that it moves the
+    result by w |v - o| times as much: the weight's rounding to the cache's type `kind`, its score's fp32
+    sum (130 roundings of its products' magnitudes), the exponent's argument and the power (2^-18: the
+    argument is rounded to 2^-24 of up to 2^5 once the base is off). Then the sums in fp32 (2^-18: single
+    roundings in chains of a few dozen). Weights of fp16 below its smallest normal one are off by 2^-25
+    each of at least one whole weight in the sum. Then the result's rounding to `out`."""
     q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
     rows, hq, hd = q.shape
     g = hq // k.shape[1]
@@ -85,9 +85,10 @@ def attention(q, k, v, ends, kind="f16", out="f32"):
             total = w.sum()
             w /= total
             o[r, h] = w @ vv
-            per = HALF_STEP[kind] + 2 * 130 * 2.0**-24 * size + 2.0**-18
-            bound[r, h] = (w * per) @ np.abs(vv) + np.abs(o[r, h]) * (w @ per - HALF_STEP[kind])
+            per = HALF_STEP[kind] + 130 * 2.0**-24 * size + 2.0**-18
+            apart = np.abs(vv - o[r, h])
+            bound[r, h] = (w * per) @ apart + 2.0**-18 * (w @ np.abs(vv) + np.abs(o[r, h]))
             if kind == "f16":
-                bound[r, h] += 2.0**-25 * np.abs(vv).sum(0) / total
+                bound[r, h] += 2.0**-25 * apart.sum(0) / total
             bound[r, h] += HALF_STEP[out] * (np.abs(o[r, h]) + bound[r, h])
     return o, bound

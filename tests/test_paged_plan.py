@@ -22,6 +22,19 @@ def _words(batch, at, n, width):
     return batch._list.numpy()[at:at + n * width].reshape(n, width)
 
 
+def _pieces(batch, at, first, groups):
+    """The parts of all work-groups: each from its first to the one that says it is the last."""
+    words, out, end = batch._list.numpy(), [], 0
+    for i in words[first:first + groups]:
+        assert i == end
+        while True:
+            out.append(words[at + 16 * end:at + 16 * end + 16])
+            end += 1
+            if out[-1][10]:
+                break
+    return out
+
+
 def _random_batch(seed):
     rng = random.Random(seed)
     size, kv_heads = rng.choice([32, 64, 256]), rng.choice([1, 2, 4])
@@ -60,8 +73,9 @@ def test_parts_cover_every_row_and_key_once(seed):
     joins = _words(batch, info.joins, info.n_joins, 8)
     seen = {}   # (sequence, query vector / 32) -> tile ranges
     slots = set()
-    for large, (at, n) in enumerate(((info.small, info.n_small), (info.large, info.n_large))):
-        for p in _words(batch, at, n, 16):
+    for large, (at, first, n) in enumerate(((info.small, info.first_small, info.n_small),
+                                            (info.large, info.first_large, info.n_large))):
+        for p in _pieces(batch, at, first, n):
             r0, nr, p0, nk, pl, vec0, t0, t1, slot, tab = (int(x) for x in p[:10])
             s = [i for i in range(len(rows)) if row0[i] == r0 and rows[i] == nr and rows[i]][0]
             assert (p0, nk) == (pos0[s], keys[s])
@@ -70,7 +84,8 @@ def test_parts_cover_every_row_and_key_once(seed):
             assert [int(x) for x in pages[tab:tab + need]] == [
                 x * cache.kv_heads * tpp for x in table[s][:need]]
             assert 0 <= t0 <= t1 <= -(-keys[s] // 32) and 0 <= vec0 < nr * g
-            vecs = min(256 if large else 32, nr * g - vec0)
+            vecs = nr * g - vec0
+            vecs = min(256 if large else 32 << p[11], vecs)
             for sub in range(-(-vecs // 32)):
                 seen.setdefault((s, vec0 // 32 + sub), []).append((t0, t1, slot + sub if slot >= 0
                                                                     else -1))
