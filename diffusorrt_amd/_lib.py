@@ -154,16 +154,15 @@ SIGNATURES = {
     "drt_op_sparse_attention": (_I32, [_VP, _I32, _VP, _I64, _I32, _VP, _I32, _I32, _I32, _I32,
                                        _I32, _I32, _I32, _I32, _VP, _I32, _I32, _VP, _I32, _VP,
                                        _SZ, _VP]),
-    "drt_op_rotate": (_I32, [_VP, _I64, _I64, _I32, _I32, _I32, _I32, C.POINTER(Rotary), _VP, _I32,
+    "drt_op_rotate": (_I32, [_VP, _I64, _I64, _I32, _I32, _I32, _I32, _VP, _VP, _I32,
                              _I32, _VP, _I64, _I64, _VP]),
     "drt_paged_plan": (_I32, [_VP, _I32, _I32, _VP, _VP, _VP, _VP, _I32, _I32, _I32, _I32, _I32,
                               _I32, _VP, _I64, C.POINTER(PagedBatch)]),
-    "drt_op_paged_append": (_I32, [C.POINTER(PagedBatch), _VP, _VP, _I64, _I64, _VP, _I64, _I64,
-                                   _VP, _I64, _I64, _I32, C.POINTER(Rotary), _VP, _I32, _VP, _VP]),
-    "drt_op_paged_load": (_I32, [C.POINTER(PagedBatch), _VP, _VP, _I32, _VP, _VP, _VP]),
+    "drt_op_paged_append": (_I32, [_VP, _VP, _VP, _I64, _I64, _VP, _I64, _I64,
+                                   _VP, _I64, _I64, _I32, _VP, _VP, _I32, _VP, _VP]),
+    "drt_op_paged_load": (_I32, [_VP, _VP, _VP, _I32, _VP, _VP, _VP]),
     "drt_op_paged_attention_workspace_bytes": (_SZ, [C.POINTER(PagedBatch)]),
-    "drt_op_paged_attention": (_I32, [C.POINTER(PagedBatch), _VP, _VP, _VP, _I32, _VP, _I32, _VP,
-                                      _SZ, _VP]),
+    "drt_op_paged_attention": (_I32, [_VP, _VP, _VP, _VP, _I32, _VP, _I32, _VP, _SZ, _VP]),
 }
 
 _lib = None

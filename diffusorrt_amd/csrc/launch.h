@@ -268,7 +268,7 @@ void rotate(const RotateCall& r, hipStream_t s);
 struct AppendCall {
   const void *q, *k, *v;  // q may be null
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
-  int type, cache_bf16, n_tiles, hq, hkv, tpp;
+  int type, cache_bf16, n_tiles, rows, hq, hkv, tpp;
   const void* tiles;
   void *cache, *q_out;
   RotaryTurns rotary;

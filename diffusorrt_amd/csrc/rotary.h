@@ -78,6 +78,25 @@ template <int DT> DRT_DEV void rotary_store8(void* p, const float (&x)[8]) {
     *(u32x4_e*)p = rotary_pack8<DT>(x);
   }
 }
+// Two neighbours, aligned to their type only.
+template <int DT> DRT_DEV void rotary_load2(const void* p, int64_t i, float& a, float& b) {
+  typedef float f32x2_e __attribute__((ext_vector_type(2), aligned(4)));
+  typedef uint16_t u16x2_e __attribute__((ext_vector_type(2), aligned(2)));
+  if constexpr (DT == 0) {
+    const f32x2_e w = *(const f32x2_e*)((const float*)p + i);
+    a = w[0];
+    b = w[1];
+  } else {
+    const u16x2_e w = *(const u16x2_e*)((const uint16_t*)p + i);
+    if constexpr (DT == 1) {
+      a = (float)__builtin_bit_cast(_Float16, (uint16_t)w[0]);
+      b = (float)__builtin_bit_cast(_Float16, (uint16_t)w[1]);
+    } else {
+      a = bf16_bits_to_float(w[0]);
+      b = bf16_bits_to_float(w[1]);
+    }
+  }
+}
 template <int DT> DRT_DEV float rotary_load1(const void* p, int64_t i) {
   if constexpr (DT == 0) return ((const float*)p)[i];
   else if constexpr (DT == 1) return (float)((const _Float16*)p)[i];

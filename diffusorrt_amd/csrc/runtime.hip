@@ -3106,6 +3106,7 @@ int32_t drt_op_paged_append(const drt_paged_batch* batch, const int32_t* list, c
     c.v_head = v_head_stride;
     c.cache_bf16 = kv_dtype == DRT_BF16;
     c.n_tiles = batch->n_tiles;
+    c.rows = batch->rows;
     c.hq = batch->hq;
     c.hkv = batch->hkv;
     c.tpp = batch->page_size / 32;

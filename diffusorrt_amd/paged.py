@@ -6,18 +6,20 @@ same page (a prefix in common).
 """
 from __future__ import annotations
 
+import ctypes as C
+
 import numpy as np
+import torch
 
 from . import _lib
-from .kernels import KV_TILE_ELEMS, _attention_out, _cache_dtype, _launch, _mask_args, _torch
-from .rotary import _type_code
+from .kernels import KV_TILE_ELEMS, _cache_dtype, _launch, _mask_args
+from .rotary import _TYPES
 
 _I32_MAX = 2**31 - 1
 
 
 def _whole_numbers(values, what):
     """int32 numpy of a list, an array or a host tensor of whole numbers."""
-    torch = _torch()
     if isinstance(values, torch.Tensor):
         if values.is_cuda:
             raise ValueError(f"{what} must be on the host")
@@ -54,7 +56,6 @@ class PagedBatch:
     as a captured graph that used it is replayed."""
 
     def __init__(self, cache, table, keys, rows, heads, positions, kind, mask_geometry):
-        torch = _torch()
         table = _table(table)
         keys, rows = _whole_numbers(keys, "keys"), _whole_numbers(rows, "rows")
         seqs = table.shape[0]
@@ -101,11 +102,17 @@ class PagedBatch:
             host = torch.empty(self.info.words, dtype=torch.int32, pin_memory=on_gpu)
             plan(host)
         host = host[:self.info.words]
+        info = self.info
+        self._address = C.addressof(info)
+        self._q_shape, self._kv_shape = (info.rows, info.hq, 128), (info.rows, info.hkv, 128)
+        self._out_shape = (info.rows, info.hq * 128)
+        self._workspace = lib.drt_op_paged_attention_workspace_bytes(info)
         if not on_gpu:
             self._list = host
             return
         with torch.cuda.device(self._index):
             self._list = host.to(cache.data.device, non_blocking=True)
+            self._at = self._list.data_ptr()
             self._ready = torch.cuda.Event()
             self._ready.record()
             self._stream = torch._C._cuda_getCurrentRawStream(self._index)
@@ -119,7 +126,7 @@ class PagedBatch:
     def heads(self) -> int:
         return self.info.hq
 
-    def _here(self, torch) -> int:
+    def _here(self) -> int:
         """The list's address, for the current stream."""
         if torch._C._cuda_getCurrentRawStream(self._index) != self._stream:
             # (while a stream is captured its other work is done: capturing began with a wait)
@@ -127,7 +134,7 @@ class PagedBatch:
                 stream = torch.cuda.current_stream(self._index)
                 stream.wait_event(self._ready)
                 self._list.record_stream(stream)
-        return self._list.data_ptr()
+        return self._at
 
 
 class PagedKVCache:
@@ -140,7 +147,6 @@ class PagedKVCache:
 
     def __init__(self, layers: int, kv_heads: int, pages: int, *, page_size: int = 64,
                  dtype="f16", device=None):
-        torch = _torch()
         self.layers, self.kv_heads, self.pages = int(layers), int(kv_heads), int(pages)
         self.page_size = int(page_size)
         if self.layers < 1 or self.kv_heads < 1 or self.pages < 1:
@@ -158,6 +164,8 @@ class PagedKVCache:
                                 device=device or "cuda")
         self._index = self.data.get_device()
         self._geometry = (self.kv_heads, self.pages, self.page_size, self._index)
+        self._data, self._layer_bytes = self.data.data_ptr(), self.data.stride(0) * 2
+        self._lib = None
 
     @property
     def nbytes(self) -> int:
@@ -179,21 +187,26 @@ class PagedKVCache:
         sequence."""
         return PagedBatch(self, pages, keys, rows, heads, positions, kind, mask_geometry)
 
-    def _check(self, layer, batch):
+    def _entry(self, layer, batch):
+        """The library, once a call's layer and batch are checked."""
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer must be in [0, {self.layers})")
         if self._index < 0:
             raise ValueError("the cache must be on a GPU")
         if not isinstance(batch, PagedBatch) or batch._geometry != self._geometry:
             raise ValueError("the batch was planned for another cache")
-
-    def _layer(self, layer):
-        return self.data.data_ptr() + layer * self.data.stride(0) * 2
+        if self._lib is None:
+            self._lib = _lib.load()
+        return self._lib
 
     def _source(self, t, shape, what):
-        if t.shape != shape or t.get_device() != self._index or t.stride(2) != 1:
-            raise ValueError(f"{what} must be {list(shape)} on the cache's device, a head's elements "
-                             "side by side")
+        """A source's strides between rows and heads."""
+        if t.shape != shape or t.get_device() != self._index:
+            raise ValueError(f"{what} must be {list(shape)} on the cache's device")
+        rows, heads, one = t.stride()
+        if one != 1:
+            raise ValueError(f"{what}: a head's elements must be side by side")
+        return rows, heads
 
     def append(self, layer: int, k, v, batch: PagedBatch, *, rotary=None, q=None):
         """Write the batch's ``k, v [rows, kv_heads, 128]`` (fp32, fp16 or bf16, views of a fused
@@ -204,57 +217,60 @@ class PagedKVCache:
         which comes back in the cache's type, ready for :meth:`attention`. Each value is rounded
         once. Raises ValueError where two sequences of the batch have rows in one tile of a page,
         or a row lies behind its sequence's keys."""
-        torch = _torch()
-        self._check(layer, batch)
-        info = batch.info
-        shape = (info.rows, self.kv_heads, 128)
-        self._source(k, shape, "append's k")
-        self._source(v, shape, "append's v")
-        code = _type_code(k.dtype)
-        if code is None or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+        lib = self._entry(layer, batch)
+        k0, k1 = self._source(k, batch._kv_shape, "append's k")
+        v0, v1 = self._source(v, batch._kv_shape, "append's v")
+        dtype = k.dtype
+        code = _TYPES.get(dtype)
+        if code is None or v.dtype is not dtype:
             raise ValueError("append takes k, v and q of one type: float32, float16 or bfloat16")
-        if rotary is not None and (rotary.dim > 128 or rotary.dim % 16 or
-                                   rotary._index != self._index):
-            raise ValueError("append's rotary must turn a multiple of 16 elements, 128 at most, "
-                             "on the cache's device")
-        out = None
-        if q is not None:
-            self._source(q, (info.rows, info.hq, 128), "append's q")
-            out = torch.empty(q.shape, dtype=self.dtype, device=q.device)
-        at = batch._here(torch)
-        _launch(torch, _lib.load().drt_op_paged_append, self._index, info, at, k.data_ptr(),
-                k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                None if q is None else q.data_ptr(), 0 if q is None else q.stride(0),
-                0 if q is None else q.stride(1), code, None if rotary is None else rotary._args,
-                self._layer(layer), self.kv_dtype, None if out is None else out.data_ptr())
+        turns = None
+        if rotary is not None:
+            if rotary.dim > 128 or rotary.dim % 16 or rotary._index != self._index:
+                raise ValueError("append's rotary must turn a multiple of 16 elements, 128 at "
+                                 "most, on the cache's device")
+            turns = rotary._address
+        if q is None:
+            out = q_at = out_at = None
+            q0 = q1 = 0
+        else:
+            q0, q1 = self._source(q, batch._q_shape, "append's q")
+            if q.dtype is not dtype:
+                raise ValueError("append takes k, v and q of one type: float32, float16 or "
+                                 "bfloat16")
+            out = q.new_empty(batch._q_shape, dtype=self.dtype)
+            q_at, out_at = q.data_ptr(), out.data_ptr()
+        _launch(torch, lib.drt_op_paged_append, self._index, batch._address, batch._here(),
+                k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, q_at, q0, q1, code, turns,
+                self._data + layer * self._layer_bytes, self.kv_dtype, out_at)
         return out
 
     def load(self, layer: int, batch: PagedBatch):
         """``(k, v) [rows, kv_heads, 128]`` of the batch's rows as the cache holds them."""
-        torch = _torch()
-        self._check(layer, batch)
-        k = torch.empty((batch.info.rows, self.kv_heads, 128), dtype=self.dtype,
-                        device=self.data.device)
-        v = torch.empty_like(k)
-        _launch(torch, _lib.load().drt_op_paged_load, self._index, batch.info, batch._here(torch),
-                self._layer(layer), self.kv_dtype, k.data_ptr(), v.data_ptr())
+        lib = self._entry(layer, batch)
+        k = self.data.new_empty(batch._kv_shape)
+        v = self.data.new_empty(batch._kv_shape)
+        _launch(torch, lib.drt_op_paged_load, self._index, batch._address, batch._here(),
+                self._data + layer * self._layer_bytes, self.kv_dtype, k.data_ptr(), v.data_ptr())
         return k, v
 
     def attention(self, layer: int, q, batch: PagedBatch, *, out_dtype=None):
         """Attention of the batch's ``q [rows, heads, 128]`` (the cache's type) over the keys that
         each row sees: ``[rows, heads * 128]`` in fp32 or bf16. A row without any gives zeros."""
-        torch = _torch()
-        self._check(layer, batch)
-        info = batch.info
-        if q.dim() != 3 or q.shape != (info.rows, info.hq, 128) or q.dtype != self.dtype or \
+        lib = self._entry(layer, batch)
+        if q.shape != batch._q_shape or q.dtype is not self.dtype or \
                 q.get_device() != self._index or not q.is_contiguous():
-            raise ValueError(f"q must be contiguous [{info.rows}, {info.hq}, 128] of the cache's "
-                             "type and device")
-        out, odt = _attention_out(torch, q, info.rows, info.hq, out_dtype)
-        lib = _lib.load()
-        need = lib.drt_op_paged_attention_workspace_bytes(info)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        _launch(torch, lib.drt_op_paged_attention, self._index, info, batch._here(torch),
-                q.data_ptr(), self._layer(layer), self.kv_dtype, out.data_ptr(), odt,
+            raise ValueError(f"q must be contiguous {list(batch._q_shape)} of the cache's type and "
+                             "device")
+        if out_dtype is None:
+            out_dtype = torch.float32
+        if out_dtype is not torch.float32 and out_dtype is not torch.bfloat16:
+            raise ValueError("attention out must be float32 or bfloat16")
+        out = q.new_empty(batch._out_shape, dtype=out_dtype)
+        need = batch._workspace
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
+        _launch(torch, lib.drt_op_paged_attention, self._index, batch._address, batch._here(),
+                q.data_ptr(), self._data + layer * self._layer_bytes, self.kv_dtype,
+                out.data_ptr(), _lib.BF16 if out_dtype is torch.bfloat16 else _lib.F32,
                 None if ws is None else ws.data_ptr(), need)
         return out

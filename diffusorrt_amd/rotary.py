@@ -5,11 +5,14 @@ frequencies are kept and the angles made where they are used, for any 32-bit pos
 """
 from __future__ import annotations
 
+import ctypes as C
 import math
 from fractions import Fraction
 
+import torch
+
 from . import _lib
-from .kernels import _launch, _torch
+from .kernels import _launch
 
 _I32_MIN, _I32_MAX = -2**31, 2**31 - 1
 _TWO_PI = 2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
@@ -107,15 +110,7 @@ def _same_places(a, b) -> bool:
         x == y or n == 1 for x, y, n in zip(a.stride(), b.stride(), a.shape))
 
 
-_TYPES = {}
-
-
-def _type_code(dtype):
-    if not _TYPES:
-        torch = _torch()
-        _TYPES.update({torch.float32: _lib.F32, torch.float16: _lib.F16,
-                       torch.bfloat16: _lib.BF16})
-    return _TYPES.get(dtype)
+_TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
 class RotaryPositions:
@@ -129,7 +124,6 @@ class RotaryPositions:
 
     def __init__(self, dim: int = 128, *, theta: float = 1e6, layout: str = "half", scaling=None,
                  frequencies=None, magnitude=None, device=None):
-        torch = _torch()
         if layout not in _LAYOUTS:
             raise ValueError(f"rotary layout is 'half' or 'interleaved', not {layout!r}")
         if frequencies is None:
@@ -153,6 +147,8 @@ class RotaryPositions:
         self._index = self.turns.get_device()
         self._args = _lib.Rotary(self.turns.data_ptr(), dim, int(layout == "interleaved"),
                                  self.magnitude)
+        self._address = C.addressof(self._args)
+        self._rotate = None
 
     def rotate(self, x, positions, *, inverse: bool = False, out=None):
         """``x [rows, heads, head_dim]`` (fp32, fp16 or bf16; any strides between rows and heads)
@@ -162,22 +158,24 @@ class RotaryPositions:
 
         ``out``: a tensor of x's shape and type, ``x`` itself or memory apart from it. Computed in
         fp32, rounded once."""
-        torch = _torch()
-        if self._index < 0:
-            raise ValueError("the rotary's frequencies must be on a GPU")
-        if x.dim() != 3 or x.shape[2] < self.dim:
+        # (a short call is mostly host time: each check once, in the order of what fails least)
+        shape, index = x.shape, self._index
+        if len(shape) != 3 or shape[2] < self.dim:
             raise ValueError(f"rotate takes x [rows, heads, head_dim >= {self.dim}]")
-        code = _type_code(x.dtype)
+        rows, heads, hd = shape
+        code = _TYPES.get(x.dtype)
         if code is None:
             raise ValueError("rotate takes float32, float16 or bfloat16")
-        rows, heads, hd = x.shape
-        if x.get_device() != self._index:
+        if index < 0:
+            raise ValueError("the rotary's frequencies must be on a GPU")
+        if x.get_device() != index:
             raise ValueError("x must be on the frequencies' device")
-        if x.stride(2) != 1 and hd > 1:
+        x0, x1, x2 = x.stride()
+        if x2 != 1:
             raise ValueError("a head's elements must be side by side")
         if isinstance(positions, torch.Tensor):
             if positions.dtype is not torch.int32 or positions.shape != (rows,) or \
-                    not positions.is_contiguous() or positions.get_device() != self._index:
+                    positions.get_device() != index or not positions.is_contiguous():
                 raise ValueError("positions must be int32 [rows] on x's device, or a number")
             at, pos0 = positions.data_ptr(), 0
         else:
@@ -187,18 +185,23 @@ class RotaryPositions:
             if not (_I32_MIN <= pos0 and pos0 + rows - 1 <= _I32_MAX):
                 raise ValueError("positions must be of 32 bits")
         if out is None:
-            out = torch.empty((rows, heads, hd), dtype=x.dtype, device=x.device)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+            y0, y1 = heads * hd, hd
         else:
-            if out.shape != x.shape or out.dtype != x.dtype or out.get_device() != self._index or \
-                    (out.stride(2) != 1 and hd > 1) or not _apart(out):
+            if out.shape != shape or out.dtype != x.dtype or out.get_device() != index or \
+                    out.stride(2) != 1 or not _apart(out):
                 raise ValueError("out must be a tensor of x's shape, type and device, its elements "
                                  "apart and a head's side by side")
+            y0, y1, _ = out.stride()
             if x.numel() and not _same_places(x, out):
                 (a, b), (c, d) = _span(x), _span(out)
                 if a < d and c < b:
                     raise ValueError("out must be x itself or memory apart from it")
-        if x.numel():
-            _launch(torch, _lib.load().drt_op_rotate, self._index, x.data_ptr(), x.stride(0),
-                    x.stride(1), code, rows, heads, hd, self._args, at, pos0, int(bool(inverse)),
-                    out.data_ptr(), out.stride(0), out.stride(1))
+        if rows and heads:
+            _launch(torch, self._rotate or self._bind(), index, x.data_ptr(), x0, x1, code, rows,
+                    heads, hd, self._address, at, pos0, 1 if inverse else 0, out.data_ptr(), y0, y1)
         return out
+
+    def _bind(self):
+        self._rotate = _lib.load().drt_op_rotate
+        return self._rotate
