@@ -93,8 +93,7 @@ class PagedBatch(C.Structure):
     _fields_ = [(n, C.c_int32) for n in (
         "rows", "appendable", "hq", "hkv", "page_size", "pages", "mask_kind", "mask_block_size",
         "n_small", "n_large", "n_joins", "n_tiles", "slots", "reserved")] + \
-        [(n, C.c_int64) for n in ("small", "large", "first_small",
-                                      "first_large", "joins", "tiles", "table", "words")]
+        [(n, C.c_int64) for n in ("small", "large", "first_large", "joins", "tiles", "table", "words")]
 
 
 _VP, _I32, _I64, _U64, _SZ = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_size_t

@@ -280,7 +280,7 @@ struct PagedAttnCall {
   const void *q, *cache;
   const int32_t* list;  // the batch's, on the device
   int n_small, n_large, n_joins, slots;
-  int64_t small, large, first_small, first_large, joins, table;
+  int64_t small, large, first_large, joins, table;
   int cache_bf16, hq, hkv, tpp, masked, block, out_type;
   void *out, *workspace;
 };

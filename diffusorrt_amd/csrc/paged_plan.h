@@ -15,8 +15,8 @@
 namespace drt {
 
 // A part of an attention: a unit of query vectors (row * G + head of the group, G = hq / hkv) of one
-// sequence over tiles [tile0, tile1) of its keys. A work-group does some that follow one another: the
-// last of them says so. Read by scalar loads: 64 bytes.
+// sequence over tiles [tile0, tile1) of its keys. A work-group of the large kernel does some that follow one
+// another: the last of them says so. Read by scalar loads: 64 bytes.
 struct PagedPiece {
   int32_t row0, rows;        // the sequence's rows in the batch
   int32_t pos0, keys, prompt_len;
@@ -52,9 +52,10 @@ struct PagedBatchArgs {
 struct PagedPlanInfo {
   // appendable: every row lies inside its sequence's keys, and none in the tile of another sequence's
   int32_t rows = 0, appendable = 1;
-  // work-groups of a K/V head for each kernel, with where each one's parts begin in `small` / `large`
+  // work-groups of a K/V head for each kernel: of the small one a part each, of the large one from part
+  // first_large[i] on to its last
   int32_t n_small = 0, n_large = 0, n_joins = 0, n_tiles = 0, slots = 0;
-  int64_t small = 0, large = 0, first_small = 0, first_large = 0;
+  int64_t small = 0, large = 0, first_large = 0;
   int64_t joins = 0, tiles = 0, table = 0, words = 0;
 };
 
@@ -161,52 +162,58 @@ inline std::vector<Share> cut(const std::vector<Unit>& units, int groups, const 
   return out;
 }
 
-// The time of work-groups, `slots` of them at once, the longest first; parts: (tiles, how many).
-inline double makespan(std::vector<std::pair<int64_t, int64_t>>& parts, int slots, const Costs& c) {
-  std::sort(parts.begin(), parts.end(), std::greater<std::pair<int64_t, int64_t>>());
+// The time of work-groups, `slots` of them at once, the longest first; parts: (us, how many).
+inline double makespan(std::vector<std::pair<double, int64_t>>& parts, int slots) {
+  std::sort(parts.begin(), parts.end(), std::greater<std::pair<double, int64_t>>());
   // rounds, each as long as its longest; or all of it evenly and the longest behind
   double rounds = 0., sum = 0.;
   int64_t room = 0;
   for (const auto& y : parts) {
-    const double us = c.fixed + c.tile * (double)y.first;
-    sum += us * (double)y.second;
+    sum += y.first * (double)y.second;
     const int64_t n = y.second - room;
     room = room > y.second ? room - y.second : 0;
     if (n > 0) {
       const int64_t r = (n + slots - 1) / slots;
-      rounds += us * (double)r;
+      rounds += y.first * (double)r;
       room = r * slots - n;
     }
   }
-  const double longest = c.fixed + c.tile * (double)parts[0].first;
-  return std::max(longest, std::min(rounds, sum / slots + longest));
+  return std::max(parts[0].first, std::min(rounds, sum / slots + parts[0].first));
 }
 
 // The longest part, in tiles, of units that are cut into equal ones, each a work-group of its own, by the
-// least time of all. all_us: what reading the keys of all sequences once takes; the nearer the
-// work-groups' own time comes to that, the more they wait for one another.
+// least time of all (c.tile: for 32 query vectors; 64 take 1.65 times as long). all_us: what reading the
+// keys of all sequences once takes; the nearer the work-groups' own time comes to that, the more they
+// wait for one another.
 inline int64_t part_length(const std::vector<Unit>& units, int hkv, double all_us, const Costs& c) {
-  std::vector<std::pair<int64_t, int64_t>> parts;
+  std::vector<std::pair<double, int64_t>> parts;
   int64_t most = 0;
   for (const Unit& u : units) most = std::max(most, u.tiles);
   double best = -1.;
   int64_t best_len = std::max<int64_t>(1, most);
-  for (int64_t len = best_len; len >= 1; len = std::min(len - 1, len * 4 / 5)) {
+  for (int64_t len = best_len; len >= 1; len = std::min(len - 1, len * 3 / 4)) {
     parts.clear();
     int64_t cuts = 0, most_cuts = 0;
     for (const Unit& u : units) {
       const int64_t n = std::max<int64_t>(1, (u.tiles + len - 1) / len);
-      parts.emplace_back((u.tiles + n - 1) / n, n * hkv);
+      parts.emplace_back(c.fixed + (u.vecs > PAGED_VECS ? 1.65 : 1.) * c.tile * (double)((u.tiles + n - 1) / n),
+                         n * hkv);
       cuts += n > 1 ? n * ((u.vecs + 31) / 32) : 0;
       most_cuts = std::max(most_cuts, n);
     }
     if (most_cuts > 128) break;
-    const double own = makespan(parts, PAGED_CUS, c), all = c.fixed + all_us;
+    const double own = makespan(parts, PAGED_CUS), all = c.fixed + all_us;
     const double us = std::sqrt(std::sqrt(own * own * own * own + all * all * all * all)) +
                       (cuts ? c.join + 0.008 * (double)(cuts * hkv) : 0.);
     if (best < 0. || us < best) {
       best = us;
       best_len = len;
+    }
+    // (whole units that take no longer than all of the work spread evenly)
+    if (len >= most) {
+      double sum = 0.;
+      for (const auto& y : parts) sum += y.first * (double)y.second;
+      if (own <= 1.1 * std::max(all, sum / PAGED_CUS)) break;
     }
   }
   return best_len;
@@ -282,7 +289,7 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
   if (std::adjacent_find(written.begin(), written.end()) != written.end()) p.appendable = 0;
 
   std::vector<PagedPiece> pieces[2];
-  std::vector<int32_t> first[2];
+  std::vector<int32_t> first;
   std::vector<PagedJoin> joins;
   int slot = 0;
   for (int k = 0; k < 2; ++k) {
@@ -296,7 +303,7 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
       for (const Unit& u : units[0]) read[u.seq] = std::max(read[u.seq], u.tiles);
       for (int64_t n : read) all += n;
       const int64_t len = part_length(units[0], a.hkv, 0.0031 * (double)(all * a.hkv),
-                                      Costs{3.5, 0.2, 5.5});
+                                      Costs{3.5, 0.24, 7.5});
       int group = 0;
       for (int i = 0; i < (int)units[0].size(); ++i) {
         const int64_t tiles = units[0][i].tiles, n = std::max<int64_t>(1, (tiles + len - 1) / len);
@@ -307,15 +314,15 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
       // whole units, or equal shares of all: by the time of either
       const Costs c{12., 0.875, 25.};
       const int groups = std::max(1, PAGED_CUS / a.hkv);
-      std::vector<std::pair<int64_t, int64_t>> len;
+      std::vector<std::pair<double, int64_t>> parts;
       double sum = 0.;
       for (const Unit& u : units[1]) {
-        len.emplace_back(u.tiles, a.hkv);
-        sum += c.fixed + c.tile * (double)u.tiles;
+        parts.emplace_back(c.fixed + c.tile * (double)u.tiles, a.hkv);
+        sum += parts.back().first;
       }
-      const double whole = makespan(len, PAGED_CUS, c);
-      const double parts = 8. * (double)(units[1].size() + groups) * a.hkv;  // (at most) written and read
-      if (whole <= sum / groups + c.fixed + c.join + 0.009 * parts) {
+      const double whole = makespan(parts, PAGED_CUS);
+      const double slots = 8. * (double)(units[1].size() + groups) * a.hkv;  // (at most) written and read
+      if (whole <= sum / groups + c.fixed + c.join + 0.009 * slots) {
         std::stable_sort(units[1].begin(), units[1].end(),
                          [](const Unit& x, const Unit& y) { return x.tiles > y.tiles; });
         for (int i = 0; i < (int)units[1].size(); ++i) shares.push_back(Share{i, i, 0, units[1][i].tiles});
@@ -331,7 +338,7 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
       for (; i < j; ++i) {
         if (i == 0 || shares[i].group != shares[i - 1].group) {
           if (i) pieces[k].back().last = 1;
-          first[k].push_back((int32_t)pieces[k].size());
+          if (k == 1) first.push_back((int32_t)pieces[k].size());
         }
         PagedPiece y{};
         y.row0 = row0[s];
@@ -361,8 +368,8 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
     }
     pieces[k].back().last = 1;
   }
-  p.n_small = (int)first[0].size();
-  p.n_large = (int)first[1].size();
+  p.n_small = (int)pieces[0].size();
+  p.n_large = (int)first.size();
   p.n_joins = (int)joins.size();
   p.n_tiles = (int)tiles.size();
   p.slots = slot;
@@ -375,8 +382,7 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
   };
   p.small = put(pieces[0].data(), pieces[0].size() * 16);
   p.large = put(pieces[1].data(), pieces[1].size() * 16);
-  p.first_small = put(first[0].data(), first[0].size());
-  p.first_large = put(first[1].data(), first[1].size());
+  p.first_large = put(first.data(), first.size());
   out.resize((out.size() + 15) / 16 * 16);
   p.joins = put(joins.data(), joins.size() * 8);
   p.tiles = put(tiles.data(), tiles.size() * 8);

@@ -3066,7 +3066,6 @@ int32_t drt_paged_plan(const int32_t* table, int32_t width, int32_t seqs, const 
     batch->slots = p.slots;
     batch->small = p.small;
     batch->large = p.large;
-    batch->first_small = p.first_small;
     batch->first_large = p.first_large;
     batch->joins = p.joins;
     batch->tiles = p.tiles;
@@ -3154,7 +3153,6 @@ int32_t drt_op_paged_attention(const drt_paged_batch* batch, const int32_t* list
     c.slots = batch->slots;
     c.small = batch->small;
     c.large = batch->large;
-    c.first_small = batch->first_small;
     c.first_large = batch->first_large;
     c.joins = batch->joins;
     c.table = batch->table;

@@ -7,6 +7,7 @@ same page (a prefix in common).
 from __future__ import annotations
 
 import ctypes as C
+import operator
 
 import numpy as np
 import torch
@@ -56,7 +57,11 @@ class PagedBatch:
     as a captured graph that used it is replayed."""
 
     def __init__(self, cache, table, keys, rows, heads, positions, kind, mask_geometry):
+        if cache._index >= 0 and torch.cuda.is_current_stream_capturing():
+            raise ValueError("a batch is planned before a graph is captured, not in it")
         table = _table(table)
+        if isinstance(heads, bool) or not isinstance(heads, int) or abs(heads) > _I32_MAX:
+            raise ValueError("heads must be a whole number")
         keys, rows = _whole_numbers(keys, "keys"), _whole_numbers(rows, "rows")
         seqs = table.shape[0]
         if keys.shape != (seqs,) or rows.shape != (seqs,):
@@ -72,8 +77,13 @@ class PagedBatch:
         else:
             if kind == "d2f_hybrid" and mask_geometry is not None and \
                     not isinstance(mask_geometry, dict):
-                first, block = mask_geometry
-                if not isinstance(first, int):  # a prompt's length for each sequence
+                try:
+                    first, block = mask_geometry
+                except (TypeError, ValueError):
+                    raise ValueError("d2f_hybrid mask geometry is (prompt length, block size)")
+                try:
+                    mask_geometry = (operator.index(first), block)
+                except TypeError:  # a prompt's length for each sequence
                     prompt = _whole_numbers(first, "prompt lengths")
                     if prompt.shape != (seqs,):
                         raise ValueError("prompt lengths are one for each sequence")
@@ -91,7 +101,7 @@ class PagedBatch:
             _lib.check(lib.drt_paged_plan(
                 table.ctypes.data, table.shape[1], seqs, rows.ctypes.data, keys.ctypes.data,
                 pos0.ctypes.data, None if prompt is None else prompt.ctypes.data, cache.page_size,
-                cache.pages, int(heads), cache.kv_heads, mask, block,
+                cache.pages, heads, cache.kv_heads, mask, block,
                 None if out is None else out.data_ptr(), 0 if out is None else out.numel(),
                 self.info))
 

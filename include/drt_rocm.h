@@ -395,7 +395,7 @@ typedef struct drt_paged_batch {
   int32_t appendable;  /* every row inside its sequence's keys, none in a tile of another's rows */
   int32_t hq, hkv, page_size, pages, mask_kind, mask_block_size;
   int32_t n_small, n_large, n_joins, n_tiles, slots, reserved;
-  int64_t small, large, first_small, first_large, joins, tiles, table;  /* where they begin in the list, in words */
+  int64_t small, large, first_large, joins, tiles, table;  /* where they begin in the list, in words */
   int64_t words;       /* of the list */
 } drt_paged_batch;
 /* Checks a batch given by host arrays and fills *batch in; where list_words >= batch->words its work list

@@ -383,6 +383,10 @@ def test_refusals():
     for call in bad:
         with pytest.raises(ValueError):
             call()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(ValueError, match="captured"):
+        with torch.cuda.graph(graph):
+            c.batch(s.table, [100, 64], [5, 9], heads=4)
     behind = c.batch(s.table, [100, 64], [5, 9], heads=4, positions=[98, 0])
     twice = c.batch([s.table[0], s.table[0]], [100, 100], [5, 9], heads=4)
     for batch in (behind, twice):

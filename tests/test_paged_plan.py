@@ -14,6 +14,9 @@ from oracle import paged as P
 pytestmark = pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="library not built")
 
 
+LARGE = set()  # (many rows, the large kernel is used, parts are joined) of the plans that were looked at
+
+
 def _cache(pages=64, page_size=64, kv_heads=2):
     return PagedKVCache(1, kv_heads, pages, page_size=page_size, device="cpu")
 
@@ -22,29 +25,35 @@ def _words(batch, at, n, width):
     return batch._list.numpy()[at:at + n * width].reshape(n, width)
 
 
-def _pieces(batch, at, first, groups):
-    """The parts of all work-groups: each from its first to the one that says it is the last."""
-    words, out, end = batch._list.numpy(), [], 0
-    for i in words[first:first + groups]:
-        assert i == end
+def _pieces(batch, large):
+    """The parts of a kernel's work-groups: one each, or (large) from its first to the one that says it
+    is the last."""
+    info, words = batch.info, batch._list.numpy()
+    if not large:
+        return list(_words(batch, info.small, info.n_small, 16))
+    out = []
+    for i in words[info.first_large:info.first_large + info.n_large]:
+        assert i == len(out)
         while True:
-            out.append(words[at + 16 * end:at + 16 * end + 16])
-            end += 1
+            at = info.large + 16 * len(out)
+            out.append(words[at:at + 16])
             if out[-1][10]:
                 break
     return out
 
 
-def _random_batch(seed):
+def _random_batch(seed, many=False):
     rng = random.Random(seed)
-    size, kv_heads = rng.choice([32, 64, 256]), rng.choice([1, 2, 4])
+    size, kv_heads = rng.choice([32, 64, 256]), rng.choice([16, 32] if many else [1, 2, 4])
     g = rng.choice([1, 2, 7, 40])
     seqs = rng.choice([1, 3, 17])
     kind = rng.choice(["full", "causal", "d2f_hybrid"])
     rows, keys, pos0, prompt = [], [], [], []
-    for _ in range(seqs):
+    for s in range(seqs):
         n = rng.choice([0, 1, 9, 32, 200])
         k = rng.choice([0, 1, 31, 32, 33, rng.randint(1, 3000)])
+        if many and s % 2 == 0:  # enough of them for the large kernel
+            n, k = rng.randint(2000, 5000) // g * g // 2 + 300, rng.choice([0, 40, 20000, 70000])
         rows.append(n)
         keys.append(k)
         pos0.append(max(0, k - n) if rng.random() < 0.7 else rng.randint(0, 4000))
@@ -63,9 +72,10 @@ def _random_batch(seed):
     return cache, batch, table, rows, keys, pos0, kind, prompt, block, g
 
 
-@pytest.mark.parametrize("seed", range(40))
-def test_parts_cover_every_row_and_key_once(seed):
-    cache, batch, table, rows, keys, pos0, kind, prompt, block, g = _random_batch(seed)
+@pytest.mark.parametrize("seed, many", [(i, False) for i in range(40)] +
+                         [(i, True) for i in range(100, 130)])
+def test_parts_cover_every_row_and_key_once(seed, many):
+    cache, batch, table, rows, keys, pos0, kind, prompt, block, g = _random_batch(seed, many)
     info, tpp = batch.info, cache.page_size // 32
     row0 = np.concatenate([[0], np.cumsum(rows)])
     assert batch.rows == sum(rows) == info.rows
@@ -73,9 +83,8 @@ def test_parts_cover_every_row_and_key_once(seed):
     joins = _words(batch, info.joins, info.n_joins, 8)
     seen = {}   # (sequence, query vector / 32) -> tile ranges
     slots = set()
-    for large, (at, first, n) in enumerate(((info.small, info.first_small, info.n_small),
-                                            (info.large, info.first_large, info.n_large))):
-        for p in _pieces(batch, at, first, n):
+    for large in (0, 1):
+        for p in _pieces(batch, large):
             r0, nr, p0, nk, pl, vec0, t0, t1, slot, tab = (int(x) for x in p[:10])
             s = [i for i in range(len(rows)) if row0[i] == r0 and rows[i] == nr and rows[i]][0]
             assert (p0, nk) == (pos0[s], keys[s])
@@ -93,6 +102,7 @@ def test_parts_cover_every_row_and_key_once(seed):
                     assert slot + sub < info.slots and slot + sub not in slots
                     slots.add(slot + sub)
     assert len(slots) == info.slots
+    LARGE.add((many, info.n_large > 0, info.n_large > 0 and info.slots > 0))
     joined = {}
     for r0, vec0, vecs, slot, step, parts, *_ in joins:
         joined[(int(r0), int(vec0))] = (int(vecs), [int(slot) + i * int(step) for i in range(parts)])
@@ -113,6 +123,11 @@ def test_parts_cover_every_row_and_key_once(seed):
                 assert vecs == min(32, n * g - 32 * u)
                 assert sorted(x[2] for x in parts) == sorted(where)
     assert not seen and not joined
+
+
+def test_both_kernels_and_both_cuts_were_planned():
+    if len(LARGE) > 1:  # (run with the tests above)
+        assert {(False, False, False), (True, True, False), (True, True, True)} <= LARGE
 
 
 @pytest.mark.parametrize("seed", range(40, 70))
@@ -163,6 +178,10 @@ def test_rows_of_two_sequences_in_one_tile_are_not_appendable():
     (dict(pages=[[1]], keys=[3], rows=[1], positions=[2**31 - 1]), "32 bits"),
     (dict(pages=[[1]], keys=[3], rows=[1], heads=3), "multiple"),
     (dict(pages=[[1]], keys=[3], rows=[1], heads=0), "multiple"),
+    (dict(pages=[[1]], keys=[3], rows=[1], heads=4.0), "whole number"),
+    (dict(pages=[[1]], keys=[3], rows=[1], heads=2**40), "whole number"),
+    (dict(pages=[[1]], keys=[3], rows=[1], kind="d2f_hybrid", mask_geometry=(0,)), "geometry"),
+    (dict(pages=[[1]], keys=[3], rows=[1], kind="d2f_hybrid", mask_geometry=(0, 2**40)), "geometry"),
     (dict(pages=[[1]], keys=[3], rows=[1], kind="window"), "mask kind"),
     (dict(pages=[[1]], keys=[3], rows=[1], mask_geometry=(0, 32)), "geometry"),
     (dict(pages=[[1]], keys=[3], rows=[1], kind="d2f_hybrid"), "geometry"),
