@@ -76,7 +76,8 @@ inline std::string paged_check(const PagedBatchArgs& a) {
   if (a.page_size < 32 || (a.page_size & (a.page_size - 1))) return "page_size must be a power of two from 32 on";
   if (a.seqs < 1 || a.width < 0 || !a.rows || !a.keys || !a.pos0 || (a.width && !a.table))
     return "a batch has a sequence at least, and rows, keys and positions of each";
-  if (a.hkv < 1 || a.hq < 1 || a.hq % a.hkv) return "query heads must be a multiple of the K/V heads";
+  if (a.hkv < 1 || a.hq < 1 || a.hq % a.hkv || a.hq > 16384)
+    return "query heads must be a multiple of the K/V heads, 16384 at most";
   if (a.pages < 1 || (int64_t)a.pages * a.hkv * (a.page_size / 32) > INT32_MAX)
     return "a layer has at most 2^31 - 1 tiles of 32 keys and one head";
   if (a.masked && a.block < 1) return "bad mask geometry";

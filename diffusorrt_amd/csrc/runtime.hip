@@ -2960,10 +2960,16 @@ int32_t drt_op_sparse_attention(const void* q, int32_t q_dtype, const void* cach
 
 }  // extern "C"
 
+// (a message is made where it is needed only: a short call is mostly host time)
+#define DRT_REQUIRE(ok, message)                     \
+  do {                                               \
+    if (!(ok)) fail(INVALID_ARGUMENT, (message));    \
+  } while (0)
+
 namespace {
 
 int elem_type(int32_t dtype, const char* what) {
-  require(dtype == DRT_F32 || dtype == DRT_F16 || dtype == DRT_BF16,
+  DRT_REQUIRE(dtype == DRT_F32 || dtype == DRT_F16 || dtype == DRT_BF16,
           std::string(what) + " takes F32, F16 or BF16");
   return dtype == DRT_F32 ? 0 : dtype == DRT_F16 ? 1 : 2;
 }
@@ -2971,7 +2977,7 @@ int elem_type(int32_t dtype, const char* what) {
 RotaryTurns turns_of(const drt_rotary* r, int hd, const char* what) {
   RotaryTurns t;
   if (!r) return t;
-  require(r->freq && ((uintptr_t)r->freq & 7) == 0 && r->dim >= 2 && r->dim % 2 == 0 && r->dim <= hd,
+  DRT_REQUIRE(r->freq && ((uintptr_t)r->freq & 7) == 0 && r->dim >= 2 && r->dim % 2 == 0 && r->dim <= hd,
           std::string(what) + ": bad rotary (dim is even and no more than the head's elements)");
   t.freq = (const uint64_t*)r->freq;
   t.magnitude = r->magnitude;
@@ -2982,11 +2988,10 @@ RotaryTurns turns_of(const drt_rotary* r, int hd, const char* what) {
 
 void require_batch(const drt_paged_batch* b, const int32_t* list, const void* cache, int32_t kv_dtype,
                    const char* what) {
-  const std::string op(what);
-  require(b && list && b->rows > 0 && b->words > 0 && ((uintptr_t)list & 15) == 0,
-          op + " needs a planned batch and its list, 16-byte aligned, on the device");
-  require(cache && ((uintptr_t)cache & 15) == 0, op + " cache must be 16-byte aligned");
-  require(kv_dtype == DRT_F16 || kv_dtype == DRT_BF16, op + " cache must be F16 or BF16");
+  DRT_REQUIRE(b && list && b->rows > 0 && b->words > 0 && ((uintptr_t)list & 15) == 0,
+          std::string(what) + " needs a planned batch and its list, 16-byte aligned, on the device");
+  DRT_REQUIRE(cache && ((uintptr_t)cache & 15) == 0, std::string(what) + " cache must be 16-byte aligned");
+  DRT_REQUIRE(kv_dtype == DRT_F16 || kv_dtype == DRT_BF16, std::string(what) + " cache must be F16 or BF16");
 }
 
 }  // namespace
@@ -2998,11 +3003,11 @@ int32_t drt_op_rotate(const void* x, int64_t x_row_stride, int64_t x_head_stride
                       const int32_t* positions, int32_t pos0, int32_t inverse, void* y,
                       int64_t y_row_stride, int64_t y_head_stride, void* stream) {
   return guarded([&] {
-    require(x && y && rows > 0 && heads > 0 && hd > 0 && rotary, "bad rotate arguments");
+    DRT_REQUIRE(x && y && rows > 0 && heads > 0 && hd > 0 && rotary, "bad rotate arguments");
     RotateCall r{};
     r.type = elem_type(dtype, "rotate");
     const uintptr_t align = r.type == 0 ? 3 : 1;
-    require((((uintptr_t)x | (uintptr_t)y) & align) == 0 && ((uintptr_t)positions & 3) == 0,
+    DRT_REQUIRE((((uintptr_t)x | (uintptr_t)y) & align) == 0 && ((uintptr_t)positions & 3) == 0,
             "rotate: unaligned tensors");
     r.rotary = turns_of(rotary, hd, "rotate");
     r.x = x;
@@ -3027,8 +3032,8 @@ int32_t drt_paged_plan(const int32_t* table, int32_t width, int32_t seqs, const 
                        int32_t mask_block_size, int32_t* list, int64_t list_words,
                        drt_paged_batch* batch) {
   return guarded([&] {
-    require(batch, "paged_plan needs a batch to fill in");
-    require(mask_kind == DRT_MASK_BIDIRECTIONAL || mask_kind == DRT_MASK_D2F_HYBRID,
+    DRT_REQUIRE(batch, "paged_plan needs a batch to fill in");
+    DRT_REQUIRE(mask_kind == DRT_MASK_BIDIRECTIONAL || mask_kind == DRT_MASK_D2F_HYBRID,
             "paged_plan mask kind must be bidirectional or d2f_hybrid");
     PagedBatchArgs a;
     a.seqs = seqs;
@@ -3045,10 +3050,10 @@ int32_t drt_paged_plan(const int32_t* table, int32_t width, int32_t seqs, const 
     a.masked = mask_kind == DRT_MASK_D2F_HYBRID;
     a.block = mask_block_size;
     const std::string wrong = paged_check(a);
-    require(wrong.empty(), wrong);
+    DRT_REQUIRE(wrong.empty(), wrong);
     static thread_local std::vector<int32_t> words;
     const PagedPlanInfo p = paged_plan(a, words);
-    require((int64_t)std::max({p.n_small, p.n_large, p.n_joins, p.n_tiles}) * hkv <= INT32_MAX,
+    DRT_REQUIRE((int64_t)std::max({p.n_small, p.n_large, p.n_joins, p.n_tiles}) * hkv <= INT32_MAX,
             "too many rows for one batch");
     *batch = drt_paged_batch{};
     batch->rows = p.rows;
@@ -3084,16 +3089,16 @@ int32_t drt_op_paged_append(const drt_paged_batch* batch, const int32_t* list, c
                             void* stream) {
   return guarded([&] {
     require_batch(batch, list, cache, kv_dtype, "paged_append");
-    require(k && v && (!q || q_out), "bad paged_append arguments");
-    require(batch->appendable,
+    DRT_REQUIRE(k && v && (!q || q_out), "bad paged_append arguments");
+    DRT_REQUIRE(batch->appendable,
             "paged_append: a row lies behind its sequence's keys, or two sequences' in one tile");
     AppendCall c{};
     c.type = elem_type(src_dtype, "paged_append");
     const uintptr_t align = c.type == 0 ? 3 : 1;
-    require((((uintptr_t)k | (uintptr_t)v | (uintptr_t)q) & align) == 0 && ((uintptr_t)q_out & 15) == 0,
+    DRT_REQUIRE((((uintptr_t)k | (uintptr_t)v | (uintptr_t)q) & align) == 0 && ((uintptr_t)q_out & 15) == 0,
             "paged_append: unaligned tensors");
     c.rotary = turns_of(rotary, 128, "paged_append");
-    require(c.rotary.dim % 16 == 0, "paged_append: rotary dim must be a multiple of 16");
+    DRT_REQUIRE(c.rotary.dim % 16 == 0, "paged_append: rotary dim must be a multiple of 16");
     c.q = q;
     c.k = k;
     c.v = v;
@@ -3120,9 +3125,9 @@ int32_t drt_op_paged_load(const drt_paged_batch* batch, const int32_t* list, con
                           int32_t kv_dtype, void* k, void* v, void* stream) {
   return guarded([&] {
     require_batch(batch, list, cache, kv_dtype, "paged_load");
-    require(k && v && (((uintptr_t)k | (uintptr_t)v) & 15) == 0,
+    DRT_REQUIRE(k && v && (((uintptr_t)k | (uintptr_t)v) & 15) == 0,
             "paged_load k, v must be 16-byte aligned");
-    require(batch->appendable,
+    DRT_REQUIRE(batch->appendable,
             "paged_load: a row lies behind its sequence's keys, or two sequences' in one tile");
     paged_load(list + batch->tiles, batch->n_tiles, cache, batch->hkv, batch->page_size / 32, k, v,
                as_stream(stream));
@@ -3138,10 +3143,10 @@ int32_t drt_op_paged_attention(const drt_paged_batch* batch, const int32_t* list
                                void* workspace, size_t workspace_bytes, void* stream) {
   return guarded([&] {
     require_batch(batch, list, cache, kv_dtype, "paged_attention");
-    require(q && out && ((uintptr_t)q & 15) == 0, "paged_attention q must be 16-byte aligned");
+    DRT_REQUIRE(q && out && ((uintptr_t)q & 15) == 0, "paged_attention q must be 16-byte aligned");
     require_out(out, out_dtype, "paged_attention");
     const size_t need = drt_op_paged_attention_workspace_bytes(batch);
-    require(workspace_bytes >= need && (workspace || !need) && ((uintptr_t)workspace & 15) == 0,
+    DRT_REQUIRE(workspace_bytes >= need && (workspace || !need) && ((uintptr_t)workspace & 15) == 0,
             "paged_attention workspace too small or not 16-byte aligned");
     PagedAttnCall c{};
     c.q = q;

@@ -24,6 +24,8 @@ def _whole_numbers(values, what):
     if isinstance(values, torch.Tensor):
         if values.is_cuda:
             raise ValueError(f"{what} must be on the host")
+        if values.is_floating_point() or values.is_complex() or values.dtype is torch.bool:
+            raise ValueError(f"{what} must be whole numbers")
         values = values.numpy()
     a = np.asarray(values)
     if a.size == 0:
@@ -54,7 +56,9 @@ def _table(pages):
 class PagedBatch:
     """New rows of several sequences, as :meth:`PagedKVCache.batch` plans them: made once a step,
     it serves ``append``, ``attention`` and ``load`` of every layer, on any stream. Keep it as long
-    as a captured graph that used it is replayed."""
+    as a captured graph that used it is replayed. How an attention is cut among the work-groups
+    follows from all of the batch's lengths: a row's result is the same from call to call, and may
+    differ in its last bits beside other sequences."""
 
     def __init__(self, cache, table, keys, rows, heads, positions, kind, mask_geometry):
         if cache._index >= 0 and torch.cuda.is_current_stream_capturing():
@@ -203,20 +207,17 @@ class PagedKVCache:
             raise ValueError(f"layer must be in [0, {self.layers})")
         if self._index < 0:
             raise ValueError("the cache must be on a GPU")
-        if not isinstance(batch, PagedBatch) or batch._geometry != self._geometry:
+        if not isinstance(batch, PagedBatch) or (batch._geometry is not self._geometry and
+                                                 batch._geometry != self._geometry):
             raise ValueError("the batch was planned for another cache")
         if self._lib is None:
             self._lib = _lib.load()
         return self._lib
 
-    def _source(self, t, shape, what):
-        """A source's strides between rows and heads."""
+    def _bad_source(self, what, t, shape):
         if t.shape != shape or t.get_device() != self._index:
             raise ValueError(f"{what} must be {list(shape)} on the cache's device")
-        rows, heads, one = t.stride()
-        if one != 1:
-            raise ValueError(f"{what}: a head's elements must be side by side")
-        return rows, heads
+        raise ValueError(f"{what}: a head's elements must be side by side")
 
     def append(self, layer: int, k, v, batch: PagedBatch, *, rotary=None, q=None):
         """Write the batch's ``k, v [rows, kv_heads, 128]`` (fp32, fp16 or bf16, views of a fused
@@ -228,15 +229,20 @@ class PagedKVCache:
         once. Raises ValueError where two sequences of the batch have rows in one tile of a page,
         or a row lies behind its sequence's keys."""
         lib = self._entry(layer, batch)
-        k0, k1 = self._source(k, batch._kv_shape, "append's k")
-        v0, v1 = self._source(v, batch._kv_shape, "append's v")
+        index, shape = self._index, batch._kv_shape
+        if k.shape != shape or k.get_device() != index or k.stride(2) != 1:
+            self._bad_source("append's k", k, shape)
+        if v.shape != shape or v.get_device() != index or v.stride(2) != 1:
+            self._bad_source("append's v", v, shape)
+        k0, k1, _ = k.stride()
+        v0, v1, _ = v.stride()
         dtype = k.dtype
         code = _TYPES.get(dtype)
         if code is None or v.dtype is not dtype:
             raise ValueError("append takes k, v and q of one type: float32, float16 or bfloat16")
         turns = None
         if rotary is not None:
-            if rotary.dim > 128 or rotary.dim % 16 or rotary._index != self._index:
+            if rotary.dim > 128 or rotary.dim % 16 or rotary._index != index:
                 raise ValueError("append's rotary must turn a multiple of 16 elements, 128 at "
                                  "most, on the cache's device")
             turns = rotary._address
@@ -244,13 +250,16 @@ class PagedKVCache:
             out = q_at = out_at = None
             q0 = q1 = 0
         else:
-            q0, q1 = self._source(q, batch._q_shape, "append's q")
+            shape = batch._q_shape
+            if q.shape != shape or q.get_device() != index or q.stride(2) != 1:
+                self._bad_source("append's q", q, shape)
+            q0, q1, _ = q.stride()
             if q.dtype is not dtype:
                 raise ValueError("append takes k, v and q of one type: float32, float16 or "
                                  "bfloat16")
-            out = q.new_empty(batch._q_shape, dtype=self.dtype)
+            out = q.new_empty(shape, dtype=self.dtype)
             q_at, out_at = q.data_ptr(), out.data_ptr()
-        _launch(torch, lib.drt_op_paged_append, self._index, batch._address, batch._here(),
+        _launch(torch, lib.drt_op_paged_append, index, batch._address, batch._here(),
                 k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, q_at, q0, q1, code, turns,
                 self._data + layer * self._layer_bytes, self.kv_dtype, out_at)
         return out

@@ -154,7 +154,8 @@ class RotaryPositions:
         """``x [rows, heads, head_dim]`` (fp32, fp16 or bf16; any strides between rows and heads)
         with row r turned by ``positions[r]`` (int32 on the device, or a number: the first row's,
         the others one further each); elements from ``dim`` on as they are. ``inverse`` turns the
-        other way, which is also the rotation's gradient: that of ``x`` from that of the result.
+        other way, by the same magnitude, which is the rotation's gradient: that of ``x`` from that
+        of the result (and takes a rotation of magnitude 1 back).
 
         ``out``: a tensor of x's shape and type, ``x`` itself or memory apart from it. Computed in
         fp32, rounded once."""

@@ -395,3 +395,37 @@ def test_refusals():
         with pytest.raises(ValueError, match="tile"):
             c.load(0, batch)
         assert torch.isfinite(c.attention(0, q, batch)).all()
+
+
+# ---------------------------------------------------------------- every key once
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("mask, geometry", [("full", None), ("causal", None), ("d2f_hybrid", (70, 32))])
+@pytest.mark.parametrize("keys, rows, g, hkv", [
+    ([1, 31, 33, 500, 4100], [1, 9, 1, 100, 1], 2, 2), ([70000], [1], 2, 2), ([20000, 64], [40, 64], 7, 1),
+    ([3000], [300], 2, 16),
+    ([8200, 77], [1024, 5], 2, 16),   # the kernel of many rows, whole units
+    ([16384], [600], 2, 16)])         # ... and equal shares
+def test_every_key_counts_once(keys, rows, g, hkv, kind, mask, geometry):
+    """Queries of zero weigh all keys alike, exactly: with values that are small whole numbers the result is
+    their sum, exact in 32 bits, over their number. A key left out, read twice or seen by a row that does
+    not see it moves some of the 128 sums by a whole number."""
+    table, pages = _tables(1, keys, 64)
+    cache = PagedKVCache(1, hkv, pages, page_size=64, dtype=kind)
+    cache.data.fill_(float("nan"))
+    total, dtype = sum(keys), TYPES[kind]
+    gen = torch.Generator(device="cuda").manual_seed(total)
+    v = torch.randint(-3, 4, (total, hkv, 128), generator=gen, device="cuda")
+    k = torch.randn((total, hkv, 128), generator=gen, device="cuda").to(dtype)
+    cache.append(0, k, v.to(dtype), cache.batch(table, keys, keys, heads=hkv))
+    batch = cache.batch(table, keys, rows, heads=g * hkv, kind=mask, mask_geometry=geometry)
+    q = torch.zeros(sum(rows), g * hkv, 128, dtype=dtype, device="cuda")
+    out = cache.attention(0, q, batch).view(-1, g * hkv, 128).double()
+    r0 = k0 = 0
+    for n, r in zip(keys, rows):
+        ends = torch.tensor(P.key_ends(mask, n - r, r, n, *(geometry or (0, 1))), device="cuda")
+        sums = v[k0:k0 + n].cumsum(0)[ends - 1].repeat_interleave(g, 1).double()
+        want = sums / ends[:, None, None]
+        # one division (and its reciprocal) and, in parts, a product with a power of two
+        assert ((out[r0:r0 + r] - want).abs() <= 2.0**-22 * want.abs()).all()
+        r0, k0 = r0 + r, k0 + n

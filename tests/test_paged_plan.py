@@ -6,6 +6,7 @@ import random
 
 import numpy as np
 import pytest
+import torch
 
 from diffusorrt_amd import _lib
 from diffusorrt_amd.paged import PagedKVCache
@@ -178,7 +179,12 @@ def test_rows_of_two_sequences_in_one_tile_are_not_appendable():
     (dict(pages=[[1]], keys=[3], rows=[1], positions=[2**31 - 1]), "32 bits"),
     (dict(pages=[[1]], keys=[3], rows=[1], heads=3), "multiple"),
     (dict(pages=[[1]], keys=[3], rows=[1], heads=0), "multiple"),
+    (dict(pages=[[1]], keys=[3], rows=[1], heads=16386), "16384"),
     (dict(pages=[[1]], keys=[3], rows=[1], heads=4.0), "whole number"),
+    (dict(pages=torch.ones(1, 1, dtype=torch.bfloat16), keys=[3], rows=[1]), "whole numbers"),
+    (dict(pages=[[1]], keys=torch.ones(1), rows=[1]), "whole numbers"),
+    (dict(pages=[1], keys=[3], rows=[1]), "list of page numbers"),
+    (dict(pages=np.ones(3, dtype=np.int32), keys=[3], rows=[1]), "sequences, width"),
     (dict(pages=[[1]], keys=[3], rows=[1], heads=2**40), "whole number"),
     (dict(pages=[[1]], keys=[3], rows=[1], kind="d2f_hybrid", mask_geometry=(0,)), "geometry"),
     (dict(pages=[[1]], keys=[3], rows=[1], kind="d2f_hybrid", mask_geometry=(0, 2**40)), "geometry"),
