@@ -34,7 +34,7 @@ def _whole_numbers(values, what):
         raise ValueError(f"{what} must be whole numbers")
     if a.size and (a.min() < -1 or a.max() > _I32_MAX):
         raise ValueError(f"{what} must be whole numbers of 32 bits")
-    return np.ascontiguousarray(a, dtype=np.int32)
+    return np.asarray(a, dtype=np.int32, order="C")
 
 
 def _table(pages):
