@@ -3,9 +3,9 @@
 // Query vectors of one K/V head are flattened (row, head of the group) within a sequence and taken in
 // units; keys come in the pages' 32-key tiles. A wave computes S^T = K Q^T and O^T += V^T P^T as 32x32x16
 // products with a running base and sum per query vector: p = 2^(s c - base), c = log2(e) / sqrt(128),
-// o = sum p v / sum p. The base is raised when a tile's largest exponent exceeds it by more than 8
-// (any base gives the same quotient; p <= 2^8). p's rounding to the products' 16-bit type is the one
-// rounding ahead of the sums; scores, base, sum and O are fp32.
+// o = sum p v / sum p. The base is raised when a tile's largest exponent has gone more than 8 over what it
+// was raised by last; any base gives the same quotient (PA_LIFT: which). p's rounding to the products'
+// 16-bit type is the one rounding ahead of the sums; scores, base, sum and O are fp32.
 //
 // A list made on the host (paged_plan.h) gives every work-group its unit and its share of the keys, so
 // sequences of any lengths fill the chip: nothing is padded to the longest, and a sequence alone is cut
@@ -21,6 +21,12 @@ using drt::PagedPiece;
 
 constexpr int PA_TILE = 16384;  // bytes
 constexpr int PA_QROW = 136;    // 16-bit elements per query vector in LDS (+ 16 bytes)
+
+// The largest exponent less the base, where it is raised. fp16 weights are 2^7 then and 2^15 at most, which
+// keeps those of down to 2^-21 of the largest normal numbers (many small ones add up over a long sequence).
+// bf16 ones, which have the exponents, are 2^-24 and 2^-16 at most: thousands of keys whose values are the
+// type's largest do not overflow the sum ahead of its division.
+template <int CT> constexpr float PA_LIFT = CT == 1 ? 7.f : -24.f;
 
 struct PaArgs {
   const uint16_t* q;    // [rows][hq][128]
@@ -212,14 +218,15 @@ __global__ __launch_bounds__(64 * PS_WAVES, 2) void paged_attn_kernel(const PaAr
 #pragma unroll
     for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, s[r]);
     const float u = ca_max_xor32(tmax) * x.c;  // -inf: no visible key
-    const bool up = u > m_run + CA_RESCALE_LOG2;
+    const bool up = u - m_run > PA_LIFT<CT> + CA_RESCALE_LOG2;  // (exact where it matters)
     if (__ballot(up)) {
-      const float alpha = up ? __builtin_amdgcn_exp2f(m_run - u) : 1.f;  // 0 from -inf
+      const float to = up ? u - PA_LIFT<CT> : m_run;
+      const float alpha = up ? __builtin_amdgcn_exp2f(m_run - to) : 1.f;  // 0 from -inf
 #pragma unroll
       for (int hb = 0; hb < 4; ++hb) o[hb] *= alpha;
       l_run *= alpha;
-      m_run = up ? u : m_run;
-      base = up ? u : base;
+      m_run = to;
+      base = up ? to : base;
       scale = __ballot(fabsf(base) > CA_LARGE) ? 1.f : x.c;
     }
     if (scale == 1.f) {
@@ -368,17 +375,18 @@ __device__ __forceinline__ void pa_large(const PaArgs& x) {
 #pragma unroll
       for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, s[j][r]);
       u[j] = ca_max_xor32(tmax) * x.c;  // -inf: no visible key
-      up[j] = u[j] > m_run[j] + CA_RESCALE_LOG2;
+      up[j] = u[j] - m_run[j] > PA_LIFT<CT> + CA_RESCALE_LOG2;
     }
     if (__ballot(up[0] || up[1])) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float alpha = up[j] ? __builtin_amdgcn_exp2f(m_run[j] - u[j]) : 1.f;  // 0 from -inf
+        const float to = up[j] ? u[j] - PA_LIFT<CT> : m_run[j];
+        const float alpha = up[j] ? __builtin_amdgcn_exp2f(m_run[j] - to) : 1.f;  // 0 from -inf
 #pragma unroll
         for (int hb = 0; hb < 4; ++hb) o[j][hb] *= alpha;
         l_run[j] *= alpha;
-        m_run[j] = up[j] ? u[j] : m_run[j];
-        base[j] = up[j] ? u[j] : base[j];
+        m_run[j] = to;
+        base[j] = up[j] ? to : base[j];
       }
       scale = __ballot(fmaxf(fabsf(base[0]), fabsf(base[1])) > CA_LARGE) ? 1.f : x.c;
     }

@@ -3053,7 +3053,9 @@ int32_t drt_paged_plan(const int32_t* table, int32_t width, int32_t seqs, const 
     DRT_REQUIRE(wrong.empty(), wrong);
     static thread_local std::vector<int32_t> words;
     const PagedPlanInfo p = paged_plan(a, words);
-    DRT_REQUIRE((int64_t)std::max({p.n_small, p.n_large, p.n_joins, p.n_tiles}) * hkv <= INT32_MAX,
+    // (a launch has fewer than 2^32 threads)
+    DRT_REQUIRE((int64_t)std::max(p.n_small, p.n_large) * hkv <= UINT32_MAX / 512 &&
+                    std::max((int64_t)p.n_joins * hkv, (int64_t)p.n_tiles) <= UINT32_MAX / 256,
             "too many rows for one batch");
     *batch = drt_paged_batch{};
     batch->rows = p.rows;

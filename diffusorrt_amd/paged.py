@@ -265,7 +265,8 @@ class PagedKVCache:
         return out
 
     def load(self, layer: int, batch: PagedBatch):
-        """``(k, v) [rows, kv_heads, 128]`` of the batch's rows as the cache holds them."""
+        """``(k, v) [rows, kv_heads, 128]`` of the batch's rows as the cache holds them. Raises
+        ValueError where :meth:`append` of the batch does."""
         lib = self._entry(layer, batch)
         k = self.data.new_empty(batch._kv_shape)
         v = self.data.new_empty(batch._kv_shape)

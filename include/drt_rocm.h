@@ -409,7 +409,7 @@ int32_t drt_paged_plan(const int32_t* table, int32_t width, int32_t seqs, const 
                        drt_paged_batch* batch);
 /* The batch's k, v [rows, hkv, 128] (src_dtype DRT_F32, DRT_F16 or DRT_BF16; strides in elements) into
  * their places in one layer's cache (kv_dtype DRT_F16 or DRT_BF16), keys turned by their positions on
- * the way where rotary is given (dim <= 128, a multiple of 16). q [rows, hq, 128], where given, is turned
+ * the way where rotary is given (dim <= 128, a multiple of 16); an appendable batch's. q [rows, hq, 128], where given, is turned
  * alike into q_out [rows, hq, 128] of kv_dtype. list: the plan's, on the device. Other rows of a tile
  * stay as they are, so calls that write different rows may overlap in time. */
 int32_t drt_op_paged_append(const drt_paged_batch* batch, const int32_t* list, const void* k,
@@ -418,7 +418,7 @@ int32_t drt_op_paged_append(const drt_paged_batch* batch, const int32_t* list, c
                             int64_t q_row_stride, int64_t q_head_stride, int32_t src_dtype,
                             const drt_rotary* rotary, void* cache, int32_t kv_dtype, void* q_out,
                             void* stream);
-/* The batch's rows as the cache holds them: k, v [rows, hkv, 128] of kv_dtype. */
+/* The batch's rows as the cache holds them: k, v [rows, hkv, 128] of kv_dtype (an appendable batch's). */
 int32_t drt_op_paged_load(const drt_paged_batch* batch, const int32_t* list, const void* cache,
                           int32_t kv_dtype, void* k, void* v, void* stream);
 /* Attention of q [rows, hq, 128] of kv_dtype over the batch's keys: out [rows, hq * 128] of out_dtype

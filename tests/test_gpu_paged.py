@@ -237,6 +237,36 @@ def test_values_that_are_not_finite_where_a_row_does_not_see_them(kind, what, ro
         assert (got[below:, 2:, 9] == what).all()
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_many_small_weights_add_up(rows):
+    # One key of each of the first eight tiles scores a^2 128 / sqrt(128) = 15.125, the others 0, so each of
+    # those weighs 2^-21.8 of it; their values are 1 and the others' 0. A weight of 2^7 2^-21.8 is off by
+    # 2^-25 at most in fp16, 2^-10.2 of itself, the largest by 2^-11, both by their scores' sums (130
+    # roundings of 15.125 in fp32, 2^-12.9) and the power (2^-18).
+    a = 1.15625
+    s = Sequences([1024], [rows], kind="f16", mask="full", hkv=2, g=1)
+    s.q.fill_(a)
+    s.k.zero_()
+    s.v.fill_(1.0)
+    s.k[:256:32] = a
+    s.v[:256:32] = 0.0
+    s.fill()
+    got = _np(s.cache.attention(0, s.q, s.batch))
+    w = 1016 * np.exp(-a * a * 128**0.5)
+    assert np.abs(got / (w / (8 + w)) - 1).max() < 2**-10.2 + 2**-11 + 2 * 2**-12.9 + 2**-17
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_values_near_the_types_largest(rows):
+    # bf16: sums ahead of the division stay finite; q of zeros, so every weight is the same
+    s = Sequences([500, 3], [rows, 1], kind="bf16", mask="full")
+    s.q.zero_()
+    s.v[..., 9] = 3e38
+    s.v[..., 10] = -3e38
+    s.fill()
+    s.check()
+
+
 def test_places_beyond_4_gib():
     # the last pages of a layer of 5.4 GB, and of the second layer
     cache = PagedKVCache(2, 8, 20480, page_size=64, dtype="bf16")

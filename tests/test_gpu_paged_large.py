@@ -183,3 +183,31 @@ def test_graph_and_other_streams():
         got = out.clone()
         assert torch.equal(got, b.cache.attention(0, b.q, b.batch))
         torch.cuda.synchronize()
+
+
+def test_many_small_weights_add_up():
+    # one key of each of the first two tiles scores 15.125, the others 0 and weigh 2^-21.8 of it each: the
+    # bound of a row's result, whose values are 1 there and 0 at the two, is that of fp16 weights of 2^7
+    # times as much (off by 2^-10.2 of themselves at most, the largest by 2^-11, both by their scores' sums
+    # of 130 fp32 roundings of 15.125, 2^-12.9, and the power, 2^-18)
+    a = 1.15625
+    b = Batch([4096], [2048], g=2, hkv=16, kind="f16", mask="full")
+    assert b.batch.info.n_large > 0 and not b.batch.info.slots
+    b.q.fill_(a)
+    b.k.zero_()
+    b.v.fill_(1.0)
+    b.k[:64:32] = a
+    b.v[:64:32] = 0.0
+    b.fill()
+    got = b.cache.attention(0, b.q, b.batch).double()
+    w = 4094 * np.exp(-a * a * 128**0.5)
+    assert (got / (w / (2 + w)) - 1).abs().max() < 2**-10.2 + 2**-11 + 2 * 2**-12.9 + 2**-17
+
+
+def test_values_near_the_types_largest():
+    b = Batch([4096], [2048], g=2, hkv=16, mask="full", kind="bf16")
+    b.q.zero_()
+    b.v[..., 9] = 3e38
+    b.v[..., 10] = -3e38
+    b.fill()
+    b.check()

@@ -220,3 +220,12 @@ def test_caches_that_are_refused():
         cache.attention(0, None, batch)
     with pytest.raises(ValueError, match="layer"):
         cache.load(1, batch)
+
+
+def test_more_work_groups_than_a_launch_has_are_refused():
+    # 2^32 threads and more: 512 for each sequence's token and K/V head
+    n = 2**20
+    ones, pages = np.ones(n, dtype=np.int32), np.zeros((n, 1), dtype=np.int32)
+    with pytest.raises(ValueError, match="too many rows"):
+        _cache(kv_heads=8).batch(pages, ones, ones, heads=8)
+    assert _cache(kv_heads=4).batch(pages, ones, ones, heads=4).rows == n
