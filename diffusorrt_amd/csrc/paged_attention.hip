@@ -32,7 +32,7 @@ struct PaArgs {
   const uint16_t* q;    // [rows][hq][128]
   const uint8_t* cache; // this layer
   const PagedPiece* pieces;
-  const int32_t* first;  // a work-group's first piece
+  const int32_t* first;  // (large kernel) a work-group's first piece
   const int32_t* table;  // a page's first tile of head 0
   int hq, hkv, tpp, masked, block;
   float c;               // log2(e) / sqrt(128)
@@ -57,7 +57,7 @@ DRT_DEV PagedPiece pa_piece(const PagedPiece* pieces, int i) {
   y.slot = p[8];
   y.table = p[9];
   y.last = p[10];
-  y.wide_log2 = p[11];
+  y.wide = p[11];
   return y;
 }
 
@@ -128,44 +128,35 @@ DRT_DEV void pa_store8(const PaArgs& x, int64_t at, f32x4 y0, f32x4 y1) {
   }
 }
 
-// Units of 32 or 64 query vectors (`wide` waves of 32 side by side) and the other waves over keys: way
-// kw takes tiles kw, kw + ways, ... of the piece, straight from memory into registers. Waves of one way
-// load the same tiles at the same time, the second from the first's lines. The ways meet in LDS at the
-// end.
+// Units of 32 query vectors: eight waves over keys, wave kw takes tiles kw, kw + 8, ... of the piece,
+// straight from memory into registers. They meet in LDS at the end.
 constexpr int PS_WAVES = 8;
 template <int CT>
-__global__ __launch_bounds__(64 * PS_WAVES, 2) void paged_attn_kernel(const PaArgs x) {
+DRT_DEV void pa_few(const PaArgs& x, const PagedPiece& pc, uint16_t* q_lds, char* ring0, char* ring1, float2* ml) {
   typedef CacheT<CT> T;
   typedef typename T::vec vec;
   constexpr int PIECES = 32, WAVE_O = 32 * PIECES * 16;
-  __shared__ __align__(16) char smem[PS_WAVES * WAVE_O];
-  __shared__ float2 ml[PS_WAVES][32];
+  // (a wave's O, 16 KiB; four in each of the rings)
+  auto o_of = [&](int w) { return (f32x4*)((w < 4 ? ring0 : ring1) + (w & 3) * WAVE_O); };
   const int lane = threadIdx.x & 63, tid = threadIdx.x;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = (int)(blockIdx.x % (uint32_t)x.hkv), G = x.hq / x.hkv;
-  // (a work-group has one piece here)
-  const PagedPiece pc = pa_piece(x.pieces, (int)(blockIdx.x / (uint32_t)x.hkv));
-  const int wide = 1 << pc.wide_log2, ways = PS_WAVES >> pc.wide_log2;
-  const int kw = wave >> pc.wide_log2, qw = wave & (wide - 1);
-  const int vecs = min(32 * wide, pc.rows * G - pc.vec0);
+  const int vecs = min(32, pc.rows * G - pc.vec0);
   auto row_of = [&](int v) { return (int)((uint32_t)(pc.vec0 + v) / (uint32_t)G); };
   auto offset_of = [&](int v) {  // of query vector v's head in q and out
     const int row = row_of(v);
     return ((int64_t)(pc.row0 + row) * x.hq + kvh * G + (pc.vec0 + v - row * G)) * 128;
   };
 
-  // the queries (behind the last query vector it again: not used), 32 query vectors a round
-  u32x4 qraw[2];
-#pragma unroll
-  for (int it = 0; it < 2; ++it)
-    if (it < wide)
-      qraw[it] = *(const u32x4*)(x.q + offset_of(min(32 * it + (tid >> 4), vecs - 1)) + (tid & 15) * 8);
+  // the queries (behind the last query vector it again: not used)
+  const int v = tid >> 4, ch = tid & 15;
+  const u32x4 qraw = *(const u32x4*)(x.q + offset_of(min(v, vecs - 1)) + ch * 8);
 
   // this wave's tiles: lane l holds the tile number in the layer of its (64 i + l)-th
-  const int n = (pc.tile1 - pc.tile0 - kw + ways - 1) >> (3 - pc.wide_log2);
+  const int n = (pc.tile1 - pc.tile0 - kw + PS_WAVES - 1) / PS_WAVES;
   const int sh = __builtin_ctz(x.tpp);
   auto numbers = [&](int i) {
-    const int t = min(pc.tile0 + kw + ways * (i + lane), pc.tile1 - 1);
+    const int t = min(pc.tile0 + kw + PS_WAVES * (i + lane), pc.tile1 - 1);
     return x.table[pc.table + (t >> sh)] + kvh * x.tpp + (t & (x.tpp - 1));
   };
   int held = n > 0 ? numbers(0) : 0;
@@ -180,15 +171,12 @@ __global__ __launch_bounds__(64 * PS_WAVES, 2) void paged_attn_kernel(const PaAr
 #pragma unroll
     for (int i = 0; i < 8; ++i) vr[i] = *(const u32x4*)(p + PA_TILE / 2 + i * 1024);
   }
-  const int q_end[1] = {pa_key_end(x, pc, row_of(min(32 * qw + (lane & 31), vecs - 1)))};
-  // (ends never fall from row to row) keys that every row of the wave sees
-  const int full_end = pa_key_end(x, pc, row_of(min(32 * qw, vecs - 1)));
-#pragma unroll
-  for (int it = 0; it < 2; ++it)
-    if (it < wide)
-      *(u32x4*)(smem + ((32 * it + (tid >> 4)) * PA_QROW + (tid & 15) * 8) * 2) = qraw[it];
+  const int q_end[1] = {pa_key_end(x, pc, row_of(min(lane & 31, vecs - 1)))};
+  // (ends never fall from row to row) keys that every row of the unit sees
+  const int full_end = pa_key_end(x, pc, row_of(0));
+  *(u32x4*)(q_lds + v * PA_QROW + ch * 8) = qraw;
   ca_lds_barrier();
-  const uint16_t* ql = (const uint16_t*)smem + (32 * qw + (lane & 31)) * PA_QROW + 8 * (lane >> 5);
+  const uint16_t* ql = q_lds + (lane & 31) * PA_QROW + 8 * (lane >> 5);
   vec qr[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) qr[i] = *(const vec*)(ql + 16 * i);
@@ -200,7 +188,7 @@ __global__ __launch_bounds__(64 * PS_WAVES, 2) void paged_attn_kernel(const PaAr
 #pragma unroll
   for (int hb = 0; hb < 4; ++hb) o[hb] = f32x16{};
   for (int it = 0; it < n; ++it) {
-    const int key0 = (pc.tile0 + kw + ways * it) * 32;
+    const int key0 = (pc.tile0 + kw + PS_WAVES * it) * 32;
     const int next = min(it + 1, n - 1);  // (the last tile's own again: loaded, not used)
     if ((next & 63) == 0 && next) held = numbers(next);
     const uint8_t* p = tile_at(next);
@@ -252,65 +240,59 @@ __global__ __launch_bounds__(64 * PS_WAVES, 2) void paged_attn_kernel(const PaAr
 
   // The ways joined: every wave leaves its O in LDS as 16-byte pieces (query v, piece p at p ^ v: every
   // bank in turn both ways), then threads with eight head dims of a query vector add the ways'.
-  __syncthreads();  // the queries have been read
   {
-    f32x4* d = (f32x4*)(smem + wave * WAVE_O);
+    f32x4* d = o_of(kw);
 #pragma unroll
     for (int b = 0; b < 4; ++b)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         d[(lane & 31) * PIECES + ((b * 8 + 2 * r + (lane >> 5)) ^ (lane & 15))] =
             f32x4{o[b][4 * r], o[b][4 * r + 1], o[b][4 * r + 2], o[b][4 * r + 3]};
-    if (lane < 32) ml[wave][lane] = make_float2(m_run, l_run);
+    if (lane < 32) ml[kw * 32 + lane] = make_float2(m_run, l_run);
   }
   __syncthreads();
-  const int v = tid >> 4, ch = tid & 15;
-  for (int it = 0; it < wide; ++it) {
-    if (32 * it + v >= vecs) break;
-    float m = -INFINITY, l = 0.f;
-    for (int k = it; k < PS_WAVES; k += wide) m = fmaxf(m, ml[k][v].x);
-    f32x4 y0 = f32x4{}, y1 = f32x4{};
-#pragma unroll 2
-    for (int k = it; k < PS_WAVES; k += wide) {
-      const f32x4* d = (const f32x4*)(smem + k * WAVE_O) + v * PIECES;
-      const float2 w = ml[k][v];
-      const float f = w.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.x - m);
-      y0 += f * d[(2 * ch) ^ (v & 15)];
-      y1 += f * d[(2 * ch + 1) ^ (v & 15)];
-      l = fmaf(f, w.y, l);
-    }
-    if (pc.slot < 0) {
-      const float inv = pc.tile1 == 0 ? 0.f : 1.f / l;  // (no key: zeros)
-      pa_store8(x, offset_of(32 * it + v) + ch * 8, y0 * inv, y1 * inv);
-    } else {
-      const int64_t at = ((int64_t)(pc.slot + it) * x.hkv + kvh) * 32 + v;
-      *(f32x4*)(x.o_part + at * 128 + ch * 8) = y0;
-      *(f32x4*)(x.o_part + at * 128 + ch * 8 + 4) = y1;
-      if (ch == 0) *(float2*)(x.ml_part + at * 2) = make_float2(m, l);
-    }
+  if (v >= vecs) return;
+  float2 w[PS_WAVES];
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int k = 0; k < PS_WAVES; ++k) {
+    w[k] = ml[k * 32 + v];
+    m = fmaxf(m, w[k].x);
+  }
+  f32x4 y0 = f32x4{}, y1 = f32x4{};
+#pragma unroll
+  for (int k = 0; k < PS_WAVES; ++k) {
+    const f32x4* d = o_of(k) + v * PIECES;
+    const float f = w[k].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w[k].x - m);
+    y0 += f * d[(2 * ch) ^ (v & 15)];
+    y1 += f * d[(2 * ch + 1) ^ (v & 15)];
+    l = fmaf(f, w[k].y, l);
+  }
+  if (pc.slot < 0) {
+    const float inv = pc.tile1 == 0 ? 0.f : 1.f / l;  // (no key: zeros)
+    pa_store8(x, offset_of(v) + ch * 8, y0 * inv, y1 * inv);
+  } else {
+    const int64_t at = ((int64_t)pc.slot * x.hkv + kvh) * 32 + v;
+    *(f32x4*)(x.o_part + at * 128 + ch * 8) = y0;
+    *(f32x4*)(x.o_part + at * 128 + ch * 8 + 4) = y1;
+    if (ch == 0) *(float2*)(x.ml_part + at * 2) = make_float2(m, l);
   }
 }
 
-// Units of 256 query vectors: four waves of 64 (two tiles of 32, for both of which a tile's operands are
-// read once) for each of two key ways, which take turns at the tiles. Tiles come by direct-to-LDS
-// loads, the next while this is worked on, queries lie in LDS for all of it.
-constexpr int PL_HELD = 4;  // steps of 16 head dims whose queries are in registers
-constexpr int PL_Q = 256, PL_WAYS = 2;
-template <int CT>
-__device__ __forceinline__ void pa_large(const PaArgs& x) {
+// Units of many query vectors: QW waves side by side of QT tiles of 32 (for all of which a key tile's operands
+// are read once), for each of 8 / QW key ways, which take turns at the tiles. Tiles come by direct-to-LDS
+// loads, one for the waves of a way together, the next while this is worked on; queries lie in LDS for
+// all of it, some of them in registers.
+template <int CT, int QW, int QT>
+DRT_DEV void pa_shared(const PaArgs& x, const PagedPiece& pc, uint16_t* q_lds, char* ring0, char* ring1, float2* ml) {
   typedef CacheT<CT> T;
   typedef typename T::vec vec;
-  __shared__ __align__(16) uint16_t q_lds[PL_Q * PA_QROW];
-  // separate arrays: the compiler knows the slot being read is not one being filled
-  __shared__ __align__(1024) char ring0[PL_WAYS * PA_TILE];
-  __shared__ __align__(1024) char ring1[PL_WAYS * PA_TILE];
-  __shared__ float2 ml[PL_Q];
+  constexpr int WAYS = 8 / QW, VW = 32 * QT, NQ = QW * VW;  // query vectors of a wave, of the unit
+  constexpr int HELD = QT == 1 ? 8 : 4;  // steps of 16 head dims whose queries are in registers
   const int lane = threadIdx.x & 63, tid = threadIdx.x;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qw = wave & 3, way = wave >> 2;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qw = wave % QW, way = wave / QW;
   const int kvh = (int)(blockIdx.x % (uint32_t)x.hkv), G = x.hq / x.hkv;
-  for (int at = x.first[blockIdx.x / (uint32_t)x.hkv];; ++at) {
-  const PagedPiece pc = pa_piece(x.pieces, at);
-  const int vecs = min(PL_Q, pc.rows * G - pc.vec0);
+  const int vecs = min(NQ, pc.rows * G - pc.vec0);
   auto row_of = [&](int v) { return (int)((uint32_t)(pc.vec0 + v) / (uint32_t)G); };
   auto offset_of = [&](int v) {
     const int row = row_of(v);
@@ -318,68 +300,71 @@ __device__ __forceinline__ void pa_large(const PaArgs& x) {
   };
 
   // this key way's tiles
-  const int n_it = (pc.tile1 - pc.tile0 + PL_WAYS - 1) / PL_WAYS;       // of the work-group
-  const int n = (pc.tile1 - pc.tile0 - way + PL_WAYS - 1) / PL_WAYS;    // of the way
+  const int n_it = (pc.tile1 - pc.tile0 + WAYS - 1) / WAYS;       // of the work-group
+  const int n = (pc.tile1 - pc.tile0 - way + WAYS - 1) / WAYS;    // of the way
   const int sh = __builtin_ctz(x.tpp);
   auto numbers = [&](int i) {
-    const int t = min(pc.tile0 + way + PL_WAYS * (i + lane), pc.tile1 - 1);
+    const int t = min(pc.tile0 + way + WAYS * (i + lane), pc.tile1 - 1);
     return x.table[pc.table + (t >> sh)] + kvh * x.tpp + (t & (x.tpp - 1));
   };
   int held = n > 0 ? numbers(0) : 0;
-  auto issue = [&](int i, char* dst) {  // this wave's quarter of the way's tile i
+  auto issue = [&](int i, char* dst) {  // this wave's share of the way's tile i
     if (i >= n) return;
     if ((i & 63) == 0 && i) held = numbers(i);
     const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(
         (void*)(x.cache + (int64_t)__builtin_amdgcn_readlane(held, i & 63) * PA_TILE), 0, PA_TILE,
         0x00020000);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < 16 / QW; ++k)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          src, (__attribute__((address_space(3))) void*)(dst + way * PA_TILE + (qw * 4 + k) * 1024), 16,
-          (uint32_t)((qw * 4 + k) * 1024 + lane * 16), 0, 0, 0);
+          src, (__attribute__((address_space(3))) void*)(dst + way * PA_TILE + (qw * (16 / QW) + k) * 1024), 16,
+          (uint32_t)((qw * (16 / QW) + k) * 1024 + lane * 16), 0, 0, 0);
   };
   issue(0, ring0);
-  u32x4 qraw[8];  // (behind the last query vector it again: not used)
+  u32x4 qraw[NQ / 32];  // (behind the last query vector it again: not used)
 #pragma unroll
-  for (int it = 0; it < 8; ++it)
+  for (int it = 0; it < NQ / 32; ++it)
     qraw[it] = *(const u32x4*)(x.q + offset_of(min((it * 512 + tid) >> 4, vecs - 1)) + (tid & 15) * 8);
 #pragma unroll
-  for (int it = 0; it < 8; ++it)
+  for (int it = 0; it < NQ / 32; ++it)
     *(u32x4*)(q_lds + ((it * 512 + tid) >> 4) * PA_QROW + (tid & 15) * 8) = qraw[it];
-  const uint16_t* ql = q_lds + (qw * 64 + (lane & 31)) * PA_QROW + 8 * (lane >> 5);
-  int q_end[2];
+  const uint16_t* ql = q_lds + (qw * VW + (lane & 31)) * PA_QROW + 8 * (lane >> 5);
+  int q_end[QT];
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
-    q_end[j] = pa_key_end(x, pc, row_of(min(qw * 64 + 32 * j + (lane & 31), vecs - 1)));
+  for (int j = 0; j < QT; ++j)
+    q_end[j] = pa_key_end(x, pc, row_of(min(qw * VW + 32 * j + (lane & 31), vecs - 1)));
   // (ends never fall from row to row) keys that every row of the wave sees, and any of them
-  const int full_end = pa_key_end(x, pc, row_of(min(qw * 64, vecs - 1)));
-  const int wave_end = qw * 64 < vecs ? pa_key_end(x, pc, row_of(min(qw * 64 + 63, vecs - 1))) : 0;
+  const int full_end = pa_key_end(x, pc, row_of(min(qw * VW, vecs - 1)));
+  const int wave_end = qw * VW < vecs ? pa_key_end(x, pc, row_of(min(qw * VW + VW - 1, vecs - 1))) : 0;
 
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-  f32x16 o[2][4];
+  float m_run[QT], l_run[QT], base[QT];  // base: m_run, or 0 before any key
+  f32x16 o[QT][4];
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < QT; ++j) {
+    m_run[j] = -INFINITY;
+    l_run[j] = base[j] = 0.f;
 #pragma unroll
     for (int hb = 0; hb < 4; ++hb) o[j][hb] = f32x16{};
+  }
 
-  f32x16 s[2];
-  vec pf[2][2];
-  float base[2] = {0.f, 0.f};  // m_run, or 0 before any key
-  float scale = x.c;           // 1 where a base is large: the scores are then scaled as it was
-  auto weights = [&] {         // of both query tiles, from their scores
-    float u[2];
-    bool up[2];
+  f32x16 s[QT];
+  vec pf[QT][2];
+  float scale = x.c;    // 1 where a base is large: the scores are then scaled as it was
+  auto weights = [&] {  // of all query tiles, from their scores
+    float u[QT], far = 0.f;
+    bool up[QT], any = false;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < QT; ++j) {
       float tmax = s[j][0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, s[j][r]);
       u[j] = ca_max_xor32(tmax) * x.c;  // -inf: no visible key
       up[j] = u[j] - m_run[j] > PA_LIFT<CT> + CA_RESCALE_LOG2;
+      any = any || up[j];
     }
-    if (__ballot(up[0] || up[1])) {
+    if (__ballot(any)) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < QT; ++j) {
         const float to = up[j] ? u[j] - PA_LIFT<CT> : m_run[j];
         const float alpha = up[j] ? __builtin_amdgcn_exp2f(m_run[j] - to) : 1.f;  // 0 from -inf
 #pragma unroll
@@ -387,17 +372,18 @@ __device__ __forceinline__ void pa_large(const PaArgs& x) {
         l_run[j] *= alpha;
         m_run[j] = to;
         base[j] = up[j] ? to : base[j];
+        far = fmaxf(far, fabsf(base[j]));
       }
-      scale = __ballot(fmaxf(fabsf(base[0]), fabsf(base[1])) > CA_LARGE) ? 1.f : x.c;
+      scale = __ballot(far > CA_LARGE) ? 1.f : x.c;
     }
     if (scale == 1.f) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < QT; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[j][r] *= x.c;
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < QT; ++j) {
 #pragma unroll
       for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
@@ -407,12 +393,12 @@ __device__ __forceinline__ void pa_large(const PaArgs& x) {
       l_run[j] = pa_add8(pf[j][1], pa_add8(pf[j][0], l_run[j]));
     }
   };
-  // A step is a tile of each way. ANY: one that not every row sees whole; the others' steps have half of
-  // the queries in registers.
-  vec qr[2][PL_HELD];
+  // A step is a tile of each way. ANY: one that not every row sees whole (the others' steps have queries in
+  // registers, where two query tiles leave room for half of them).
+  vec qr[QT][HELD];
   auto step = [&](int i, const char* here, char* next, auto any) {
     constexpr bool ANY = decltype(any)::value;
-    const int key0 = (pc.tile0 + way + PL_WAYS * i) * 32;
+    const int key0 = (pc.tile0 + way + WAYS * i) * 32;
     const bool mine = ANY ? i < n && key0 < wave_end : wave_end > 0;
     const bool part = ANY && key0 + 32 > full_end;
     const uint16_t* kt = (const uint16_t*)(here + way * PA_TILE) + lane * 8;
@@ -421,19 +407,21 @@ __device__ __forceinline__ void pa_large(const PaArgs& x) {
     asm volatile("" ::: "memory");
     if (i + 1 < n_it) issue(i + 1, next);
     if (mine) {
-      s[0] = s[1] = f32x16{};
+#pragma unroll
+      for (int j = 0; j < QT; ++j) s[j] = f32x16{};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const vec kf = *(const vec*)(kt + e * 512);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          s[j] = T::mma(kf, !ANY && e < PL_HELD ? qr[j][e < PL_HELD ? e : 0]
-                                                : *(const vec*)(ql + j * 32 * PA_QROW + 16 * e),
+        for (int j = 0; j < QT; ++j)
+          s[j] = T::mma(kf, (!ANY || QT == 1) && e < HELD
+                               ? qr[j][e < HELD ? e : 0]
+                               : *(const vec*)(ql + j * 32 * PA_QROW + 16 * e),
                         s[j]);
       }
       if (part) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < QT; ++j)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             s[j][r] = key0 + mfma_row(r, lane) < q_end[j] ? s[j][r] : -INFINITY;
@@ -441,8 +429,10 @@ __device__ __forceinline__ void pa_large(const PaArgs& x) {
       weights();
 #pragma unroll
       for (int hb = 0; hb < 4; ++hb) {
-        f32x16* const at[2] = {&o[0][hb], &o[1][hb]};
-        pa_values<CT, 2>(*(const u32x4*)(kt + 4096 + hb * 1024),
+        f32x16* at[QT];
+#pragma unroll
+        for (int j = 0; j < QT; ++j) at[j] = &o[j][hb];
+        pa_values<CT, QT>(*(const u32x4*)(kt + 4096 + hb * 1024),
                          *(const u32x4*)(kt + 4096 + hb * 1024 + 512), pf, part, key0, q_end, lane, at);
       }
     }
@@ -451,12 +441,12 @@ __device__ __forceinline__ void pa_large(const PaArgs& x) {
   };
   __syncthreads();  // the queries are in LDS
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < QT; ++j)
 #pragma unroll
-    for (int e = 0; e < PL_HELD; ++e) qr[j][e] = *(const vec*)(ql + j * 32 * PA_QROW + 16 * e);
+    for (int e = 0; e < HELD; ++e) qr[j][e] = *(const vec*)(ql + j * 32 * PA_QROW + 16 * e);
   // (a whole number of both rings' steps) tiles that every row of the unit sees, of both ways
   const int whole = min(pa_key_end(x, pc, row_of(0)) >> 5, pc.tile1) - pc.tile0;
-  const int n_whole = max(whole, 0) / PL_WAYS & ~1;
+  const int n_whole = max(whole, 0) / WAYS & ~1;
   int it = 0;
   for (; it < n_whole; it += 2) {
     step(it, ring0, ring1, std::false_type{});
@@ -468,41 +458,57 @@ __device__ __forceinline__ void pa_large(const PaArgs& x) {
     step(it + 1, ring1, ring0, std::true_type{});
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j) l_run[j] += __shfl_xor(l_run[j], 32, 64);
+  for (int j = 0; j < QT; ++j) l_run[j] += __shfl_xor(l_run[j], 32, 64);
 
-  // The second way's part to the first, which has the same queries in the same registers, 32 head dims
-  // of both query tiles at a time; the first way's waves write theirs out, eight head dims a lane.
-  char* const mine = (qw & 2 ? ring1 : ring0) + (qw & 1) * PA_TILE;  // 16 KiB
-  float f0[2], f1[2];
+  // The other ways' parts to the first, which has the same queries in the same registers, half a head
+  // at a time; the first way's waves write theirs out, eight head dims a lane.
+  constexpr int REGION = QT * 8192, IN_RING = WAYS * PA_TILE / REGION;
+  static_assert((WAYS - 1) * QW <= 2 * IN_RING, "half a head of the other ways' queries fits the rings");
+  auto region = [&](int w) {  // of way w's wave of these queries
+    const int i = (w - 1) * QW + qw;
+    return (i < IN_RING ? ring0 + i * REGION : ring1 + (i - IN_RING) * REGION) + lane * 16;
+  };
+  float f[QT][WAYS];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    __syncthreads();  // the ring, or the first half, has been read
+    __syncthreads();  // the rings, or the first half, have been read
     if (way) {
+      char* const mine = region(way);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < QT; ++j) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const f32x16& y = o[j][2 * half + b];
-            *(f32x4*)(mine + ((j * 2 + b) * 4 + r) * 1024 + lane * 16) =
+            *(f32x4*)(mine + ((j * 2 + b) * 4 + r) * 1024) =
                 f32x4{y[4 * r], y[4 * r + 1], y[4 * r + 2], y[4 * r + 3]};
           }
-        if (half == 0 && lane < 32) ml[qw * 64 + j * 32 + lane] = make_float2(m_run[j], l_run[j]);
+        if (half == 0 && lane < 32)
+          ml[(way - 1) * NQ + qw * VW + j * 32 + lane] = make_float2(m_run[j], l_run[j]);
       }
     }
     __syncthreads();
     if (!way) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int v = qw * 64 + j * 32 + (lane & 31);
+      for (int j = 0; j < QT; ++j) {
+        const int v = qw * VW + j * 32 + (lane & 31);
         if (half == 0) {
-          const float2 z = ml[v];
-          const float m = fmaxf(m_run[j], z.x);
-          f0[j] = m_run[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[j] - m);
-          f1[j] = z.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(z.x - m);
+          float2 z[WAYS];
+          z[0] = make_float2(m_run[j], l_run[j]);
+          float m = m_run[j], l = 0.f;
+#pragma unroll
+          for (int w = 1; w < WAYS; ++w) {
+            z[w] = ml[(w - 1) * NQ + v];
+            m = fmaxf(m, z[w].x);
+          }
+#pragma unroll
+          for (int w = 0; w < WAYS; ++w) {
+            f[j][w] = z[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(z[w].x - m);
+            l = fmaf(f[j][w], z[w].y, l);
+          }
           m_run[j] = m;
-          l_run[j] = f0[j] * l_run[j] + f1[j] * z.y;
+          l_run[j] = l;
         }
         const float inv = pc.slot >= 0 ? 1.f : pc.tile1 == 0 ? 0.f : 1.f / l_run[j];  // (no key: zeros)
         const bool there = v < vecs;
@@ -520,8 +526,10 @@ __device__ __forceinline__ void pa_large(const PaArgs& x) {
             for (int g = 0; g < 2; ++g) {
               const f32x16& z = o[j][2 * half + b];
               y[g] = f32x4{z[4 * (r + g)], z[4 * (r + g) + 1], z[4 * (r + g) + 2], z[4 * (r + g) + 3]} *
-                         f0[j] +
-                     *(const f32x4*)(mine + ((j * 2 + b) * 4 + r + g) * 1024 + lane * 16) * f1[j];
+                     f[j][0];
+#pragma unroll
+              for (int w = 1; w < WAYS; ++w)
+                y[g] += *(const f32x4*)(region(w) + ((j * 2 + b) * 4 + r + g) * 1024) * f[j][w];
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -542,14 +550,33 @@ __device__ __forceinline__ void pa_large(const PaArgs& x) {
       }
     }
   }
-  if (pc.last) return;
-  __syncthreads();  // the next part's queries and tiles go where this one's O was
-  }
 }
-// (the buffer resource type is not known to the host pass: the body is a device function)
-template <int CT> __global__ __launch_bounds__(512, 2) void paged_attn_large_kernel(const PaArgs x) {
+
+// (the buffer resource type is not known to the host pass: the bodies are device functions)
+// (separate arrays: the compiler knows the slot being read is not one being filled)
+template <int CT> __global__ __launch_bounds__(512, 2) void paged_attn_kernel(const PaArgs x) {
+  __shared__ __align__(16) uint16_t q_lds[64 * PA_QROW];
+  __shared__ __align__(1024) char ring0[4 * PA_TILE];
+  __shared__ __align__(1024) char ring1[4 * PA_TILE];
+  __shared__ float2 ml[8 * 32];
 #if defined(__HIP_DEVICE_COMPILE__)
-  pa_large<CT>(x);
+  const PagedPiece pc = pa_piece(x.pieces, (int)(blockIdx.x / (uint32_t)x.hkv));
+  if (pc.wide) pa_shared<CT, 2, 1>(x, pc, q_lds, ring0, ring1, ml);
+  else pa_few<CT>(x, pc, q_lds, ring0, ring1, ml);
+#endif
+}
+template <int CT> __global__ __launch_bounds__(512, 2) void paged_attn_large_kernel(const PaArgs x) {
+  __shared__ __align__(16) uint16_t q_lds[256 * PA_QROW];
+  __shared__ __align__(1024) char ring0[2 * PA_TILE];
+  __shared__ __align__(1024) char ring1[2 * PA_TILE];
+  __shared__ float2 ml[256];
+#if defined(__HIP_DEVICE_COMPILE__)
+  for (int at = x.first[blockIdx.x / (uint32_t)x.hkv];; ++at) {
+    const PagedPiece pc = pa_piece(x.pieces, at);
+    pa_shared<CT, 4, 2>(x, pc, q_lds, ring0, ring1, ml);
+    if (pc.last) return;
+    __syncthreads();  // the next part's queries and tiles go where this one's O was
+  }
 #endif
 }
 
@@ -647,8 +674,8 @@ void paged_attention(const PagedAttnCall& c, hipStream_t s) {
   if (c.n_small) {
     a.pieces = (const PagedPiece*)(c.list + c.small);
     const dim3 grid((unsigned)c.n_small * (unsigned)c.hkv);
-    if (c.cache_bf16) hipLaunchKernelGGL(paged_attn_kernel<2>, grid, dim3(64 * PS_WAVES), 0, s, a);
-    else hipLaunchKernelGGL(paged_attn_kernel<1>, grid, dim3(64 * PS_WAVES), 0, s, a);
+    if (c.cache_bf16) hipLaunchKernelGGL(paged_attn_kernel<2>, grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL(paged_attn_kernel<1>, grid, dim3(512), 0, s, a);
     DRT_HIP(hipGetLastError());
   }
   if (c.n_large) {

@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <map>
 #include <string>
 #include <vector>
 
@@ -25,7 +26,7 @@ struct PagedPiece {
   int32_t slot;              // where its part goes (32 query vectors a slot); < 0: the whole unit
   int32_t table;             // the sequence's first page in the list
   int32_t last;              // a work-group's last
-  int32_t wide_log2;         // (small kernel) its unit is of 32 << wide_log2 query vectors (0 or 1)
+  int32_t wide;              // (small kernel) its unit is of up to 64 query vectors, not 32
   int32_t unused[4];
 };
 // 32 query vectors of a unit whose keys are split: their parts are in slots slot, slot + step, ...
@@ -60,7 +61,7 @@ struct PagedPlanInfo {
 };
 
 // Query vectors of a unit: of the small kernel, 32 or 64, and of the large one.
-constexpr int PAGED_VECS = 32, PAGED_VECS_L = 256;
+constexpr int PAGED_VECS = 32, PAGED_VECS_M = 64, PAGED_VECS_L = 256;
 constexpr int PAGED_CUS = 256;
 
 // The number of keys that the row at position p sees, always the first ones.
@@ -107,13 +108,19 @@ namespace paged_detail {
 struct Unit {
   int seq, vec0, vecs;
   int64_t tiles;
+  double beside = 1.;  // units of the sequence
 };
 
-// Times in us. A part: `fixed` (its queries in, its result out) and `tile` for 32 keys, alone on its CU;
-// `join`: the second launch that a cut needs.
+// Times in us. A part: `fixed` (its queries in, its result out) and `tile` for 32 keys, on its CU; where
+// units read the same keys side by side those come from the L2, else each is `alone` in waiting for memory;
+// `join`: the second launch that a cut needs. Fitted to 157 batches of 1 to 48 sequences (1 to 1000 rows,
+// 300 to 60000 keys, 16 heads on 8, 28 on 4, 32 on 2), in each of which units of 32 and of 64 were timed at
+// several cuts: what these times choose is 2.4 % slower on average than the fastest seen in each (choosing by
+// one cost a tile for all was 11 %).
 struct Costs {
-  double fixed, tile, join;
+  double fixed, tile, join, alone;
 };
+constexpr Costs SMALL{5., 0.147, 3.3, 0.143}, MEDIUM{7., 0.235, 3.3, 0.13}, LARGE{12., 0.74, 20., 0.};
 // The part [tile0, tile1) of unit `unit` for work-group `group`.
 struct Share {
   int unit, group;
@@ -163,30 +170,39 @@ inline std::vector<Share> cut(const std::vector<Unit>& units, int groups, const 
   return out;
 }
 
-// The time of work-groups, `slots` of them at once, the longest first; parts: (us, how many).
+// The time of work-groups, `slots` of them at once, the longest first, each where one before it ends; parts:
+// (us, how many). Times within 2 % are taken as one. (Places are an XCD's, to which a work-group belongs by
+// its number: where some wait for one they end later than that by up to half of the longest of them.)
 inline double makespan(std::vector<std::pair<double, int64_t>>& parts, int slots) {
   std::sort(parts.begin(), parts.end(), std::greater<std::pair<double, int64_t>>());
-  // rounds, each as long as its longest; or all of it evenly and the longest behind
-  double rounds = 0., sum = 0.;
-  int64_t room = 0;
-  for (const auto& y : parts) {
-    sum += y.first * (double)y.second;
-    const int64_t n = y.second - room;
-    room = room > y.second ? room - y.second : 0;
-    if (n > 0) {
-      const int64_t r = (n + slots - 1) / slots;
-      rounds += y.first * (double)r;
-      room = r * slots - n;
+  std::map<double, int64_t> free_at{{0., slots}};
+  double last = 0., sum = 0., waits = 0.;
+  int64_t before = 0;
+  for (size_t i = 0; i < parts.size();) {
+    const double us = parts[i].first;
+    int64_t n = 0;
+    for (; i < parts.size() && parts[i].first > 0.98 * us; ++i) n += parts[i].second;
+    sum += us * (double)n;
+    if (before <= slots && before + n > slots) waits = us;
+    before += n;
+    while (n > 0) {
+      const auto at = free_at.begin();
+      const int64_t k = std::min(n, at->second);
+      const double end = at->first + us;
+      n -= k;
+      at->second -= k;
+      if (at->second == 0) free_at.erase(at);
+      free_at[end] += k;
+      last = std::max(last, end);
     }
   }
-  return std::max(parts[0].first, std::min(rounds, sum / slots + parts[0].first));
+  return std::max(last, sum / slots + 0.5 * waits);
 }
 
-// The longest part, in tiles, of units that are cut into equal ones, each a work-group of its own, by the
-// least time of all (c.tile: for 32 query vectors; 64 take 1.65 times as long). all_us: what reading the
-// keys of all sequences once takes; the nearer the work-groups' own time comes to that, the more they
-// wait for one another.
-inline int64_t part_length(const std::vector<Unit>& units, int hkv, double all_us, const Costs& c) {
+// (us, longest part in tiles) of units that are cut into equal parts, each a work-group of its own, by the
+// least time of all. all_us: what reading the keys of all sequences once takes; the nearer the work-groups'
+// own time comes to that, the more they wait for one another.
+inline std::pair<double, int64_t> part_length(const std::vector<Unit>& units, int hkv, double all_us) {
   std::vector<std::pair<double, int64_t>> parts;
   int64_t most = 0;
   for (const Unit& u : units) most = std::max(most, u.tiles);
@@ -197,15 +213,15 @@ inline int64_t part_length(const std::vector<Unit>& units, int hkv, double all_u
     int64_t cuts = 0, most_cuts = 0;
     for (const Unit& u : units) {
       const int64_t n = std::max<int64_t>(1, (u.tiles + len - 1) / len);
-      parts.emplace_back(c.fixed + (u.vecs > PAGED_VECS ? 1.65 : 1.) * c.tile * (double)((u.tiles + n - 1) / n),
-                         n * hkv);
+      const Costs& c = u.vecs > PAGED_VECS ? MEDIUM : SMALL;
+      parts.emplace_back(c.fixed + (c.tile + c.alone / u.beside) * (double)((u.tiles + n - 1) / n), n * hkv);
       cuts += n > 1 ? n * ((u.vecs + 31) / 32) : 0;
       most_cuts = std::max(most_cuts, n);
     }
     if (most_cuts > 128) break;
-    const double own = makespan(parts, PAGED_CUS), all = c.fixed + all_us;
+    const double own = makespan(parts, PAGED_CUS), all = SMALL.fixed + all_us;
     const double us = std::sqrt(std::sqrt(own * own * own * own + all * all * all * all)) +
-                      (cuts ? c.join + 0.008 * (double)(cuts * hkv) : 0.);
+                      (cuts ? SMALL.join + 0.008 * (double)(cuts * hkv) : 0.);
     if (best < 0. || us < best) {
       best = us;
       best_len = len;
@@ -217,7 +233,65 @@ inline int64_t part_length(const std::vector<Unit>& units, int hkv, double all_u
       if (own <= 1.1 * std::max(all, sum / PAGED_CUS)) break;
     }
   }
-  return best_len;
+  return {best, best_len};
+}
+
+// Units of the large kernel: each a work-group of its own, or all of them in equal shares whose parts are
+// joined (0.009 us for 32 query vectors of a part written and read).
+struct LargeTimes {
+  double whole = 0., cut = 0.;
+};
+inline LargeTimes large_times(const std::vector<Unit>& units, int hkv) {
+  LargeTimes y;
+  if (units.empty()) return y;
+  const int groups = std::max(1, PAGED_CUS / hkv);
+  std::vector<std::pair<double, int64_t>> parts;
+  double sum = 0.;
+  for (const Unit& u : units) {
+    parts.emplace_back(LARGE.fixed + LARGE.tile * (double)u.tiles, hkv);
+    sum += parts.back().first;
+  }
+  y.whole = makespan(parts, PAGED_CUS);
+  y.cut = sum / groups + LARGE.fixed + LARGE.join + 0.009 * 8. * (double)(units.size() + groups) * hkv;
+  return y;
+}
+
+// The order of the small kernel's pieces: the longest first. Work-groups go round the 8 XCDs, each with an
+// L2 of its own, and a piece's K/V heads follow one another: pieces of one sequence's same keys (`same`) are
+// put so that they come to the same XCDs, as long as there are others to take the places between (17 rows x
+// 28 heads on 4 over 16000 keys 15.1 us, of 60000 32.6; side by side in turn 16.4 and 36.1).
+inline void side_by_side(std::vector<PagedPiece>& pieces, const std::vector<std::pair<int, int>>& same,
+                         int hkv) {
+  int lanes = 8;
+  for (int h = hkv; lanes > 1 && h % 2 == 0; h /= 2) lanes /= 2;
+  std::vector<int> order(pieces.size());
+  for (size_t i = 0; i < order.size(); ++i) order[i] = (int)i;
+  std::stable_sort(order.begin(), order.end(), [&](int x, int y) {
+    return pieces[x].tile1 - pieces[x].tile0 > pieces[y].tile1 - pieces[y].tile0;
+  });
+  std::map<std::pair<int, int>, int> lane_of;
+  std::vector<std::vector<int>> lane(lanes);
+  std::vector<size_t> size(lanes, 0);
+  std::map<std::pair<int, int>, size_t> count;
+  for (const auto& y : same) ++count[y];
+  for (const int i : order) {
+    auto at = lane_of.find(same[i]);
+    if (at == lane_of.end()) {
+      // (of many, a lane's each: enough to be beside one another)
+      const int shortest = (int)(std::min_element(size.begin(), size.end()) - size.begin());
+      at = lane_of.emplace(same[i], 2 * lanes * count[same[i]] <= pieces.size() ? shortest : -1).first;
+    }
+    const int to = at->second >= 0 ? at->second
+                                   : (int)(std::min_element(size.begin(), size.end()) - size.begin());
+    lane[to].push_back(i);
+    size[to] += pieces[i].tile1 - pieces[i].tile0 + 20;
+  }
+  std::vector<PagedPiece> out;
+  out.reserve(pieces.size());
+  for (size_t i = 0; out.size() < pieces.size(); ++i)
+    for (int l = 0; l < lanes; ++l)
+      if (i < lane[l].size()) out.push_back(pieces[lane[l][i]]);
+  pieces.swap(out);
 }
 
 }  // namespace paged_detail
@@ -229,32 +303,50 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
   const int G = a.hq / a.hkv, tpp = a.page_size / 32;
   std::vector<int32_t> row0(a.seqs);
   std::vector<int64_t> table0(a.seqs);
-  std::vector<Unit> units[2];
+  std::vector<Unit> units[2], units64;
   std::vector<PagedTile> tiles;
   std::vector<int32_t> written;  // the tiles' numbers, to find two rows in one place
   int64_t n_table = 0;
-  // Sequences of many query vectors: by the large kernel where the others' is estimated to take longer. A
-  // tile of 256 query vectors is 0.88 us there and 1.32 in four units of 64; beginning, end and balance
-  // are 48 and 6 (2048 rows x 16 heads: over 16384 keys 267 us and 335, over 2048 57 and 38).
-  double work = 0.;  // tiles of 256 query vectors, of a CU
-  int64_t n64 = 0;
   const auto unit_tiles = [&](int s, int64_t last_vec) {
     const int64_t end = paged_key_end(a.pos0[s] + last_vec / G, a.keys[s], a.masked != 0,
                                       a.prompt_len ? a.prompt_len[s] : 0, a.block);
     return (end + 31) / 32;
   };
-  for (int s = 0; s < a.seqs; ++s) {
+  const auto units_of = [&](int s, int step, std::vector<Unit>& to) {
     const int64_t vecs = (int64_t)a.rows[s] * G;
-    n64 += (vecs + 63) / 64 * a.hkv;
-    if (vecs < PAGED_VECS_L) continue;
-    const int64_t n = (vecs + PAGED_VECS_L - 1) / PAGED_VECS_L;
-    work += 0.5 * (double)(n * (unit_tiles(s, 0) + unit_tiles(s, vecs - 1))) * a.hkv / PAGED_CUS;
+    for (int64_t v = 0; v < vecs; v += step) {
+      const int n = (int)std::min<int64_t>(step, vecs - v);
+      to.push_back(Unit{s, (int)v, n, unit_tiles(s, v + n - 1), (double)((vecs + step - 1) / step)});
+    }
+  };
+  // What reading the keys of all of the units' sequences once takes, at 5.3 TB/s.
+  const auto read_us = [&](const std::vector<Unit>& of) {
+    std::vector<int64_t> read(a.seqs, 0);
+    int64_t all = 0;
+    for (const Unit& u : of) read[u.seq] = std::max(read[u.seq], u.tiles);
+    for (int64_t n : read) all += n;
+    return 0.0031 * (double)(all * a.hkv);
+  };
+  // Sequences of many query vectors: by the large kernel where that takes less time than units of 64. (Work:
+  // that of a CU, in tiles of 256 query vectors, about a us each. Of 40 of them no batch was faster there, of
+  // 400 none was slower.)
+  double work = 0.;
+  bool others = false;
+  for (int s = 0; s < a.seqs; ++s) {
+    if ((int64_t)a.rows[s] * G >= PAGED_VECS_L) units_of(s, PAGED_VECS_L, units[1]);
+    else others = others || a.rows[s];
   }
-  const bool many = 0.88 * work + 48. < 1.32 * work + 6.;
-  // Units of 64 (whose tiles are read for 32 query vectors twice, by waves side by side) where they fill
-  // the chip: a chunk of 500 rows x 16 heads over 4097 keys beside 31 tokens 56 us, of 32 67; 512 rows
-  // over 16384 alone 148 and 92.
-  const int small_vecs = n64 >= 192 ? 2 * PAGED_VECS : PAGED_VECS;
+  for (const Unit& u : units[1]) work += (double)(u.tiles * a.hkv) / PAGED_CUS;
+  const LargeTimes large_us = large_times(units[1], a.hkv);
+  bool many = work > 400.;
+  if (!many && work > 40.) {
+    std::vector<Unit> small;
+    for (int s = 0; s < a.seqs; ++s)
+      if ((int64_t)a.rows[s] * G >= PAGED_VECS_L) units_of(s, PAGED_VECS_M, small);
+    many = std::min(large_us.whole, large_us.cut) + (others ? 8. : 0.) <
+           part_length(small, a.hkv, read_us(small)).first;
+  }
+  if (!many) units[1].clear();
   for (int s = 0; s < a.seqs; ++s) {
     row0[s] = p.rows;
     p.rows += a.rows[s];
@@ -262,10 +354,9 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
     n_table += (a.keys[s] + (int64_t)a.page_size - 1) / a.page_size;
     const int64_t vecs = (int64_t)a.rows[s] * G;
     const bool large = many && vecs >= PAGED_VECS_L;
-    const int step = large ? PAGED_VECS_L : small_vecs;
-    for (int64_t v = 0; v < vecs; v += step) {
-      const int n = (int)std::min<int64_t>(step, vecs - v);
-      units[large].push_back(Unit{s, (int)v, n, unit_tiles(s, v + n - 1)});
+    if (!large) {
+      units_of(s, PAGED_VECS, units[0]);
+      units_of(s, PAGED_VECS_M, units64);
     }
     // the tiles that rows inside the sequence's keys lie in
     const int32_t* pg = a.table + (int64_t)s * a.width;
@@ -296,39 +387,36 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
   for (int k = 0; k < 2; ++k) {
     if (units[k].empty()) continue;
     std::vector<Share> shares;
+    std::vector<std::pair<int, int>> same;  // the sequence of a share, and which of its parts
     if (k == 0) {
-      std::stable_sort(units[0].begin(), units[0].end(),
-                       [](const Unit& x, const Unit& y) { return x.tiles > y.tiles; });
-      int64_t all = 0;  // (units of one sequence follow one another, the longest first)
-      std::vector<int64_t> read(a.seqs, 0);
-      for (const Unit& u : units[0]) read[u.seq] = std::max(read[u.seq], u.tiles);
-      for (int64_t n : read) all += n;
-      const int64_t len = part_length(units[0], a.hkv, 0.0031 * (double)(all * a.hkv),
-                                      Costs{3.5, 0.24, 7.5});
+      const auto longest = [](const Unit& x, const Unit& y) { return x.tiles > y.tiles; };
+      std::stable_sort(units[0].begin(), units[0].end(), longest);
+      const double all_us = read_us(units[0]);
+      auto best = part_length(units[0], a.hkv, all_us);
+      if (units64.size() < units[0].size()) {
+        const auto other = part_length(units64, a.hkv, all_us);
+        if (other.first < best.first) {
+          best = other;
+          units[0].swap(units64);
+          std::stable_sort(units[0].begin(), units[0].end(), longest);
+        }
+      }
+      const int64_t len = best.second;
       int group = 0;
       for (int i = 0; i < (int)units[0].size(); ++i) {
         const int64_t tiles = units[0][i].tiles, n = std::max<int64_t>(1, (tiles + len - 1) / len);
-        for (int64_t j = 0; j < n; ++j)
+        for (int64_t j = 0; j < n; ++j) {
           shares.push_back(Share{i, group++, tiles * j / n, tiles * (j + 1) / n});
+          same.emplace_back(units[0][i].seq, (int)j);
+        }
       }
     } else {
-      // whole units, or equal shares of all: by the time of either
-      const Costs c{12., 0.875, 25.};
-      const int groups = std::max(1, PAGED_CUS / a.hkv);
-      std::vector<std::pair<double, int64_t>> parts;
-      double sum = 0.;
-      for (const Unit& u : units[1]) {
-        parts.emplace_back(c.fixed + c.tile * (double)u.tiles, a.hkv);
-        sum += parts.back().first;
-      }
-      const double whole = makespan(parts, PAGED_CUS);
-      const double slots = 8. * (double)(units[1].size() + groups) * a.hkv;  // (at most) written and read
-      if (whole <= sum / groups + c.fixed + c.join + 0.009 * slots) {
+      if (large_us.whole <= large_us.cut) {
         std::stable_sort(units[1].begin(), units[1].end(),
                          [](const Unit& x, const Unit& y) { return x.tiles > y.tiles; });
         for (int i = 0; i < (int)units[1].size(); ++i) shares.push_back(Share{i, i, 0, units[1][i].tiles});
       } else {
-        shares = cut(units[1], groups, c);
+        shares = cut(units[1], std::max(1, PAGED_CUS / a.hkv), Costs{LARGE.fixed, 0.875, 0., 0.});
       }
     }
     for (size_t i = 0; i < shares.size();) {
@@ -352,7 +440,7 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
         y.tile1 = (int)shares[i].tile1;
         y.slot = parts > 1 ? slot : -1;
         y.table = (int)table0[s];
-        y.wide_log2 = u.vecs > PAGED_VECS;
+        y.wide = u.vecs > PAGED_VECS;
         pieces[k].push_back(y);
         if (parts > 1) slot += subs;
       }
@@ -368,6 +456,7 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
       }
     }
     pieces[k].back().last = 1;
+    if (k == 0) side_by_side(pieces[0], same, a.hkv);
   }
   p.n_small = (int)pieces[0].size();
   p.n_large = (int)first.size();

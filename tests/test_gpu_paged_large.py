@@ -101,16 +101,16 @@ class Batch:
 @pytest.mark.parametrize("mask, geometry", [("causal", None), ("full", None), ("d2f_hybrid", (5000, 32)),
                                             ("d2f_hybrid", (0, 1000))])
 def test_masks(kind, mask, geometry):
-    Batch([8001], [1023], g=2, hkv=16, kind=kind, mask=mask, geometry=geometry).check()
+    Batch([8001], [1023], g=2, hkv=64, kind=kind, mask=mask, geometry=geometry).check()
 
 
-@pytest.mark.parametrize("g, hkv, rows, keys", [(1, 32, 1000, 6700), (7, 4, 1200, 7100), (40, 4, 200, 8000),
-                                                (3, 64, 257, 5000), (5, 9, 555, 9999)])
+@pytest.mark.parametrize("g, hkv, rows, keys", [(1, 32, 2000, 9100), (7, 4, 2300, 9500), (40, 4, 400, 9000),
+                                                (3, 64, 257, 5000), (5, 9, 1111, 19999)])
 def test_head_groups(g, hkv, rows, keys):
     Batch([keys], [rows], g=g, hkv=hkv, seed=g).check("bf16")
 
 
-@pytest.mark.parametrize("cut, rows, keys", [(False, 2048, 8192), (True, 600, 16384)])
+@pytest.mark.parametrize("cut, rows, keys", [(False, 2048, 8192), (True, 600, 40000)])
 def test_whole_units_and_shares(cut, rows, keys):
     b = Batch([keys], [rows], g=2, hkv=16, size=256, seed=1, scale=2.0)
     got = b.check(cut=cut)
@@ -126,25 +126,25 @@ def test_ragged_sequences_beside_small_ones():
 
 
 def test_rows_without_keys_beside_others():
-    b = Batch([9000, 0, 40], [900, 300, 5], g=2, hkv=16, mask="full", positions=[8100, 0, 35])
+    b = Batch([9000, 0, 40], [1900, 300, 5], g=2, hkv=32, mask="full", positions=[7100, 0, 35])
     got = b.check()
-    assert (got[900:1200] == 0).all()
+    assert (got[1900:2200] == 0).all()
 
 
 def test_from_the_first_key_on():
-    Batch([3500, 100], [3500, 100], g=4, hkv=16).check()
+    Batch([6000, 100], [6000, 100], g=4, hkv=16).check()
 
 
 def test_large_scores():
-    Batch([8000], [1024], g=2, hkv=16, scale=1e4, seed=4).check()
+    Batch([9000], [2048], g=2, hkv=16, scale=1e4, seed=4).check()
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
 def test_values_that_are_not_finite_where_a_row_does_not_see_them(kind, what):
-    b = Batch([8192], [1024], g=2, hkv=16, kind=kind)
+    b = Batch([9000], [2048], g=2, hkv=16, kind=kind)
     want, bound = b.want()
-    at = 8192 - 1024 + 500
+    at = 9000 - 2048 + 500
     b.k[at + 1, 0, 5] = what
     b.v[at, 3, 9] = what
     b.fill()
@@ -166,7 +166,7 @@ def test_values_that_are_not_finite_where_a_row_does_not_see_them(kind, what):
 
 
 def test_graph_and_other_streams():
-    b = Batch([9000, 50], [800, 1], g=2, hkv=16)
+    b = Batch([9000, 50], [2000, 1], g=2, hkv=16)
     want = b.cache.attention(0, b.q, b.batch)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
