@@ -129,7 +129,12 @@ DRT_DEV void pa_store8(const PaArgs& x, int64_t at, f32x4 y0, f32x4 y1) {
 }
 
 // Units of 32 query vectors: eight waves over keys, wave kw takes tiles kw, kw + 8, ... of the piece,
-// straight from memory into registers. They meet in LDS at the end.
+// straight from memory into registers, the next while this is worked on. They meet in LDS at the end.
+// Bound by the keys' bytes where those are many: one row x 16 heads over 131072 keys 96 us (537 MB at 5.8
+// TB/s of the kernel's 92), 32 tokens x 28 heads over up to 16384 52 (251 MB at 5.2 of 48). A CU alone draws
+// 55 GB/s so, 0.29 us a tile; where units of the same keys run beside one another tiles come from the L2,
+// 0.15. One row over 1337 keys: 5.6 us, of which a tile each wave and the joins; 3.0 more joins its parts.
+// Four waves a work-group (two of them a CU) are slower where memory bounds (131072 keys 118 us).
 constexpr int PS_WAVES = 8;
 template <int CT>
 DRT_DEV void pa_few(const PaArgs& x, const PagedPiece& pc, uint16_t* q_lds, char* ring0, char* ring1, float2* ml) {
@@ -283,6 +288,14 @@ DRT_DEV void pa_few(const PaArgs& x, const PagedPiece& pc, uint16_t* q_lds, char
 // are read once), for each of 8 / QW key ways, which take turns at the tiles. Tiles come by direct-to-LDS
 // loads, one for the waves of a way together, the next while this is worked on; queries lie in LDS for
 // all of it, some of them in registers.
+// 64 query vectors (2 x 1 and four ways): 0.245 us a tile, 0.15 for 32 of them above; it begins and ends 2 us
+// slower, so it takes over where keys are long (16 sequences of 32 rows x 16 heads 47 us, 50 above; 150 rows
+// x 28 heads over 16000 keys 53 and 66, over 1300 17.7 and 11.2).
+// 256 (4 x 2 and two ways): 0.74 us a tile. Bound by the matrix unit at the clock that the card's power
+// leaves it: 2048 rows x 28 heads over 10240 keys 286 us, 1.13 PFLOP/s in the steps, as much as a large
+// library product; the rest is the first and last 20 us of a work-group and rows that see fewer keys
+// finishing early. With zeros for data it is 26 % faster. Below, not faster: the two ways half a step apart
+// with a barrier between, priorities around the products, five or six of eight query steps in registers.
 template <int CT, int QW, int QT>
 DRT_DEV void pa_shared(const PaArgs& x, const PagedPiece& pc, uint16_t* q_lds, char* ring0, char* ring1, float2* ml) {
   typedef CacheT<CT> T;
@@ -582,7 +595,9 @@ template <int CT> __global__ __launch_bounds__(512, 2) void paged_attn_large_ker
 
 // The parts of a unit joined: WIDE, a wave for each query vector, lane (sg, ch) adding head dims 8 ch ..
 // + 8 of parts sg, sg + 4, ...; the four groups meet by lane exchanges. Otherwise sixteen lanes for each,
-// four query vectors a wave. All loads of a batch of parts are on their way before their use.
+// four query vectors a wave. All loads of a batch of parts are on their way before their use. 3.0 to 4.3 us, a
+// launch and one chain of loads. (Joined by the last work-group of a unit to arrive instead: 64 rows x 16
+// heads over 2048 keys 16.8 us, 12.3 with this launch.)
 template <bool WIDE>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PaArgs x, const PagedJoin* joins) {
   const int kvh = (int)(blockIdx.x % (uint32_t)x.hkv), G = x.hq / x.hkv;
@@ -687,7 +702,9 @@ void paged_attention(const PagedAttnCall& c, hipStream_t s) {
     DRT_HIP(hipGetLastError());
   }
   if (c.n_joins) {
-    // Few query vectors of many parts by a wave each, many of few by a quarter.
+    // Few query vectors of many parts by a wave each, many of few by a quarter (both launches, us with a wave
+    // and a quarter: one row over 16000 keys, 25 parts, 17.7 and 20.6; over 60000, 105 parts, 20.6 and 32.8;
+    // 64 rows x 32 heads in 128 parts of 32 units 31.8 and 31.2).
     const bool wide = c.slots > 4 * c.n_joins || (int64_t)c.n_joins * c.hkv < 64;
     const unsigned n = (unsigned)c.n_joins * (unsigned)c.hkv;
     const PagedJoin* joins = (const PagedJoin*)(c.list + c.joins);
