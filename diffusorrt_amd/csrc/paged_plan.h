@@ -171,29 +171,44 @@ inline std::vector<Share> cut(const std::vector<Unit>& units, int groups, const 
 }
 
 // The time of work-groups, `slots` of them at once, the longest first, each where one before it ends; parts:
-// (us, how many). Times within 2 % are taken as one. (Places are an XCD's, to which a work-group belongs by
-// its number: where some wait for one they end later than that by up to half of the longest of them.)
+// (us, how many). Times within 4 % are taken as one, and many rounds as even ones: a plan is made once a step.
+// (Places are an XCD's, to which a work-group belongs by its number: where some wait for one they end later
+// than that by up to half of the longest of them.)
 inline double makespan(std::vector<std::pair<double, int64_t>>& parts, int slots) {
+  int64_t all = 0;
+  double longest = 0., sum = 0.;
+  for (const auto& y : parts) {
+    all += y.second;
+    longest = std::max(longest, y.first);
+    sum += y.first * (double)y.second;
+  }
+  if (all <= slots) return longest;
   std::sort(parts.begin(), parts.end(), std::greater<std::pair<double, int64_t>>());
-  std::map<double, int64_t> free_at{{0., slots}};
-  double last = 0., sum = 0., waits = 0.;
+  double last = longest, waits = 0.;
   int64_t before = 0;
-  for (size_t i = 0; i < parts.size();) {
-    const double us = parts[i].first;
-    int64_t n = 0;
-    for (; i < parts.size() && parts[i].first > 0.98 * us; ++i) n += parts[i].second;
-    sum += us * (double)n;
-    if (before <= slots && before + n > slots) waits = us;
-    before += n;
-    while (n > 0) {
-      const auto at = free_at.begin();
-      const int64_t k = std::min(n, at->second);
-      const double end = at->first + us;
-      n -= k;
-      at->second -= k;
-      if (at->second == 0) free_at.erase(at);
-      free_at[end] += k;
-      last = std::max(last, end);
+  for (const auto& y : parts) {
+    before += y.second;
+    if (before > slots) {
+      waits = y.first;
+      break;
+    }
+  }
+  if (all <= 4 * slots) {
+    std::map<double, int64_t> free_at{{0., slots}};
+    for (size_t i = 0; i < parts.size();) {
+      const double us = parts[i].first;
+      int64_t n = 0;
+      for (; i < parts.size() && parts[i].first > 0.96 * us; ++i) n += parts[i].second;
+      while (n > 0) {
+        const auto at = free_at.begin();
+        const int64_t k = std::min(n, at->second);
+        const double end = at->first + us;
+        n -= k;
+        at->second -= k;
+        if (at->second == 0) free_at.erase(at);
+        free_at[end] += k;
+        last = std::max(last, end);
+      }
     }
   }
   return std::max(last, sum / slots + 0.5 * waits);
@@ -260,29 +275,28 @@ inline LargeTimes large_times(const std::vector<Unit>& units, int hkv) {
 // L2 of its own, and a piece's K/V heads follow one another: pieces of one sequence's same keys (`same`) are
 // put so that they come to the same XCDs, as long as there are others to take the places between (17 rows x
 // 28 heads on 4 over 16000 keys 15.1 us, of 60000 32.6; side by side in turn 16.4 and 36.1).
-inline void side_by_side(std::vector<PagedPiece>& pieces, const std::vector<std::pair<int, int>>& same,
-                         int hkv) {
+inline void side_by_side(std::vector<PagedPiece>& pieces, const std::vector<int>& same, int hkv) {
   int lanes = 8;
   for (int h = hkv; lanes > 1 && h % 2 == 0; h /= 2) lanes /= 2;
-  std::vector<int> order(pieces.size());
+  std::vector<int> order(pieces.size()), count, lane_of;
   for (size_t i = 0; i < order.size(); ++i) order[i] = (int)i;
   std::stable_sort(order.begin(), order.end(), [&](int x, int y) {
     return pieces[x].tile1 - pieces[x].tile0 > pieces[y].tile1 - pieces[y].tile0;
   });
-  std::map<std::pair<int, int>, int> lane_of;
+  for (const int y : same) {
+    if (y >= (int)count.size()) count.resize(y + 1);
+    ++count[y];
+  }
+  lane_of.assign(count.size(), -1);
   std::vector<std::vector<int>> lane(lanes);
   std::vector<size_t> size(lanes, 0);
-  std::map<std::pair<int, int>, size_t> count;
-  for (const auto& y : same) ++count[y];
   for (const int i : order) {
-    auto at = lane_of.find(same[i]);
-    if (at == lane_of.end()) {
-      // (of many, a lane's each: enough to be beside one another)
-      const int shortest = (int)(std::min_element(size.begin(), size.end()) - size.begin());
-      at = lane_of.emplace(same[i], 2 * lanes * count[same[i]] <= pieces.size() ? shortest : -1).first;
+    int to = lane_of[same[i]];
+    if (to < 0) {
+      to = (int)(std::min_element(size.begin(), size.end()) - size.begin());
+      // (of very many, each to a lane of its own: enough of them are beside one another)
+      if (2 * lanes * (size_t)count[same[i]] <= pieces.size()) lane_of[same[i]] = to;
     }
-    const int to = at->second >= 0 ? at->second
-                                   : (int)(std::min_element(size.begin(), size.end()) - size.begin());
     lane[to].push_back(i);
     size[to] += pieces[i].tile1 - pieces[i].tile0 + 20;
   }
@@ -343,8 +357,10 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
     std::vector<Unit> small;
     for (int s = 0; s < a.seqs; ++s)
       if ((int64_t)a.rows[s] * G >= PAGED_VECS_L) units_of(s, PAGED_VECS_M, small);
-    many = std::min(large_us.whole, large_us.cut) + (others ? 8. : 0.) <
-           part_length(small, a.hkv, read_us(small)).first;
+    const double us = std::min(large_us.whole, large_us.cut) + (others ? 8. : 0.);
+    double least = 0.;  // what any cut of them takes
+    for (const Unit& u : small) least += (MEDIUM.fixed + MEDIUM.tile * (double)u.tiles) * a.hkv / PAGED_CUS;
+    many = us < least || us < part_length(small, a.hkv, read_us(small)).first;
   }
   if (!many) units[1].clear();
   for (int s = 0; s < a.seqs; ++s) {
@@ -387,7 +403,7 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
   for (int k = 0; k < 2; ++k) {
     if (units[k].empty()) continue;
     std::vector<Share> shares;
-    std::vector<std::pair<int, int>> same;  // the sequence of a share, and which of its parts
+    std::vector<int> same;  // a number for each sequence and part of its keys: which a share has
     if (k == 0) {
       const auto longest = [](const Unit& x, const Unit& y) { return x.tiles > y.tiles; };
       std::stable_sort(units[0].begin(), units[0].end(), longest);
@@ -402,12 +418,21 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
         }
       }
       const int64_t len = best.second;
-      int group = 0;
+      int group = 0, numbers = 0;
+      std::vector<std::pair<int, int>> number(a.seqs);  // (of a sequence the first, how many)
+      for (const Unit& u : units[0]) {
+        int& n = number[u.seq].second;
+        n = std::max(n, (int)((u.tiles + len - 1) / len));
+      }
+      for (auto& y : number) {
+        y.first = numbers;
+        numbers += std::max(1, y.second);
+      }
       for (int i = 0; i < (int)units[0].size(); ++i) {
         const int64_t tiles = units[0][i].tiles, n = std::max<int64_t>(1, (tiles + len - 1) / len);
         for (int64_t j = 0; j < n; ++j) {
           shares.push_back(Share{i, group++, tiles * j / n, tiles * (j + 1) / n});
-          same.emplace_back(units[0][i].seq, (int)j);
+          same.push_back(number[units[0][i].seq].first + (int)j);
         }
       }
     } else {
