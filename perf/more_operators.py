@@ -354,12 +354,14 @@ def _run_plain(st):
 
 def _prepare_own(state):
     from diffusorrt_amd.paged import PagedKVCache
-    from diffusorrt_amd.rotary import RotaryPositions
+    from diffusorrt_amd.rotary import RotaryPositions, rotary_frequencies
 
     case = state["case"]
-    if case["kind"] != "attend":  # the frequencies that a model keeps
-        state["rotary"] = RotaryPositions(case.get("dim", HD), theta=THETA,
-                                          layout=case["layout"], scaling=_scaling(case))
+    if case["kind"] != "attend":  # the frequencies that a model keeps (yarn's by turns, as above)
+        dim = case.get("dim", HD)
+        frequencies, magnitude = rotary_frequencies(dim, THETA, _scaling(case))
+        state["rotary"] = RotaryPositions(dim, layout=case["layout"], frequencies=frequencies,
+                                          magnitude=magnitude)
     if case["kind"] == "rotate":
         return state
     hq, hkv = HEADS[case["arch"]]
