@@ -47,7 +47,7 @@ def rotary_frequencies(dim: int, theta: float = 1e6, scaling=None):
     * ``yarn``: pair i makes r = original_max_position_embeddings * f / 2 pi turns over the
       original positions; f stays where r >= beta_fast (32), is divided by s where r <= beta_slow
       (1), and lies between the two in proportion to r (arXiv 2309.00071, 3.2). The magnitude is
-      ``attention_factor``, by default 0.1 ln s + 1.
+      ``attention_factor``, by default 0.1 ln s + 1, or 1 for a factor of no more than 1.
     """
     return _frequencies(dim, theta, scaling, _kept_by_turns)
 
@@ -110,7 +110,7 @@ def _frequencies(dim, theta, scaling, kept):
         raise ValueError("yarn scaling needs beta_fast > beta_slow")
     out = [f * (keep + (1.0 - keep) / factor)
            for f, keep in zip(plain, kept(dim, theta, plain, original, fast, slow))]
-    return out, _number(scaling, "attention_factor", 0.1 * math.log(factor) + 1.0)
+    return out, _number(scaling, "attention_factor", 0.1 * math.log(max(factor, 1.0)) + 1.0)
 
 
 def _turns(f: float) -> int:

@@ -91,3 +91,12 @@ def test_a_yarn_without_a_ramp_is_refused(dim, theta, original):
         configured_frequencies(dim, theta, scaling)
     with pytest.raises(ValueError, match="yarn"):
         RotaryPositions(dim, theta=theta, scaling=scaling, device="cpu")
+
+
+@pytest.mark.parametrize("frequencies", [configured_frequencies, rotary_frequencies])
+@pytest.mark.parametrize("factor", [1.0, 0.5, 1e-5])
+def test_yarn_of_no_extension_has_magnitude_one(frequencies, factor):
+    scaling = {"type": "yarn", "factor": factor, "original_max_position_embeddings": 4096}
+    assert frequencies(128, 1e6, scaling)[1] == 1.0
+    assert frequencies(128, 1e6, scaling | {"attention_factor": 0.25})[1] == 0.25
+    assert frequencies(128, 1e6, scaling | {"factor": 1 + 2.0**-20})[1] > 1.0
