@@ -81,6 +81,16 @@ def _kept_by_index(dim, theta, plain, original, fast, slow):
 
 
 def _frequencies(dim, theta, scaling, kept):
+    try:
+        frequencies, magnitude = _scaled(dim, theta, scaling, kept)
+    except (OverflowError, ZeroDivisionError):
+        frequencies = [math.inf]
+    if not all(map(math.isfinite, frequencies)):
+        raise ValueError("rotary frequencies of this theta and scaling are beyond a double")
+    return frequencies, magnitude
+
+
+def _scaled(dim, theta, scaling, kept):
     if isinstance(dim, bool) or not isinstance(dim, int) or dim < 2 or dim % 2:
         raise ValueError("rotary dim must be an even number from 2 on")
     theta = float(theta)
@@ -149,8 +159,9 @@ class RotaryPositions:
     ``layout``: ``"half"`` pairs elements ``(i, i + dim / 2)``, ``"interleaved"``
     ``(2 i, 2 i + 1)``. ``theta`` and ``scaling`` (a configuration's ``rope_scaling``) as in
     :func:`configured_frequencies`; or ``frequencies``, ``dim / 2`` radians a position of any other
-    form, and ``magnitude`` (so :func:`rotary_frequencies` gives the paper's yarn). The frequencies are kept as 64-bit fractions of a turn on ``device`` (the current GPU): an angle is
-    right to 2^-31 of a turn at any position of 32 bits, cosine and sine to 2^-22."""
+    form, and ``magnitude`` (so :func:`rotary_frequencies` gives the paper's yarn). The frequencies
+    are kept as 64-bit fractions of a turn on ``device`` (the current GPU): an angle is right to
+    2^-31 of a turn at any position of 32 bits, cosine and sine to 2^-22."""
 
     def __init__(self, dim: int = 128, *, theta: float = 1e6, layout: str = "half", scaling=None,
                  frequencies=None, magnitude=None, device=None):
@@ -169,8 +180,8 @@ class RotaryPositions:
                     not all(math.isfinite(f) for f in self.frequencies):
                 raise ValueError("rotary frequencies must be dim / 2 finite numbers")
             self.magnitude = 1.0 if magnitude is None else float(magnitude)
-            if not math.isfinite(self.magnitude):
-                raise ValueError("rotary magnitude must be finite")
+        if not abs(self.magnitude) <= torch.finfo(torch.float32).max:
+            raise ValueError("rotary magnitude must be a finite number of fp32")
         self.dim, self.layout = dim, layout
         self.turns = torch.tensor([_turns(f) for f in self.frequencies], dtype=torch.int64,
                                   device=device or "cuda")

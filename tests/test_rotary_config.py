@@ -100,3 +100,18 @@ def test_yarn_of_no_extension_has_magnitude_one(frequencies, factor):
     assert frequencies(128, 1e6, scaling)[1] == 1.0
     assert frequencies(128, 1e6, scaling | {"attention_factor": 0.25})[1] == 0.25
     assert frequencies(128, 1e6, scaling | {"factor": 1 + 2.0**-20})[1] > 1.0
+
+
+@pytest.mark.parametrize("call", [
+    dict(theta=5e-324),                                      # theta^-126/128 is beyond a double
+    dict(scaling={"type": "linear", "factor": 1e-320}),      # so is the first pair's 1 / factor
+    dict(scaling={"type": "ntk", "factor": 1e308}),          # and the base
+    dict(scaling={"type": "ntk", "factor": 5e-324}),         # a base of 0
+    dict(scaling={"type": "yarn", "factor": 1e-320, "original_max_position_embeddings": 4096}),
+    dict(frequencies=[1.0] * 64, magnitude=1e39),            # infinity in fp32
+    dict(scaling={"type": "yarn", "factor": 2.0, "original_max_position_embeddings": 4096,
+                  "attention_factor": 1e39}),
+])
+def test_frequencies_and_magnitudes_beyond_their_types_are_refused(call):
+    with pytest.raises(ValueError):
+        RotaryPositions(**({"device": "cpu"} | call))
