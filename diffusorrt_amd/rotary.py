@@ -205,6 +205,8 @@ class RotaryPositions:
         if len(shape) != 3 or shape[2] < self.dim:
             raise ValueError(f"rotate takes x [rows, heads, head_dim >= {self.dim}]")
         rows, heads, hd = shape
+        if rows > _I32_MAX or heads > _I32_MAX or hd > _I32_MAX:
+            raise ValueError("rotate takes fewer than 2^31 rows, heads and elements of a head")
         code = _TYPES.get(x.dtype)
         if code is None:
             raise ValueError("rotate takes float32, float16 or bfloat16")
