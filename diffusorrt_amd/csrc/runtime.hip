@@ -3009,6 +3009,7 @@ int32_t drt_op_rotate(const void* x, int64_t x_row_stride, int64_t x_head_stride
     const uintptr_t align = r.type == 0 ? 3 : 1;
     DRT_REQUIRE((((uintptr_t)x | (uintptr_t)y) & align) == 0 && ((uintptr_t)positions & 3) == 0,
             "rotate: unaligned tensors");
+    DRT_REQUIRE(positions || (int64_t)pos0 + rows - 1 <= INT32_MAX, "rotate: positions must be of 32 bits");
     r.rotary = turns_of(rotary, hd, "rotate");
     r.x = x;
     r.y = y;

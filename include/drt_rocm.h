@@ -376,7 +376,8 @@ typedef struct drt_rotary {
 /* x [rows, heads, hd] of dtype (DRT_F32, DRT_F16, DRT_BF16) to y, the same type and shape, elements
  * beyond dim as they are; strides in elements, a head's elements side by side. y may be x (the same
  * strides) and must not overlap it otherwise. Row r is at positions[r] (int32 [rows] on the device) or,
- * with positions NULL, at pos0 + r; negative positions turn backwards, as inverse != 0 does. */
+ * with positions NULL, at pos0 + r (of 32 bits for every row); negative positions turn backwards, as
+ * inverse != 0 does. */
 int32_t drt_op_rotate(const void* x, int64_t x_row_stride, int64_t x_head_stride, int32_t dtype,
                       int32_t rows, int32_t heads, int32_t hd, const drt_rotary* rotary,
                       const int32_t* positions, int32_t pos0, int32_t inverse, void* y,
