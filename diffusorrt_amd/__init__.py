@@ -7,7 +7,7 @@ Layers:
   * :mod:`.runtime`  -- ``Runtime`` / ``DeviceSession`` (the device-session contract);
   * :mod:`.decode`   -- host control plane of the fixed-quota strategies;
   * :mod:`.kernels`  -- per-op kernel table (rms_norm / linear / rope / swiglu / attention);
-  * :mod:`.rotary`   -- rotary positions of any form (``RotaryPositions``);
+  * :mod:`.rotary`   -- rotary positions (``RotaryPositions``);
   * :mod:`.paged`    -- a K/V cache in pages that sequences share, its appends and attention
     (``PagedKVCache``);
   * :mod:`.synthetic` -- seeded synthetic models and inputs for the workloads.

@@ -1,4 +1,5 @@
-"""Rotary positions of any form the models' configurations name: :class:`RotaryPositions`.
+"""Rotary positions: :class:`RotaryPositions`, of plain frequencies, linear, ntk and yarn scalings,
+or frequencies of the caller's (other forms that configurations name are refused by their name).
 
 :func:`.kernels.rope` takes fp32 rows and tables of the caller's (the reference's seam); here the
 frequencies are kept and the angles made where they are used, for any 32-bit position.
@@ -7,8 +8,11 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import numbers
+import operator
 from fractions import Fraction
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -27,10 +31,19 @@ _SCALING_FIELDS = {
 
 def _number(scaling, key, default=None):
     value = scaling.get(key, default)
-    if isinstance(value, bool) or not isinstance(value, (int, float)) or \
+    if isinstance(value, bool) or not isinstance(value, numbers.Real) or \
             not math.isfinite(value) or value <= 0:
         raise ValueError(f"rope scaling needs a positive {key}")
     return float(value)
+
+
+def _whole(value, what):
+    try:
+        if isinstance(value, (bool, np.bool_)):
+            raise TypeError
+        return operator.index(value)
+    except TypeError:
+        raise ValueError(f"{what} must be a whole number")
 
 
 def rotary_frequencies(dim: int, theta: float = 1e6, scaling=None):
@@ -91,7 +104,8 @@ def _frequencies(dim, theta, scaling, kept):
 
 
 def _scaled(dim, theta, scaling, kept):
-    if isinstance(dim, bool) or not isinstance(dim, int) or dim < 2 or dim % 2:
+    dim = _whole(dim, "rotary dim")
+    if dim < 2 or dim % 2:
         raise ValueError("rotary dim must be an even number from 2 on")
     theta = float(theta)
     if not (math.isfinite(theta) and theta > 0):
@@ -167,6 +181,7 @@ class RotaryPositions:
                  frequencies=None, magnitude=None, device=None):
         if layout not in _LAYOUTS:
             raise ValueError(f"rotary layout is 'half' or 'interleaved', not {layout!r}")
+        dim = _whole(dim, "rotary dim")
         if frequencies is None:
             if magnitude is not None:
                 raise ValueError("magnitude comes with frequencies of the caller's own")
@@ -175,9 +190,8 @@ class RotaryPositions:
             if scaling is not None:
                 raise ValueError("rotary takes either scaling or frequencies")
             self.frequencies = [float(f) for f in frequencies]
-            if isinstance(dim, bool) or not isinstance(dim, int) or dim < 2 or \
-                    2 * len(self.frequencies) != dim or \
-                    not all(math.isfinite(f) for f in self.frequencies):
+            if dim < 2 or 2 * len(self.frequencies) != dim or not all(
+                    map(math.isfinite, self.frequencies)):
                 raise ValueError("rotary frequencies must be dim / 2 finite numbers")
             self.magnitude = 1.0 if magnitude is None else float(magnitude)
         if not abs(self.magnitude) <= torch.finfo(torch.float32).max:
@@ -223,9 +237,9 @@ class RotaryPositions:
                 raise ValueError("positions must be int32 [rows] on x's device, or a number")
             at, pos0 = positions.data_ptr(), 0
         else:
-            if isinstance(positions, bool) or not isinstance(positions, int):
-                raise ValueError("positions must be int32 [rows] on x's device, or a number")
             at, pos0 = None, positions
+            if type(positions) is not int:
+                pos0 = _whole(positions, "positions, where no int32 tensor on x's device,")
             if not (_I32_MIN <= pos0 and pos0 + rows - 1 <= _I32_MAX):
                 raise ValueError("positions must be of 32 bits")
         if out is None:

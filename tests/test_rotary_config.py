@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import math
 
+import numpy as np
 import pytest
 
 from diffusorrt_amd.rotary import RotaryPositions, configured_frequencies, rotary_frequencies
@@ -115,3 +116,16 @@ def test_yarn_of_no_extension_has_magnitude_one(frequencies, factor):
 def test_frequencies_and_magnitudes_beyond_their_types_are_refused(call):
     with pytest.raises(ValueError):
         RotaryPositions(**({"device": "cpu"} | call))
+
+
+def test_numpy_numbers_are_numbers():
+    scaling = {"type": "yarn", "factor": np.float32(4), "original_max_position_embeddings": np.int64(4096)}
+    r = RotaryPositions(np.int64(64), theta=np.float64(1e4), scaling=scaling, device="cpu")
+    assert type(r.dim) is int and r.dim == 64
+    assert r.frequencies == configured_frequencies(
+        64, 1e4, {"type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096})[0]
+    own = RotaryPositions(np.int32(4), frequencies=np.array([1.0, 0.5], np.float32), device="cpu")
+    assert own.frequencies == [1.0, 0.5]
+    for dim in (np.float64(64), np.True_, "64"):
+        with pytest.raises(ValueError):
+            RotaryPositions(dim, device="cpu")
