@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from .kernels import KV_TILE_ELEMS, _cache_dtype, _launch, _mask_args
-from .rotary import _TYPES
+from .rotary import _TYPES, _lend
 
 _I32_MAX = 2**31 - 1
 
@@ -246,6 +246,8 @@ class PagedKVCache:
                 raise ValueError("append's rotary must turn a multiple of 16 elements, 128 at "
                                  "most, on the cache's device")
             turns = rotary._address
+            if torch._C._cuda_getCurrentRawStream(index) not in rotary._streams:
+                _lend(rotary.turns, index, rotary._streams)
         if q is None:
             out = q_at = out_at = None
             q0 = q1 = 0

@@ -167,6 +167,16 @@ def _same_places(a, b) -> bool:
 _TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
+def _lend(tensor, index, streams):
+    """The current stream, none of the tensor's ``streams`` yet, reads it: the allocator is told, so
+    that dropping the tensor does not give its memory away under a launch. (In a capture there is
+    nothing to tell: what a graph reads is the caller's to keep.)"""
+    with torch.cuda.device(index):
+        if not torch.cuda.is_current_stream_capturing():
+            tensor.record_stream(torch.cuda.current_stream(index))
+            streams.add(torch._C._cuda_getCurrentRawStream(index))
+
+
 class RotaryPositions:
     """The rotation of the first ``dim`` elements of heads by their rows' positions.
 
@@ -175,7 +185,8 @@ class RotaryPositions:
     :func:`configured_frequencies`; or ``frequencies``, ``dim / 2`` radians a position of any other
     form, and ``magnitude`` (so :func:`rotary_frequencies` gives the paper's yarn). The frequencies
     are kept as 64-bit fractions of a turn on ``device`` (the current GPU): an angle is right to
-    2^-31 of a turn at any position of 32 bits, cosine and sine to 2^-22."""
+    2^-31 of a turn at any position of 32 bits, cosine and sine to 2^-22. Any stream may use them;
+    keep the object as long as a captured graph that used it is replayed."""
 
     def __init__(self, dim: int = 128, *, theta: float = 1e6, layout: str = "half", scaling=None,
                  frequencies=None, magnitude=None, device=None):
@@ -200,6 +211,8 @@ class RotaryPositions:
         self.turns = torch.tensor([_turns(f) for f in self.frequencies], dtype=torch.int64,
                                   device=device or "cuda")
         self._index = self.turns.get_device()
+        # (they are on the device: the copy of pageable memory waits for itself)
+        self._streams = {torch._C._cuda_getCurrentRawStream(self._index)} if self._index >= 0 else ()
         self._args = _lib.Rotary(self.turns.data_ptr(), dim, int(layout == "interleaved"),
                                  self.magnitude)
         self._address = C.addressof(self._args)
@@ -256,6 +269,8 @@ class RotaryPositions:
                 if a < d and c < b:
                     raise ValueError("out must be x itself or memory apart from it")
         if rows and heads:
+            if torch._C._cuda_getCurrentRawStream(index) not in self._streams:
+                _lend(self.turns, index, self._streams)
             _launch(torch, self._rotate or self._bind(), index, x.data_ptr(), x0, x1, code, rows,
                     heads, hd, self._address, at, pos0, 1 if inverse else 0, out.data_ptr(), y0, y1)
         return out
