@@ -157,7 +157,11 @@ class PagedKVCache:
     ``"bf16"``. Pages hold the 32-key tiles of :class:`.kernels.PrefixKVCache`.
 
     Which pages a sequence has, and in which order, is the caller's: :meth:`batch` takes the
-    lists. A page may be given to another sequence without clearing it."""
+    lists. A page may be given to another sequence without clearing it.
+
+    Calls may be on any stream; a call that reads what another stream's wrote waits for it (the
+    caller's to see to, as for any tensor). Keep the cache as long as a captured graph that used it
+    is replayed."""
 
     def __init__(self, layers: int, kv_heads: int, pages: int, *, page_size: int = 64,
                  dtype="f16", device=None):
@@ -173,10 +177,20 @@ class PagedKVCache:
         if self.kv_dtype == _lib.I8:
             raise ValueError("a paged cache's dtype is 'f16' or 'bf16'")
         self.dtype = torch.bfloat16 if self.kv_dtype == _lib.BF16 else torch.float16
+        device = torch.device(device or "cuda")
+        if device.type == "cuda":
+            with torch.cuda.device(device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise ValueError("a cache is made before a graph is captured, not in it")
         self.data = torch.zeros((self.layers, self.pages, self.kv_heads,
                                  self.page_size // 32 * KV_TILE_ELEMS), dtype=self.dtype,
-                                device=device or "cuda")
+                                device=device)
         self._index = self.data.get_device()
+        self._streams = ()
+        if self._index >= 0:  # the zeros are there before any stream writes rows
+            stream = torch.cuda.current_stream(self._index)
+            stream.synchronize()
+            self._streams = {stream.cuda_stream}
         self._geometry = (self.kv_heads, self.pages, self.page_size, self._index)
         self._data, self._layer_bytes = self.data.data_ptr(), self.data.stride(0) * 2
         self._lib = None
@@ -210,6 +224,8 @@ class PagedKVCache:
         if not isinstance(batch, PagedBatch) or (batch._geometry is not self._geometry and
                                                  batch._geometry != self._geometry):
             raise ValueError("the batch was planned for another cache")
+        if torch._C._cuda_getCurrentRawStream(self._index) not in self._streams:
+            _lend(self.data, self._index, self._streams)
         if self._lib is None:
             self._lib = _lib.load()
         return self._lib

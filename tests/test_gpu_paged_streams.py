@@ -1,0 +1,57 @@
+"""The paged cache on other streams than its own."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from diffusorrt_amd.paged import PagedKVCache
+
+pytestmark = pytest.mark.gpu
+BUSY = 20_000_000  # cycles, about 10 ms
+
+
+def _randn(seed, *shape, dtype=torch.float16):
+    return torch.from_numpy(np.random.default_rng(seed).standard_normal(shape, np.float32)).cuda().to(dtype)
+
+
+def test_the_zeros_do_not_overtake_another_streams_rows():
+    k, v = _randn(1, 40, 3, 128), _randn(2, 40, 3, 128)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(BUSY)
+    cache = PagedKVCache(1, 3, 4)
+    with torch.cuda.stream(side):
+        batch = cache.batch([[2]], [40], [40], heads=3)
+        cache.append(0, k, v, batch)
+    torch.cuda.synchronize()
+    k2, v2 = cache.load(0, batch)
+    assert torch.equal(k2, k) and torch.equal(v2, v)
+
+
+def test_a_cache_dropped_after_a_call_on_another_stream():
+    k, v = _randn(3, 40, 3, 128), _randn(4, 40, 3, 128)
+    cache = PagedKVCache(1, 3, 2)
+    batch = cache.batch([[1]], [40], [40], heads=3)
+    cache.append(0, k, v, batch)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(BUSY)
+        k2, v2 = cache.load(0, batch)
+    n = cache.data.numel()
+    del cache
+    taken = [torch.ones(n, dtype=torch.float16, device="cuda") for _ in range(16)]
+    torch.cuda.synchronize()
+    assert torch.equal(k2, k) and torch.equal(v2, v) and len(taken) == 16
+
+
+def test_no_cache_is_made_in_a_capture():
+    x = torch.zeros(4, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError, match="captured"):
+            PagedKVCache(1, 1, 1)
+        x += 1
+    graph.replay()
+    assert torch.equal(x.cpu(), torch.ones(4))
