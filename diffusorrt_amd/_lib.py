@@ -157,6 +157,7 @@ SIGNATURES = {
                              _I32, _VP, _I64, _I64, _VP]),
     "drt_paged_plan": (_I32, [_VP, _I32, _I32, _VP, _VP, _VP, _VP, _I32, _I32, _I32, _I32, _I32,
                               _I32, _VP, _I64, C.POINTER(PagedBatch)]),
+    "drt_event_wait": (_I32, [_VP]),
     "drt_op_paged_append": (_I32, [_VP, _VP, _VP, _I64, _I64, _VP, _I64, _I64,
                                    _VP, _I64, _I64, _I32, _VP, _VP, _I32, _VP, _VP]),
     "drt_op_paged_load": (_I32, [_VP, _VP, _VP, _I32, _VP, _VP, _VP]),

@@ -3084,6 +3084,18 @@ int32_t drt_paged_plan(const int32_t* table, int32_t width, int32_t seqs, const 
   });
 }
 
+int32_t drt_event_wait(void* event) {
+  return guarded([&] {
+    DRT_REQUIRE(event, "event_wait needs an event");
+    // (a capture forbids its thread waits, but for those that it says are none of the capture's)
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    DRT_HIP(hipThreadExchangeStreamCaptureMode(&mode));
+    const hipError_t waited = hipEventSynchronize((hipEvent_t)event);
+    DRT_HIP(hipThreadExchangeStreamCaptureMode(&mode));
+    DRT_HIP(waited);
+  });
+}
+
 int32_t drt_op_paged_append(const drt_paged_batch* batch, const int32_t* list, const void* k,
                             int64_t k_row_stride, int64_t k_head_stride, const void* v,
                             int64_t v_row_stride, int64_t v_head_stride, const void* q,

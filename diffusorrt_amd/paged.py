@@ -61,8 +61,10 @@ class PagedBatch:
     differ in its last bits beside other sequences."""
 
     def __init__(self, cache, table, keys, rows, heads, positions, kind, mask_geometry):
-        if cache._index >= 0 and torch.cuda.is_current_stream_capturing():
-            raise ValueError("a batch is planned before a graph is captured, not in it")
+        if cache._index >= 0:
+            with torch.cuda.device(cache._index):
+                if torch.cuda.is_current_stream_capturing():
+                    raise ValueError("a batch is planned before a graph is captured, not in it")
         table = _table(table)
         if isinstance(heads, bool) or not isinstance(heads, int) or abs(heads) > _I32_MAX:
             raise ValueError("heads must be a whole number")
@@ -143,12 +145,19 @@ class PagedBatch:
     def _here(self) -> int:
         """The list's address, for the current stream."""
         if torch._C._cuda_getCurrentRawStream(self._index) != self._stream:
-            # (while a stream is captured its other work is done: capturing began with a wait)
-            if not torch.cuda.is_current_stream_capturing():
-                stream = torch.cuda.current_stream(self._index)
-                stream.wait_event(self._ready)
-                self._list.record_stream(stream)
+            self._elsewhere()
         return self._at
+
+    def _elsewhere(self):
+        """The list is used on a stream that is not the one it was copied on."""
+        with torch.cuda.device(self._index):
+            if torch.cuda.is_current_stream_capturing():
+                # (a stream's wait would become the graph's, and the copy is no part of it)
+                _lib.check(_lib.load().drt_event_wait(self._ready.cuda_event))
+                return
+            stream = torch.cuda.current_stream(self._index)
+            stream.wait_event(self._ready)
+            self._list.record_stream(stream)
 
 
 class PagedKVCache:

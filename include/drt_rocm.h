@@ -408,6 +408,10 @@ int32_t drt_paged_plan(const int32_t* table, int32_t width, int32_t seqs, const 
                        int32_t page_size, int32_t pages, int32_t hq, int32_t hkv, int32_t mask_kind,
                        int32_t mask_block_size, int32_t* list, int64_t list_words,
                        drt_paged_batch* batch);
+/* Waits on the host for the work before the record of a hipEvent_t, also while the calling thread captures
+ * a stream: what a graph reads but does not write (a batch's list) has to be there before a replay. The
+ * event's own record is no part of a capture. */
+int32_t drt_event_wait(void* event);
 /* The batch's k, v [rows, hkv, 128] (src_dtype DRT_F32, DRT_F16 or DRT_BF16; strides in elements) into
  * their places in one layer's cache (kv_dtype DRT_F16 or DRT_BF16), keys turned by their positions on
  * the way where rotary is given (dim <= 128, a multiple of 16); an appendable batch's. q [rows, hq, 128], where given, is turned

@@ -55,3 +55,36 @@ def test_no_cache_is_made_in_a_capture():
         x += 1
     graph.replay()
     assert torch.equal(x.cpu(), torch.ones(4))
+
+
+@pytest.mark.parametrize("bare", [False, True])
+def test_a_batch_is_on_the_device_before_a_captured_graph_is_replayed(bare):
+    k, v, q = _randn(5, 300, 2, 128), _randn(6, 300, 2, 128), _randn(7, 3, 4, 128)
+    cache = PagedKVCache(1, 2, 8)
+    pages, rows = [[7, 2, 5, 0, 3]], [300]
+    cache.append(0, k, v, cache.batch(pages, rows, rows, heads=4))
+    want = cache.attention(0, q, cache.batch(pages, rows, [3], heads=4))
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    if bare:  # no wait begins it
+        torch.cuda._sleep(BUSY)
+        batch = cache.batch(pages, rows, [3], heads=4)
+        with torch.cuda.stream(side):
+            graph.capture_begin()
+            out = cache.attention(0, q, batch)
+            graph.capture_end()
+            graph.replay()
+    else:
+        batch = cache.batch(pages, rows, [3], heads=4)
+        with torch.cuda.graph(graph, stream=side):
+            out = cache.attention(0, q, batch)
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    for _ in range(3):
+        out.zero_()
+        eager = cache.attention(0, q, batch)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(eager, want)
