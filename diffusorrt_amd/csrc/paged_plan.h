@@ -79,7 +79,7 @@ inline std::string paged_check(const PagedBatchArgs& a) {
     return "a batch has a sequence at least, and rows, keys and positions of each";
   if (a.hkv < 1 || a.hq < 1 || a.hq % a.hkv || a.hq > 16384)
     return "query heads must be a multiple of the K/V heads, 16384 at most";
-  if (a.pages < 1 || (int64_t)a.pages * a.hkv * (a.page_size / 32) > INT32_MAX)
+  if (a.pages < 1 || a.pages > INT32_MAX / ((int64_t)a.hkv * (a.page_size / 32)))
     return "a layer has at most 2^31 - 1 tiles of 32 keys and one head";
   if (a.masked && a.block < 1) return "bad mask geometry";
   int64_t total = 0;

@@ -1,6 +1,8 @@
 """What the paged cache's C entries refuse, on the CPU."""
 from __future__ import annotations
 
+import ctypes as C
+
 import pytest
 
 from diffusorrt_amd import _lib
@@ -10,3 +12,30 @@ pytestmark = pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="library not 
 
 def test_no_event_is_refused():
     assert _lib.load().drt_event_wait(None) == _lib.INVALID_ARGUMENT
+
+
+def _plan(page_size, pages, hq, hkv, keys=(1,), rows=(1,), table=None, width=1):
+    n = len(keys)
+    i32 = C.c_int32 * n
+    table = (C.c_int32 * (n * width))() if table is None else table
+    info = _lib.PagedBatch()
+    status = _lib.load().drt_paged_plan(
+        C.addressof(table) if isinstance(table, C.Array) else table.ctypes.data, width, n, i32(*rows),
+        i32(*keys), i32(*[k - r for k, r in zip(keys, rows)]), None, page_size, pages, hq, hkv,
+        _lib.MASK_BIDIRECTIONAL, 1, None, 0, info)
+    return status, info
+
+
+@pytest.mark.parametrize("page_size, pages, hkv", [
+    (2**25, 2**30, 2**14),      # 2^20 * 2^30 * 2^14 tiles: 2^64
+    (2**30, 2**30, 2**14),      # 2^69
+    (2**30, 2**31 - 1, 2**13),  # a product whose 64 bits are negative
+    (32, 2**31 - 1, 2), (2**30, 64, 1)])
+def test_layers_of_more_tiles_than_31_bits_are_refused(page_size, pages, hkv):
+    status, _ = _plan(page_size, pages, hkv, hkv)
+    assert status == _lib.INVALID_ARGUMENT and "tiles" in _lib.last_error()
+
+
+def test_the_largest_layer_is_taken():
+    assert _plan(32, 2**31 - 1, 7, 1)[0] == _lib.OK
+    assert _plan(2**30, 63, 1, 1)[0] == _lib.OK
