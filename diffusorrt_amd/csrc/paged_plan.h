@@ -82,7 +82,9 @@ inline std::string paged_check(const PagedBatchArgs& a) {
   if (a.pages < 1 || a.pages > INT32_MAX / ((int64_t)a.hkv * (a.page_size / 32)))
     return "a layer has at most 2^31 - 1 tiles of 32 keys and one head";
   if (a.masked && a.block < 1) return "bad mask geometry";
-  int64_t total = 0;
+  int64_t total = 0, listed = 0;
+  for (int s = 0; s < a.seqs; ++s) listed += (std::max(a.keys[s], 0) + (int64_t)a.page_size - 1) / a.page_size;
+  if (listed > INT32_MAX) return "too many pages for one batch";
   for (int s = 0; s < a.seqs; ++s) {
     const int64_t rows = a.rows[s], keys = a.keys[s], pos0 = a.pos0[s];
     if (rows < 0 || keys < 0 || pos0 < 0 || pos0 + rows > INT32_MAX)

@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import ctypes as C
 
+import numpy as np
 import pytest
 
 from diffusorrt_amd import _lib
@@ -39,3 +40,11 @@ def test_layers_of_more_tiles_than_31_bits_are_refused(page_size, pages, hkv):
 def test_the_largest_layer_is_taken():
     assert _plan(32, 2**31 - 1, 7, 1)[0] == _lib.OK
     assert _plan(2**30, 63, 1, 1)[0] == _lib.OK
+
+
+def test_lists_of_more_pages_than_31_bits_are_refused():
+    # 33 sequences of 2^26 - 2 pages each (one page again and again: zeros that no memory stands behind)
+    width = 2**26 - 2
+    table = np.zeros(33 * width, dtype=np.int32)
+    status, _ = _plan(32, 1, 1, 1, keys=[width * 32 - 1] * 33, rows=[1] * 33, table=table, width=width)
+    assert status == _lib.INVALID_ARGUMENT and "pages" in _lib.last_error()
