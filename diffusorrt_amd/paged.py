@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from .kernels import KV_TILE_ELEMS, _cache_dtype, _launch, _mask_args
-from .rotary import _TYPES, _lend
+from .rotary import _TYPES, _lend, _whole
 
 _I32_MAX = 2**31 - 1
 
@@ -66,7 +66,8 @@ class PagedBatch:
                 if torch.cuda.is_current_stream_capturing():
                     raise ValueError("a batch is planned before a graph is captured, not in it")
         table = _table(table)
-        if isinstance(heads, bool) or not isinstance(heads, int) or abs(heads) > _I32_MAX:
+        heads = _whole(heads, "heads")
+        if abs(heads) > _I32_MAX:
             raise ValueError("heads must be a whole number")
         keys, rows = _whole_numbers(keys, "keys"), _whole_numbers(rows, "rows")
         seqs = table.shape[0]

@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 
 from diffusorrt_amd import _lib
+from diffusorrt_amd.paged import PagedKVCache
 
 pytestmark = pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="library not built")
 
@@ -48,3 +49,11 @@ def test_lists_of_more_pages_than_31_bits_are_refused():
     table = np.zeros(33 * width, dtype=np.int32)
     status, _ = _plan(32, 1, 1, 1, keys=[width * 32 - 1] * 33, rows=[1] * 33, table=table, width=width)
     assert status == _lib.INVALID_ARGUMENT and "pages" in _lib.last_error()
+
+
+def test_numpy_heads():
+    cache = PagedKVCache(1, 2, 4, device="cpu")
+    assert cache.batch([[1]], [3], [1], heads=np.int64(4)).heads == 4
+    for bad in (np.float64(4), True, np.True_, "4", None):
+        with pytest.raises(ValueError, match="whole number"):
+            cache.batch([[1]], [3], [1], heads=bad)
