@@ -88,3 +88,37 @@ def test_a_batch_is_on_the_device_before_a_captured_graph_is_replayed(bare):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(eager, want)
+
+
+@pytest.mark.parametrize("src", [torch.float32, torch.float16])
+def test_appends_of_other_rows_of_the_same_tiles_overlap_in_time(src):
+    # even rows' batches on one stream, odd ones on another: every tile is written by both at once, and
+    # both again and again, as neither waits for the other
+    size, hkv, n, times = 64, 4, 8, 6
+    cache = PagedKVCache(1, hkv, n, page_size=size)
+    pages = [[i] for i in range(n)]
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    halves = [(0, 7), (7, 20), (20, 33), (33, 45), (45, 50), (50, 64)]  # they part inside groups of eight
+    work = [[], []]
+    want = torch.zeros(2, n, size, hkv, 128, dtype=torch.float16, device="cuda")
+    for i, (lo, hi) in enumerate(halves):
+        k, v = (_randn(10 * i + j, n * (hi - lo), hkv, 128, dtype=src) for j in (0, 1))
+        batch = cache.batch(pages, [size] * n, [hi - lo] * n, heads=hkv, positions=[lo] * n)
+        want[0][:, lo:hi] = k.half().view(n, hi - lo, hkv, 128)
+        want[1][:, lo:hi] = v.half().view(n, hi - lo, hkv, 128)
+        work[i % 2].append((k, v, batch))
+    whole = cache.batch(pages, [size] * n, [size] * n, heads=hkv)
+    for _ in range(5):
+        cache.data.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for side in sides:
+            with torch.cuda.stream(side):
+                torch.cuda._sleep(BUSY // 10)  # both streams' appends are queued before either begins
+        for _ in range(times):
+            for side, calls in zip(sides, work):
+                with torch.cuda.stream(side):
+                    for k, v, batch in calls:
+                        cache.append(0, k, v, batch)
+        torch.cuda.synchronize()
+        k2, v2 = cache.load(0, whole)
+        assert torch.equal(k2.view_as(want[0]), want[0]) and torch.equal(v2.view_as(want[1]), want[1])

@@ -44,7 +44,7 @@ def test_kernels_and_cuts(sequences, hq, hkv, small, large, cut):
 
 
 @pytest.mark.parametrize("sequences, hq, hkv, wide", [
-    ([(1337, 1)], 16, 8, 0), ([(16384, 1), (3000, 1)], 28, 4, 0), ([(8224, 32)] * 16, 16, 8, 1)])
+    ([(1337, 1)], 16, 8, 0), ([(16384, 1), (3000, 1)], 28, 4, 0), ([(300 + 500 * i, 32) for i in range(16)], 16, 8, 1)])
 def test_units_of_32_and_of_64_query_vectors(sequences, hq, hkv, wide):
     info, words = _plan(sequences, hq, hkv)
     pieces = words[info.small:info.small + 16 * info.n_small].reshape(-1, 16)
