@@ -115,14 +115,19 @@ struct Unit {
 
 // Times in us. A part: `fixed` (its queries in, its result out) and `tile` for 32 keys, on its CU; where
 // units read the same keys side by side those come from the L2, else each is `alone` in waiting for memory;
-// `join`: the second launch that a cut needs. Fitted to 157 batches of 1 to 48 sequences (1 to 1000 rows,
-// 300 to 60000 keys, 16 heads on 8, 28 on 4, 32 on 2), in each of which units of 32 and of 64 were timed at
-// several cuts: what these times choose is 2.4 % slower on average than the fastest seen in each (choosing by
-// one cost a tile for all was 11 %).
+// JOIN, LARGE_JOIN: the second launch that a cut needs. Of 181 batches of 1 to 48 sequences (1 to 1000 rows, 300 to
+// 60000 keys, 16 heads on 8, 28 on 4, 32 on 2; profiles/paged_plan_batches.csv) what these times choose is
+// 2.2 % slower on average than the fastest of both units at up to 15 lengths of parts, in 30 of them by more
+// than 5 %, by 25 % at worst (48 tokens x 28 heads over 12000 keys: 134 us, 108 in parts a quarter as long).
 struct Costs {
-  double fixed, tile, join, alone;
+  double fixed, tile, alone;
 };
-constexpr Costs SMALL{5., 0.147, 3.3, 0.143}, MEDIUM{7., 0.235, 3.3, 0.13}, LARGE{12., 0.74, 20., 0.};
+constexpr Costs SMALL{5., 0.147, 0.143}, MEDIUM{7., 0.235, 0.13}, LARGE{12., 0.74, 0.};
+constexpr double JOIN = 3.3, LARGE_JOIN = 20.;
+// What the large kernel's equal shares are cut by: a tile counts for more than in a whole unit's time. Cut by
+// LARGE, eight of ten batches take 0 to 2 % longer (700 rows x 28 heads over 16000 keys 200 us for 196, 2048 over
+// 70000 1830 for 1821; 1400 rows x 64 heads beside tokens 933 for 947).
+constexpr Costs LARGE_SHARES{12., 0.875, 0.};
 // The part [tile0, tile1) of unit `unit` for work-group `group`.
 struct Share {
   int unit, group;
@@ -238,7 +243,7 @@ inline std::pair<double, int64_t> part_length(const std::vector<Unit>& units, in
     if (most_cuts > 128) break;
     const double own = makespan(parts, PAGED_CUS), all = SMALL.fixed + all_us;
     const double us = std::sqrt(std::sqrt(own * own * own * own + all * all * all * all)) +
-                      (cuts ? SMALL.join + 0.008 * (double)(cuts * hkv) : 0.);
+                      (cuts ? JOIN + 0.008 * (double)(cuts * hkv) : 0.);
     if (best < 0. || us < best) {
       best = us;
       best_len = len;
@@ -269,7 +274,7 @@ inline LargeTimes large_times(const std::vector<Unit>& units, int hkv) {
     sum += parts.back().first;
   }
   y.whole = makespan(parts, PAGED_CUS);
-  y.cut = sum / groups + LARGE.fixed + LARGE.join + 0.009 * 8. * (double)(units.size() + groups) * hkv;
+  y.cut = sum / groups + LARGE.fixed + LARGE_JOIN + 0.009 * 8. * (double)(units.size() + groups) * hkv;
   return y;
 }
 
@@ -444,7 +449,7 @@ inline PagedPlanInfo paged_plan(const PagedBatchArgs& a, std::vector<int32_t>& o
                          [](const Unit& x, const Unit& y) { return x.tiles > y.tiles; });
         for (int i = 0; i < (int)units[1].size(); ++i) shares.push_back(Share{i, i, 0, units[1][i].tiles});
       } else {
-        shares = cut(units[1], std::max(1, PAGED_CUS / a.hkv), Costs{LARGE.fixed, 0.875, 0., 0.});
+        shares = cut(units[1], std::max(1, PAGED_CUS / a.hkv), LARGE_SHARES);
       }
     }
     for (size_t i = 0; i < shares.size();) {
