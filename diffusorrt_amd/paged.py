@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from .kernels import KV_TILE_ELEMS, _cache_dtype, _launch, _mask_args
-from .rotary import _TYPES, _lend, _whole
+from .rotary import _TYPES, _capturing, _lend, _whole
 
 _I32_MAX = 2**31 - 1
 
@@ -61,10 +61,8 @@ class PagedBatch:
     differ in its last bits beside other sequences."""
 
     def __init__(self, cache, table, keys, rows, heads, positions, kind, mask_geometry):
-        if cache._index >= 0:
-            with torch.cuda.device(cache._index):
-                if torch.cuda.is_current_stream_capturing():
-                    raise ValueError("a batch is planned before a graph is captured, not in it")
+        if cache._index >= 0 and _capturing(cache._index):
+            raise ValueError("a batch is planned before a graph is captured, not in it")
         table = _table(table)
         heads = _whole(heads, "heads")
         if abs(heads) > _I32_MAX:
@@ -151,14 +149,13 @@ class PagedBatch:
 
     def _elsewhere(self):
         """The list is used on a stream that is not the one it was copied on."""
-        with torch.cuda.device(self._index):
-            if torch.cuda.is_current_stream_capturing():
-                # (a stream's wait would become the graph's, and the copy is no part of it)
-                _lib.check(_lib.load().drt_event_wait(self._ready.cuda_event))
-                return
-            stream = torch.cuda.current_stream(self._index)
-            stream.wait_event(self._ready)
-            self._list.record_stream(stream)
+        if _capturing(self._index):
+            # (a stream's wait would become the graph's, and the copy is no part of it)
+            _lib.check(_lib.load().drt_event_wait(self._ready.cuda_event))
+            return
+        stream = torch.cuda.current_stream(self._index)
+        stream.wait_event(self._ready)
+        self._list.record_stream(stream)
 
 
 class PagedKVCache:

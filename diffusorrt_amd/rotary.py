@@ -167,14 +167,21 @@ def _same_places(a, b) -> bool:
 _TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
+def _capturing(index):
+    """Whether the current stream of device ``index`` is being captured."""
+    if torch._C._cuda_getDevice() == index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _lend(tensor, index, streams):
     """The current stream, none of the tensor's ``streams`` yet, reads it: the allocator is told, so
     that dropping the tensor does not give its memory away under a launch. (In a capture there is
     nothing to tell: what a graph reads is the caller's to keep.)"""
-    with torch.cuda.device(index):
-        if not torch.cuda.is_current_stream_capturing():
-            tensor.record_stream(torch.cuda.current_stream(index))
-            streams.add(torch._C._cuda_getCurrentRawStream(index))
+    if not _capturing(index):
+        tensor.record_stream(torch.cuda.current_stream(index))
+        streams.add(torch._C._cuda_getCurrentRawStream(index))
 
 
 class RotaryPositions:
