@@ -192,8 +192,9 @@ __global__ __launch_bounds__(256) void paged_load_kernel(const PagedTile* tiles,
   }
 }
 
-// Work-groups a tile that share its K/V heads: one each, or one for two where there are many tiles (loads, us with
-// one and two: 125 tiles x 8 heads 6.5 and 7.4, 16 x 8 3.8 and 4.6; 2000 x 8 both 21.6, where fewer begin).
+// Work-groups a tile that share its K/V heads: one each, or one for two where there are many tiles and half as
+// many do (us a head each and two: loads of 125 tiles x 8 heads 5.9 and 6.9, 42 x 8 3.9 and 4.7, 16 x 8 3.3 and 4.1;
+// 2000 x 8 100 and 101, its append 229 and 230 to 235).
 int heads_of(int n_tiles, int hkv) { return (int64_t)n_tiles * hkv <= 1024 ? hkv : (hkv + 1) / 2; }
 
 }  // namespace

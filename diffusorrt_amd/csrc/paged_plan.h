@@ -279,10 +279,11 @@ inline LargeTimes large_times(const std::vector<Unit>& units, int hkv) {
 }
 
 // The order of the small kernel's pieces: the longest first (lengths within 8 tiles are one: 32 rows x 28 heads
-// over 60000 keys 47 us by unit and part, 50 sorted to the tile). Work-groups go round the 8 XCDs, each with an
+// over 60000 keys 48.5 us, sorted to the tile 50.1). Work-groups go round the 8 XCDs, each with an
 // L2 of its own, and a piece's K/V heads follow one another: pieces of one sequence's same keys (`same`) are
-// put so that they come to the same XCDs, as long as there are others to take the places between (17 rows x
-// 28 heads on 4 over 16000 keys 15.1 us, of 60000 32.6; side by side in turn 16.4 and 36.1).
+// put so that they come to the same XCDs, as long as there are others to take the places between (eight
+// sequences of 9 rows x 28 heads over up to 2500 keys 12.1 us with their join, in the units' order 13.3; sixteen
+// of 32 rows 52 and 54; 17 or 32 rows alone alike).
 inline void side_by_side(std::vector<PagedPiece>& pieces, const std::vector<int>& same, int hkv) {
   int lanes = 8;
   for (int h = hkv; lanes > 1 && h % 2 == 0; h /= 2) lanes /= 2;

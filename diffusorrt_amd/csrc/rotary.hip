@@ -2,8 +2,8 @@
 //
 // Bound by its bytes, each read and written once: a thread makes the cosines and sines of 8 pairs (half
 // layout) or 4 (interleaved) once and turns those of one or two heads, 16 or 32 bytes a load. 8192 rows x 16 heads
-// of bf16: 11.8 us, 67 MB at 5.7 TB/s (a large copy's 4.85 is of more than the last-level cache holds); 1000
-// rows x 28 heads of fp32 7.3; one row 2.3, its launch.
+// of bf16: 11.8 us, 67 MB at 5.7 TB/s (a large copy's 4.9 is of more than the last-level cache holds); 1000
+// rows x 28 heads of fp32 7.0; one row 2.3, its launch.
 #include "launch.h"
 #include "rotary.h"
 
@@ -76,7 +76,8 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotateArgs a) {
   }
 }
 
-// Any even dim: a thread a pair, then one an element that is not turned.
+// Any even dim: a thread a pair, then one an element that is not turned. Bound by its index divisions and
+// narrow loads: 4096 rows x 16 heads of bf16, 72 of 128 elements 24.6 us, 34 MB at 1.4 TB/s; 250 of 256 31.7.
 template <int DT>
 __global__ __launch_bounds__(256) void rotate_any_kernel(const RotateArgs a, bool half) {
   const int pairs = a.dim / 2, per_head = pairs + (a.hd - a.dim);
@@ -128,8 +129,8 @@ void rotate(const RotateCall& r, hipStream_t s) {
     const int rest = r.x == r.y ? 0 : (a.hd - a.dim) / 8;  // (in place they are there already)
     a.items = turned + rest;
     // Two heads a thread, which share the angles, where that leaves work for the chip (bf16, us with two and
-    // one: 2048 rows x 16 heads 5.5 and 5.9, 4096 7.6 and 8.9, 8192 12.7 and 14.1, 1000 4.6 both; with four
-    // or eight as with two or, of 65536 rows, 6 to 28 % longer).
+    // one: 2048 rows x 16 heads 5.3 and 5.6, 4096 7.7 and 8.2, 8192 12.0 and 12.9, 65536 94 and 96, 1000 3.9 both;
+    // four take 0 to 7 % longer than two, eight 2 to 50 %).
     a.per = (int64_t)a.rows * a.items * a.heads > 131072 ? 2 : 1;
     a.groups = (a.heads + a.per - 1) / a.per;
     const int64_t threads = (int64_t)a.rows * a.items * a.groups;

@@ -55,8 +55,9 @@ def _table(pages):
 
 class PagedBatch:
     """New rows of several sequences, as :meth:`PagedKVCache.batch` plans them: made once a step,
-    it serves ``append``, ``attention`` and ``load`` of every layer, on any stream. Keep it as long
-    as a captured graph that used it is replayed. How an attention is cut among the work-groups
+    it serves ``append``, ``attention`` and ``load`` of every layer, on any stream. Its lengths and
+    pages are fixed, and none is planned inside a capture: a graph that used it is of its step
+    alone. Keep it as long as that graph is replayed. How an attention is cut among the work-groups
     follows from all of the batch's lengths: a row's result is the same from call to call, and may
     differ in its last bits beside other sequences."""
 
@@ -301,7 +302,11 @@ class PagedKVCache:
 
     def attention(self, layer: int, q, batch: PagedBatch, *, out_dtype=None):
         """Attention of the batch's ``q [rows, heads, 128]`` (the cache's type) over the keys that
-        each row sees: ``[rows, heads * 128]`` in fp32 or bf16. A row without any gives zeros."""
+        each row sees: ``[rows, heads * 128]`` in fp32 or bf16. A row without any gives zeros.
+
+        Scores, softmax sums and results are held in fp32; the weights are rounded to the cache's
+        type for their product with the values (a row's result in fp32 is off by up to about 2.5
+        parts in 10^4 of its size over an fp16 cache, 2 in 10^3 over a bf16 one)."""
         lib = self._entry(layer, batch)
         if q.shape != batch._q_shape or q.dtype is not self.dtype or \
                 q.get_device() != self._index or not q.is_contiguous():
