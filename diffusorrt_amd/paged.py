@@ -6,6 +6,7 @@ same page (a prefix in common).
 """
 from __future__ import annotations
 
+import copy
 import ctypes as C
 import operator
 
@@ -142,11 +143,8 @@ class PagedBatch:
     def heads(self) -> int:
         return self.info.hq
 
-    def _here(self) -> int:
-        """The list's address, for the current stream."""
-        if torch._C._cuda_getCurrentRawStream(self._index) != self._stream:
-            self._elsewhere()
-        return self._at
+    def __deepcopy__(self, memo):
+        return self  # (a plan does not change)
 
     def _elsewhere(self):
         """The list is used on a stream that is not the one it was copied on."""
@@ -194,14 +192,26 @@ class PagedKVCache:
                                  self.page_size // 32 * KV_TILE_ELEMS), dtype=self.dtype,
                                 device=device)
         self._index = self.data.get_device()
+        self._own_streams()
+        self._geometry = (self.kv_heads, self.pages, self.page_size, self._index)
+        self._layer_bytes = self.data.stride(0) * 2
+        self._lib = None
+
+    def __deepcopy__(self, memo):
+        if self._index >= 0 and _capturing(self._index):
+            raise ValueError("a cache is copied before a graph is captured, not in it")
+        other = copy.copy(self)
+        other.data = self.data.clone()
+        other._own_streams()
+        return other
+
+    def _own_streams(self):
+        """The tensor was made on the current stream: what fills it is done before any other uses it."""
         self._streams = ()
-        if self._index >= 0:  # the zeros are there before any stream writes rows
+        if self._index >= 0:
             stream = torch.cuda.current_stream(self._index)
             stream.synchronize()
             self._streams = {stream.cuda_stream}
-        self._geometry = (self.kv_heads, self.pages, self.page_size, self._index)
-        self._data, self._layer_bytes = self.data.data_ptr(), self.data.stride(0) * 2
-        self._lib = None
 
     @property
     def nbytes(self) -> int:
@@ -224,7 +234,8 @@ class PagedKVCache:
         return PagedBatch(self, pages, keys, rows, heads, positions, kind, mask_geometry)
 
     def _entry(self, layer, batch):
-        """The library, once a call's layer and batch are checked."""
+        """The library, the batch's list on the device and the layer's pages, once a call's layer and
+        batch are checked and both are the current stream's to use."""
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer must be in [0, {self.layers})")
         if self._index < 0:
@@ -232,11 +243,14 @@ class PagedKVCache:
         if not isinstance(batch, PagedBatch) or (batch._geometry is not self._geometry and
                                                  batch._geometry != self._geometry):
             raise ValueError("the batch was planned for another cache")
-        if torch._C._cuda_getCurrentRawStream(self._index) not in self._streams:
+        stream = torch._C._cuda_getCurrentRawStream(self._index)
+        if stream not in self._streams:
             _lend(self.data, self._index, self._streams)
+        if stream != batch._stream:
+            batch._elsewhere()
         if self._lib is None:
             self._lib = _lib.load()
-        return self._lib
+        return self._lib, batch._at, self.data.data_ptr() + layer * self._layer_bytes
 
     def _bad_source(self, what, t, shape):
         if t.shape != shape or t.get_device() != self._index:
@@ -252,7 +266,7 @@ class PagedKVCache:
         which comes back in the cache's type, ready for :meth:`attention`. Each value is rounded
         once. Raises ValueError where two sequences of the batch have rows in one tile of a page,
         or a row lies behind its sequence's keys."""
-        lib = self._entry(layer, batch)
+        lib, plan, pages = self._entry(layer, batch)
         index, shape = self._index, batch._kv_shape
         if k.shape != shape or k.get_device() != index or k.stride(2) != 1:
             self._bad_source("append's k", k, shape)
@@ -285,19 +299,19 @@ class PagedKVCache:
                                  "bfloat16")
             out = q.new_empty(shape, dtype=self.dtype)
             q_at, out_at = q.data_ptr(), out.data_ptr()
-        _launch(torch, lib.drt_op_paged_append, index, batch._address, batch._here(),
+        _launch(torch, lib.drt_op_paged_append, index, batch._address, plan,
                 k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, q_at, q0, q1, code, turns,
-                self._data + layer * self._layer_bytes, self.kv_dtype, out_at)
+                pages, self.kv_dtype, out_at)
         return out
 
     def load(self, layer: int, batch: PagedBatch):
         """``(k, v) [rows, kv_heads, 128]`` of the batch's rows as the cache holds them. Raises
         ValueError where :meth:`append` of the batch does."""
-        lib = self._entry(layer, batch)
+        lib, plan, pages = self._entry(layer, batch)
         k = self.data.new_empty(batch._kv_shape)
         v = self.data.new_empty(batch._kv_shape)
-        _launch(torch, lib.drt_op_paged_load, self._index, batch._address, batch._here(),
-                self._data + layer * self._layer_bytes, self.kv_dtype, k.data_ptr(), v.data_ptr())
+        _launch(torch, lib.drt_op_paged_load, self._index, batch._address, plan,
+                pages, self.kv_dtype, k.data_ptr(), v.data_ptr())
         return k, v
 
     def attention(self, layer: int, q, batch: PagedBatch, *, out_dtype=None):
@@ -307,7 +321,7 @@ class PagedKVCache:
         Scores, softmax sums and results are held in fp32; the weights are rounded to the cache's
         type for their product with the values (a row's result in fp32 is off by up to about 2.5
         parts in 10^4 of its size over an fp16 cache, 2 in 10^3 over a bf16 one)."""
-        lib = self._entry(layer, batch)
+        lib, plan, pages = self._entry(layer, batch)
         if q.shape != batch._q_shape or q.dtype is not self.dtype or \
                 q.get_device() != self._index or not q.is_contiguous():
             raise ValueError(f"q must be contiguous {list(batch._q_shape)} of the cache's type and "
@@ -319,8 +333,8 @@ class PagedKVCache:
         out = q.new_empty(batch._out_shape, dtype=out_dtype)
         need = batch._workspace
         ws = q.new_empty(need, dtype=torch.uint8) if need else None
-        _launch(torch, lib.drt_op_paged_attention, self._index, batch._address, batch._here(),
-                q.data_ptr(), self._data + layer * self._layer_bytes, self.kv_dtype,
+        _launch(torch, lib.drt_op_paged_attention, self._index, batch._address, plan,
+                q.data_ptr(), pages, self.kv_dtype,
                 out.data_ptr(), _lib.BF16 if out_dtype is torch.bfloat16 else _lib.F32,
                 None if ws is None else ws.data_ptr(), need)
         return out

@@ -170,7 +170,7 @@ _TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib
 def _capturing(index):
     """Whether the current stream of device ``index`` is being captured."""
     if torch._C._cuda_getDevice() == index:
-        return torch.cuda.is_current_stream_capturing()
+        return torch._C._cuda_isCurrentStreamCapturing()
     with torch.cuda.device(index):
         return torch.cuda.is_current_stream_capturing()
 
@@ -224,6 +224,9 @@ class RotaryPositions:
                                  self.magnitude)
         self._address = C.addressof(self._args)
         self._rotate = None
+
+    def __deepcopy__(self, memo):
+        return self  # (frequencies do not change)
 
     def rotate(self, x, positions, *, inverse: bool = False, out=None):
         """``x [rows, heads, head_dim]`` (fp32, fp16 or bf16; any strides between rows and heads)
