@@ -53,6 +53,17 @@ def test_dropped_after_a_call_on_another_stream(call):
     assert torch.equal(got, want) and len(taken) == 64
 
 
+def test_no_rotation_is_made_in_a_capture():
+    x = torch.zeros(4, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError, match="captured"):
+            RotaryPositions(8)
+        x += 1
+    graph.replay()
+    assert torch.equal(x.cpu(), torch.ones(4))
+
+
 def test_streams_are_told_once_and_captures_never():
     rotary = RotaryPositions(8)
     x = torch.zeros(2, 1, 8, device="cuda")

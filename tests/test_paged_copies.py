@@ -47,3 +47,15 @@ def test_rows_of_a_copy_are_not_the_caches():
     del cache
     q = torch.zeros(5, 1, 128, dtype=torch.float16, device="cuda")
     assert torch.equal(other.attention(0, q, batch), torch.full((5, 128), 3.0, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_no_cache_is_copied_in_a_capture():
+    x, cache = torch.zeros(4, device="cuda"), PagedKVCache(1, 1, 1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError, match="captured"):
+            copy.deepcopy(cache)
+        x += 1
+    graph.replay()
+    assert torch.equal(x.cpu(), torch.ones(4))
