@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from .kernels import KV_TILE_ELEMS, _cache_dtype, _launch, _mask_args
-from .rotary import _TYPES, _capturing, _lend, _whole
+from .rotary import _TYPES, _before_captures, _capturing, _lend, _whole
 
 _I32_MAX = 2**31 - 1
 
@@ -165,9 +165,9 @@ class PagedKVCache:
     Which pages a sequence has, and in which order, is the caller's: :meth:`batch` takes the
     lists. A page may be given to another sequence without clearing it.
 
-    Calls may be on any stream; a call that reads what another stream's wrote waits for it (the
-    caller's to see to, as for any tensor). Keep the cache as long as a captured graph that used it
-    is replayed."""
+    Calls may be on any stream; that one which reads comes behind the one which wrote is the
+    caller's to see to, as for any tensor. Keep the cache as long as a captured graph that used it
+    is replayed. A deep copy has pages of its own, and takes the same batches."""
 
     def __init__(self, layers: int, kv_heads: int, pages: int, *, page_size: int = 64,
                  dtype="f16", device=None):
@@ -183,14 +183,9 @@ class PagedKVCache:
         if self.kv_dtype == _lib.I8:
             raise ValueError("a paged cache's dtype is 'f16' or 'bf16'")
         self.dtype = torch.bfloat16 if self.kv_dtype == _lib.BF16 else torch.float16
-        device = torch.device(device or "cuda")
-        if device.type == "cuda":
-            with torch.cuda.device(device):
-                if torch.cuda.is_current_stream_capturing():
-                    raise ValueError("a cache is made before a graph is captured, not in it")
         self.data = torch.zeros((self.layers, self.pages, self.kv_heads,
                                  self.page_size // 32 * KV_TILE_ELEMS), dtype=self.dtype,
-                                device=device)
+                                device=_before_captures(device, "a cache"))
         self._index = self.data.get_device()
         self._own_streams()
         self._geometry = (self.kv_heads, self.pages, self.page_size, self._index)
@@ -198,8 +193,7 @@ class PagedKVCache:
         self._lib = None
 
     def __deepcopy__(self, memo):
-        if self._index >= 0 and _capturing(self._index):
-            raise ValueError("a cache is copied before a graph is captured, not in it")
+        _before_captures(self.data.device, "a cache's copy")
         other = copy.copy(self)
         other.data = self.data.clone()
         other._own_streams()

@@ -175,6 +175,17 @@ def _capturing(index):
         return torch.cuda.is_current_stream_capturing()
 
 
+def _before_captures(device, what):
+    """The device that ``what`` is made on, where no graph is being captured: what fills it would be
+    the graph's."""
+    device = torch.device(device or "cuda")
+    if device.type == "cuda":
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError(f"{what} is made before a graph is captured, not in it")
+    return device
+
+
 def _lend(tensor, index, streams):
     """The current stream, none of the tensor's ``streams`` yet, reads it: the allocator is told, so
     that dropping the tensor does not give its memory away under a launch. (In a capture there is
@@ -216,7 +227,7 @@ class RotaryPositions:
             raise ValueError("rotary magnitude must be a finite number of fp32")
         self.dim, self.layout = dim, layout
         self.turns = torch.tensor([_turns(f) for f in self.frequencies], dtype=torch.int64,
-                                  device=device or "cuda")
+                                  device=_before_captures(device, "a rotation"))
         self._index = self.turns.get_device()
         # (they are on the device: the copy of pageable memory waits for itself)
         self._streams = {torch._C._cuda_getCurrentRawStream(self._index)} if self._index >= 0 else ()
